@@ -409,6 +409,116 @@ int migemm_gemm_plan(int transA, int transB, int M, int N, int K,
                      const float *bias, float *C, int64_t ldc, int64_t strideC,
                      int batch, int flags, char *plan, size_t plan_len);
 
+/* ------------------------------------------------------------------------------- */
+/* (6) Serving in 8 bits: layers whose weights, and a paged cache whose keys and values, are
+ *     held as int8 with float32 scales. The reference has no counterpart.
+ *
+ * Activations are float32 or bfloat16 (`type`); scales, sums, softmax statistics and bias
+ * are 32-bit. Row strides (ld*) are in elements of their operand; rows are contiguous.
+ * The scale of a set of values with largest magnitude a is s = fl(a / 127), 0 where that is
+ * subnormal and NaN where a value is not finite; a value x is held as
+ * rint(fl(x * fl(1 / s))), half to even (s = 0: as 0; s = NaN: the bytes hold nothing, and
+ * what is computed from them is NaN).
+ * Lengths, counts, tables and slots are read on the GPU: entries out of range are never
+ * followed (each entry says what it does with them). */
+#define MIGEMM_FLOAT32 0
+#define MIGEMM_BFLOAT16 1
+
+/* values[r, k] and scales[r] of the rows of X [rows, cols]. ldv >= cols rounded up to 16
+ * (the added columns are written as 0), ldv % 16 == 0, values 16-byte aligned. */
+int migemm_quantize_rows(void *stream, const void *X, int type, int64_t ldx, int8_t *values,
+                         int64_t ldv, float *scales, int rows, int cols);
+
+/* C[m, n] = (sum_k A[m, k] * B[n, k]) * a_scales[m] * b_scales[n] (+ bias[n] if not NULL):
+ * A [M, K] and B [N, K] int8, C [M, N] of `type`. The sum is exact (int32; K <= 131071).
+ * K, lda and ldb multiples of 16, A and B 16-byte aligned, lda and ldb <= 2^23. */
+int migemm_matmul_int8(void *stream, const int8_t *A, int64_t lda, const float *a_scales,
+                       const int8_t *B, int64_t ldb, const float *b_scales, const float *bias,
+                       void *C, int type, int64_t ldc, int M, int N, int K);
+
+/* Y = the product above of the quantised rows of X [M, cols] (X and Y of `type`) and
+ * W [N, K], K = cols rounded up to 16 (as migemm_quantize_rows leaves a weight [N, cols]).
+ * One launch for a few rows; otherwise the quantised rows go to the stream's workspace. */
+int migemm_linear_int8(void *stream, const void *X, int type, int64_t ldx, const int8_t *W,
+                       int64_t ldw, const float *w_scales, const float *bias, void *Y,
+                       int64_t ldy, int M, int N, int cols);
+
+/* The paged cache: keys int8 [pages, kv_heads, page_size, width], values int8 [pages,
+ * kv_heads, width, page_size] (a head's values transposed within a page), float32 scales
+ * [pages, kv_heads] of each. width = head_dim rounded up to 32 (to 64 above 128);
+ * head_dim a multiple of 8 up to 256, page_size 16, 32, 64 or 128, all four pointers 16-byte
+ * aligned (scales 4). Slot s is token s % page_size of page s / page_size; a request's token
+ * at position p is in page table[request, p / page_size] (table [requests, max_pages]). */
+
+/* The pages and slots of a step that adds counts[i] tokens to each request of lengths[i]
+ * tokens. Requests are packed in order: starts [requests + 1] are their first tokens' places
+ * (at most `tokens`, the size of slots and positions). Request i needs ceil((length + count)
+ * / page_size) - ceil(length / page_size) new pages; it is admitted if its table row and
+ * `tokens` hold it and it needs none or all it needs are left when the requests before it
+ * (that fit) have theirs. New pages come from the end of free_pages[0 .. *free_count)
+ * (read as at most free_capacity, the size of free_pages) and are written to the table.
+ * slots[t] and positions[t] are token t's, -1 where its request is not admitted or t is past
+ * the step's tokens. new_lengths = lengths + counts where admitted, else lengths; *new_free =
+ * the pages left. Negative lengths and counts are read as 0, a page number that is negative
+ * or has no int32 slot gives slot and position -1. Only table, slots, positions, starts, new_lengths and new_free are
+ * written: the same call again gives the same results, until the caller takes new_lengths and
+ * new_free as its lengths and free_count. */
+int migemm_cache_tables(void *stream, const int *lengths, const int *counts, int requests,
+                        int *table, int max_pages, int page_size, const int *free_pages,
+                        const int *free_count, int free_capacity, int *slots,
+                        int *positions, int *starts, int *new_lengths, int *new_free,
+                        int tokens);
+
+/* The slots, positions and starts alone, of tokens lengths[i] .. lengths[i] + counts[i] of
+ * each request in the pages that its table row already names (e.g. lengths 0 and counts the
+ * lengths: every token of the cache). */
+int migemm_cache_slots(void *stream, const int *lengths, const int *counts, int requests,
+                       const int *table, int max_pages, int page_size, int *slots,
+                       int *positions, int *starts, int tokens);
+
+/* Gives the pages of each request i with finished[i] != 0 back: they are added at the end of
+ * free_pages (which holds `pages`), *free_count grows, its table entries become -1 and its
+ * length 0. Pages outside the pool, or beyond what free_pages holds, are dropped. */
+int migemm_cache_release(void *stream, const int *finished, int *lengths, int requests,
+                         int *table, int max_pages, int page_size, int *free_pages, int pages,
+                         int *free_count);
+
+/* Writes K and V [tokens, kv_heads, head_dim] (tokens ldk / ldv elements apart) into their
+ * slots. The tokens of one page are neighbours in the call (as migemm_cache_tables gives
+ * them); slots outside the pool are skipped. For each page and head that gets tokens the new
+ * scale is the larger of the old one and of the new tokens', the old one dropped where the
+ * page's first slot is among the new; where it grew, what the page holds is rounded anew:
+ * rint(fl(v * fl(old / new))). A value that is not finite makes its page's scale NaN for that
+ * head, until the page is begun again. */
+int migemm_cache_append(void *stream, const void *K, const void *V, int type, int64_t ldk,
+                        int64_t ldv, const int *slots, int tokens, int8_t *keys,
+                        int8_t *values, float *key_scales, float *value_scales, int pages,
+                        int kv_heads, int head_dim, int page_size);
+
+/* K and V [tokens, kv_heads, head_dim] (contiguous, of `type`) = what the cache holds at
+ * slots; 0 for slots outside the pool. */
+int migemm_cache_read(void *stream, const int8_t *keys, const int8_t *values,
+                      const float *key_scales, const float *value_scales, int pages,
+                      int kv_heads, int head_dim, int page_size, const int *slots, int tokens,
+                      void *K, void *V, int type);
+
+/* O[t, h] = softmax(scale * Q[t, h] . keys) values over positions 0 .. positions[t] of token
+ * t's request, head h / (heads / kv_heads) of the cache: Q (tokens ldq elements apart) and O
+ * (contiguous) [tokens, heads, head_dim] of `type`, heads a multiple of kv_heads. Request i
+ * has tokens starts[i] .. starts[i + 1]; tokens past starts[requests] and those with position
+ * -1 give 0. Positions are read as below max_pages * page_size, starts as within [0, tokens];
+ * cached tokens whose table entry is outside the pool are left out.
+ * max_count (most tokens of one request, 0: unknown) and max_length (longest request after
+ * the step, 0: unknown) shape the launch; results are right whatever they say.
+ * Contexts are cut in ranges where the requests alone do not fill the GPU; their partial
+ * results go to the stream's workspace and are joined in order: the same bits every time. */
+int migemm_cache_attention(void *stream, const void *Q, int type, int64_t ldq,
+                           const int8_t *keys, const int8_t *values, const float *key_scales,
+                           const float *value_scales, int pages, int kv_heads, int head_dim,
+                           int page_size, const int *table, int max_pages, const int *starts,
+                           const int *positions, int requests, int tokens, int heads,
+                           float scale, int max_count, int max_length, void *O);
+
 #ifdef __cplusplus
 }
 #endif

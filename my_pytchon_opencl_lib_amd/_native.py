@@ -22,6 +22,10 @@ MIGEMM_ERR_NO_QUEUE = 7
 
 MIGEMM_GEMM_ACCUMULATE = 1  # migemm_gemm_strided_batched_ex flag: C += result
 
+# Activation types of the 8-bit operators
+MIGEMM_FLOAT32 = 0
+MIGEMM_BFLOAT16 = 1
+
 # Kernel-family policies (migemm_set_gemm_policy)
 MIGEMM_POLICY_AUTO = 0
 MIGEMM_POLICY_TILED = 1
@@ -80,6 +84,7 @@ _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
 _ip = ctypes.POINTER(ctypes.c_int)
+_f32 = ctypes.c_float
 SIGNATURES = {
     "migemm_gemm_strided_batched": ([_vp, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _vp,
                                      _i64, _i64, _vp, _vp, _i64, _i64, _i32], _i32),
@@ -136,6 +141,21 @@ SIGNATURES = {
     "migemm_stream_read": ([_vp, _vp, _sz, _vp, _i32], _i32),
     "migemm_gemm_plan": ([_i32, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
                           _vp, _i64, _i64, _i32, _i32, ctypes.c_char_p, _sz], _i32),
+    "migemm_quantize_rows": ([_vp, _vp, _i32, _i64, _vp, _i64, _vp, _i32, _i32], _i32),
+    "migemm_matmul_int8": ([_vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _i64, _i32,
+                            _i32, _i32], _i32),
+    "migemm_linear_int8": ([_vp, _vp, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32,
+                            _i32], _i32),
+    "migemm_cache_tables": ([_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32] +
+                            [_vp] * 5 + [_i32], _i32),
+    "migemm_cache_slots": ([_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _i32], _i32),
+    "migemm_cache_release": ([_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _i32, _vp], _i32),
+    "migemm_cache_append": ([_vp, _vp, _vp, _i32, _i64, _i64, _vp, _i32] + [_vp] * 4 +
+                            [_i32] * 4, _i32),
+    "migemm_cache_read": ([_vp] * 5 + [_i32] * 4 + [_vp, _i32, _vp, _vp, _i32], _i32),
+    "migemm_cache_attention": ([_vp, _vp, _i32, _i64] + [_vp] * 4 + [_i32] * 4 +
+                               [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _i32, _i32, _vp],
+                               _i32),
 }
 
 _lib = None

@@ -11,11 +11,12 @@ import sys
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libmigemm.so")
-SOURCES = ["gemm_direct_256.hip", "gemm_direct_128x256.hip", "gemm_direct_128.hip",
+SOURCES = ["cache_attention_f32.hip", "cache_attention_bf16.hip", "gemm_int8.hip",
+           "gemm_direct_256.hip", "gemm_direct_128x256.hip", "gemm_direct_128.hip",
            "gemm_direct_64.hip", "gemm_split_256x128.hip", "gemm_split_128.hip",
            "gemm_split.hip", "gemm_mfma.hip", "api.hip", "gemm_direct.hip", "gemm_small.hip",
            "gemm_skinny.hip", "aux_kernels.hip", "runtime.hip", "gemm_panel.hip",
-           "gemm_tiny.hip"]
+           "gemm_tiny.hip", "quantize_rows.hip", "cache8.hip", "serve_api.hip"]
 ARCH = "gfx950"
 
 

@@ -1,0 +1,425 @@
+// The 8-bit paged cache: its tables and slots, and the kernels that write and read tokens.
+// The layouts and rules are those of include/migemm.h (6).
+#include "int8_common.h"
+
+namespace migemm {
+namespace {
+
+// ---------------------------------------------------------------------- tables and slots
+constexpr int TW = 1024;  // threads of a work-group, and tokens that one fills
+
+// Inclusive scan over the work-group (part: 16 ints of LDS, free again on return).
+template <typename F>
+__device__ __forceinline__ int scan_block(int v, int *part, F op) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o);
+        if (lane >= o) v = op(u, v);
+    }
+    if (lane == 63) part[wave] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TW / 64; ++w)
+        if (w < wave) v = op(part[w], v);
+    __syncthreads();
+    return v;
+}
+
+// One launch, no work-group waits for another: each runs over all requests (a scan of the
+// counts for the tokens' places, a scan of the pages asked for their pages; 8 bytes a request
+// from L2) and keeps, in LDS, what the requests that own tokens of its window of 1024 tokens
+// need; then one thread a token. Bound by latency: a step of a few hundred requests is one
+// round of loads, two scans and one more dependent load. The token at a new page's first
+// place writes that page to the table, so each entry has one writer; tokens in new pages take
+// them from the free list and never read an entry that another work-group may be writing.
+// GROW false: slots of the pages that the table already names, nothing is allocated.
+template <bool GROW>
+__global__ void __launch_bounds__(TW) cache_tables_kernel(TablesArgs a, int shift) {
+    __shared__ int part[TW / 64];
+    __shared__ int owner[TW], place[TW], ends[TW], first[TW], rank[TW];
+    __shared__ int taken;
+    const int tid = threadIdx.x;
+    const int w0 = blockIdx.x * TW;
+    const int cap = a.tokens + 1;  // places are added up to this: no sum overflows
+    const int mask = (1 << shift) - 1;
+    const int held = GROW ? min(max(*a.free_count, 0), a.free_capacity) : 0;
+    owner[tid] = -1;
+    if (tid == 0) taken = 0;
+    auto capped = [cap](int x, int y) { return min(x + y, cap); };
+    auto plus = [](int x, int y) { return x + y; };
+    int end0 = 0, asks0 = 0;  // sums over the requests of earlier rounds
+    __syncthreads();
+    for (int base = 0; base < a.requests; base += TW) {
+        const int r = base + tid;
+        const bool is = r < a.requests;
+        const int n = is ? max(a.lengths[r], 0) : 0;
+        const int count = is ? max(a.counts[r], 0) : 0;
+        const int c = min(count, cap);
+        const int end = min(scan_block(c, part, capped) + end0, cap);
+        const int start = end - c;
+        const bool fits = is && (int64_t)n + count <= ((int64_t)a.max_pages << shift) &&
+                          end <= a.tokens;  // (end is exact where it is below the cap)
+        const int have = GROW ? (int)(((int64_t)n + mask) >> shift) : a.max_pages;
+        const int asks = GROW && fits ? ((n + count + mask) >> shift) - have : 0;
+        int upto = 0;
+        if constexpr (GROW) upto = scan_block(asks, part, plus) + asks0;
+        const bool ok = fits && (asks == 0 || upto <= held);
+        if (is && blockIdx.x == 0) {
+            a.starts[r + 1] = min(end, a.tokens);
+            if (r == 0) a.starts[0] = 0;
+            if constexpr (GROW) {
+                a.new_lengths[r] = ok ? n + count : n;
+                if (ok && asks > 0) atomicMax(&taken, upto);
+            }
+        }
+        if (ok && c > 0 && end > w0 && start < w0 + TW) {
+            const int at = max(start - w0, 0);
+            owner[at] = r;
+            place[at] = n - start;
+            ends[at] = end;
+            first[at] = have;
+            rank[at] = upto - asks;
+        }
+        // carries: the last thread's sums
+        __syncthreads();
+        if (tid == TW - 1) {
+            part[0] = end;
+            part[1] = upto;
+        }
+        __syncthreads();
+        end0 = part[0];
+        asks0 = part[1];
+        __syncthreads();
+    }
+    __syncthreads();
+    if (GROW && blockIdx.x == 0 && tid == 0) *a.new_free = held - taken;
+    const int own = scan_block(owner[tid] >= 0 ? tid : -1, part,
+                               [](int x, int y) { return max(x, y); });
+    const int t = w0 + tid;
+    if (t >= a.tokens) return;
+    int slot = -1, pos = -1;
+    if (own >= 0 && t < ends[own]) {
+        const int r = owner[own];
+        const int p = place[own] + t;
+        const int j = p >> shift;
+        int *entry = a.table + (int64_t)r * a.max_pages + j;
+        int page;
+        if (GROW && j >= first[own]) {
+            page = a.free_pages[held - 1 - (rank[own] + j - first[own])];
+            if ((p & mask) == 0) *entry = page;
+        } else {
+            page = *entry;
+        }
+        if (page >= 0 && page <= INT32_MAX >> shift) {  // (else no page, or no int32 slot)
+            slot = (page << shift) + (p & mask);
+            pos = p;
+        }
+    }
+    a.slots[t] = slot;
+    a.positions[t] = pos;
+}
+
+// One work-group: a scheduler frees a few requests at a time, in order.
+__global__ void __launch_bounds__(TW)
+cache_release_kernel(const int *finished, int *lengths, int requests, int *table, int max_pages,
+                     int shift, int *free_pages, int pages, int *free_count) {
+    __shared__ int part[TW / 64];
+    __shared__ int last;
+    const int tid = threadIdx.x;
+    const int mask = (1 << shift) - 1;
+    int count = min(max(*free_count, 0), pages);
+    for (int r = 0; r < requests; ++r) {
+        if (finished[r] == 0) continue;  // the same for every thread
+        const int n = (int)min(((int64_t)max(lengths[r], 0) + mask) >> shift,
+                               (int64_t)max_pages);
+        for (int base = 0; base < n; base += TW) {
+            const int j = base + tid;
+            int *entry = table + (int64_t)r * max_pages + j;
+            const int page = j < n ? *entry : -1;
+            const int is = page >= 0 && page < pages;
+            const int upto = scan_block(is, part, [](int x, int y) { return x + y; });
+            if (is && count + upto <= pages) free_pages[count + upto - 1] = page;
+            if (j < n) *entry = -1;
+            if (tid == TW - 1) last = upto;
+            __syncthreads();
+            count = min(count + last, pages);
+            __syncthreads();
+        }
+        __syncthreads();
+        if (tid == 0) lengths[r] = 0;
+    }
+    __syncthreads();
+    if (tid == 0) *free_count = count;
+}
+
+// ------------------------------------------------------------------------------ append
+__device__ __forceinline__ int page_of(int slot, int shift, int pages) {
+    const int page = slot >> shift;
+    return slot >= 0 && page < pages ? page : -1;
+}
+
+struct AppendArgs {
+    const void *x[2];  // K, V
+    int64_t ld[2];
+    const int *slots;
+    int tokens, chunk;
+    Cache8 c;
+    int shift;
+};
+
+// A work-group takes the pages that begin (in the order of tokens) in its chunk of tokens, for
+// one head and one of K and V, one after the other, so that each page and head has one owner:
+// no atomics, and the scale, the rounding anew and the new tokens follow each other behind
+// barriers. Reads the new tokens twice (maximum, then rounding; the second time from L2).
+// Values are transposed through LDS so that a page's rows are written in whole words.
+// Bound by memory for prompts, by latency for single tokens; a page is rounded anew only
+// where its scale grew.
+template <typename T>
+__global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
+    __shared__ uint32_t most_part[4];
+    __shared__ int token_at[128];
+    __shared__ int run_end, fresh;
+    extern __shared__ __attribute__((aligned(16))) int8_t tile[];  // values: [page_size][W + 4]
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int h = blockIdx.y;
+    const bool is_v = blockIdx.z != 0;
+    const T *x = static_cast<const T *>(a.x[is_v]) + (int64_t)h * a.c.dim;
+    const int64_t ld = a.ld[is_v];
+    const int P = a.c.page_size, W = a.c.width, D = a.c.dim, d8 = D / 8;
+    const int c0 = blockIdx.x * a.chunk;
+    // which tokens of the chunk begin a page (chunk <= 64: every wavefront finds the same)
+    bool begins = false;
+    if (lane < a.chunk && c0 + lane < a.tokens) {
+        const int pg = page_of(a.slots[c0 + lane], a.shift, a.c.pages);
+        begins = pg >= 0 && (c0 + lane == 0 ||
+                             page_of(a.slots[c0 + lane - 1], a.shift, a.c.pages) != pg);
+    }
+    uint64_t todo = __ballot(begins);
+    while (todo != 0) {
+        const int t0 = c0 + __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int page = a.slots[t0] >> a.shift;
+        if (tid < P) token_at[tid] = -1;
+        if (tid == 0) {
+            run_end = t0 + P;
+            fresh = 0;
+        }
+        __syncthreads();
+        // the run: the tokens from t0 on that stay in the page, at most as many as it holds
+        if (tid < P) {
+            const int t = t0 + tid;
+            const bool in = t < a.tokens && page_of(a.slots[t], a.shift, a.c.pages) == page;
+            if (!in) atomicMin(&run_end, t);
+        }
+        __syncthreads();
+        const int n = run_end - t0;
+        if (tid < n) {
+            const int off = a.slots[t0 + tid] & (P - 1);
+            atomicMax(&token_at[off], tid);
+            if (off == 0) fresh = 1;
+        }
+        uint32_t most = 0;
+        for (int i = tid; i < n * d8; i += 256) {
+            const int t = i / d8, e = i - t * d8;
+            float v[8];
+            load_f32<T, 8>(x + (int64_t)(t0 + t) * ld + e * 8, 8, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t b = __float_as_uint(v[k]) & 0x7fffffffu;
+                most = b > most ? b : most;
+            }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint32_t b = __shfl_xor(most, o);
+            most = b > most ? b : most;
+        }
+        if (lane == 0) most_part[tid >> 6] = most;
+        const int64_t ph = (int64_t)page * a.c.heads + h;
+        float *scale = (is_v ? a.c.value_scales : a.c.key_scales) + ph;
+        const float was = *scale;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) most = most_part[w] > most ? most_part[w] : most;
+        const float old = fresh ? 0.0f : was;
+        const float mine = scale_of(most);
+        // the larger; NaN where either is
+        const float now = old != old ? old : (mine != mine || mine > old ? mine : old);
+        if (tid == 0) *scale = now;
+        int8_t *base = (is_v ? a.c.values : a.c.keys) + ph * P * W;
+        if (!fresh && now > old) {  // (not where now is NaN: the bytes hold nothing then)
+            const float ratio = old / now;
+            for (int i = tid; i < P * W / 16; i += 256) {
+                uint4 q = reinterpret_cast<uint4 *>(base)[i];
+                uint32_t *w = reinterpret_cast<uint32_t *>(&q);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t b[4];
+#pragma unroll
+                    for (int m = 0; m < 4; ++m)
+                        b[m] = held_byte((float)(int8_t)(w[k] >> (8 * m)), ratio);
+                    w[k] = pack4(b[0], b[1], b[2], b[3]);
+                }
+                reinterpret_cast<uint4 *>(base)[i] = q;
+            }
+        }
+        __syncthreads();
+        const float inv = inverse_scale(now);
+        for (int i = tid; i < n * d8; i += 256) {
+            const int t = i / d8, e = i - t * d8;
+            const int off = a.slots[t0 + t] & (P - 1);
+            if (token_at[off] != t) continue;
+            float v[8];
+            load_f32<T, 8>(x + (int64_t)(t0 + t) * ld + e * 8, 8, v);
+            uint2 q;
+            q.x = pack4(held_byte(v[0], inv), held_byte(v[1], inv), held_byte(v[2], inv),
+                        held_byte(v[3], inv));
+            q.y = pack4(held_byte(v[4], inv), held_byte(v[5], inv), held_byte(v[6], inv),
+                        held_byte(v[7], inv));
+            if (!is_v)
+                *reinterpret_cast<uint2 *>(base + off * W + e * 8) = q;
+            else {
+                *reinterpret_cast<uint32_t *>(tile + off * (W + 4) + e * 8) = q.x;
+                *reinterpret_cast<uint32_t *>(tile + off * (W + 4) + e * 8 + 4) = q.y;
+            }
+        }
+        if (is_v) {
+            __syncthreads();
+            const int groups = P / 4;  // of four neighbouring offsets
+            for (int i = tid; i < D * groups; i += 256) {
+                const int d = i / groups, off = (i - d * groups) * 4;
+                uint32_t b[4];
+                int here = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    b[k] = (uint8_t)tile[(off + k) * (W + 4) + d];
+                    here |= (token_at[off + k] >= 0) << k;
+                }
+                int8_t *out = base + (int64_t)d * P + off;
+                if (here == 15)
+                    *reinterpret_cast<uint32_t *>(out) = pack4(b[0], b[1], b[2], b[3]);
+                else if (here != 0) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (here >> k & 1) out[k] = (int8_t)b[k];
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// -------------------------------------------------------------------------------- read
+// 64 tokens of one head, of K or of V. Values are read along a page's tokens (neighbouring
+// slots are neighbouring bytes) and turned in LDS.
+template <typename T>
+__global__ void __launch_bounds__(256)
+cache_read_kernel(Cache8 c, const int *slots, int tokens, T *K, T *V, int shift) {
+    extern __shared__ __attribute__((aligned(16))) int8_t tile[];  // values: [64][W + 4]
+    __shared__ float scales[64];
+    __shared__ int64_t bases[64];
+    const int tid = threadIdx.x;
+    const int h = blockIdx.y;
+    const bool is_v = blockIdx.z != 0;
+    const int t0 = blockIdx.x * 64;
+    const int n = min(64, tokens - t0);
+    const int P = c.page_size, W = c.width, D = c.dim, d8 = D / 8;
+    if (tid < n) {
+        const int slot = slots[t0 + tid];
+        const int page = page_of(slot, shift, c.pages);
+        const int64_t ph = (int64_t)page * c.heads + h;
+        const int off = slot & (P - 1);
+        scales[tid] = page < 0 ? 0.f : (is_v ? c.value_scales : c.key_scales)[ph];
+        bases[tid] = page < 0 ? -1 : ph * P * W + (is_v ? off : off * W);
+    }
+    __syncthreads();
+    if (is_v) {
+        for (int i = tid; i < 64 * D; i += 256) {
+            const int t = i & 63, d = i >> 6;
+            if (t < n && bases[t] >= 0) tile[t * (W + 4) + d] = c.values[bases[t] + d * P];
+        }
+        __syncthreads();
+    }
+    T *out = (is_v ? V : K) + ((int64_t)t0 * c.heads + h) * D;
+    for (int i = tid; i < n * d8; i += 256) {
+        const int t = i / d8, e = i - t * d8;
+        uint32_t w[2] = {0, 0};
+        const float s = scales[t];
+        if (bases[t] >= 0) {
+            const int8_t *from = is_v ? tile + t * (W + 4) + e * 8 : c.keys + bases[t] + e * 8;
+            w[0] = *reinterpret_cast<const uint32_t *>(from);
+            w[1] = *reinterpret_cast<const uint32_t *>(from + 4);
+        }
+        struct {
+            T t[8];
+        } r;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            r.t[k] = from_f32<T>((float)(int8_t)(w[k / 4] >> (8 * (k & 3))) * s);
+        store_any(out + (int64_t)t * c.heads * D + e * 8, r);
+    }
+}
+
+int shift_of(int page_size) { return __builtin_ctz((unsigned)page_size); }
+}  // namespace
+
+int launch_cache_tables(hipStream_t stream, const TablesArgs &a) {
+    const unsigned blocks = a.tokens > 0 ? (unsigned)((a.tokens + TW - 1) / TW) : 1u;
+    const int shift = shift_of(a.page_size);
+    if (a.free_pages != nullptr)
+        MIGEMM_LAUNCH((cache_tables_kernel<true>), dim3(blocks), dim3(TW), 0, stream, a, shift);
+    else
+        MIGEMM_LAUNCH((cache_tables_kernel<false>), dim3(blocks), dim3(TW), 0, stream, a, shift);
+    return launch_status("cache_tables_kernel launch");
+}
+
+int launch_cache_release(hipStream_t stream, const int *finished, int *lengths, int requests,
+                         int *table, int max_pages, int page_size, int *free_pages, int pages,
+                         int *free_count) {
+    MIGEMM_LAUNCH(cache_release_kernel, dim3(1), dim3(TW), 0, stream, finished, lengths,
+                  requests, table, max_pages, shift_of(page_size), free_pages, pages,
+                  free_count);
+    return launch_status("cache_release_kernel launch");
+}
+
+int launch_cache_append(hipStream_t stream, const void *K, const void *V, int type,
+                        int64_t ldk, int64_t ldv, const int *slots, int tokens,
+                        const Cache8 &c) {
+    AppendArgs a{};
+    a.x[0] = K;
+    a.x[1] = V;
+    a.ld[0] = ldk;
+    a.ld[1] = ldv;
+    a.slots = slots;
+    a.tokens = tokens;
+    a.c = c;
+    a.shift = shift_of(c.page_size);
+    // work-groups for each CU several times over before one takes more than one page's tokens
+    const int64_t want = (int64_t)tokens * c.heads * 2 / 2048;
+    a.chunk = 1;
+    while (a.chunk < 64 && a.chunk < c.page_size && a.chunk < want) a.chunk *= 2;
+    const dim3 grid((tokens + a.chunk - 1) / a.chunk, c.heads, 2);
+    const size_t lds = (size_t)c.page_size * (c.width + 4);
+    if (type == MIGEMM_FLOAT32)
+        MIGEMM_LAUNCH((cache_append_kernel<float>), grid, dim3(256), lds, stream, a);
+    else
+        MIGEMM_LAUNCH((cache_append_kernel<Bf16>), grid, dim3(256), lds, stream, a);
+    return launch_status("cache_append_kernel launch");
+}
+
+int launch_cache_read(hipStream_t stream, const Cache8 &c, const int *slots, int tokens,
+                      void *K, void *V, int type) {
+    const dim3 grid((tokens + 63) / 64, c.heads, 2);
+    const size_t lds = (size_t)64 * (c.width + 4);
+    const int shift = shift_of(c.page_size);
+    if (type == MIGEMM_FLOAT32)
+        MIGEMM_LAUNCH((cache_read_kernel<float>), grid, dim3(256), lds, stream, c, slots, tokens,
+                      static_cast<float *>(K), static_cast<float *>(V), shift);
+    else
+        MIGEMM_LAUNCH((cache_read_kernel<Bf16>), grid, dim3(256), lds, stream, c, slots, tokens,
+                      static_cast<Bf16 *>(K), static_cast<Bf16 *>(V), shift);
+    return launch_status("cache_read_kernel launch");
+}
+
+}  // namespace migemm

@@ -13,7 +13,7 @@ NnClGlob.LinearForward) is the bias-epilogue form.
 import numpy as np
 import torch
 
-from .nncl_glob import NnClGlob, ShapeError, _require
+from .nncl_glob import NnClGlob, ShapeError, _check_typed, _require
 
 
 class Linear:
@@ -48,3 +48,36 @@ class Linear:
 
     def parameters(self):
         return [self.weight, self.bias]
+
+
+class LinearInt8:
+    """A Linear layer for serving, its weight held in 8 bits with a scale for each output:
+    y[..., out] = x[..., in] @ weight^T (+ bias). weight [out, in] is a float tensor or array
+    (e.g. Linear.weight), quantised here once; x and y are float32 or bfloat16."""
+
+    def __init__(self, weight, bias=None, nnclglob=None):
+        self.nnclglob = nnclglob if nnclglob is not None else NnClGlob()
+        dev = self.nnclglob.device
+        w = weight if isinstance(weight, torch.Tensor) else torch.as_tensor(
+            np.asarray(weight, dtype=np.float32))
+        _require(w.dim() == 2, "weight must be [out, in]")
+        self.out_channels, self.in_features = w.shape
+        if w.dtype != torch.bfloat16:
+            w = w.to(torch.float32)
+        self.weight, self.scales = self.nnclglob.QuantizeRows(w.to(dev).contiguous())
+        self.bias = None
+        if bias is not None:
+            b = bias if isinstance(bias, torch.Tensor) else torch.as_tensor(np.asarray(bias))
+            self.bias = b.to(dev, torch.float32).contiguous()
+            _check_typed("bias", self.bias, torch.float32, (self.out_channels,))
+
+    def forward(self, x):
+        if not isinstance(x, torch.Tensor) or not x.dim() or x.shape[-1] != self.in_features:
+            raise ShapeError(f"x must end in {self.in_features} features (got "
+                             f"{list(getattr(x, 'shape', []))})")
+        return self.nnclglob.LinearInt8(x, self.weight, self.scales, self.bias)
+
+    __call__ = forward
+
+    def parameters(self):
+        return [self.weight, self.scales] + ([self.bias] if self.bias is not None else [])

@@ -17,6 +17,10 @@ Reference interfaces mirrored (paths relative to the reference repository;
   permute(x, axes)                    :148     NnClGlob.permute(x, axes)
   bmm_backward(grad_output, A, B)     :283     NnClGlob.bmm_backward(grad_output, A, B)
 
+Beyond the reference, for serving in 8 bits: QuantizeRows, MatmulInt8, LinearInt8 (layers with
+int8 weights) and CacheTables, CacheSlots, CacheRelease, CacheAppend, CacheRead,
+CacheAttention (an int8 paged cache, cache.Int8Cache, and the attention that reads it).
+
 Tensors are torch float32 tensors resident on the GPU (torch is only the device-memory and
 stream plumbing); every operator enqueues a HIP kernel of libmigemm.so on the current torch
 stream through the C ABI. There is no CPU fallback: a CPU tensor or a missing library raises.
@@ -133,6 +137,53 @@ def _check_tensor(name, t):
     _require(t.dtype == torch.float32, f"{name} must be float32 (got {t.dtype})")
     _require(t.is_cuda, f"{name} must live on the GPU: the matmul path has no CPU fallback")
     _require(t.is_contiguous(), f"{name} must be contiguous (row-major, as Tensor.cs:283-295)")
+
+
+# Activations of the 8-bit operators.
+_TYPES = {torch.float32: _native.MIGEMM_FLOAT32, torch.bfloat16: _native.MIGEMM_BFLOAT16}
+
+
+def _check_rows(name, t, dim=None):
+    """An activation tensor of the 8-bit operators: float32 or bfloat16, on the GPU, its rows
+    contiguous (_row_stride). Returns the type's code."""
+    _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
+    if t.dtype not in _TYPES:
+        raise ShapeError(f"{name} must be float32 or bfloat16 (got {t.dtype})")
+    _require(t.is_cuda, f"{name} must live on the GPU: there is no CPU fallback")
+    if dim is not None and t.dim() != dim:
+        raise ShapeError(f"{name} must have {dim} axes (got {list(t.shape)})")
+    return _TYPES[t.dtype]
+
+
+def _row_stride(name, t):
+    """Elements between the rows t[i] of a tensor whose rows are contiguous blocks."""
+    if t.is_contiguous():
+        return t.numel() // t.shape[0] if t.shape[0] else 0
+    want = 1
+    for n, step in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if n != 1 and step != want:
+            raise ShapeError(f"the rows of {name} must be contiguous (strides "
+                             f"{list(t.stride())} of {list(t.shape)})")
+        want *= n
+    if t.shape[0] <= 1:
+        return want
+    if t.stride(0) < want:
+        raise ShapeError(f"the rows of {name} overlap (strides {list(t.stride())} of "
+                         f"{list(t.shape)})")
+    return t.stride(0)
+
+
+def _check_typed(name, t, dtype, shape=None):
+    """A contiguous GPU tensor of one type (and shape; None in it: any size)."""
+    _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise ShapeError(f"{name} must be {dtype} (got {t.dtype})")
+    _require(t.is_cuda, f"{name} must live on the GPU: there is no CPU fallback")
+    if not t.is_contiguous():
+        raise ShapeError(f"{name} must be contiguous (strides {list(t.stride())})")
+    if shape is not None and (t.dim() != len(shape) or
+                              any(a is not None and a != b for a, b in zip(shape, t.shape))):
+        raise ShapeError(f"{name} must have the shape {list(shape)} (got {list(t.shape)})")
 
 
 class NnClGlob:
@@ -449,3 +500,206 @@ class NnClGlob:
                 b3.shape[2], sB, _ptr(bias) if bias is not None else None, _ptr(out), n, m * n,
                 batch)
         return out.view(m, n) if squeeze else out
+
+    # ---------------------------------------------------------------- serving in 8 bits
+    # The reference has no counterpart. Activations are float32 or bfloat16; rows of a larger
+    # tensor (a slice of a fused projection) are taken as they lie. All of these only enqueue
+    # work on the current stream; nothing is read back.
+    def QuantizeRows(self, x):
+        """(values, scales) of x[..., K] in 8 bits, a scale for each row: scales [rows] =
+        max |x| / 127 over the row, values int8 [rows, K rounded up to 16] = x / scale rounded
+        half to even, the added columns 0. A weight [out, in] is laid out by it once; a row
+        with a value that is not finite gets the scale NaN."""
+        code = _check_rows("x", x)
+        k = x.shape[-1] if x.dim() else 0
+        if x.dim() < 1 or k < 1:
+            raise ShapeError(f"x must have rows of at least one value (got {list(x.shape)})")
+        x2 = x if x.dim() == 2 else x.reshape(-1, k)
+        rows = x2.shape[0]
+        values = torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+        if rows:
+            _launch("migemm_quantize_rows", (x2, values, scales), _ptr(x2), code,
+                    _row_stride("x", x2), _ptr(values), values.shape[1], _ptr(scales), rows, k)
+        return values, scales
+
+    def MatmulInt8(self, a, aScales, b, bScales, bias=None, dtype=torch.float32):
+        """C[M, N] = (a[M, K] @ b[N, K]^T) * aScales[M] * bScales[N] (+ bias[N]) of dtype: int8
+        rows as QuantizeRows gives them (K a multiple of 16, at most 131071; rows may lie
+        further apart than K). The integer sum is exact."""
+        if dtype not in _TYPES:
+            raise ShapeError(f"dtype must be float32 or bfloat16 (got {dtype})")
+        for name, t in (("a", a), ("b", b)):
+            _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
+            if t.dtype != torch.int8 or t.dim() != 2:
+                raise ShapeError(f"{name} must be int8 [rows, K] (got {t.dtype} "
+                                 f"{list(t.shape)})")
+            _require(t.is_cuda, f"{name} must live on the GPU: there is no CPU fallback")
+        m, k = a.shape
+        n = b.shape[0]
+        if b.shape[1] != k:
+            raise ShapeError(f"inner dimensions differ: {k} != {b.shape[1]}")
+        _check_typed("aScales", aScales, torch.float32, (m,))
+        _check_typed("bScales", bScales, torch.float32, (n,))
+        if bias is not None:
+            _check_typed("bias", bias, torch.float32, (n,))
+        c = torch.empty((m, n), dtype=dtype, device=a.device)
+        if m and n:
+            if not k:
+                raise ShapeError("K must be at least 1")
+            extra = (bias,) if bias is not None else ()
+            _launch("migemm_matmul_int8", (a, b, aScales, bScales, c) + extra, _ptr(a),
+                    _row_stride("a", a), _ptr(aScales), _ptr(b), _row_stride("b", b),
+                    _ptr(bScales), _ptr(bias) if bias is not None else None, _ptr(c),
+                    _TYPES[dtype], n, m, n, k)
+        return c
+
+    def LinearInt8(self, x, weight, scales, bias=None):
+        """y[..., N] = x[..., K] @ W^T (+ bias[N], float32) with W [N, K] as QuantizeRows left
+        it (weight int8 [N, K rounded up to 16], scales [N]); the rows of x are quantised on
+        the way. y has the type of x. One launch for up to four rows."""
+        code = _check_rows("x", x)
+        _check_typed("weight", weight, torch.int8, (None, None))
+        n, kp = weight.shape
+        k = x.shape[-1] if x.dim() else 0
+        if k < 1 or (k + 15) // 16 * 16 != kp:
+            raise ShapeError(f"x must end in the weight's features (got {list(x.shape)} and "
+                             f"rows of {kp} bytes)")
+        _check_typed("scales", scales, torch.float32, (n,))
+        if bias is not None:
+            _check_typed("bias", bias, torch.float32, (n,))
+        x2 = x if x.dim() == 2 else x.reshape(-1, k)
+        m = x2.shape[0]
+        y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        if m and n:
+            extra = (bias,) if bias is not None else ()
+            _launch("migemm_linear_int8", (x2, weight, scales, y) + extra, _ptr(x2), code,
+                    _row_stride("x", x2), _ptr(weight), kp, _ptr(scales),
+                    _ptr(bias) if bias is not None else None, _ptr(y), n, m, n, k)
+        return y if x.dim() == 2 else y.reshape(list(x.shape[:-1]) + [n])
+
+    def CacheTables(self, lengths, counts, table, free, freeCount, tokens, pageSize):
+        """The pages and slots of a step that adds counts[i] tokens to each request of
+        lengths[i] tokens: (slots [tokens], positions [tokens], starts [requests + 1], the new
+        lengths [requests], the pages left [1]), all int32; table [requests, pages a request]
+        gets the new pages' numbers, taken from the end of free[0 .. freeCount). Requests are
+        packed in order; `tokens` is the size of the step's buffers, tokens past the step's
+        end get slot and position -1. A request is admitted if its table row and `tokens` hold
+        it and it needs no new page or enough are left after the requests before it; else
+        its tokens get -1 and its length stays. The lengths and freeCount given are not
+        changed: a caller goes on with the ones returned."""
+        requests = lengths.numel() if isinstance(lengths, torch.Tensor) else 0
+        _check_typed("lengths", lengths, torch.int32, (None,))
+        _check_typed("counts", counts, torch.int32, (requests,))
+        _check_typed("table", table, torch.int32, (requests, None))
+        _check_typed("free", free, torch.int32, (None,))
+        _check_typed("freeCount", freeCount, torch.int32, (1,))
+        tokens = int(tokens)
+        _require(tokens >= 0, "tokens must not be negative")
+        # one buffer: five allocations would cost more than the kernel
+        out = torch.empty(2 * tokens + 2 * requests + 2, dtype=torch.int32,
+                          device=lengths.device)
+        slots, positions, starts, new, left = torch.split(
+            out, (tokens, tokens, requests + 1, requests, 1))
+        at = _ptr(out)
+        _launch("migemm_cache_tables", (lengths, counts, table, free, freeCount, out),
+                _ptr(lengths), _ptr(counts), requests, _ptr(table), table.shape[1],
+                int(pageSize), _ptr(free), _ptr(freeCount), free.numel(), at, at + 4 * tokens,
+                at + 8 * tokens, at + 8 * tokens + 4 * requests + 4,
+                at + 8 * tokens + 8 * requests + 4, tokens)
+        return slots, positions, starts, new, left
+
+    def CacheSlots(self, lengths, counts, table, tokens, pageSize):
+        """(slots [tokens], positions [tokens], starts [requests + 1]) of the tokens lengths[i]
+        .. lengths[i] + counts[i] of each request in the pages that its table row names: with
+        lengths 0 and the lengths as counts, every cached token."""
+        requests = lengths.numel() if isinstance(lengths, torch.Tensor) else 0
+        _check_typed("lengths", lengths, torch.int32, (None,))
+        _check_typed("counts", counts, torch.int32, (requests,))
+        _check_typed("table", table, torch.int32, (requests, None))
+        tokens = int(tokens)
+        _require(tokens >= 0, "tokens must not be negative")
+        out = torch.empty(2 * tokens + requests + 1, dtype=torch.int32, device=lengths.device)
+        slots, positions, starts = torch.split(out, (tokens, tokens, requests + 1))
+        at = _ptr(out)
+        _launch("migemm_cache_slots", (lengths, counts, table, out), _ptr(lengths),
+                _ptr(counts), requests, _ptr(table), table.shape[1], int(pageSize),
+                at, at + 4 * tokens, at + 8 * tokens, tokens)
+        return slots, positions, starts
+
+    def CacheRelease(self, finished, lengths, table, free, freeCount, pageSize):
+        """Gives the pages of every request with finished[i] != 0 back: added at the end of
+        free[0 .. freeCount) (free has room for the whole pool), its table row becomes -1 and
+        its length 0. In place."""
+        requests = lengths.numel() if isinstance(lengths, torch.Tensor) else 0
+        _check_typed("lengths", lengths, torch.int32, (None,))
+        _check_typed("finished", finished, torch.int32, (requests,))
+        _check_typed("table", table, torch.int32, (requests, None))
+        _check_typed("free", free, torch.int32, (None,))
+        _check_typed("freeCount", freeCount, torch.int32, (1,))
+        _launch("migemm_cache_release", (finished, lengths, table, free, freeCount),
+                _ptr(finished), _ptr(lengths), requests, _ptr(table), table.shape[1],
+                int(pageSize), _ptr(free), free.numel(), _ptr(freeCount))
+
+    def CacheAppend(self, k, v, slots, cache):
+        """Writes the keys k and values v [tokens, kv heads, head size] of a step into their
+        slots of an Int8Cache (slots of CacheTables; -1 skips a token; the tokens of one page
+        are neighbours). A page and head whose scale is too small for the new tokens gets
+        theirs, and what it holds is rounded anew."""
+        code = _check_rows("k", k, 3)
+        if _check_rows("v", v, 3) != code:
+            raise ShapeError(f"k and v must have one type (got {k.dtype} and {v.dtype})")
+        tokens = k.shape[0]
+        want = [tokens, cache.kvHeads, cache.headDim]
+        if list(k.shape) != want or list(v.shape) != want:
+            raise ShapeError(f"k and v must be {want} (got {list(k.shape)} and "
+                             f"{list(v.shape)})")
+        _check_typed("slots", slots, torch.int32, (tokens,))
+        if tokens:
+            _launch("migemm_cache_append", (k, v, slots, cache.keys), _ptr(k), _ptr(v), code,
+                    _row_stride("k", k), _row_stride("v", v), _ptr(slots), tokens,
+                    *cache.pointers, *cache.sizes)
+
+    def CacheRead(self, cache, slots, dtype=torch.float32):
+        """(k, v) [tokens, kv heads, head size] of dtype: what the cache holds at slots (e.g.
+        of CacheSlots), 0 where a slot is -1. For products over a cached context through Bmm."""
+        if dtype not in _TYPES:
+            raise ShapeError(f"dtype must be float32 or bfloat16 (got {dtype})")
+        _check_typed("slots", slots, torch.int32, (None,))
+        tokens = slots.numel()
+        k = torch.empty((tokens, cache.kvHeads, cache.headDim), dtype=dtype,
+                        device=slots.device)
+        v = torch.empty_like(k)
+        if tokens:
+            _launch("migemm_cache_read", (slots, cache.keys, k, v), *cache.pointers,
+                    *cache.sizes, _ptr(slots), tokens, _ptr(k), _ptr(v), _TYPES[dtype])
+        return k, v
+
+    def CacheAttention(self, q, cache, table, starts, positions, scale=None, maxCount=0,
+                       maxLength=0):
+        """Causal attention of a step's queries q [tokens, heads, head size] over an Int8Cache:
+        query t of request i (starts[i] <= t < starts[i + 1]) sees the request's tokens 0 ..
+        positions[t] (its own, already appended, among them), head h the kv head
+        h // (heads / kv heads). scale: 1 / sqrt(head size) if None. Tokens without a position
+        (-1) or request give 0. starts and positions are CacheTables'; maxCount (most tokens of
+        one request) and maxLength (longest request) shape the launches if the caller knows
+        them, the result does not depend on them. Returns [tokens, heads, head size] of q's
+        type."""
+        code = _check_rows("q", q, 3)
+        tokens, heads, dim = q.shape
+        if dim != cache.headDim or heads % cache.kvHeads or not heads:
+            raise ShapeError(f"q must be [tokens, a multiple of {cache.kvHeads} heads, "
+                             f"{cache.headDim}] (got {list(q.shape)})")
+        _check_typed("table", table, torch.int32, (None, None))
+        requests = table.shape[0]
+        _check_typed("starts", starts, torch.int32, (requests + 1,))
+        _check_typed("positions", positions, torch.int32, (tokens,))
+        o = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        if tokens:
+            _launch("migemm_cache_attention",
+                    (q, cache.keys, table, starts, positions, o), _ptr(q), code,
+                    _row_stride("q", q), *cache.pointers, *cache.sizes, _ptr(table),
+                    table.shape[1], _ptr(starts), _ptr(positions), requests, tokens, heads,
+                    dim ** -0.5 if scale is None else float(scale), int(maxCount),
+                    int(maxLength), _ptr(o))
+        return o
