@@ -166,20 +166,24 @@ struct AppendArgs {
     int tokens, chunk;
     Cache8 c;
     int shift;
+    FastDiv d8;  // head_dim / 8
 };
 
 // A work-group takes the pages that begin (in the order of tokens) in its chunk of tokens, for
 // one head and one of K and V, one after the other, so that each page and head has one owner:
 // no atomics, and the scale, the rounding anew and the new tokens follow each other behind
-// barriers. Reads the new tokens twice (maximum, then rounding; the second time from L2).
-// Values are transposed through LDS so that a page's rows are written in whole words.
-// Bound by memory for prompts, by latency for single tokens; a page is rounded anew only
-// where its scale grew.
+// barriers. New tokens stay in registers between the maximum and the rounding (up to 8192
+// values; what is beyond is read again). Values are transposed through LDS so that a page's rows
+// are written in whole words. Bound by memory for prompts; for single tokens by latency: two
+// loads that wait for each other (slots; tokens and scale). A page is rounded anew only where
+// its scale grew.
 template <typename T>
-__global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4)))
+cache_append_kernel(AppendArgs a) {
+    constexpr int KEEP = 4;  // items of 8 values that a thread keeps
     __shared__ uint32_t most_part[4];
     __shared__ int token_at[128];
-    __shared__ int run_end, fresh;
+    __shared__ int window[256];  // slots of tokens c0 - 1 ..: -1 outside the pool and the call
     extern __shared__ __attribute__((aligned(16))) int8_t tile[];  // values: [page_size][W + 4]
     const int tid = threadIdx.x, lane = tid & 63;
     const int h = blockIdx.y;
@@ -187,48 +191,76 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
     const T *x = static_cast<const T *>(a.x[is_v]) + (int64_t)h * a.c.dim;
     const int64_t ld = a.ld[is_v];
     const int P = a.c.page_size, W = a.c.width, D = a.c.dim, d8 = D / 8;
+    // item i: eight features from 8 e on of token t of the run
+    auto split = [&](int i, int &t, int &e) {
+        t = (int)fast_div((uint32_t)i, a.d8);
+        e = i - t * d8;
+    };
     const int c0 = blockIdx.x * a.chunk;
-    // which tokens of the chunk begin a page (chunk <= 64: every wavefront finds the same)
-    bool begins = false;
-    if (lane < a.chunk && c0 + lane < a.tokens) {
-        const int pg = page_of(a.slots[c0 + lane], a.shift, a.c.pages);
-        begins = pg >= 0 && (c0 + lane == 0 ||
-                             page_of(a.slots[c0 + lane - 1], a.shift, a.c.pages) != pg);
+    {  // chunk <= 64 and a page's 128 tokens: a window of 193 at most
+        const int t = c0 - 1 + tid;
+        const int slot = t >= 0 && t < a.tokens ? a.slots[t] : -1;
+        window[tid] = page_of(slot, a.shift, a.c.pages) >= 0 ? slot : -1;
     }
+    __syncthreads();
+    // which tokens of the chunk begin a page (every wavefront finds the same); slots of -1 have
+    // the page -1
+    const bool begins = lane < a.chunk && window[lane + 1] >= 0 &&
+                        window[lane] >> a.shift != window[lane + 1] >> a.shift;
     uint64_t todo = __ballot(begins);
+#pragma unroll 1
     while (todo != 0) {
-        const int t0 = c0 + __builtin_ctzll(todo);
+        const int at = __builtin_ctzll(todo) + 1;  // the page's first token in the window
         todo &= todo - 1;
-        const int page = a.slots[t0] >> a.shift;
-        if (tid < P) token_at[tid] = -1;
-        if (tid == 0) {
-            run_end = t0 + P;
-            fresh = 0;
-        }
-        __syncthreads();
+        const int t0 = c0 + at - 1;
+        const int page = window[at] >> a.shift;
+        const int64_t ph = (int64_t)page * a.c.heads + h;
+        float *scale = (is_v ? a.c.value_scales : a.c.key_scales) + ph;
+        const float was = *scale;
         // the run: the tokens from t0 on that stay in the page, at most as many as it holds
-        if (tid < P) {
-            const int t = t0 + tid;
-            const bool in = t < a.tokens && page_of(a.slots[t], a.shift, a.c.pages) == page;
-            if (!in) atomicMin(&run_end, t);
+        // (every wavefront finds the same)
+        int n = 0;
+        bool fresh = false;
+#pragma unroll 1
+        for (int base = 0; base < P; base += 64) {
+            const int i = at + base + lane;
+            const int slot = base + lane < P ? window[i] : -1;
+            const uint64_t in = __ballot(slot >= 0 && slot >> a.shift == page);
+            const int run = in == ~0ull ? 64 : __builtin_ctzll(~in);
+            const uint64_t zero = __ballot(lane < run && (slot & (P - 1)) == 0);
+            fresh = fresh || zero != 0;
+            n += run;
+            if (run < 64) break;
         }
-        __syncthreads();
-        const int n = run_end - t0;
-        if (tid < n) {
-            const int off = a.slots[t0 + tid] & (P - 1);
-            atomicMax(&token_at[off], tid);
-            if (off == 0) fresh = 1;
-        }
-        uint32_t most = 0;
-        for (int i = tid; i < n * d8; i += 256) {
-            const int t = i / d8, e = i - t * d8;
-            float v[8];
-            load_f32<T, 8>(x + (int64_t)(t0 + t) * ld + e * 8, 8, v);
+        const int items = n * d8;
+        float v[KEEP][8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t b = __float_as_uint(v[k]) & 0x7fffffffu;
+        for (int k = 0; k < KEEP; ++k) {
+            const int i = tid + 256 * k;
+            int t, e;
+            split(i, t, e);
+            // (past the run: its first item again, so that no register depends on a branch)
+            load_f32<T, 8>(x + (i < items ? (int64_t)(t0 + t) * ld + e * 8 : (int64_t)t0 * ld), 8,
+                           v[k]);
+        }
+        if (tid < P) token_at[tid] = -1;
+        uint32_t most = 0;
+        auto largest = [&most](const float(&y)[8]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t b = __float_as_uint(y[j]) & 0x7fffffffu;
                 most = b > most ? b : most;
             }
+        };
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k) largest(v[k]);
+#pragma unroll 1
+        for (int i = tid + 256 * KEEP; i < items; i += 256) {
+            int t, e;
+            split(i, t, e);
+            float y[8];
+            load_f32<T, 8>(x + (int64_t)(t0 + t) * ld + e * 8, 8, y);
+            largest(y);
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
@@ -236,12 +268,10 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
             most = b > most ? b : most;
         }
         if (lane == 0) most_part[tid >> 6] = most;
-        const int64_t ph = (int64_t)page * a.c.heads + h;
-        float *scale = (is_v ? a.c.value_scales : a.c.key_scales) + ph;
-        const float was = *scale;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < 4; ++w) most = most_part[w] > most ? most_part[w] : most;
+        if (tid < n) atomicMax(&token_at[window[at + tid] & (P - 1)], tid);
         const float old = fresh ? 0.0f : was;
         const float mine = scale_of(most);
         // the larger; NaN where either is
@@ -250,6 +280,7 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
         int8_t *base = (is_v ? a.c.values : a.c.keys) + ph * P * W;
         if (!fresh && now > old) {  // (not where now is NaN: the bytes hold nothing then)
             const float ratio = old / now;
+#pragma unroll 1
             for (int i = tid; i < P * W / 16; i += 256) {
                 uint4 q = reinterpret_cast<uint4 *>(base)[i];
                 uint32_t *w = reinterpret_cast<uint32_t *>(&q);
@@ -266,29 +297,44 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
         }
         __syncthreads();
         const float inv = inverse_scale(now);
-        for (int i = tid; i < n * d8; i += 256) {
-            const int t = i / d8, e = i - t * d8;
-            const int off = a.slots[t0 + t] & (P - 1);
-            if (token_at[off] != t) continue;
-            float v[8];
-            load_f32<T, 8>(x + (int64_t)(t0 + t) * ld + e * 8, 8, v);
+        auto put = [&](const float(&y)[8], int i) {
+            int t, e;
+            split(i, t, e);
+            const int off = window[at + t] & (P - 1);
+            if (token_at[off] != t) return;
             uint2 q;
-            q.x = pack4(held_byte(v[0], inv), held_byte(v[1], inv), held_byte(v[2], inv),
-                        held_byte(v[3], inv));
-            q.y = pack4(held_byte(v[4], inv), held_byte(v[5], inv), held_byte(v[6], inv),
-                        held_byte(v[7], inv));
-            if (!is_v)
+            q.x = pack4(held_byte(y[0], inv), held_byte(y[1], inv), held_byte(y[2], inv),
+                        held_byte(y[3], inv));
+            q.y = pack4(held_byte(y[4], inv), held_byte(y[5], inv), held_byte(y[6], inv),
+                        held_byte(y[7], inv));
+            if (!is_v) {
                 *reinterpret_cast<uint2 *>(base + off * W + e * 8) = q;
-            else {
+            } else {
                 *reinterpret_cast<uint32_t *>(tile + off * (W + 4) + e * 8) = q.x;
                 *reinterpret_cast<uint32_t *>(tile + off * (W + 4) + e * 8 + 4) = q.y;
             }
+        };
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k)
+            if (tid + 256 * k < items) put(v[k], tid + 256 * k);
+#pragma unroll 1
+        for (int i = tid + 256 * KEEP; i < items; i += 256) {
+            int t, e;
+            split(i, t, e);
+            float y[8];
+            load_f32<T, 8>(x + (int64_t)(t0 + t) * ld + e * 8, 8, y);
+            put(y, i);
         }
-        if (is_v) {
-            __syncthreads();
-            const int groups = P / 4;  // of four neighbouring offsets
+        if (is_v) __syncthreads();
+        if (is_v && n == 1) {  // (a single token's bytes lie apart)
+            const int off = window[at] & (P - 1);
+#pragma unroll 1
+            for (int d = tid; d < D; d += 256) base[(int64_t)d * P + off] = tile[off * (W + 4) + d];
+        } else if (is_v) {
+            const int groups = P / 4, per = a.shift - 2;  // groups of four neighbouring offsets
+#pragma unroll 1
             for (int i = tid; i < D * groups; i += 256) {
-                const int d = i / groups, off = (i - d * groups) * 4;
+                const int d = i >> per, off = (i & (groups - 1)) * 4;
                 uint32_t b[4];
                 int here = 0;
 #pragma unroll
@@ -311,53 +357,88 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
 }
 
 // -------------------------------------------------------------------------------- read
-// 64 tokens of one head, of K or of V. Values are read along a page's tokens (neighbouring
-// slots are neighbouring bytes) and turned in LDS.
+// 64 tokens of one head, of K or of V: a thread takes four tokens' eight features at a time.
+// Values are read along a page's tokens, four neighbouring slots a load (wherever they begin),
+// and turned in registers. Two loads that wait for each other (slots; bytes and scales), then
+// 16 bytes or more a store: bound by memory.
 template <typename T>
 __global__ void __launch_bounds__(256)
 cache_read_kernel(Cache8 c, const int *slots, int tokens, T *K, T *V, int shift) {
-    extern __shared__ __attribute__((aligned(16))) int8_t tile[];  // values: [64][W + 4]
-    __shared__ float scales[64];
-    __shared__ int64_t bases[64];
     const int tid = threadIdx.x;
     const int h = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
-    const int t0 = blockIdx.x * 64;
-    const int n = min(64, tokens - t0);
-    const int P = c.page_size, W = c.width, D = c.dim, d8 = D / 8;
-    if (tid < n) {
-        const int slot = slots[t0 + tid];
-        const int page = page_of(slot, shift, c.pages);
-        const int64_t ph = (int64_t)page * c.heads + h;
-        const int off = slot & (P - 1);
-        scales[tid] = page < 0 ? 0.f : (is_v ? c.value_scales : c.key_scales)[ph];
-        bases[tid] = page < 0 ? -1 : ph * P * W + (is_v ? off : off * W);
-    }
-    __syncthreads();
-    if (is_v) {
-        for (int i = tid; i < 64 * D; i += 256) {
-            const int t = i & 63, d = i >> 6;
-            if (t < n && bases[t] >= 0) tile[t * (W + 4) + d] = c.values[bases[t] + d * P];
-        }
-        __syncthreads();
-    }
-    T *out = (is_v ? V : K) + ((int64_t)t0 * c.heads + h) * D;
-    for (int i = tid; i < n * d8; i += 256) {
-        const int t = i / d8, e = i - t * d8;
-        uint32_t w[2] = {0, 0};
-        const float s = scales[t];
-        if (bases[t] >= 0) {
-            const int8_t *from = is_v ? tile + t * (W + 4) + e * 8 : c.keys + bases[t] + e * 8;
-            w[0] = *reinterpret_cast<const uint32_t *>(from);
-            w[1] = *reinterpret_cast<const uint32_t *>(from + 4);
-        }
-        struct {
-            T t[8];
-        } r;
+    const int t0 = blockIdx.x * 64 + (tid & 15) * 4;
+    if (t0 >= tokens) return;
+    const int n = min(4, tokens - t0);
+    const int P = c.page_size, W = c.width, D = c.dim;
+    // Outside the pool: page 0's bytes, and the scale 0. All loads are made (in branches each
+    // would be waited for).
+    int64_t at[4];
+    float scale[4];
+    int slot[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            r.t[k] = from_f32<T>((float)(int8_t)(w[k / 4] >> (8 * (k & 3))) * s);
-        store_any(out + (int64_t)t * c.heads * D + e * 8, r);
+    for (int j = 0; j < 4; ++j) slot[j] = slots[min(t0 + j, tokens - 1)];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int page = page_of(slot[j], shift, c.pages);
+        const int64_t ph = (int64_t)max(page, 0) * c.heads + h;
+        const int off = slot[j] & (P - 1);
+        at[j] = ph * P * W + (is_v ? off : off * W);
+        const float s = (is_v ? c.value_scales : c.key_scales)[ph];
+        scale[j] = page < 0 ? 0.f : s;
+    }
+    const bool four = slot[1] == slot[0] + 1 && slot[2] == slot[0] + 2 &&
+                      slot[3] == slot[0] + 3 && (slot[0] & (P - 1)) + 3 < P;
+    T *out = (is_v ? V : K) + ((int64_t)t0 * c.heads + h) * D;
+    for (int e = (tid >> 4) * 8; e < D; e += 128) {
+        uint32_t w[4][2];  // eight bytes of each token
+        if (!is_v) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint2 x = load_any<uint2>(c.keys + at[j] + e);
+                w[j][0] = x.x;
+                w[j][1] = x.y;
+            }
+        } else {
+            uint32_t f[8];  // four tokens of each feature
+            const int8_t *from = c.values + (int64_t)e * P;
+            if (four) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) f[k] = load_any<uint32_t>(from + at[0] + k * P);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    f[k] = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        f[k] |= (uint32_t)(uint8_t)from[at[j] + k * P] << (8 * j);
+                }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t *g = f + 4 * half;
+                // bytes (0, 0', 1, 1'), (2, 2', 3, 3') of two features, then of four
+                const uint32_t a = __builtin_amdgcn_perm(g[1], g[0], 0x05010400u);
+                const uint32_t b = __builtin_amdgcn_perm(g[1], g[0], 0x07030602u);
+                const uint32_t x = __builtin_amdgcn_perm(g[3], g[2], 0x05010400u);
+                const uint32_t y = __builtin_amdgcn_perm(g[3], g[2], 0x07030602u);
+                w[0][half] = __builtin_amdgcn_perm(x, a, 0x05040100u);
+                w[1][half] = __builtin_amdgcn_perm(x, a, 0x07060302u);
+                w[2][half] = __builtin_amdgcn_perm(y, b, 0x05040100u);
+                w[3][half] = __builtin_amdgcn_perm(y, b, 0x07060302u);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            struct {
+                T t[8];
+            } r;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                r.t[k] =
+                    from_f32<T>((float)(int8_t)(w[j][k / 4] >> (8 * (k & 3))) * scale[j]);
+            if (j < n) store_any(out + (int64_t)j * c.heads * D + e, r);
+        }
     }
 }
 
@@ -395,6 +476,7 @@ int launch_cache_append(hipStream_t stream, const void *K, const void *V, int ty
     a.tokens = tokens;
     a.c = c;
     a.shift = shift_of(c.page_size);
+    a.d8 = make_fastdiv((uint32_t)c.dim / 8);
     // work-groups for each CU several times over before one takes more than one page's tokens
     const int64_t want = (int64_t)tokens * c.heads * 2 / 2048;
     a.chunk = 1;
@@ -411,13 +493,12 @@ int launch_cache_append(hipStream_t stream, const void *K, const void *V, int ty
 int launch_cache_read(hipStream_t stream, const Cache8 &c, const int *slots, int tokens,
                       void *K, void *V, int type) {
     const dim3 grid((tokens + 63) / 64, c.heads, 2);
-    const size_t lds = (size_t)64 * (c.width + 4);
     const int shift = shift_of(c.page_size);
     if (type == MIGEMM_FLOAT32)
-        MIGEMM_LAUNCH((cache_read_kernel<float>), grid, dim3(256), lds, stream, c, slots, tokens,
+        MIGEMM_LAUNCH((cache_read_kernel<float>), grid, dim3(256), 0, stream, c, slots, tokens,
                       static_cast<float *>(K), static_cast<float *>(V), shift);
     else
-        MIGEMM_LAUNCH((cache_read_kernel<Bf16>), grid, dim3(256), lds, stream, c, slots, tokens,
+        MIGEMM_LAUNCH((cache_read_kernel<Bf16>), grid, dim3(256), 0, stream, c, slots, tokens,
                       static_cast<Bf16 *>(K), static_cast<Bf16 *>(V), shift);
     return launch_status("cache_read_kernel launch");
 }

@@ -5,12 +5,12 @@
 // O = sum p vs v8 / sum p, with c = scale log2 e, k8 and v8 the bytes, ks and vs the scales
 // of their page and head; one pass over the keys with the running maximum and sum, in fp32.
 //
-// The bytes are exact in bf16 (7 bits), so both products run on the bf16 matrix cores with
-// the cache's side exact. A bf16 query is exact too. A float32 query, and p vs, are cut into
-// bf16 parts whose products add up in the fp32 accumulator: three parts (24 bits) for float32
-// calls, so that they are as exact as float32 arithmetic; for bf16 calls two in the few-rows
-// kernel (it waits for memory) and one in the many-rows kernel, which sums the rounded weights
-// for the denominator too: their roundings average over the keys and stay below the result's.
+// The bytes are exact in bf16 (7 bits), so products run on the bf16 matrix cores with the
+// cache's side exact. A bf16 query is exact too. A float32 query, and p vs, are cut into bf16
+// parts whose products add up in the fp32 accumulator: three parts (24 bits) for float32
+// calls, so that they are as exact as float32 arithmetic. For bf16 calls p vs is one part, and
+// the denominator is summed over the rounded weights too: their roundings average over the
+// keys and stay below the result's. (The few-rows kernel's first product is integer, below.)
 //
 // The transposed products S^T = K Q^T and O^T = V^T P^T keep everything in registers: a lane
 // holds keys of one row, the exponentials come out where the second product wants them, and
@@ -34,14 +34,17 @@ struct AttnArgs {
     int cap;            // tokens a table row holds
     float c;            // scale * log2 e
     int chunk, splits;  // keys of a range (the last takes the rest), ranges
-    int both;           // few- and many-rows kernels run, each takes its requests
-    int units;          // many-rows kernel: tiles of rows that the grid covers
+    int both;           // few and many rows in one launch, each part takes its requests
+    int units;          // many rows: tiles of rows that the grid covers
     float *part_o;      // [tokens * heads][splits][width]
     float *part_ml;     // [tokens * heads][splits][2]
 };
 
 constexpr int kFewRows = 16;
-constexpr int kManyRows = 128;
+// Wavefronts (of 32 rows) of a many-rows work-group: eight, two on each SIMD, where the
+// registers allow that.
+constexpr int many_waves(int width, int bytes) { return 4; }
+constexpr float kLag = 8.f;  // (weights stay below 2^8)
 
 namespace {
 
@@ -81,6 +84,17 @@ union Frag {
 // Eight neighbouring values of a query row from d on (0 at and after `left`), in N parts.
 template <typename T, int N>
 __device__ __forceinline__ void query_frag(const T *q, int left, Frag (&f)[N]) {
+    if constexpr (std::is_same<T, Bf16>::value && N == 1) {
+        if (left >= 8) {
+            f[0] = load_any<Frag>(q);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                f[0].u[i] = (2 * i < left ? q[2 * i].b : 0u) |
+                            (2 * i + 1 < left ? (uint32_t)q[2 * i + 1].b << 16 : 0u);
+        }
+        return;
+    }
     float x[8];
     load_f32<T, 8>(q, left, x);
 #pragma unroll
@@ -99,27 +113,41 @@ __device__ __forceinline__ bool row_is_whole(const AttnArgs &p, int limit) {
 
 // ------------------------------------------------------------------------- few rows
 // Up to 16 rows (queries x heads that share a kv head): decoding. Bound by reading the cache
-// once. A work-group takes one request, kv head and range of keys; its four wavefronts take
-// tiles of 64 tokens in turn, straight from memory to registers (the next tile's loads fly
-// while one is computed), on v_mfma_f32_16x16x32_bf16. Row m of subtile u is token
-// 16 (m / 4) + 4 u + m % 4 of the tile, so that lane group g ends up with the scores of
-// tokens 16 g .. 16 g + 15, whose bytes of V^T are 16 neighbours: one load a row of V.
-template <typename T, int W>
-__global__ void __launch_bounds__(256) attention_few_kernel(AttnArgs p) {
-    constexpr int QP = std::is_same<T, float>::value ? 3 : 1;
-    constexpr int PP = std::is_same<T, float>::value ? 3 : 2;
-    constexpr int ST = W / 32;   // steps of the first product
-    constexpr int KD = W / 16;   // dwords of a K row that a lane takes
-    constexpr int DT = W / 16;   // blocks of the second product
-    constexpr int OS = W + 4;    // LDS row
-    __shared__ __attribute__((aligned(16))) float o_lds[4 * 16 * OS];
-    __shared__ float m_lds[4][16], l_lds[4][16];
+// once, if little enough is done for each byte: the vector units have about 40 instructions'
+// time for each 64 bytes of the cache. A work-group takes one request, kv head and range of
+// keys; its four wavefronts take tiles of 64 tokens in turn, straight from memory to registers
+// (K of the next tile flies from the first product on, V from the second).
+//
+// The first product runs on the int8 matrix cores, so K needs no conversion at all: a row of q
+// is held as three signed bytes a value, q = max|q| / (127 * 2^16) * (h 2^16 + m 2^8 + l) to
+// 2^-24 of the row's largest, and the three sums are exact.
+//
+// v_mfma_i32_16x16x64_i8: row m of subtile u is token 16 (m / 4) + 4 u + m % 4 of the tile, so
+// that lane group g ends up with the scores of tokens 16 g .. 16 g + 15, whose bytes of V^T are
+// 16 neighbours: one load a row of V.
+template <int W, int NW = 4>
+struct FewLds {
+    alignas(16) float o[NW * 16 * (W + 4)];
+    float m[NW][16], l[NW][16];
+};
+
+template <typename T, int W, int NW>
+__device__ __forceinline__ void few_rows(const AttnArgs &p, int id, FewLds<W, NW> &lds) {
+    constexpr int STEP = 64 * NW;  // tokens that the work-group takes at a time
+    constexpr int PP = std::is_same<T, float>::value ? 3 : 1;
+    constexpr int SK = (W + 63) / 64;  // steps of 64 features of the first product
+    constexpr bool HALF = W % 64 != 0; // of the last one only 32 are there: lane groups 2 and 3
+                                       // take 0 and 1's bytes of K, and zeros of q
+    constexpr int DT = W / 16;         // blocks of the second product
+    constexpr int OS = W + 4;          // LDS row
+    float *const o_lds = lds.o;
+    auto &m_lds = lds.m;
+    auto &l_lds = lds.l;
 
     const CacheAttention &a = p.a;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
-    int id = blockIdx.x;
     const int split = id % p.splits;
     id /= p.splits;
     const int h = id % a.c.heads;
@@ -136,9 +164,8 @@ __global__ void __launch_bounds__(256) attention_few_kernel(AttnArgs p) {
         const int j = row0 + col;
         const int tok = s0 + j / p.group;
         const int head = h * p.group + j % p.group;
-        const int limit = j < rows && r < a.requests
-                              ? keys_of(a.positions[tok], p.cap)
-                              : 0;
+        const int limit =
+            j < rows && r < a.requests ? keys_of(a.positions[tok], p.cap) : 0;
         int most = limit;
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o));
@@ -147,108 +174,167 @@ __global__ void __launch_bounds__(256) attention_few_kernel(AttnArgs p) {
         const int hi = split == p.splits - 1 ? most : min(most, lo + p.chunk);
         if (split > 0 && lo >= most) continue;  // (the same for the whole work-group)
 
-        Frag q[ST][QP];
-        {
-            const T *qp = static_cast<const T *>(a.Q) + (int64_t)(j < rows ? tok : s0) * a.ldq +
-                          (int64_t)head * a.c.dim;
-            if (j >= rows) qp = static_cast<const T *>(a.Q) + (int64_t)s0 * a.ldq;
-#pragma unroll
-            for (int s = 0; s < ST; ++s) {
-                const int d = g * (W / 4) + 8 * s;
-                query_frag<T, QP>(qp + d, j < rows ? a.c.dim - d : 0, q[s]);
-            }
-        }
-
-        uint32_t kb[4][KD];
+        uint32_t kb[4][4 * SK];
         v4i vb[DT];
         float ks = 0.f, vs = 0.f;
         int page = -1;
-        auto find = [&](int t0) {  // the page of lane group g's 16 tokens
-            const int t = t0 + 16 * g;
-            const int pg = t < hi ? table[t >> p.shift] : -1;
-            return pg >= 0 && pg < a.c.pages ? pg : -1;
-        };
-        auto load = [&](int t0, int pg) {
+        // The table's entry for lane group g's 16 tokens: as it stands, and looked at only where
+        // the tile is loaded. (A check here would wait for the entry, and as loads come back in
+        // order, for every load before it.)
+        auto find = [&](int t0) { return table[min(t0 + 16 * g, p.cap - 1) >> p.shift]; };
+        auto load_k = [&](int t0, int entry) {
+            const int pg = t0 + 16 * g < hi && entry >= 0 && entry < a.c.pages ? entry : -1;
             page = pg;
             const int64_t mine = (int64_t)max(pg, 0) * a.c.heads + h;
             ks = a.c.key_scales[mine];
             vs = a.c.value_scales[mine];
             const int kpage = max(__shfl(pg, (col >> 2) * 16), 0);
             const int8_t *kp = a.c.keys + ((int64_t)kpage * a.c.heads + h) * page_bytes +
-                               ((t0 + 16 * (col >> 2) + (col & 3)) & (P - 1)) * W + g * (W / 4);
+                               ((t0 + 16 * (col >> 2) + (col & 3)) & (P - 1)) * W;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                if constexpr (W / 4 >= 16) {
 #pragma unroll
-                    for (int i = 0; i < W / 64; ++i) {
-                        const v4i x = *reinterpret_cast<const v4i *>(kp + u * 4 * W + 16 * i);
+                for (int i = 0; i < SK; ++i) {
+                    const int at = HALF && i == SK - 1 ? g & 1 : g;
+                    const v4i x =
+                        *reinterpret_cast<const v4i *>(kp + u * 4 * W + 64 * i + 16 * at);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) kb[u][4 * i + e] = x[e];
-                    }
-                }
-                if constexpr (W % 64 != 0) {
-                    const uint2 x =
-                        *reinterpret_cast<const uint2 *>(kp + u * 4 * W + W / 64 * 16);
-                    kb[u][W / 64 * 4] = x.x;
-                    kb[u][W / 64 * 4 + 1] = x.y;
+                    for (int e = 0; e < 4; ++e) kb[u][4 * i + e] = x[e];
                 }
             }
-            const int8_t *vp = a.c.values + mine * page_bytes + col * P + ((t0 + 16 * g) & (P - 1));
+        };
+        auto load_v = [&](int t0) {  // (of the pages of the last load_k)
+            const int64_t mine = (int64_t)max(page, 0) * a.c.heads + h;
+            const int8_t *vp =
+                a.c.values + mine * page_bytes + col * P + ((t0 + 16 * g) & (P - 1));
 #pragma unroll
             for (int d = 0; d < DT; ++d)
                 vb[d] = *reinterpret_cast<const v4i *>(vp + d * 16 * P);
         };
+        int t0 = lo + 64 * wave;
+        int entry = 0, next = 0;
+        if (t0 < hi) {
+            entry = find(t0);
+            next = find(t0 + STEP);
+            load_k(t0, entry);
+            load_v(t0);
+        }
+
+        // q's bytes: lane (col, g) holds features 64 i + 16 g .. + 15
+        uint32_t q[3][4 * SK];
+        float qs;
+        {
+            const T *qp = static_cast<const T *>(a.Q);
+            if (j < rows) qp += (int64_t)tok * a.ldq + (int64_t)head * a.c.dim;
+            const int left = j < rows ? a.c.dim : 0;
+            float x[2 * SK][8];
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 2 * SK; ++i) {
+                const int d = 64 * (i / 2) + 16 * g + 8 * (i % 2);
+                load_f32<T, 8>(qp + d, left - d, x[i]);  // (dim <= W: zeros past a half step)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t bits = __float_as_uint(x[i][e]) & 0x7fffffffu;
+                    top = bits > top ? bits : top;
+                }
+            }
+#pragma unroll
+            for (int o = 16; o < 64; o <<= 1) {
+                const uint32_t other = __shfl_xor(top, o);
+                top = other > top ? other : top;
+            }
+            // (subnormal rows count as 0; where a value is not finite the scale is NaN)
+            const float big = __uint_as_float(top);
+            const bool fine = big >= 0x1p-126f && top < 0x7f800000u;
+            const float inv = fine ? 1.f / big : 0.f;
+            qs = (top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fine ? big : 0.f) *
+                 (1.f / 8323072.f) * p.c;
+#pragma unroll
+            for (int i = 0; i < 2 * SK; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t byte[3][4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int t = __float2int_rn(x[i][4 * e + k] * inv * 8323072.f);
+                        const int t1 = (t - (int8_t)t) >> 8;
+                        byte[2][k] = (uint32_t)t;
+                        byte[1][k] = (uint32_t)t1;
+                        byte[0][k] = (uint32_t)((t1 - (int8_t)t1) >> 8);
+                    }
+#pragma unroll
+                    for (int n = 0; n < 3; ++n)
+                        q[n][2 * i + e] =
+                            pack4(byte[n][0], byte[n][1], byte[n][2], byte[n][3]);
+                }
+        }
 
         float m = -INFINITY, l = 0.f;
         v4f o[DT];
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
+        const v4i zero = {0, 0, 0, 0};
 
-        int t0 = lo + 64 * wave;
-        int next = -1;
-        if (t0 < hi) {
-            load(t0, find(t0));
-            if (t0 + 256 < hi) next = find(t0 + 256);
-        }
-        for (; t0 < hi; t0 += 256) {
-            // first product, then this tile's K registers are free for the next tile
+        for (; t0 < hi; t0 += STEP) {
             v4f s[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                s[u] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int st = 0; st < ST; ++st) {
-                    const v8bf k = bytes8_to_bf16(kb[u][2 * st], kb[u][2 * st + 1]);
-#pragma unroll
-                    for (int n = QP - 1; n >= 0; --n)
-                        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[st][n].v, s[u], 0, 0,
-                                                                       0);
-                }
-            }
-            const float sc = ks * p.c;
-            const float vscale = vs;
-            const int seen = page < 0 ? 0 : limit - t0 - 16 * g;  // of this lane's 16 tokens
-            v4i v[DT];
-#pragma unroll
-            for (int d = 0; d < DT; ++d) v[d] = vb[d];
-            if (t0 + 256 < hi) {
-                load(t0 + 256, next);
-                if (t0 + 512 < hi) next = find(t0 + 512);
-            }
             float top = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < 4; ++u) {
+                v4i sum[3];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[u][i] = 4 * u + i < seen ? s[u][i] * sc : -INFINITY;
-                    top = fmaxf(top, s[u][i]);
+                for (int n = 0; n < 3; ++n) {
+                    sum[n] = zero;
+#pragma unroll
+                    for (int i = 0; i < SK; ++i) {
+                        v4i k, x;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            k[e] = (int)kb[u][4 * i + e];
+                            x[e] = (int)q[n][4 * i + e];
+                        }
+                        sum[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, x, sum[n], 0, 0, 0);
+                    }
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s[u][i] = fmaf((float)((sum[0][i] << 8) + sum[1][i]), 256.f,
+                                   (float)sum[2][i]);
+            }
+            float sc = ks * qs;
+            const float vscale = vs;
+            const int seen = page < 0 ? 0 : limit - t0 - 16 * g;  // of this lane's 16 tokens
+            // The next tile; behind the last one the same again, from L2: loads in a branch
+            // would make every wait below one for all loads.
+            const bool more = t0 + STEP < hi;
+            const int ahead = more ? t0 + STEP : t0;
+            entry = more ? next : entry;
+            load_k(ahead, entry);
+            next = find(t0 + 2 * STEP);
+            // Scores are s * sc: scaled at once only where some are masked.
+            if (__ballot(seen < 16) == 0) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, s[u][i]);
+                top *= sc;
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[u][i] = 4 * u + i < seen ? s[u][i] * sc : -INFINITY;
+                        top = fmaxf(top, s[u][i]);
+                    }
+                sc = 1.f;
+            }
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float now = fmaxf(m, top);
-            const float base = now == -INFINITY ? 0.f : now;
-            if (__ballot(now != m) != 0) {
-                const float alpha = __builtin_amdgcn_exp2f(m - base);
+            // m is any number near the largest score: it follows only where it would be left
+            // behind by more than kLag, so the sums are rarely scaled anew
+            if (__ballot(top > m + kLag) != 0) {
+                const float now = fmaxf(m, top);
+                const float alpha = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.f : now));
                 l *= alpha;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
@@ -256,39 +342,64 @@ __global__ void __launch_bounds__(256) attention_few_kernel(AttnArgs p) {
                     for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
                 m = now;
             }
+            const float base = m == -INFINITY ? 0.f : m;
             Frag w[2][PP];
+            if (PP == 1 && __ballot(!(vscale >= 0x1p-90f)) == 0) {
+                // one part: the sum is taken over the rounded weights, so that numerator and
+                // denominator round alike (a row that sees one key gives its value, whatever
+                // the scale's bits; p vs alone would be off by the same 2^-9 in all of a page)
+                const float less = __builtin_amdgcn_logf(vscale) - base;  // (log2)
+                float sum = 0.f;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                float e[4];
+                for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    e[i] = __builtin_amdgcn_exp2f(s[u][i] - base);
-                    l += e[i];
-                    e[i] = 4 * u + i < seen ? e[i] * vscale : 0.f;
-                }
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t e =
+                            pack_bf16(__builtin_amdgcn_exp2f(fmaf(s[u][2 * i], sc, less)),
+                                      __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], sc, less)));
+                        w[u / 2][0].u[2 * (u & 1) + i] = e;
+                        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, e),
+                                                              v2bf{(__bf16)1.f, (__bf16)1.f},
+                                                              sum, false);
+                    }
+                l = fmaf(sum, __builtin_amdgcn_rcpf(vscale), l);
+            } else {  // (a scale of 0, a tiny one, NaN, or float32)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t part[PP];
-                    split_pair<PP>(e[2 * i], e[2 * i + 1], part);
+                for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int n = 0; n < PP; ++n) w[u / 2][n].u[2 * (u & 1) + i] = part[n];
-                }
+                    for (int i = 0; i < 2; ++i) {
+                        float e[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const float z = fmaf(s[u][2 * i + k], sc, -base);
+                            e[k] = __builtin_amdgcn_exp2f(z);
+                            l += e[k];
+                            e[k] = z != -INFINITY ? e[k] * vscale : 0.f;
+                        }
+                        uint32_t part[PP];
+                        split_pair<PP>(e[0], e[1], part);
+#pragma unroll
+                        for (int n = 0; n < PP; ++n)
+                            w[u / 2][n].u[2 * (u & 1) + i] = part[n];
+                    }
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const v8bf x = bytes8_to_bf16(v[d][0], v[d][1]);
-                const v8bf y = bytes8_to_bf16(v[d][2], v[d][3]);
+                pin(vb[d]);
+                const v8bf x = bytes8_to_bf16(vb[d][0], vb[d][1]);
+                const v8bf y = bytes8_to_bf16(vb[d][2], vb[d][3]);
 #pragma unroll
                 for (int n = PP - 1; n >= 0; --n) {
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, w[0][n].v, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, w[1][n].v, o[d], 0, 0, 0);
                 }
             }
+            load_v(ahead);
         }
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
 
-        // the four wavefronts' results under their common maximum, added in order
+        // the wavefronts' results under their common maximum, added in order
         if (g == 0) {
             m_lds[wave][col] = m;
             l_lds[wave][col] = l;
@@ -296,7 +407,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(AttnArgs p) {
         __syncthreads();
         float top = m_lds[0][col];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][col]);
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, m_lds[w][col]);
         const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
@@ -309,7 +420,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(AttnArgs p) {
         if (lane < 16 && wave == 0) {  // (m_lds, l_lds: now the joined ones)
             float sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 const float mw = m_lds[w][col], lw = l_lds[w][col];
                 sum += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f(mw - top);
             }
@@ -317,13 +428,13 @@ __global__ void __launch_bounds__(256) attention_few_kernel(AttnArgs p) {
             l_lds[0][col] = sum;
         }
         __syncthreads();
-        for (int e = tid; e < 16 * (W / 4); e += 256) {
+        for (int e = tid; e < 16 * (W / 4); e += STEP) {
             const int c = e / (W / 4), d = (e - c * (W / 4)) * 4;
             const int jj = row0 + c;
             if (jj >= rows) continue;
             v4f x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 const v4f y = *reinterpret_cast<const v4f *>(o_lds + (w * 16 + c) * OS + d);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] += y[i];
@@ -356,47 +467,58 @@ __global__ void __launch_bounds__(256) attention_few_kernel(AttnArgs p) {
 }
 
 // ------------------------------------------------------------------------ many rows
-// Prompts: 128 rows (queries x heads that share a kv head) a work-group, 32 a wavefront, on
+// Prompts: 32 rows (queries x heads that share a kv head) a wavefront, 4 or 8 wavefronts, on
 // v_mfma_f32_32x32x16_bf16. Tiles of 64 tokens are read as bytes, turned into bf16 once for
 // the work-group and shared in LDS (two buffers: the next tile's bytes fly during a tile's
 // work, one barrier a tile). Bound by the matrix cores and by the exponentials and
 // conversions beside them. LDS rows are padded by 16 bytes: the 16 lanes of a read phase fall
 // on different banks.
-template <typename T, int W>
-__global__ void __launch_bounds__(256)
-__attribute__((amdgpu_waves_per_eu(std::is_same<T, float>::value || W > 128 ? 1 : 2)))
-attention_many_kernel(AttnArgs p) {
+template <int W, int NW>
+struct ManyLds {
+    alignas(16) uint16_t k[2][64 * (W + 8)];
+    alignas(16) uint16_t v[2][W * (64 + 8)];
+    float scales[2][8];  // ks c of the tile's four groups of 16 tokens, then vs
+    uint32_t flags[2];
+    int most[NW];
+};
+
+template <typename T, int W, int NW>
+__device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, NW> &lds) {
+    constexpr int ROWS = 32 * NW;
+    constexpr int NT = 64 * NW;
     constexpr int QP = std::is_same<T, float>::value ? 3 : 1;
     constexpr int PP = QP;
     constexpr int ST = W / 16;       // steps of the first product
     constexpr int DT = W / 32;       // blocks of the second product
     constexpr int KR = W + 8;        // LDS rows, in bf16
     constexpr int VR = 64 + 8;
-    constexpr int KD = W / 16;       // dwords of K a thread moves
-    constexpr int VU = (W * 4 + 255) / 256;  // units of 16 bytes of V a thread moves
-    __shared__ __attribute__((aligned(16))) uint16_t k_lds[2][64 * KR];
-    __shared__ __attribute__((aligned(16))) uint16_t v_lds[2][W * VR];
-    __shared__ float scale_lds[2][8];  // ks c of the tile's four groups of 16 tokens, then vs
-    __shared__ uint32_t lost_lds[2];
+    constexpr int CH = W / 16;       // units of 16 bytes in a row of K
+    constexpr int MU = (4 * W + NT - 1) / NT;  // units of K, and of V, that a thread moves
+    constexpr bool EVEN = 4 * W % NT == 0;     // (as many for every thread)
+    auto &k_lds = lds.k;
+    auto &v_lds = lds.v;
+    auto &scale_lds = lds.scales;
+    auto &lost_lds = lds.flags;
+    auto &most_lds = lds.most;
 
     const CacheAttention &a = p.a;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lo32 = lane & 31, hi32 = lane >> 5;
 
-    int id = blockIdx.x;
     const int h = id % a.c.heads;
     id /= a.c.heads;
     const int split = id % p.splits;
     id /= p.splits;
-    // which request's tile: requests in order, 64 at a time
+    // which request's tile: requests in order (tiles that run together share keys in L2), 64 at
+    // a time
     int r = -1, tile = 0, s0 = 0, s1 = 0;
     for (int base = 0, before = 0; base <= a.requests; base += 64) {
         int x0 = 0, x1 = 0, n = 0;
         if (base + lane <= a.requests) {
             request_tokens(a, base + lane, x0, x1);
             const int rows = (x1 - x0) * p.group;
-            n = rows > kFewRows || !p.both ? (rows + kManyRows - 1) / kManyRows : 0;
+            n = rows > kFewRows ? (rows + ROWS - 1) / ROWS : 0;
         }
         int upto = n;
 #pragma unroll
@@ -425,28 +547,76 @@ attention_many_kernel(AttnArgs p) {
     const int *table = a.table + (int64_t)(r < a.requests ? r : 0) * a.max_pages;
     const int64_t page_bytes = (int64_t)P * W;
 
-    const int j = tile * kManyRows + wave * 32 + lo32;
+    const int j = tile * ROWS + wave * 32 + lo32;
     const int tok = j < rows ? s0 + j / p.group : s0;
     const int head = j < rows ? h * p.group + j % p.group : 0;
-    const int limit =
-        j < rows && r < a.requests ? keys_of(a.positions[tok], p.cap) : 0;
-    // the work-group's longest row, and this wavefront's shortest
-    __shared__ int most_lds[4];
-    int most = limit, least = j < rows ? limit : INT32_MAX;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        most = max(most, __shfl_xor(most, o));
-        least = min(least, __shfl_xor(least, o));
-    }
-    least = __builtin_amdgcn_readfirstlane(least);
-    if (lane == 0) most_lds[wave] = most;
-    __syncthreads();
-    most = max(max(most_lds[0], most_lds[1]), max(most_lds[2], most_lds[3]));
-    most = __builtin_amdgcn_readfirstlane(most);
+    // What the first tile needs is asked for at once, before it is known whether any row sees it
+    // (a work-group's beginning is a chain of loads that wait for each other).
     const int lo = split * p.chunk;
-    const int hi = split == p.splits - 1 ? most : min(most, lo + p.chunk);
-    if (split > 0 && lo >= most) return;
+    // this thread's units of 16 bytes of a tile: of K row unit / CH (a token), of V row unit / 4
+    // (a feature) and group unit % 4 (of 16 tokens)
+    v4i kb[MU], vb[MU];
+    float sc = 0.f;
+    auto entry_at = [&](int t) { return table[min(t, p.cap - 1) >> p.shift]; };
+    auto page_of = [&](int entry) { return entry >= 0 && entry < a.c.pages ? entry : -1; };
+    auto token_of = [&](int i) { return min((tid + NT * i) / CH, 63); };
+    // A tile's table entries are read a tile before its bytes, and looked at only then (a check
+    // at once would wait for them, and as loads come back in order, for every load before).
+    int kentry[MU], ventry = -1;
+    auto find = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < MU; ++i) kentry[i] = entry_at(t0 + (token_of(i) & 48));
+        ventry = entry_at(t0 + 16 * (tid & 3));
+    };
+    uint32_t gone = 0;
+    auto load = [&](int t0) {
+        int kpage[MU];
+#pragma unroll
+        for (int i = 0; i < MU; ++i) kpage[i] = page_of(kentry[i]);
+        const int vpage = page_of(ventry);
+        gone = (uint32_t)__ballot(lane < 4 && vpage < 0);
+#pragma unroll
+        for (int i = 0; i < MU; ++i)
+            kb[i] = *reinterpret_cast<const v4i *>(
+                a.c.keys + ((int64_t)max(kpage[i], 0) * a.c.heads + h) * page_bytes +
+                ((t0 + token_of(i)) & (P - 1)) * W + (tid + NT * i) % CH * 16);
+        const int8_t *vp = a.c.values + ((int64_t)max(vpage, 0) * a.c.heads + h) * page_bytes +
+                           ((t0 + 16 * (tid & 3)) & (P - 1));
+#pragma unroll
+        for (int i = 0; i < MU; ++i) {
+            const int d = (tid + NT * i) >> 2;
+            vb[i] = *reinterpret_cast<const v4i *>(vp + (EVEN ? d : min(d, W - 1)) * P);
+        }
+        if (tid < 8) {  // tid & 3: the group
+            const int64_t at = (int64_t)max(vpage, 0) * a.c.heads + h;
+            sc = tid < 4 ? a.c.key_scales[at] * p.c : a.c.value_scales[at];
+        }
+    };
+    auto stage = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < MU; ++i) {
+            const int unit = tid + NT * i;
+            if (EVEN || unit < 4 * W) {
+                pin(kb[i]);
+                pin(vb[i]);
+                uint16_t *kp = k_lds[b] + unit / CH * KR + unit % CH * 16;
+                *reinterpret_cast<v8bf *>(kp) = bytes8_to_bf16(kb[i][0], kb[i][1]);
+                *reinterpret_cast<v8bf *>(kp + 8) = bytes8_to_bf16(kb[i][2], kb[i][3]);
+                // a half-wavefront's eight tokens of each 16 are neighbours: 0-3, 8-11 and
+                // 4-7, 12-15, as the rows of the first product fall
+                uint16_t *vp = v_lds[b] + (unit >> 2) * VR + (tid & 3) * 16;
+                *reinterpret_cast<v8bf *>(vp) = bytes8_to_bf16(vb[i][0], vb[i][2]);
+                *reinterpret_cast<v8bf *>(vp + 8) = bytes8_to_bf16(vb[i][1], vb[i][3]);
+            }
+        }
+        if (tid < 8) scale_lds[b][tid] = sc;
+        // (bit 4: the four value scales are plain numbers)
+        const bool plain = (__ballot(sc >= 0x1p-90f) >> 4 & 15) == 15;
+        if (tid == 0) lost_lds[b] = gone | (uint32_t)plain << 4;
+    };
 
+    find(lo);
+    const int position = j < rows && r < a.requests ? a.positions[tok] : -1;
     Frag q[ST][QP];
     {
         const T *qp = static_cast<const T *>(a.Q) + (int64_t)tok * a.ldq +
@@ -457,71 +627,26 @@ attention_many_kernel(AttnArgs p) {
             query_frag<T, QP>(qp + d, j < rows ? a.c.dim - d : 0, q[s]);
         }
     }
-
-    // this thread's part of a tile: a quarter row of K (token tid / 4: group = wave), units of
-    // 16 bytes of V (row d = unit / 4, group unit % 4)
-    uint32_t kb[KD];
-    v4i vb[VU];
-    float sc = 0.f;
-    auto page_at = [&](int t) {
-        const int pg = t < hi ? table[t >> p.shift] : -1;
-        return pg >= 0 && pg < a.c.pages ? pg : -1;
-    };
-    // (the pages of a tile are looked up a tile before its bytes are loaded)
-    int kpage = -1, vpage = -1;
-    auto find = [&](int t0) {
-        kpage = page_at(t0 + 16 * wave);
-        vpage = page_at(t0 + 16 * (tid & 3));
-    };
-    uint32_t gone = 0;
-    auto load = [&](int t0) {
-        gone = (uint32_t)__ballot(lane < 4 && t0 + 16 * lane < hi && vpage < 0);
-        const int8_t *kp = a.c.keys + ((int64_t)max(kpage, 0) * a.c.heads + h) * page_bytes +
-                           ((t0 + (tid >> 2)) & (P - 1)) * W + (tid & 3) * (W / 4);
-        if constexpr (W / 4 >= 16) {
+    load(lo);
+    find(lo + 64);
+    const int limit = keys_of(position, p.cap);
+    // the work-group's longest row, this wavefront's and its shortest
+    int most = limit, least = j < rows ? limit : INT32_MAX;
 #pragma unroll
-            for (int i = 0; i < W / 64; ++i) {
-                const v4i x = *reinterpret_cast<const v4i *>(kp + 16 * i);
+    for (int o = 16; o > 0; o >>= 1) {
+        most = max(most, __shfl_xor(most, o));
+        least = min(least, __shfl_xor(least, o));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    const int mine = __builtin_amdgcn_readfirstlane(most);
+    if (lane == 0) most_lds[wave] = most;
+    stage(0);
+    __syncthreads();
 #pragma unroll
-                for (int e = 0; e < 4; ++e) kb[4 * i + e] = x[e];
-            }
-        }
-        if constexpr (W % 64 != 0) {
-            const uint2 x = *reinterpret_cast<const uint2 *>(kp + W / 64 * 16);
-            kb[W / 64 * 4] = x.x;
-            kb[W / 64 * 4 + 1] = x.y;
-        }
-        const int8_t *vp = a.c.values + ((int64_t)max(vpage, 0) * a.c.heads + h) * page_bytes +
-                           ((t0 + 16 * (tid & 3)) & (P - 1));
-#pragma unroll
-        for (int i = 0; i < VU; ++i) {
-            const int d = (tid + 256 * i) >> 2;
-            vb[i] = *reinterpret_cast<const v4i *>(vp + min(d, W - 1) * P);
-        }
-        if (tid < 8) {  // tid & 3: the group
-            const int64_t at = (int64_t)max(vpage, 0) * a.c.heads + h;
-            sc = tid < 4 ? a.c.key_scales[at] * p.c : a.c.value_scales[at];
-        }
-    };
-    auto stage = [&](int b) {
-        uint16_t *kp = k_lds[b] + (tid >> 2) * KR + (tid & 3) * (W / 4);
-#pragma unroll
-        for (int i = 0; i < KD / 2; ++i)
-            *reinterpret_cast<v8bf *>(kp + 8 * i) = bytes8_to_bf16(kb[2 * i], kb[2 * i + 1]);
-#pragma unroll
-        for (int i = 0; i < VU; ++i) {
-            const int d = (tid + 256 * i) >> 2;
-            if (W * 4 % 256 == 0 || d < W) {
-                // a half-wavefront's eight tokens of each 16 are neighbours: 0-3, 8-11 and
-                // 4-7, 12-15, as the rows of the first product fall
-                uint16_t *vp = v_lds[b] + d * VR + (tid & 3) * 16;
-                *reinterpret_cast<v8bf *>(vp) = bytes8_to_bf16(vb[i][0], vb[i][2]);
-                *reinterpret_cast<v8bf *>(vp + 8) = bytes8_to_bf16(vb[i][1], vb[i][3]);
-            }
-        }
-        if (tid < 8) scale_lds[b][tid] = sc;
-        if (tid == 0) lost_lds[b] = gone;
-    };
+    for (int w = 0; w < NW; ++w) most = max(most, most_lds[w]);
+    most = __builtin_amdgcn_readfirstlane(most);
+    const int hi = split == p.splits - 1 ? most : min(most, lo + p.chunk);
+    if (split > 0 && lo >= most) return;
 
     float m = -INFINITY, l = 0.f;
     v16f o[DT];
@@ -530,36 +655,39 @@ attention_many_kernel(AttnArgs p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
 
-    if (lo < hi) {
-        find(lo);
-        load(lo);
-        find(lo + 64);
-        stage(0);
-    }
-    __syncthreads();
     int buf = 0;
     for (int t0 = lo; t0 < hi; t0 += 64, buf ^= 1) {
         const bool more = t0 + 64 < hi;
-        if (more) {
-            load(t0 + 64);
-            find(t0 + 128);
-        }
+        if (more) load(t0 + 64);
+        find(t0 + 128);  // (always: a value that only a branch loads is copied, and waited for)
+        if (t0 < mine) {  // (else none of this wavefront's rows sees the tile)
         // pages of the tile that are outside the pool (one bit for each group of 16 tokens)
-        const uint32_t lost = lost_lds[buf];
+        const uint32_t flags = __builtin_amdgcn_readfirstlane(lost_lds[buf]);
+        const uint32_t lost = flags & 15;
 
+        // The first product's and the second's operands are read from LDS a step ahead; the
+        // accumulators of neighbouring instructions are different ones.
         v16f s[2];
+        const v16f zero = {};
+        const uint16_t *kp = k_lds[buf] + lo32 * KR + 8 * hi32;
+        v8bf kf[2][2];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < 2; ++b) kf[0][b] = *reinterpret_cast<const v8bf *>(kp + 32 * b * KR);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+        for (int st = 0; st < ST; ++st) {
+            if (st + 1 < ST) {
 #pragma unroll
-            for (int st = 0; st < ST; ++st) {
-                const v8bf k = *reinterpret_cast<const v8bf *>(
-                    k_lds[buf] + (32 * b + lo32) * KR + 16 * st + 8 * hi32);
-#pragma unroll
-                for (int n = QP - 1; n >= 0; --n)
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[st][n].v, s[b], 0, 0, 0);
+                for (int b = 0; b < 2; ++b)
+                    kf[(st + 1) & 1][b] =
+                        *reinterpret_cast<const v8bf *>(kp + 32 * b * KR + 16 * (st + 1));
             }
+#pragma unroll
+            for (int n = QP - 1; n >= 0; --n)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        kf[st & 1][b], q[st][n].v, st == 0 && n == QP - 1 ? zero : s[b], 0, 0,
+                        0);
         }
         float ks[4], vs[4];
 #pragma unroll
@@ -567,25 +695,36 @@ attention_many_kernel(AttnArgs p) {
             ks[w] = scale_lds[buf][w];
             vs[w] = scale_lds[buf][4 + w];
         }
-        const bool whole = t0 + 64 <= least && lost == 0;  // the same for the wavefront
+        // Scores are s * ks. Where some are masked, a ks that -inf could not be multiplied with
+        // (0, tiny, NaN) is multiplied first.
+        if (t0 + 64 > least || lost != 0) {  // the same for the wavefront
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int seen = lost >> w & 1 ? 0 : limit - t0 - 16 * w - 4 * hi32;
+                const bool odd = !(ks[w] >= 0x1p-100f);
+                const float by = odd ? ks[w] : 1.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = s[w >> 1][8 * (w & 1) + i] * by;
+                    s[w >> 1][8 * (w & 1) + i] = 8 * (i >> 2) + (i & 3) < seen ? x : -INFINITY;
+                }
+                ks[w] = odd ? 1.f : ks[w];
+            }
+        }
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < 4; ++w) {
+            float x = s[w >> 1][8 * (w & 1)];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float x = s[w >> 1][8 * (w & 1) + i] * ks[w];
-                if (!whole) {
-                    const int t = t0 + 16 * w + 8 * (i >> 2) + 4 * hi32 + (i & 3);
-                    x = t < limit && !(lost >> w & 1) ? x : -INFINITY;
-                }
-                s[w >> 1][8 * (w & 1) + i] = x;
-                top = fmaxf(top, x);
-            }
+            for (int i = 1; i < 8; ++i) x = fmaxf(x, s[w >> 1][8 * (w & 1) + i]);
+            top = fmaxf(top, x * ks[w]);
+        }
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float now = fmaxf(m, top);
-        const float base = now == -INFINITY ? 0.f : now;
-        if (__ballot(now != m) != 0) {
-            const float alpha = __builtin_amdgcn_exp2f(m - base);
+        // m is any number near the largest score: it follows only where it would be left behind
+        // by more than kLag, so the sums are rarely scaled anew
+        if (__ballot(top > m + kLag) != 0) {
+            const float now = fmaxf(m, top);
+            const float alpha = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.f : now));
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -593,27 +732,29 @@ attention_many_kernel(AttnArgs p) {
                 for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
             m = now;
         }
+        const float base = m == -INFINITY ? 0.f : m;
         Frag w[4][PP];
-        const bool plain_scales = vs[0] >= 0x1p-90f && vs[1] >= 0x1p-90f &&
-                                  vs[2] >= 0x1p-90f && vs[3] >= 0x1p-90f;
-        if (PP == 1 && plain_scales) {
+        if (PP == 1 && flags >> 4 != 0) {
             // one part: the sum is taken over the rounded weights, so that numerator and
             // denominator round alike (a row that sees one key gives its value, whatever the
             // scale's bits; p vs alone would be off by the same 2^-9 in all of a page)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
+                const float less = __builtin_amdgcn_logf(vs[x]) - base;  // (log2)
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float e[2];
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
-                        e[k] = __builtin_amdgcn_exp2f(s[x >> 1][8 * (x & 1) + 2 * i + k] -
-                                                      base) * vs[x];
+                        e[k] = __builtin_amdgcn_exp2f(
+                            fmaf(s[x >> 1][8 * (x & 1) + 2 * i + k], ks[x], less));
                     w[x][0].u[i] = pack_bf16(e[0], e[1]);
-                    sum += bf16_low(w[x][0].u[i]) + bf16_high(w[x][0].u[i]);
+                    sum = __builtin_amdgcn_fdot2_f32_bf16(
+                        __builtin_bit_cast(v2bf, w[x][0].u[i]), v2bf{(__bf16)1.f, (__bf16)1.f},
+                        sum, false);
                 }
-                l += sum * __builtin_amdgcn_rcpf(vs[x]);
+                l = fmaf(sum, __builtin_amdgcn_rcpf(vs[x]), l);
             }
         } else {  // (a scale of 0, a tiny one, NaN, or float32)
 #pragma unroll
@@ -623,10 +764,10 @@ attention_many_kernel(AttnArgs p) {
                     float e[2];
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const float z = s[x >> 1][8 * (x & 1) + 2 * i + k];
-                        e[k] = __builtin_amdgcn_exp2f(z - base);
+                        const float z = fmaf(s[x >> 1][8 * (x & 1) + 2 * i + k], ks[x], -base);
+                        e[k] = __builtin_amdgcn_exp2f(z);
                         l += e[k];
-                        e[k] = whole || z != -INFINITY ? e[k] * vs[x] : 0.f;
+                        e[k] = z != -INFINITY ? e[k] * vs[x] : 0.f;
                     }
                     uint32_t part[PP];
                     split_pair<PP>(e[0], e[1], part);
@@ -634,16 +775,26 @@ attention_many_kernel(AttnArgs p) {
                     for (int n = 0; n < PP; ++n) w[x][n].u[i] = part[n];
                 }
         }
+        const uint16_t *vp = v_lds[buf] + lo32 * VR + 8 * hi32;
+        v8bf vf[2][DT];
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int d = 0; d < DT; ++d) vf[0][d] = *reinterpret_cast<const v8bf *>(vp + 32 * d * VR);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const v8bf v = *reinterpret_cast<const v8bf *>(
-                    v_lds[buf] + (32 * d + lo32) * VR + 16 * x + 8 * hi32);
+        for (int x = 0; x < 4; ++x) {
+            if (x < 3) {
 #pragma unroll
-                for (int n = PP - 1; n >= 0; --n)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w[x][n].v, o[d], 0, 0, 0);
+                for (int d = 0; d < DT; ++d)
+                    vf[(x + 1) & 1][d] =
+                        *reinterpret_cast<const v8bf *>(vp + 32 * d * VR + 16 * (x + 1));
             }
+#pragma unroll
+            for (int n = PP - 1; n >= 0; --n)
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x & 1][d], w[x][n].v, o[d],
+                                                                   0, 0, 0);
+        }
+        }
         if (more) stage(buf ^ 1);
         __syncthreads();
     }
@@ -654,6 +805,7 @@ attention_many_kernel(AttnArgs p) {
         const bool direct = row_is_whole(p, limit);
         if (direct && split > 0) return;
         const int64_t at = row * p.splits + split;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         if (!direct && hi32 == 0) {
             p.part_ml[at * 2] = m;
             p.part_ml[at * 2 + 1] = l;
@@ -674,7 +826,7 @@ attention_many_kernel(AttnArgs p) {
                     } y;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        y.t[k] = from_f32<T>(l == 0.f ? 0.f : x[k] / l);
+                        y.t[k] = from_f32<T>(x[k] * inv);
                     store_any(static_cast<T *>(a.O) + row * a.c.dim + dd, y);
                 }
             }
@@ -739,21 +891,41 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnArgs p) {
     }
 }
 
-// few, many: which kernels the call runs.
 template <typename T, int W>
-int launch_width(hipStream_t stream, const AttnArgs &p, bool few, bool many) {
-    if (many) {
-        const int64_t blocks = (int64_t)p.units * p.splits * p.a.c.heads;
-        MIGEMM_LAUNCH((attention_many_kernel<T, W>), dim3((unsigned)blocks), dim3(256), 0,
-                      stream, p);
-        if (const int rc = launch_status("attention_many_kernel launch")) return rc;
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W <= 128 ? 2 : 1)))
+attention_few_kernel(AttnArgs p) {
+    __shared__ FewLds<W> lds;
+    few_rows<T, W, 4>(p, blockIdx.x, lds);
+}
+
+// Both in one launch, each request's rows where they belong: the few-rows work-groups first.
+template <typename T, int W, int NW>
+__global__ void __launch_bounds__(64 * NW)
+__attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 || W > 128 ? 1 : 2)))
+attention_both_kernel(AttnArgs p, int few) {
+    __shared__ union {
+        FewLds<W, NW> few;
+        ManyLds<W, NW> many;
+    } lds;
+    if ((int)blockIdx.x < few) {
+        few_rows<T, W, NW>(p, blockIdx.x, lds.few);
+    } else {
+        many_rows<T, W, NW>(p, blockIdx.x - few, lds.many);
     }
-    if (few) {
-        const int64_t blocks = (int64_t)p.splits * p.a.c.heads * (p.a.requests + 1);
-        MIGEMM_LAUNCH((attention_few_kernel<T, W>), dim3((unsigned)blocks), dim3(256), 0, stream,
+}
+
+template <typename T, int W>
+int launch_width(hipStream_t stream, const AttnArgs &p) {
+    const int few = p.splits * p.a.c.heads * (p.a.requests + 1);
+    constexpr int NW = many_waves(W, sizeof(T));
+    if (p.both)
+        MIGEMM_LAUNCH((attention_both_kernel<T, W, NW>),
+                      dim3((unsigned)(few + p.units * p.splits * p.a.c.heads)), dim3(64 * NW),
+                      0, stream, p, few);
+    else
+        MIGEMM_LAUNCH((attention_few_kernel<T, W>), dim3((unsigned)few), dim3(256), 0, stream,
                       p);
-        if (const int rc = launch_status("attention_few_kernel launch")) return rc;
-    }
+    if (const int rc = launch_status("attention kernel launch")) return rc;
     if (p.splits > 1) {
         const int64_t rows = (int64_t)p.a.tokens * p.a.heads;
         MIGEMM_LAUNCH((attention_join_kernel<T, W>), dim3((unsigned)rows), dim3(256), 0, stream,
@@ -764,19 +936,19 @@ int launch_width(hipStream_t stream, const AttnArgs &p, bool few, bool many) {
 }
 
 template <typename T>
-int launch_widths(hipStream_t stream, const AttnArgs &p, bool few, bool many) {
+int launch_widths(hipStream_t stream, const AttnArgs &p) {
     switch (p.a.c.width) {
-        case 32: return launch_width<T, 32>(stream, p, few, many);
-        case 64: return launch_width<T, 64>(stream, p, few, many);
-        case 96: return launch_width<T, 96>(stream, p, few, many);
-        case 128: return launch_width<T, 128>(stream, p, few, many);
-        case 192: return launch_width<T, 192>(stream, p, few, many);
-        default: return launch_width<T, 256>(stream, p, few, many);
+        case 32: return launch_width<T, 32>(stream, p);
+        case 64: return launch_width<T, 64>(stream, p);
+        case 96: return launch_width<T, 96>(stream, p);
+        case 128: return launch_width<T, 128>(stream, p);
+        case 192: return launch_width<T, 192>(stream, p);
+        default: return launch_width<T, 256>(stream, p);
     }
 }
 }  // namespace
 
-int launch_attention_f32(hipStream_t stream, const AttnArgs &p, bool few, bool many);
-int launch_attention_bf16(hipStream_t stream, const AttnArgs &p, bool few, bool many);
+int launch_attention_f32(hipStream_t stream, const AttnArgs &p);
+int launch_attention_bf16(hipStream_t stream, const AttnArgs &p);
 
 }  // namespace migemm

@@ -3,8 +3,8 @@
 
 namespace migemm {
 
-int launch_attention_bf16(hipStream_t stream, const AttnArgs &p, bool few, bool many) {
-    return launch_widths<Bf16>(stream, p, few, many);
+int launch_attention_bf16(hipStream_t stream, const AttnArgs &p) {
+    return launch_widths<Bf16>(stream, p);
 }
 
 }  // namespace migemm

@@ -3,8 +3,8 @@
 
 namespace migemm {
 
-int launch_attention_f32(hipStream_t stream, const AttnArgs &p, bool few, bool many) {
-    return launch_widths<float>(stream, p, few, many);
+int launch_attention_f32(hipStream_t stream, const AttnArgs &p) {
+    return launch_widths<float>(stream, p);
 }
 
 }  // namespace migemm

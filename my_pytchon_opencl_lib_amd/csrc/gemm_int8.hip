@@ -8,10 +8,10 @@
 // Three kernels:
 //   gemm_int8_kernel     tiles through LDS on v_mfma_i32_32x32x32_i8, bound by the matrix
 //                        cores (and the loads that feed them) for large M
-//   rows_int8_kernel     M <= 64: bound by streaming B once; a work-group takes 16 rows of B,
+//   rows_int8_kernel     few rows: bound by streaming B once; a work-group takes 16 rows of B,
 //                        its wavefronts split K, operands go straight to registers
-//   rows_int8_kernel with x in float: the same for M <= 4, x quantised by every work-group
-//                        (x is small and in L2): one launch instead of two
+//   rows_int8_kernel with x in float: the same for one or two rows, x quantised by every
+//                        work-group (x is small and in L2): one launch instead of two
 #include "gemm_direct.h"
 #include "int8_common.h"
 
@@ -31,16 +31,31 @@ __device__ __forceinline__ void put(T *c, int sum, float sa, float sb, float bia
     *c = from_f32<T>((float)sum * sa * sb + bias);
 }
 
+// This lane's 16 bytes of each load of the tail tile kt, zero at k >= K. K is a multiple of 16
+// bytes, so each is wholly inside or outside; all loads are made (outside: at the row's start)
+// and fly together.
+template <int BK, typename Op>
+__device__ __forceinline__ void fetch_tail(const Op &op, typename Op::Tail &t, int kt, int K,
+                                           int64_t ld) {
+    const char *tb = op.tile_base(kt, ld);
+#pragma unroll
+    for (int j = 0; j < Op::NS; ++j) {
+        const bool in = kt * BK + op.kk[j] < K;
+        t.v[j] = *reinterpret_cast<const f4 *>(in ? tb + op.voff[j]
+                                                  : op.base + (op.voff[j] - 4 * op.kk[j]));
+        if (!in) t.v[j] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+}
+
 // ---------------------------------------------------------------------------- large tiles
 // BM x BN tiles, 128 bytes of K a stage, loaded straight into LDS (DlOperand, whose unit of
 // four bytes holds four values of K here) and swizzled by 16-byte chunks; a fragment read of
 // 16 bytes a lane is one operand of v_mfma_i32_32x32x32_i8. The order of waits, barrier and
 // loads is gemm_direct_kernel's: a tile's loads run D tiles ahead, and every fragment read of
 // a stage is issued before the barrier that frees it.
-template <typename T, int BM, int BN, int WM, int WN, int S, int D, int OCC>
+template <typename T, int BM, int BN, int WM, int WN, int S, int D, int OCC, int BK>
 __global__ void __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(OCC)))
 gemm_int8_kernel(Int8Args p) {
-    constexpr int BK = 32;  // units of four bytes
     constexpr int NT = WM * WN * 64;
     constexpr int FM = BM / WM / 32, FN = BN / WN / 32;
     constexpr int G = BK / 8;
@@ -48,6 +63,7 @@ gemm_int8_kernel(Int8Args p) {
     typedef DlOperand<NT, true, BK, BN, 4> OpB;
     constexpr int A_FL = OpA::FLOATS, B_FL = OpB::FLOATS;
     constexpr int LPT = OpA::NS + OpB::NS;
+    static_assert(S >= 2 && S <= 4 && D >= 2 && D <= S, "the loop below takes S steps of 2..4");
     __shared__ __attribute__((aligned(16))) float lds_a[S * A_FL];
     __shared__ __attribute__((aligned(16))) float lds_b[S * B_FL];
 
@@ -114,6 +130,16 @@ gemm_int8_kernel(Int8Args p) {
         mfmas(fa[(G - 1) & 1], fb[(G - 1) & 1]);
     };
 
+    // The tail tile's loads are issued first where registers allow (a short k loop does not
+    // hide their latency at its end); being the oldest, every wait below covers them.
+    constexpr bool EARLY = OpA::NS + OpB::NS <= 4 && BM * BN < 256 * 256;
+    typename OpA::Tail ta;
+    typename OpB::Tail tb;
+    if (EARLY && kf < kt1) {
+        fetch_tail<BK>(opa, ta, kf, K, p.t.lda);
+        fetch_tail<BK>(opb, tb, kf, K, p.t.ldb);
+    }
+
     int kt = kt0;
     if (kt0 < kf) {
 #pragma unroll
@@ -138,10 +164,10 @@ gemm_int8_kernel(Int8Args p) {
     }
     wait_vmcnt<0>();
     if (kt < kt1) {  // the tail tile: k >= K zero in both operands
-        typename OpA::Tail ta;
-        typename OpB::Tail tb;
-        opa.tail_fetch(ta, kt, K, p.t.lda);
-        opb.tail_fetch(tb, kt, K, p.t.ldb);
+        if (!EARLY) {
+            fetch_tail<BK>(opa, ta, kt, K, p.t.lda);
+            fetch_tail<BK>(opb, tb, kt, K, p.t.ldb);
+        }
         __syncthreads();
         opa.tail_put(ta, lds_a, lane);
         opb.tail_put(tb, lds_b, lane);
@@ -160,7 +186,8 @@ gemm_int8_kernel(Int8Args p) {
     const int lo = lane & 31, hi = lane >> 5;
     const int r0 = tc.m0 + wm * (BM / WM), c0 = tc.n0 + wn * (BN / WN);
     if (p.t.splits > 1) {
-        int32_t *out = p.partial + (int64_t)tc.split * p.t.M * p.t.N;
+        const int ld = (p.t.N + 3) & ~3;
+        int32_t *out = p.partial + (int64_t)tc.split * p.t.M * ld;
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -170,7 +197,7 @@ gemm_int8_kernel(Int8Args p) {
                     const int row = r0 + i * 32 + 8 * (r >> 2) + 4 * hi + (r & 3);
                     const int col = c0 + j * 32 + lo;
                     if (row < p.t.M && col < p.t.N)
-                        out[(int64_t)row * p.t.N + col] = acc[i][j][r];
+                        out[(int64_t)row * ld + col] = acc[i][j][r];
                 }
         return;
     }
@@ -197,22 +224,29 @@ gemm_int8_kernel(Int8Args p) {
         }
 }
 
-// The k ranges' sums added (exactly) and scaled.
+// The k ranges' sums added (exactly) and scaled: four neighbouring columns a thread.
 template <typename T>
 __global__ void __launch_bounds__(256)
-join_int8_kernel(const int32_t *partial, int splits, int M, int N, const float *sa,
-                 const float *sb, const float *bias, T *C, int64_t ldc) {
-    const int64_t total = (int64_t)M * N;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    const int row = (int)(i / N), col = (int)(i - (int64_t)row * N);
-    int sum = 0;
-    for (int s = 0; s < splits; ++s) sum += partial[s * total + i];
-    put(C + (int64_t)row * ldc + col, sum, sa[row], sb[col],
-        bias != nullptr ? bias[col] : 0.f);
+join_int8_kernel(const int32_t *partial, int splits, int M, int N, int64_t plane, FastDiv quads,
+                 const float *sa, const float *sb, const float *bias, T *C, int64_t ldc) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    const int row = (int)fast_div(i, quads), col = (int)(i - row * quads.d) * 4;
+    if (row >= M) return;
+    const int n = min(4, N - col);
+    int sum[4] = {0, 0, 0, 0};
+    const int32_t *from = partial + (int64_t)row * (quads.d * 4) + col;  // (rows padded to 4)
+    for (int s = 0; s < splits; ++s) {
+        const v4i x = *reinterpret_cast<const v4i *>(from + s * plane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += x[e];
+    }
+    const float a = sa[row];
+    for (int e = 0; e < n; ++e)
+        put(C + (int64_t)row * ldc + col + e, sum[e], a, sb[col + e],
+            bias != nullptr ? bias[col + e] : 0.f);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int S, int D, int OCC>
+template <typename T, int BM, int BN, int WM, int WN, int S, int D, int OCC, int BK = 32>
 int launch_tiles(hipStream_t stream, const Int8Product &p, int splits) {
     Int8Args a{};
     TiledArgs &t = a.t;
@@ -226,7 +260,7 @@ int launch_tiles(hipStream_t stream, const Int8Product &p, int splits) {
     t.batch = 1;
     t.tiles_m = (p.M + BM - 1) / BM;
     t.tiles_n = (p.N + BN - 1) / BN;
-    const int nk = (t.K + 31) / 32;
+    const int nk = (t.K + BK - 1) / BK;
     const int want = splits < nk ? splits : nk;
     t.kt_per_split = (nk + want - 1) / want;
     t.splits = (nk + t.kt_per_split - 1) / t.kt_per_split;
@@ -241,19 +275,21 @@ int launch_tiles(hipStream_t stream, const Int8Product &p, int splits) {
     a.bias = p.bias;
     a.C = p.C;
     a.ldc = p.ldc;
+    const uint32_t quads = (uint32_t)(p.N + 3) / 4;
+    const int64_t plane = (int64_t)p.M * quads * 4;
     if (t.splits > 1) {
         int rc = MIGEMM_OK;
         a.partial = static_cast<int32_t *>(
-            workspace(stream, (size_t)t.splits * p.M * p.N * sizeof(int32_t), &rc, 0));
+            workspace(stream, (size_t)t.splits * plane * sizeof(int32_t), &rc, 0));
         if (a.partial == nullptr) return rc;
     }
-    MIGEMM_LAUNCH((gemm_int8_kernel<T, BM, BN, WM, WN, S, D, OCC>), dim3(t.total),
+    MIGEMM_LAUNCH((gemm_int8_kernel<T, BM, BN, WM, WN, S, D, OCC, BK>), dim3(t.total),
                   dim3(WM * WN * 64), 0, stream, a);
     if (const int rc = launch_status("gemm_int8_kernel launch")) return rc;
     if (t.splits > 1) {
-        const int64_t blocks = ((int64_t)p.M * p.N + 255) / 256;
+        const int64_t blocks = (plane / 4 + 255) / 256;
         MIGEMM_LAUNCH((join_int8_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream,
-                      a.partial, t.splits, p.M, p.N, p.sa, p.sb, p.bias,
+                      a.partial, t.splits, p.M, p.N, plane, make_fastdiv(quads), p.sa, p.sb, p.bias,
                       static_cast<T *>(p.C), p.ldc);
         if (const int rc = launch_status("join_int8_kernel launch")) return rc;
     }
@@ -269,6 +305,7 @@ int launch_tiles(hipStream_t stream, const Int8Product &p, int splits) {
 // row is one whole 128-byte line and two instructions.
 // X != void: A is not given but x [M, K] in X, and each work-group quantises it into LDS
 // itself (its first loads of B are on their way meanwhile).
+constexpr int kKeep = 2;  // steps of x (NW * 512 values each) that stay in registers
 struct RowsArgs {
     const int8_t *A, *B;
     const void *X;
@@ -293,8 +330,8 @@ __global__ void __launch_bounds__(NW * 64) rows_int8_kernel(RowsArgs p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     int32_t *sums = reinterpret_cast<int32_t *>(lds);  // [NW][16 MT][16]
     int8_t *held = reinterpret_cast<int8_t *>(lds + NW * MT * 1024);  // FUSED: [M][K + 16]
-    __shared__ uint32_t most[16];
-    __shared__ float scales[16];
+    __shared__ uint32_t most[kKeep];
+    __shared__ float scales[kKeep];
 
     v4i rb[U][2];
     auto load_b = [&](int u, int piece) {
@@ -305,49 +342,66 @@ __global__ void __launch_bounds__(NW * 64) rows_int8_kernel(RowsArgs p) {
                            ? *reinterpret_cast<const v4i *>(b + (int64_t)piece * 128 + 16 * h)
                            : v4i{0, 0, 0, 0};
     };
+    if constexpr (!FUSED) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_b(u, wave + u * NW);
-
-    if constexpr (FUSED) {
+        for (int u = 0; u < U; ++u) load_b(u, wave + u * NW);
+    } else {
         typedef typename std::conditional<FUSED, X, float>::type Xt;
-        if (tid < 16) most[tid] = 0;
+        constexpr int STEP = NW * 64 * 8;  // values that the work-group takes at a time
+        const int per_row = (p.K + STEP - 1) / STEP;
+        float v[kKeep][8];
+        auto at = [&](int c, int &m, int &k) {  // step c: row m, this thread's first column k
+            m = c / per_row;
+            k = (c - m * per_row) * STEP + tid * 8;
+        };
+        // x first: loads come back in order, and x is in L2
+#pragma unroll
+        for (int c = 0; c < kKeep; ++c) {
+            int m, k;
+            at(c, m, k);
+            if (m < p.M)
+                load_f32<Xt, 8>(static_cast<const Xt *>(p.X) + (int64_t)m * p.ldx + k,
+                                p.cols - k, v[c]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_b(u, wave + u * NW);
+        if (tid < kKeep) most[tid] = 0;
         __syncthreads();
-        for (int m = 0; m < p.M; ++m) {
-            const Xt *x = static_cast<const Xt *>(p.X) + (int64_t)m * p.ldx;
-            uint32_t top = 0;
-            for (int k = tid * 8; k < p.cols; k += NW * 64 * 8) {
-                float v[8];
-                load_f32<Xt, 8>(x + k, p.cols - k, v);
+#pragma unroll
+        for (int c = 0; c < kKeep; ++c) {
+            int m, k;
+            at(c, m, k);
+            if (m < p.M) {
+                uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint32_t bits = __float_as_uint(v[i]) & 0x7fffffffu;
+                    const uint32_t bits = __float_as_uint(v[c][i]) & 0x7fffffffu;
                     top = bits > top ? bits : top;
                 }
-            }
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                const uint32_t other = __shfl_xor(top, o);
-                top = other > top ? other : top;
+                for (int o = 32; o > 0; o >>= 1) {
+                    const uint32_t other = __shfl_xor(top, o);
+                    top = other > top ? other : top;
+                }
+                if (lane == 0) atomicMax(&most[m], top);  // (a maximum: in any order the same)
             }
-            if (lane == 0) atomicMax(&most[m], top);  // (a maximum: in any order the same)
         }
         __syncthreads();
-        for (int m = 0; m < p.M; ++m) {
-            const Xt *x = static_cast<const Xt *>(p.X) + (int64_t)m * p.ldx;
-            const float s = scale_of(most[m]);
-            const float inv = inverse_scale(s);
-            if (tid == 0) scales[m] = s;
-            for (int k = tid * 8; k < p.K; k += NW * 64 * 8) {
-                float v[8];
-                load_f32<Xt, 8>(x + k, p.cols - k, v);
+#pragma unroll
+        for (int c = 0; c < kKeep; ++c) {
+            int m, k;
+            at(c, m, k);
+            if (m < p.M && k < p.K) {
+                const float inv = inverse_scale(scale_of(most[m]));
                 uint2 q;
-                q.x = pack4(held_byte(v[0], inv), held_byte(v[1], inv), held_byte(v[2], inv),
-                            held_byte(v[3], inv));
-                q.y = pack4(held_byte(v[4], inv), held_byte(v[5], inv), held_byte(v[6], inv),
-                            held_byte(v[7], inv));
+                q.x = pack4(held_byte(v[c][0], inv), held_byte(v[c][1], inv),
+                            held_byte(v[c][2], inv), held_byte(v[c][3], inv));
+                q.y = pack4(held_byte(v[c][4], inv), held_byte(v[c][5], inv),
+                            held_byte(v[c][6], inv), held_byte(v[c][7], inv));
                 *reinterpret_cast<uint2 *>(held + (int64_t)m * (p.K + 16) + k) = q;
             }
         }
+        if (tid < p.M) scales[tid] = scale_of(most[tid]);
         __syncthreads();
     }
 
@@ -434,29 +488,57 @@ RowsArgs rows_args(const Int8Product &p) {
     return a;
 }
 
+// What a choice costs, in work of one CU at the best tiles' rate: rounds of work-groups over
+// the 256 CUs, a tile's products over the rate that its shape reaches. Rates measured against
+// 256 x 256 (2500 TOP/s at 8192^3): 128 x 256 0.88, 128 x 128 0.84, 64 x 128 0.70, 64 x 64 0.55.
+struct TileChoice {
+    int bm, bn;
+    float rate;
+};
+constexpr TileChoice kTiles[] = {
+    {256, 256, 1.f}, {128, 256, 0.88f}, {128, 128, 0.84f}, {64, 128, 0.70f}, {64, 64, 0.55f}};
+
 template <typename T>
 int launch_product(hipStream_t stream, const Int8Product &p) {
-    if (p.M <= 64) {
+    // Few rows over few columns: 16 columns a work-group (24 x 4096 x 2048: 4.2 us, tiles 6.8);
+    // over many the tiles stream B as well and read A once for 64 columns (16 x 11008 x 4096:
+    // 11.1 us, 14.3 by rows).
+    if (p.M <= 32 && (int64_t)p.N * p.K <= (int64_t)12 << 20) {
         const RowsArgs a = rows_args(p);
-        if (p.M <= 16) return launch_rows<T, void, 1, 8>(stream, a);
-        if (p.M <= 32) return launch_rows<T, void, 2, 8>(stream, a);
-        return launch_rows<T, void, 4, 8>(stream, a);
+        return p.M <= 16 ? launch_rows<T, void, 1, 8>(stream, a)
+                         : launch_rows<T, void, 2, 8>(stream, a);
     }
-    auto tiles = [&](int bm, int bn) {
-        return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn);
+    auto tiles = [&](const TileChoice &c) {
+        return (int64_t)((p.M + c.bm - 1) / c.bm) * ((p.N + c.bn - 1) / c.bn);
     };
-    if (tiles(256, 256) >= 192)
-        return launch_tiles<T, 256, 256, 4, 2, 2, 2, 2>(stream, p, 1);
-    if (tiles(128, 128) >= 128)
-        return launch_tiles<T, 128, 128, 2, 2, 2, 2, 2>(stream, p, 1);
-    const int64_t n = tiles(64, 64);
-    const int splits = n >= 256 ? 1 : (int)(512 / n);
-    const int most = (p.K + 511) / 512;  // at least four stages a range
-    return launch_tiles<T, 64, 64, 2, 2, 4, 3, 2>(stream, p, splits < most ? splits : most);
+    int best = 0;
+    float least = INFINITY;
+    for (int i = 0; i < 5; ++i) {
+        const TileChoice &c = kTiles[i];
+        const float cost = (float)((tiles(c) + 255) / 256) * (float)(c.bm * c.bn) / c.rate;
+        if (cost < least) {
+            least = cost;
+            best = i;
+        }
+    }
+    switch (best) {
+        case 0: return launch_tiles<T, 256, 256, 8, 2, 2, 2, 4>(stream, p, 1);
+        case 1: return launch_tiles<T, 128, 256, 4, 4, 3, 3, 4>(stream, p, 1);
+        case 2: return launch_tiles<T, 128, 128, 4, 4, 2, 2, 4>(stream, p, 1);
+        case 3: return launch_tiles<T, 64, 128, 2, 4, 3, 3, 4>(stream, p, 1);
+    }
+    // Too few of the smallest tiles for the CUs: k ranges, each of 16 stages at least (they
+    // cost a second launch).
+    const int64_t n = tiles(kTiles[4]);
+    const int splits = n >= 128 ? 1 : (int)(256 / n);
+    const int most = p.K / 2048 > 1 ? p.K / 2048 : 1;
+    return launch_tiles<T, 64, 64, 2, 2, 3, 3, 3>(stream, p, splits < most ? splits : most);
 }
 
-// M <= 4 rows whose bytes fit beside the sums: every work-group quantises them itself.
-bool fused_rows(int M, int K) { return M <= 4 && (int64_t)M * K <= 32768; }
+// One or two rows that a work-group of 8 wavefronts holds in its registers: quantised by each
+// (1 x 4096 to 11008, weights from HBM: 10.4 us, against 3 and 10.5 by two launches; 2 x 4096
+// to 4096: 5.9, and 3 and 5.0).
+bool fused_rows(int M, int K) { return M <= kKeep && M * ((K + 4095) / 4096) <= kKeep; }
 }  // namespace
 
 int launch_product_int8(hipStream_t stream, const Int8Product &p) {

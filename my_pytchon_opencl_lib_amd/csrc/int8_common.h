@@ -142,6 +142,10 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
     return lo | (hi << 16);
 }
 
+// What a loop loaded a round ahead, at its use: keeps the compiler from unpacking it where it was
+// loaded (which waits for the load there, and spills).
+__device__ __forceinline__ void pin(v4i &x) { asm volatile("" : "+v"(x)); }
+
 // Four signed bytes as bf16: exact (|v| <= 127 has 7 significant bits), so only the upper
 // half of each float is kept.
 __device__ __forceinline__ void bytes_to_bf16(uint32_t v, uint32_t &lo, uint32_t &hi) {
@@ -162,12 +166,10 @@ __device__ __forceinline__ v8bf bytes8_to_bf16(uint32_t a, uint32_t b) {
     return r.v;
 }
 // Two floats as two bf16, rounded to nearest even.
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-    v2bf v = {(__bf16)a, (__bf16)b};
-    uint32_t u;
-    __builtin_memcpy(&u, &v, 4);
-    return u;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2bf));
 }
 __device__ __forceinline__ float bf16_low(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t u) {

@@ -454,27 +454,27 @@ int launch_cache_attention(hipStream_t stream, const CacheAttention &a) {
     const int64_t count = a.max_count > 0 && a.max_count < a.tokens ? a.max_count : a.tokens;
     const int64_t length =
         a.max_length > 0 && a.max_length < p.cap ? a.max_length : p.cap;
-    // Requests of at most 16 rows go to the few-rows kernel, the others to the many-rows
-    // kernel; where one request alone may bring more, both run, and each takes its own.
+    // Requests of at most 16 rows are computed one way, others another; where one request may
+    // bring more, one launch holds both ways.
     const bool many = count * p.group > kFewRows;
     p.both = many;
-    const int64_t units = (int64_t)a.tokens * p.group / kManyRows + a.requests + 1;
+    const int tile = 32 * many_waves(a.c.width, type_size(a.type));
+    const int64_t units = (int64_t)a.tokens * p.group / tile + a.requests + 1;
     p.units = (int)units;
-    // Work-groups before contexts are cut: about so many requests and tiles a kv head. Cut in
-    // ranges of whole rounds of the few-rows kernel (256 tokens) until there are about 1024.
+    // Contexts are cut in ranges (of whole rounds of a few-rows work-group, 256 tokens) where the
+    // requests, tiles and kv heads alone make too few work-groups: single tokens until there are
+    // about 1024 (they wait for memory), prompts only until there is one for each CU (their
+    // partial results, four bytes a feature and row and range, cost more than an uneven end).
     const int64_t base =
-        (a.requests + (many ? (int64_t)a.tokens * p.group / kManyRows : 0)) * a.c.heads;
-    const int64_t want = (1024 + base - 1) / base;
+        (a.requests + (many ? (int64_t)a.tokens * p.group / tile : 0)) * a.c.heads;
+    const int64_t want = many ? (base < 256 ? 256 / base : 1) : (1024 + base - 1) / base;
     int64_t chunk = (length + want - 1) / want;
     chunk = (chunk + 255) / 256 * 256;
-    if (want == 1) chunk = (length + 255) / 256 * 256;
     p.chunk = (int)chunk;
     p.splits = (int)((length + chunk - 1) / chunk);
     const int64_t rows = (int64_t)a.tokens * a.heads;
-    MIGEMM_TRY(check_grid("cache_attention", (int64_t)p.splits * a.c.heads * (a.requests + 1),
-                          256));
-    if (many)
-        MIGEMM_TRY(check_grid("cache_attention", units * p.splits * a.c.heads, 256));
+    MIGEMM_TRY(check_grid("cache_attention", (int64_t)p.splits * a.c.heads *
+                                                  (a.requests + 1 + (many ? units : 0)), 512));
     if (p.splits > 1) {
         MIGEMM_TRY(check_grid("cache_attention", rows, 256));
         const size_t parts = (size_t)rows * p.splits;
@@ -484,8 +484,8 @@ int launch_cache_attention(hipStream_t stream, const CacheAttention &a) {
         if (p.part_o == nullptr) return rc;
         p.part_ml = p.part_o + parts * a.c.width;
     }
-    return a.type == MIGEMM_FLOAT32 ? launch_attention_f32(stream, p, true, many)
-                                    : launch_attention_bf16(stream, p, true, many);
+    return a.type == MIGEMM_FLOAT32 ? launch_attention_f32(stream, p)
+                                    : launch_attention_bf16(stream, p);
 }
 
 }  // namespace migemm

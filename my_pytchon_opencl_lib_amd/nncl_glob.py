@@ -144,15 +144,18 @@ _TYPES = {torch.float32: _native.MIGEMM_FLOAT32, torch.bfloat16: _native.MIGEMM_
 
 
 def _check_rows(name, t, dim=None):
-    """An activation tensor of the 8-bit operators: float32 or bfloat16, on the GPU, its rows
-    contiguous (_row_stride). Returns the type's code."""
+    """An activation tensor of the 8-bit operators: float32 or bfloat16, on the GPU. Returns the
+    type's code. (Here and below what usually holds is checked in one expression, and a message
+    is made only where it does not: a step of a small batch is a few microseconds of GPU work.)"""
+    if isinstance(t, torch.Tensor) and t.is_cuda and (dim is None or t.dim() == dim):
+        code = _TYPES.get(t.dtype)
+        if code is not None:
+            return code
     _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
     if t.dtype not in _TYPES:
         raise ShapeError(f"{name} must be float32 or bfloat16 (got {t.dtype})")
     _require(t.is_cuda, f"{name} must live on the GPU: there is no CPU fallback")
-    if dim is not None and t.dim() != dim:
-        raise ShapeError(f"{name} must have {dim} axes (got {list(t.shape)})")
-    return _TYPES[t.dtype]
+    raise ShapeError(f"{name} must have {dim} axes (got {list(t.shape)})")
 
 
 def _row_stride(name, t):
@@ -173,17 +176,30 @@ def _row_stride(name, t):
     return t.stride(0)
 
 
-def _check_typed(name, t, dtype, shape=None):
-    """A contiguous GPU tensor of one type (and shape; None in it: any size)."""
+def _check_typed(name, t, dtype, shape=None, dim=None):
+    """A contiguous GPU tensor of one type, and of a shape or a number of axes."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.is_contiguous() and \
+            (shape is None or t.shape == shape) and (dim is None or t.dim() == dim):
+        return
     _require(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
     if t.dtype != dtype:
         raise ShapeError(f"{name} must be {dtype} (got {t.dtype})")
     _require(t.is_cuda, f"{name} must live on the GPU: there is no CPU fallback")
     if not t.is_contiguous():
         raise ShapeError(f"{name} must be contiguous (strides {list(t.stride())})")
-    if shape is not None and (t.dim() != len(shape) or
-                              any(a is not None and a != b for a, b in zip(shape, t.shape))):
-        raise ShapeError(f"{name} must have the shape {list(shape)} (got {list(t.shape)})")
+    raise ShapeError(f"{name} must have the shape {list(shape)} (got {list(t.shape)})"
+                     if shape is not None else
+                     f"{name} must have {dim} axes (got {list(t.shape)})")
+
+
+def _check_table(lengths, table):
+    """Lengths [requests] and a block table [requests, pages]; returns the table's shape."""
+    _check_typed("lengths", lengths, torch.int32, dim=1)
+    _check_typed("table", table, torch.int32, dim=2)
+    requests, columns = table.shape
+    if lengths.shape[0] != requests:
+        raise ShapeError(f"table must have {lengths.shape[0]} rows (got {requests})")
+    return requests, columns
 
 
 class NnClGlob:
@@ -557,12 +573,12 @@ class NnClGlob:
     def LinearInt8(self, x, weight, scales, bias=None):
         """y[..., N] = x[..., K] @ W^T (+ bias[N], float32) with W [N, K] as QuantizeRows left
         it (weight int8 [N, K rounded up to 16], scales [N]); the rows of x are quantised on
-        the way. y has the type of x. One launch for up to four rows."""
+        the way. y has the type of x. One launch for one or two rows."""
         code = _check_rows("x", x)
-        _check_typed("weight", weight, torch.int8, (None, None))
+        _check_typed("weight", weight, torch.int8, dim=2)
         n, kp = weight.shape
         k = x.shape[-1] if x.dim() else 0
-        if k < 1 or (k + 15) // 16 * 16 != kp:
+        if k < 1 or (k + 15) & -16 != kp:
             raise ShapeError(f"x must end in the weight's features (got {list(x.shape)} and "
                              f"rows of {kp} bytes)")
         _check_typed("scales", scales, torch.float32, (n,))
@@ -570,7 +586,7 @@ class NnClGlob:
             _check_typed("bias", bias, torch.float32, (n,))
         x2 = x if x.dim() == 2 else x.reshape(-1, k)
         m = x2.shape[0]
-        y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        y = x.new_empty((m, n))
         if m and n:
             extra = (bias,) if bias is not None else ()
             _launch("migemm_linear_int8", (x2, weight, scales, y) + extra, _ptr(x2), code,
@@ -588,57 +604,47 @@ class NnClGlob:
         it and it needs no new page or enough are left after the requests before it; else
         its tokens get -1 and its length stays. The lengths and freeCount given are not
         changed: a caller goes on with the ones returned."""
-        requests = lengths.numel() if isinstance(lengths, torch.Tensor) else 0
-        _check_typed("lengths", lengths, torch.int32, (None,))
+        requests, columns = _check_table(lengths, table)
         _check_typed("counts", counts, torch.int32, (requests,))
-        _check_typed("table", table, torch.int32, (requests, None))
-        _check_typed("free", free, torch.int32, (None,))
+        _check_typed("free", free, torch.int32, dim=1)
         _check_typed("freeCount", freeCount, torch.int32, (1,))
         tokens = int(tokens)
         _require(tokens >= 0, "tokens must not be negative")
         # one buffer: five allocations would cost more than the kernel
-        out = torch.empty(2 * tokens + 2 * requests + 2, dtype=torch.int32,
-                          device=lengths.device)
-        slots, positions, starts, new, left = torch.split(
-            out, (tokens, tokens, requests + 1, requests, 1))
+        out = lengths.new_empty(2 * tokens + 2 * requests + 2)
         at = _ptr(out)
+        rest = at + 8 * tokens
         _launch("migemm_cache_tables", (lengths, counts, table, free, freeCount, out),
-                _ptr(lengths), _ptr(counts), requests, _ptr(table), table.shape[1],
-                int(pageSize), _ptr(free), _ptr(freeCount), free.numel(), at, at + 4 * tokens,
-                at + 8 * tokens, at + 8 * tokens + 4 * requests + 4,
-                at + 8 * tokens + 8 * requests + 4, tokens)
-        return slots, positions, starts, new, left
+                _ptr(lengths), _ptr(counts), requests, _ptr(table), columns, int(pageSize),
+                _ptr(free), _ptr(freeCount), free.shape[0], at, at + 4 * tokens, rest,
+                rest + 4 * requests + 4, rest + 8 * requests + 4, tokens)
+        return out.split_with_sizes((tokens, tokens, requests + 1, requests, 1))
 
     def CacheSlots(self, lengths, counts, table, tokens, pageSize):
         """(slots [tokens], positions [tokens], starts [requests + 1]) of the tokens lengths[i]
         .. lengths[i] + counts[i] of each request in the pages that its table row names: with
         lengths 0 and the lengths as counts, every cached token."""
-        requests = lengths.numel() if isinstance(lengths, torch.Tensor) else 0
-        _check_typed("lengths", lengths, torch.int32, (None,))
+        requests, columns = _check_table(lengths, table)
         _check_typed("counts", counts, torch.int32, (requests,))
-        _check_typed("table", table, torch.int32, (requests, None))
         tokens = int(tokens)
         _require(tokens >= 0, "tokens must not be negative")
-        out = torch.empty(2 * tokens + requests + 1, dtype=torch.int32, device=lengths.device)
-        slots, positions, starts = torch.split(out, (tokens, tokens, requests + 1))
+        out = lengths.new_empty(2 * tokens + requests + 1)
         at = _ptr(out)
         _launch("migemm_cache_slots", (lengths, counts, table, out), _ptr(lengths),
-                _ptr(counts), requests, _ptr(table), table.shape[1], int(pageSize),
-                at, at + 4 * tokens, at + 8 * tokens, tokens)
-        return slots, positions, starts
+                _ptr(counts), requests, _ptr(table), columns, int(pageSize), at,
+                at + 4 * tokens, at + 8 * tokens, tokens)
+        return out.split_with_sizes((tokens, tokens, requests + 1))
 
     def CacheRelease(self, finished, lengths, table, free, freeCount, pageSize):
         """Gives the pages of every request with finished[i] != 0 back: added at the end of
         free[0 .. freeCount) (free has room for the whole pool), its table row becomes -1 and
         its length 0. In place."""
-        requests = lengths.numel() if isinstance(lengths, torch.Tensor) else 0
-        _check_typed("lengths", lengths, torch.int32, (None,))
+        requests, columns = _check_table(lengths, table)
         _check_typed("finished", finished, torch.int32, (requests,))
-        _check_typed("table", table, torch.int32, (requests, None))
-        _check_typed("free", free, torch.int32, (None,))
+        _check_typed("free", free, torch.int32, dim=1)
         _check_typed("freeCount", freeCount, torch.int32, (1,))
         _launch("migemm_cache_release", (finished, lengths, table, free, freeCount),
-                _ptr(finished), _ptr(lengths), requests, _ptr(table), table.shape[1],
+                _ptr(finished), _ptr(lengths), requests, _ptr(table), columns,
                 int(pageSize), _ptr(free), free.numel(), _ptr(freeCount))
 
     def CacheAppend(self, k, v, slots, cache):
@@ -650,9 +656,9 @@ class NnClGlob:
         if _check_rows("v", v, 3) != code:
             raise ShapeError(f"k and v must have one type (got {k.dtype} and {v.dtype})")
         tokens = k.shape[0]
-        want = [tokens, cache.kvHeads, cache.headDim]
-        if list(k.shape) != want or list(v.shape) != want:
-            raise ShapeError(f"k and v must be {want} (got {list(k.shape)} and "
+        want = (tokens, cache.kvHeads, cache.headDim)
+        if k.shape != want or v.shape != want:
+            raise ShapeError(f"k and v must be {list(want)} (got {list(k.shape)} and "
                              f"{list(v.shape)})")
         _check_typed("slots", slots, torch.int32, (tokens,))
         if tokens:
@@ -665,7 +671,7 @@ class NnClGlob:
         of CacheSlots), 0 where a slot is -1. For products over a cached context through Bmm."""
         if dtype not in _TYPES:
             raise ShapeError(f"dtype must be float32 or bfloat16 (got {dtype})")
-        _check_typed("slots", slots, torch.int32, (None,))
+        _check_typed("slots", slots, torch.int32, dim=1)
         tokens = slots.numel()
         k = torch.empty((tokens, cache.kvHeads, cache.headDim), dtype=dtype,
                         device=slots.device)
@@ -690,16 +696,16 @@ class NnClGlob:
         if dim != cache.headDim or heads % cache.kvHeads or not heads:
             raise ShapeError(f"q must be [tokens, a multiple of {cache.kvHeads} heads, "
                              f"{cache.headDim}] (got {list(q.shape)})")
-        _check_typed("table", table, torch.int32, (None, None))
-        requests = table.shape[0]
+        _check_typed("table", table, torch.int32, dim=2)
+        requests, columns = table.shape
         _check_typed("starts", starts, torch.int32, (requests + 1,))
         _check_typed("positions", positions, torch.int32, (tokens,))
-        o = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        o = q.new_empty((tokens, heads, dim))
         if tokens:
             _launch("migemm_cache_attention",
                     (q, cache.keys, table, starts, positions, o), _ptr(q), code,
                     _row_stride("q", q), *cache.pointers, *cache.sizes, _ptr(table),
-                    table.shape[1], _ptr(starts), _ptr(positions), requests, tokens, heads,
+                    columns, _ptr(starts), _ptr(positions), requests, tokens, heads,
                     dim ** -0.5 if scale is None else float(scale), int(maxCount),
                     int(maxLength), _ptr(o))
         return o
