@@ -36,11 +36,15 @@ struct AttnArgs {
     int chunk, splits;  // keys of a range (the last takes the rest), ranges
     int both;           // few and many rows in one launch, each part takes its requests
     int units;          // many rows: tiles of rows that the grid covers
-    float *part_o;      // [tokens * heads][splits][width]
-    float *part_ml;     // [tokens * heads][splits][2]
+    int shares;         // work-groups of few_shares (0: ranges)
+    int *firsts;        // [2][requests + 2]: its scan, for the join
+    float *part_o;      // [tokens * heads][splits][width], or [2 shares][16][width]
+    float *part_ml;     // likewise, 2 (the largest score, the sum)
 };
 
 constexpr int kFewRows = 16;
+constexpr int kShareRequests = 1022;  // few_shares keeps a scan of the requests in LDS
+constexpr int kSnap = 2;              // (its cuts)
 // Wavefronts (of 32 rows) of a many-rows work-group: eight, two on each SIMD, where the
 // registers allow that.
 constexpr int many_waves(int width, int bytes) { return 4; }
@@ -81,28 +85,35 @@ union Frag {
     v8bf v;
 };
 
-// Eight neighbouring values of a query row from d on (0 at and after `left`), in N parts.
+// Eight neighbouring values of a query row as float32 (head sizes are multiples of 8: all of
+// them are there or none, which reads `row` itself and gives zeros; no branch waits for a load).
+template <typename T>
+__device__ __forceinline__ void query_values(const T *row, int d, bool there, float (&x)[8]) {
+    struct Raw {
+        T t[8];
+    };
+    const Raw v = load_any<Raw>(row + (there ? d : 0));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = there ? to_f32(v.t[i]) : 0.f;
+}
+
+// The same in N parts.
 template <typename T, int N>
-__device__ __forceinline__ void query_frag(const T *q, int left, Frag (&f)[N]) {
+__device__ __forceinline__ void query_frag(const T *row, int d, bool there, Frag (&f)[N]) {
     if constexpr (std::is_same<T, Bf16>::value && N == 1) {
-        if (left >= 8) {
-            f[0] = load_any<Frag>(q);
-        } else {
+        f[0] = load_any<Frag>(row + (there ? d : 0));
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                f[0].u[i] = (2 * i < left ? q[2 * i].b : 0u) |
-                            (2 * i + 1 < left ? (uint32_t)q[2 * i + 1].b << 16 : 0u);
+        for (int i = 0; i < 4; ++i) f[0].u[i] = there ? f[0].u[i] : 0u;
+    } else {
+        float x[8];
+        query_values(row, d, there, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t part[N];
+            split_pair<N>(x[2 * i], x[2 * i + 1], part);
+#pragma unroll
+            for (int n = 0; n < N; ++n) f[n].u[i] = part[n];
         }
-        return;
-    }
-    float x[8];
-    load_f32<T, 8>(q, left, x);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t part[N];
-        split_pair<N>(x[2 * i], x[2 * i + 1], part);
-#pragma unroll
-        for (int n = 0; n < N; ++n) f[n].u[i] = part[n];
     }
 }
 
@@ -131,8 +142,15 @@ struct FewLds {
     float m[NW][16], l[NW][16];
 };
 
+// 16 rows from row0 on of request r (tokens from s0 on) and kv head h, over its keys lo .. end - 1
+// (as far as a row sees them). part: kWhole (all its keys: the result), a place for a part, or -2 - range where rows go by
+// row_is_whole.
+constexpr int kWhole = -1;
+
 template <typename T, int W, int NW>
-__device__ __forceinline__ void few_rows(const AttnArgs &p, int id, FewLds<W, NW> &lds) {
+__device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, int rows, int h,
+                                            int row0, int lo, int end, int part,
+                                            FewLds<W, NW> &lds) {
     constexpr int STEP = 64 * NW;  // tokens that the work-group takes at a time
     constexpr int PP = std::is_same<T, float>::value ? 3 : 1;
     constexpr int SK = (W + 63) / 64;  // steps of 64 features of the first product
@@ -148,6 +166,323 @@ __device__ __forceinline__ void few_rows(const AttnArgs &p, int id, FewLds<W, NW
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
+    const int P = a.c.page_size;
+    const int *table = a.table + (int64_t)(r < a.requests ? r : 0) * a.max_pages;
+    const int64_t page_bytes = (int64_t)P * W;
+    const int split = part < kWhole ? -2 - part : 0;
+
+    const int j = row0 + col;
+    const int tok = j < rows ? s0 + j / p.group : min(s0, a.tokens - 1);
+    const int head = h * p.group + j % p.group;
+
+    uint32_t kb[4][4 * SK];
+    v4i vb[DT];
+    float ks = 0.f, vs = 0.f;
+    int page = -1;
+    // The table's entry for lane group g's 16 tokens: as it stands, and looked at only where
+    // the tile is loaded. (A check here would wait for the entry, and as loads come back in
+    // order, for every load before it.)
+    auto find = [&](int t0) { return table[min(t0 + 16 * g, p.cap - 1) >> p.shift]; };
+    // (not live: behind the last tile, where every lane reads the same few bytes)
+    auto load_k = [&](int t0, int entry, bool live) {
+        const int pg = entry >= 0 && entry < a.c.pages ? entry : -1;
+        page = pg;
+        const int64_t mine = (int64_t)max(pg, 0) * a.c.heads + h;
+        ks = a.c.key_scales[mine];
+        vs = a.c.value_scales[mine];
+        const int kpage = max(__shfl(pg, (col >> 2) * 16), 0);
+        const int64_t at = ((int64_t)kpage * a.c.heads + h) * page_bytes +
+                           ((t0 + 16 * (col >> 2) + (col & 3)) & (P - 1)) * W;
+        const int8_t *kp = a.c.keys + (live ? at : 0);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+#pragma unroll
+            for (int i = 0; i < SK; ++i) {
+                const int group = HALF && i == SK - 1 ? g & 1 : g;
+                const v4i x = __builtin_nontemporal_load(
+                    reinterpret_cast<const v4i *>(kp + u * 4 * W + 64 * i + 16 * group));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) kb[u][4 * i + e] = x[e];
+            }
+        }
+    };
+    auto load_v = [&](int t0, bool live) {  // (of the pages of the last load_k)
+        const int64_t at = ((int64_t)max(page, 0) * a.c.heads + h) * page_bytes + col * P +
+                           ((t0 + 16 * g) & (P - 1));
+        const int8_t *vp = a.c.values + (live ? at : 0);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+            vb[d] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(vp + d * 16 * P));
+    };
+    // What the first tile needs is asked for at once, before it is known whether a row sees it
+    // (a segment begins with loads that wait for each other).
+    int t0 = lo + 64 * wave;
+    const int entry = find(t0);
+    int next = find(t0 + STEP);
+    const int position = a.positions[tok];
+    load_k(t0, entry, t0 < end);
+    load_v(t0, t0 < end);
+
+    // q's bytes: lane (col, g) holds features 64 i + 16 g .. + 15
+    uint32_t q[3][4 * SK];
+    float qs;
+    {
+        const T *qp = static_cast<const T *>(a.Q) +
+                      (j < rows ? (int64_t)tok * a.ldq + (int64_t)head * a.c.dim : 0);
+        float x[2 * SK][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * SK; ++i) {
+            const int d = 64 * (i / 2) + 16 * g + 8 * (i % 2);
+            query_values(qp, d, j < rows && d < a.c.dim, x[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t bits = __float_as_uint(x[i][e]) & 0x7fffffffu;
+                top = bits > top ? bits : top;
+            }
+        }
+#pragma unroll
+        for (int o = 16; o < 64; o <<= 1) {
+            const uint32_t other = __shfl_xor(top, o);
+            top = other > top ? other : top;
+        }
+        // (subnormal rows count as 0; where a value is not finite the scale is NaN)
+        const float big = __uint_as_float(top);
+        const bool fine = big >= 0x1p-126f && top < 0x7f800000u;
+        const float inv = fine ? 1.f / big : 0.f;
+        qs = (top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fine ? big : 0.f) *
+             (1.f / 8323072.f) * p.c;
+#pragma unroll
+        for (int i = 0; i < 2 * SK; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t byte[3][4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int t = __float2int_rn(x[i][4 * e + k] * inv * 8323072.f);
+                    const int t1 = (t - (int8_t)t) >> 8;
+                    byte[2][k] = (uint32_t)t;
+                    byte[1][k] = (uint32_t)t1;
+                    byte[0][k] = (uint32_t)((t1 - (int8_t)t1) >> 8);
+                }
+#pragma unroll
+                for (int n = 0; n < 3; ++n)
+                    q[n][2 * i + e] =
+                        pack4(byte[n][0], byte[n][1], byte[n][2], byte[n][3]);
+            }
+    }
+
+    const int limit = j < rows && r < a.requests ? keys_of(position, p.cap) : 0;
+    int most = limit;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o));
+    most = __builtin_amdgcn_readfirstlane(most);
+    const int hi = min(most, end);
+    if (split > 0 && lo >= most) return;  // (the same for the whole work-group)
+
+    float m = -INFINITY, l = 0.f;
+    v4f o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
+    const v4i zero = {0, 0, 0, 0};
+
+    for (; t0 < hi; t0 += STEP) {
+        v4f s[4];
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            v4i sum[3];
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                sum[n] = zero;
+#pragma unroll
+                for (int i = 0; i < SK; ++i) {
+                    v4i k, x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        k[e] = (int)kb[u][4 * i + e];
+                        x[e] = (int)q[n][4 * i + e];
+                    }
+                    sum[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, x, sum[n], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s[u][i] = fmaf((float)((sum[0][i] << 8) + sum[1][i]), 256.f,
+                               (float)sum[2][i]);
+        }
+        float sc = ks * qs;
+        const float vscale = vs;
+        const int seen = page < 0 ? 0 : limit - t0 - 16 * g;  // of this lane's 16 tokens
+        // The next tile's loads, behind the last one too: loads in a branch would make every
+        // wait below one for all loads.
+        const bool more = t0 + STEP < hi;
+        load_k(t0 + STEP, next, more);
+        next = find(t0 + 2 * STEP);
+        // Scores are s * sc: scaled at once only where some are masked.
+        if (__ballot(seen < 16) == 0) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, s[u][i]);
+            top *= sc;
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[u][i] = 4 * u + i < seen ? s[u][i] * sc : -INFINITY;
+                    top = fmaxf(top, s[u][i]);
+                }
+            sc = 1.f;
+        }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        // m is any number near the largest score: it follows only where it would be left
+        // behind by more than kLag, so the sums are rarely scaled anew
+        if (__ballot(top > m + kLag) != 0) {
+            const float now = fmaxf(m, top);
+            const float alpha = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.f : now));
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
+            m = now;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        Frag w[2][PP];
+        if (PP == 1 && __ballot(!(vscale >= 0x1p-90f)) == 0) {
+            // one part: the sum is taken over the rounded weights, so that numerator and
+            // denominator round alike (a row that sees one key gives its value, whatever
+            // the scale's bits; p vs alone would be off by the same 2^-9 in all of a page)
+            const float less = __builtin_amdgcn_logf(vscale) - base;  // (log2)
+            float sum = 0.f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t e =
+                        pack_bf16(__builtin_amdgcn_exp2f(fmaf(s[u][2 * i], sc, less)),
+                                  __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], sc, less)));
+                    w[u / 2][0].u[2 * (u & 1) + i] = e;
+                    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, e),
+                                                          v2bf{(__bf16)1.f, (__bf16)1.f},
+                                                          sum, false);
+                }
+            l = fmaf(sum, __builtin_amdgcn_rcpf(vscale), l);
+        } else {  // (a scale of 0, a tiny one, NaN, or float32)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float e[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float z = fmaf(s[u][2 * i + k], sc, -base);
+                        e[k] = __builtin_amdgcn_exp2f(z);
+                        l += e[k];
+                        e[k] = z != -INFINITY ? e[k] * vscale : 0.f;
+                    }
+                    uint32_t part[PP];
+                    split_pair<PP>(e[0], e[1], part);
+#pragma unroll
+                    for (int n = 0; n < PP; ++n)
+                        w[u / 2][n].u[2 * (u & 1) + i] = part[n];
+                }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            pin(vb[d]);
+            const v8bf x = bytes8_to_bf16(vb[d][0], vb[d][1]);
+            const v8bf y = bytes8_to_bf16(vb[d][2], vb[d][3]);
+#pragma unroll
+            for (int n = PP - 1; n >= 0; --n) {
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, w[0][n].v, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, w[1][n].v, o[d], 0, 0, 0);
+            }
+        }
+        load_v(t0 + STEP, more);
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+
+    // the wavefronts' results under their common maximum, added in order
+    if (g == 0) {
+        m_lds[wave][col] = m;
+        l_lds[wave][col] = l;
+    }
+    __syncthreads();
+    float top = m_lds[0][col];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) top = fmaxf(top, m_lds[w][col]);
+    const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+        v4f x = o[d];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] *= f;
+        *reinterpret_cast<v4f *>(o_lds + (wave * 16 + col) * OS + d * 16 + 4 * g) = x;
+    }
+    __syncthreads();
+    if (lane < 16 && wave == 0) {  // (m_lds, l_lds: now the joined ones)
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float mw = m_lds[w][col], lw = l_lds[w][col];
+            sum += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f(mw - top);
+        }
+        m_lds[0][col] = top;
+        l_lds[0][col] = sum;
+    }
+    __syncthreads();
+    for (int e = tid; e < 16 * (W / 4); e += STEP) {
+        const int c = e / (W / 4), d = (e - c * (W / 4)) * 4;
+        const int jj = row0 + c;
+        if (jj >= rows) continue;
+        v4f x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const v4f y = *reinterpret_cast<const v4f *>(o_lds + (w * 16 + c) * OS + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] += y[i];
+        }
+        const int tk = s0 + jj / p.group;
+        const int64_t row = (int64_t)tk * a.heads + h * p.group + jj % p.group;
+        bool whole = part == kWhole;
+        int64_t at = (int64_t)part * 16 + c;
+        if (part < kWhole) {
+            const int lim = r < a.requests ? keys_of(a.positions[tk], p.cap) : 0;
+            whole = row_is_whole(p, lim);
+            if (whole && split > 0) continue;
+            at = row * p.splits + split;
+        }
+        const float sum = l_lds[0][c];
+        if (whole) {
+            if (d < a.c.dim) {
+                struct {
+                    T t[4];
+                } y;
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y.t[i] = from_f32<T>(x[i] * inv);
+                store_any(static_cast<T *>(a.O) + row * a.c.dim + d, y);
+            }
+        } else {
+            *reinterpret_cast<v4f *>(p.part_o + at * W + d) = x;
+            if (d == 0) {
+                p.part_ml[at * 2] = m_lds[0][c];
+                p.part_ml[at * 2 + 1] = sum;
+            }
+        }
+    }
+    __syncthreads();
+}
+
+// One request, kv head and range of its keys, all its rows.
+template <typename T, int W, int NW>
+__device__ __forceinline__ void few_rows(const AttnArgs &p, int id, FewLds<W, NW> &lds) {
+    const CacheAttention &a = p.a;
     const int split = id % p.splits;
     id /= p.splits;
     const int h = id % a.c.heads;
@@ -156,313 +491,120 @@ __device__ __forceinline__ void few_rows(const AttnArgs &p, int id, FewLds<W, NW
     request_tokens(a, r, s0, s1);
     const int rows = (s1 - s0) * p.group;
     if (p.both && rows > kFewRows) return;
-    const int P = a.c.page_size;
-    const int *table = a.table + (int64_t)(r < a.requests ? r : 0) * a.max_pages;
-    const int64_t page_bytes = (int64_t)P * W;
+    const int lo = split * p.chunk;
+    for (int row0 = 0; row0 < rows; row0 += 16)
+        few_segment<T, W, NW>(p, r, s0, rows, h, row0, lo,
+                              split == p.splits - 1 ? p.cap : lo + p.chunk, -2 - split, lds);
+}
 
-    for (int row0 = 0; row0 < rows; row0 += 16) {
-        const int j = row0 + col;
-        const int tok = s0 + j / p.group;
-        const int head = h * p.group + j % p.group;
-        const int limit =
-            j < rows && r < a.requests ? keys_of(a.positions[tok], p.cap) : 0;
-        int most = limit;
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o));
-        most = __builtin_amdgcn_readfirstlane(most);
-        const int lo = split * p.chunk;
-        const int hi = split == p.splits - 1 ? most : min(most, lo + p.chunk);
-        if (split > 0 && lo >= most) continue;  // (the same for the whole work-group)
+// Single tokens in even shares: the tiles (of 64 tokens) of all requests and kv heads in one
+// line, cut into p.shares equal pieces, one a work-group, all of which run at once; a decoding
+// batch's contexts differ, and work-groups of whole ranges would leave CUs idle at the end.
+// A unit is one request, kv head and 16 rows (its rows beyond 16 are further units, and a unit
+// without keys has one tile, which writes its zeros). Cuts within two tiles of a unit's end
+// are moved there. A unit that is cut is joined afterwards (attention_share_join_kernel, which
+// finds the same cuts): a share has at most one unit that began before it (part 2 w) and one
+// that goes on after it (part 2 w + 1).
+struct Shares {
+    int total, each;  // tiles of all units, of a share
+};
+__device__ __forceinline__ Shares shares_of(const AttnArgs &p, int tiles) {
+    const int total = tiles * p.a.c.heads;
+    return {total, max(4, (total + p.shares - 1) / p.shares)};
+}
 
-        uint32_t kb[4][4 * SK];
-        v4i vb[DT];
-        float ks = 0.f, vs = 0.f;
-        int page = -1;
-        // The table's entry for lane group g's 16 tokens: as it stands, and looked at only where
-        // the tile is loaded. (A check here would wait for the entry, and as loads come back in
-        // order, for every load before it.)
-        auto find = [&](int t0) { return table[min(t0 + 16 * g, p.cap - 1) >> p.shift]; };
-        auto load_k = [&](int t0, int entry) {
-            const int pg = t0 + 16 * g < hi && entry >= 0 && entry < a.c.pages ? entry : -1;
-            page = pg;
-            const int64_t mine = (int64_t)max(pg, 0) * a.c.heads + h;
-            ks = a.c.key_scales[mine];
-            vs = a.c.value_scales[mine];
-            const int kpage = max(__shfl(pg, (col >> 2) * 16), 0);
-            const int8_t *kp = a.c.keys + ((int64_t)kpage * a.c.heads + h) * page_bytes +
-                               ((t0 + 16 * (col >> 2) + (col & 3)) & (P - 1)) * W;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-#pragma unroll
-                for (int i = 0; i < SK; ++i) {
-                    const int at = HALF && i == SK - 1 ? g & 1 : g;
-                    const v4i x =
-                        *reinterpret_cast<const v4i *>(kp + u * 4 * W + 64 * i + 16 * at);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) kb[u][4 * i + e] = x[e];
-                }
-            }
-        };
-        auto load_v = [&](int t0) {  // (of the pages of the last load_k)
-            const int64_t mine = (int64_t)max(page, 0) * a.c.heads + h;
-            const int8_t *vp =
-                a.c.values + mine * page_bytes + col * P + ((t0 + 16 * g) & (P - 1));
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-                vb[d] = *reinterpret_cast<const v4i *>(vp + d * 16 * P);
-        };
-        int t0 = lo + 64 * wave;
-        int entry = 0, next = 0;
-        if (t0 < hi) {
-            entry = find(t0);
-            next = find(t0 + STEP);
-            load_k(t0, entry);
-            load_v(t0);
+struct ShareLds {
+    int first[kShareRequests + 2];  // tiles of one head of the requests before r
+    int units[kShareRequests + 2];  // tiles of a unit of r
+    int token[kShareRequests + 2];  // r's first token
+    int rows[kShareRequests + 2];
+};
+
+template <typename T, int W, int NW>
+__device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W, NW> &lds,
+                                           ShareLds &scan) {
+    const CacheAttention &a = p.a;
+    auto &first = scan.first;
+    auto &units = scan.units;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    auto &sums = lds.m[0];
+    int before = 0;
+    for (int base = 0; base <= a.requests; base += 64 * NW) {
+        const int r = base + tid;
+        int n = 0, unit = 1;
+        if (r <= a.requests) {
+            int s0, s1, most = 0;
+            request_tokens(a, r, s0, s1);
+            if (r < a.requests)
+                for (int t = s0; t < s1; ++t) most = max(most, keys_of(a.positions[t], p.cap));
+            unit = max(1, (most + 63) / 64);
+            n = ((s1 - s0) * p.group + 15) / 16 * unit;
+            units[r] = unit;
+            scan.token[r] = s0;
+            scan.rows[r] = (s1 - s0) * p.group;
         }
-
-        // q's bytes: lane (col, g) holds features 64 i + 16 g .. + 15
-        uint32_t q[3][4 * SK];
-        float qs;
-        {
-            const T *qp = static_cast<const T *>(a.Q);
-            if (j < rows) qp += (int64_t)tok * a.ldq + (int64_t)head * a.c.dim;
-            const int left = j < rows ? a.c.dim : 0;
-            float x[2 * SK][8];
-            uint32_t top = 0;
+        int upto = n;
 #pragma unroll
-            for (int i = 0; i < 2 * SK; ++i) {
-                const int d = 64 * (i / 2) + 16 * g + 8 * (i % 2);
-                load_f32<T, 8>(qp + d, left - d, x[i]);  // (dim <= W: zeros past a half step)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t bits = __float_as_uint(x[i][e]) & 0x7fffffffu;
-                    top = bits > top ? bits : top;
-                }
-            }
-#pragma unroll
-            for (int o = 16; o < 64; o <<= 1) {
-                const uint32_t other = __shfl_xor(top, o);
-                top = other > top ? other : top;
-            }
-            // (subnormal rows count as 0; where a value is not finite the scale is NaN)
-            const float big = __uint_as_float(top);
-            const bool fine = big >= 0x1p-126f && top < 0x7f800000u;
-            const float inv = fine ? 1.f / big : 0.f;
-            qs = (top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fine ? big : 0.f) *
-                 (1.f / 8323072.f) * p.c;
-#pragma unroll
-            for (int i = 0; i < 2 * SK; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    uint32_t byte[3][4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int t = __float2int_rn(x[i][4 * e + k] * inv * 8323072.f);
-                        const int t1 = (t - (int8_t)t) >> 8;
-                        byte[2][k] = (uint32_t)t;
-                        byte[1][k] = (uint32_t)t1;
-                        byte[0][k] = (uint32_t)((t1 - (int8_t)t1) >> 8);
-                    }
-#pragma unroll
-                    for (int n = 0; n < 3; ++n)
-                        q[n][2 * i + e] =
-                            pack4(byte[n][0], byte[n][1], byte[n][2], byte[n][3]);
-                }
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(upto, o);
+            if (lane >= o) upto += u;
         }
-
-        float m = -INFINITY, l = 0.f;
-        v4f o[DT];
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
-        const v4i zero = {0, 0, 0, 0};
-
-        for (; t0 < hi; t0 += STEP) {
-            v4f s[4];
-            float top = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                v4i sum[3];
-#pragma unroll
-                for (int n = 0; n < 3; ++n) {
-                    sum[n] = zero;
-#pragma unroll
-                    for (int i = 0; i < SK; ++i) {
-                        v4i k, x;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            k[e] = (int)kb[u][4 * i + e];
-                            x[e] = (int)q[n][4 * i + e];
-                        }
-                        sum[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, x, sum[n], 0, 0, 0);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s[u][i] = fmaf((float)((sum[0][i] << 8) + sum[1][i]), 256.f,
-                                   (float)sum[2][i]);
-            }
-            float sc = ks * qs;
-            const float vscale = vs;
-            const int seen = page < 0 ? 0 : limit - t0 - 16 * g;  // of this lane's 16 tokens
-            // The next tile; behind the last one the same again, from L2: loads in a branch
-            // would make every wait below one for all loads.
-            const bool more = t0 + STEP < hi;
-            const int ahead = more ? t0 + STEP : t0;
-            entry = more ? next : entry;
-            load_k(ahead, entry);
-            next = find(t0 + 2 * STEP);
-            // Scores are s * sc: scaled at once only where some are masked.
-            if (__ballot(seen < 16) == 0) {
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, s[u][i]);
-                top *= sc;
-            } else {
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s[u][i] = 4 * u + i < seen ? s[u][i] * sc : -INFINITY;
-                        top = fmaxf(top, s[u][i]);
-                    }
-                sc = 1.f;
-            }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            // m is any number near the largest score: it follows only where it would be left
-            // behind by more than kLag, so the sums are rarely scaled anew
-            if (__ballot(top > m + kLag) != 0) {
-                const float now = fmaxf(m, top);
-                const float alpha = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.f : now));
-                l *= alpha;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
-                m = now;
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-            Frag w[2][PP];
-            if (PP == 1 && __ballot(!(vscale >= 0x1p-90f)) == 0) {
-                // one part: the sum is taken over the rounded weights, so that numerator and
-                // denominator round alike (a row that sees one key gives its value, whatever
-                // the scale's bits; p vs alone would be off by the same 2^-9 in all of a page)
-                const float less = __builtin_amdgcn_logf(vscale) - base;  // (log2)
-                float sum = 0.f;
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t e =
-                            pack_bf16(__builtin_amdgcn_exp2f(fmaf(s[u][2 * i], sc, less)),
-                                      __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], sc, less)));
-                        w[u / 2][0].u[2 * (u & 1) + i] = e;
-                        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, e),
-                                                              v2bf{(__bf16)1.f, (__bf16)1.f},
-                                                              sum, false);
-                    }
-                l = fmaf(sum, __builtin_amdgcn_rcpf(vscale), l);
-            } else {  // (a scale of 0, a tiny one, NaN, or float32)
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        float e[2];
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const float z = fmaf(s[u][2 * i + k], sc, -base);
-                            e[k] = __builtin_amdgcn_exp2f(z);
-                            l += e[k];
-                            e[k] = z != -INFINITY ? e[k] * vscale : 0.f;
-                        }
-                        uint32_t part[PP];
-                        split_pair<PP>(e[0], e[1], part);
-#pragma unroll
-                        for (int n = 0; n < PP; ++n)
-                            w[u / 2][n].u[2 * (u & 1) + i] = part[n];
-                    }
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                pin(vb[d]);
-                const v8bf x = bytes8_to_bf16(vb[d][0], vb[d][1]);
-                const v8bf y = bytes8_to_bf16(vb[d][2], vb[d][3]);
-#pragma unroll
-                for (int n = PP - 1; n >= 0; --n) {
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, w[0][n].v, o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, w[1][n].v, o[d], 0, 0, 0);
-                }
-            }
-            load_v(ahead);
-        }
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
-
-        // the wavefronts' results under their common maximum, added in order
-        if (g == 0) {
-            m_lds[wave][col] = m;
-            l_lds[wave][col] = l;
-        }
+        if (lane == 63) sums[wave] = __int_as_float(upto);
         __syncthreads();
-        float top = m_lds[0][col];
+        int all = 0;
 #pragma unroll
-        for (int w = 1; w < NW; ++w) top = fmaxf(top, m_lds[w][col]);
-        const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - top);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            v4f x = o[d];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] *= f;
-            *reinterpret_cast<v4f *>(o_lds + (wave * 16 + col) * OS + d * 16 + 4 * g) = x;
+        for (int w = 0; w < NW; ++w) {
+            const int x = __float_as_int(sums[w]);
+            upto += w < wave ? x : 0;
+            all += x;
         }
+        if (r <= a.requests) first[r + 1] = before + upto;
+        before += all;
         __syncthreads();
-        if (lane < 16 && wave == 0) {  // (m_lds, l_lds: now the joined ones)
-            float sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const float mw = m_lds[w][col], lw = l_lds[w][col];
-                sum += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f(mw - top);
-            }
-            m_lds[0][col] = top;
-            l_lds[0][col] = sum;
+    }
+    if (tid == 0) first[0] = 0;
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int i = tid; i <= a.requests + 1; i += 64 * NW) {
+            p.firsts[i] = first[i];
+            p.firsts[a.requests + 2 + i] = i <= a.requests ? units[i] : 1;
         }
-        __syncthreads();
-        for (int e = tid; e < 16 * (W / 4); e += STEP) {
-            const int c = e / (W / 4), d = (e - c * (W / 4)) * 4;
-            const int jj = row0 + c;
-            if (jj >= rows) continue;
-            v4f x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const v4f y = *reinterpret_cast<const v4f *>(o_lds + (w * 16 + c) * OS + d);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] += y[i];
-            }
-            const int tk = s0 + jj / p.group;
-            const int64_t row = (int64_t)tk * a.heads + h * p.group + jj % p.group;
-            const int lim = r < a.requests ? keys_of(a.positions[tk], p.cap) : 0;
-            const float sum = l_lds[0][c];
-            if (row_is_whole(p, lim)) {
-                if (split == 0 && d < a.c.dim) {
-                    struct {
-                        T t[4];
-                    } y;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        y.t[i] = from_f32<T>(sum == 0.f ? 0.f : x[i] / sum);
-                    store_any(static_cast<T *>(a.O) + row * a.c.dim + d, y);
-                }
-            } else {
-                const int64_t at = row * p.splits + split;
-                *reinterpret_cast<v4f *>(p.part_o + at * W + d) = x;
-                if (d == 0) {
-                    p.part_ml[at * 2] = m_lds[0][c];
-                    p.part_ml[at * 2 + 1] = sum;
-                }
-            }
-        }
-        __syncthreads();
+    const Shares s = shares_of(p, before);
+    auto request_at = [&](int tile) {  // the last request that begins at or before the tile
+        int r = -1;
+        for (int base = 0; base <= a.requests; base += 64)
+            r += __builtin_popcountll(__ballot(
+                base + lane <= a.requests && first[min(base + lane, a.requests)] *
+                                                     a.c.heads <= tile));
+        return r;
+    };
+    auto cut = [&](int w) {
+        const int64_t at = (int64_t)w * s.each;
+        if (at >= s.total) return s.total;
+        const int r = request_at((int)at);
+        const int in = ((int)at - first[r] * a.c.heads) % units[r];
+        if (in <= kSnap) return (int)at - in;
+        return units[r] - in <= kSnap ? (int)at + units[r] - in : (int)at;
+    };
+    const int w = blockIdx.x;
+    int at = __builtin_amdgcn_readfirstlane(cut(w));
+    const int stop = __builtin_amdgcn_readfirstlane(cut(w + 1));
+    while (at < stop) {
+        const int r = request_at(at);
+        const int unit = __builtin_amdgcn_readfirstlane(units[r]);
+        const int n = __builtin_amdgcn_readfirstlane(first[r + 1] - first[r]);
+        const int in = at - __builtin_amdgcn_readfirstlane(first[r]) * a.c.heads;
+        const int h = in / n;
+        const int block = (in - h * n) / unit;
+        const int tile = in - h * n - block * unit;
+        const int last = min(unit, tile + stop - at);
+        const bool ends = last == unit;
+        const int s0 = __builtin_amdgcn_readfirstlane(scan.token[r]);
+        const int rows = __builtin_amdgcn_readfirstlane(scan.rows[r]);
+        few_segment<T, W, NW>(p, r, s0, rows, h, block * 16, tile * 64,
+                              last * 64,
+                              tile == 0 && ends ? kWhole : 2 * w + (tile == 0 ? 1 : 0), lds);
+        at += last - tile;
     }
 }
 
@@ -624,7 +766,7 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
 #pragma unroll
         for (int s = 0; s < ST; ++s) {
             const int d = 16 * s + 8 * hi32;
-            query_frag<T, QP>(qp + d, j < rows ? a.c.dim - d : 0, q[s]);
+            query_frag<T, QP>(qp, d, j < rows && d < a.c.dim, q[s]);
         }
     }
     load(lo);
@@ -891,6 +1033,88 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnArgs p) {
     }
 }
 
+// Joins what few_shares cut: one request and query head a work-group (a row of each token),
+// parts side by side over its thread groups and in order within them, under their common
+// maximum.
+template <typename T, int W>
+__global__ void __launch_bounds__(256) attention_share_join_kernel(AttnArgs p) {
+    constexpr int Q = W / 4;    // threads that hold a row of O
+    constexpr int N = 256 / Q;  // parts at a time
+    __shared__ __attribute__((aligned(16))) float o_lds[N][W + 4];
+    __shared__ float l_lds[N];
+    const CacheAttention &a = p.a;
+    const int r = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+    const int h = head / p.group;
+    const int before = p.firsts[r], n = p.firsts[r + 1] - before;
+    const int tiles = p.firsts[a.requests + 1], unit = p.firsts[a.requests + 2 + r];
+    if (n == 0 || unit <= 2 * kSnap) return;
+    const Shares s = shares_of(p, tiles);
+    int s0, s1;
+    request_tokens(a, r, s0, s1);
+    const int g = threadIdx.x / Q, d = threadIdx.x % Q * 4;
+    for (int tok = s0; tok < s1; ++tok) {
+        const int j = (tok - s0) * p.group + head % p.group;
+        const int begin = before * a.c.heads + h * n + j / 16 * unit;
+        const int cut0 = (begin + kSnap) / s.each + 1;         // the first cut inside
+        const int cut1 = (begin + unit - kSnap - 1) / s.each;  // and the last
+        const int parts = cut1 - cut0 + 2;
+        if (parts < 2) continue;
+        auto place = [&](int k) {
+            return (int64_t)(k == 0 ? 2 * (cut0 - 1) + 1 : 2 * (cut0 + k - 1)) * 16 + j % 16;
+        };
+        float top = -INFINITY;
+        for (int k = threadIdx.x & 63; k < parts; k += 64)
+            top = fmaxf(top, p.part_ml[place(k) * 2]);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        if (g < N) {
+            float l = 0.f;
+            v4f x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int k = g; k < parts; k += N) {
+                const int64_t at = place(k);
+                const float ms = p.part_ml[at * 2], ls = p.part_ml[at * 2 + 1];
+                // (a part whose scores were all NaN has sum NaN and no maximum)
+                const float f = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.f)
+                                                : __builtin_amdgcn_exp2f(ms - top);
+                const v4f y = *reinterpret_cast<const v4f *>(p.part_o + at * W + d);
+                l += ls * f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] += y[i] * f;
+            }
+            *reinterpret_cast<v4f *>(&o_lds[g][d]) = x;
+            if (d == 0) l_lds[g] = l;
+        }
+        __syncthreads();
+        if (threadIdx.x < Q && d < a.c.dim) {
+            float l = 0.f;
+            v4f x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                l += l_lds[k];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] += o_lds[k][d + i];
+            }
+            struct {
+                T t[4];
+            } y;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y.t[i] = from_f32<T>(x[i] * inv);
+            store_any(static_cast<T *>(a.O) + ((int64_t)tok * a.heads + head) * a.c.dim + d, y);
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W <= 128 ? 2 : 1)))
+attention_share_kernel(AttnArgs p) {
+    __shared__ FewLds<W> lds;
+    __shared__ ShareLds scan;
+    few_shares<T, W, 4>(p, lds, scan);
+}
+
 template <typename T, int W>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W <= 128 ? 2 : 1)))
 attention_few_kernel(AttnArgs p) {
@@ -916,6 +1140,15 @@ attention_both_kernel(AttnArgs p, int few) {
 
 template <typename T, int W>
 int launch_width(hipStream_t stream, const AttnArgs &p) {
+    if (p.shares != 0) {
+        MIGEMM_LAUNCH((attention_share_kernel<T, W>), dim3((unsigned)p.shares), dim3(256), 0,
+                      stream, p);
+        if (const int rc = launch_status("attention kernel launch")) return rc;
+        if (p.cap <= 64 * (2 * kSnap + 1)) return MIGEMM_OK;  // (no unit is long enough to cut)
+        MIGEMM_LAUNCH((attention_share_join_kernel<T, W>),
+                      dim3((unsigned)(p.a.requests * p.a.heads)), dim3(256), 0, stream, p);
+        return launch_status("attention_share_join_kernel launch");
+    }
     const int few = p.splits * p.a.c.heads * (p.a.requests + 1);
     constexpr int NW = many_waves(W, sizeof(T));
     if (p.both)
