@@ -117,6 +117,13 @@ __device__ __forceinline__ void query_frag(const T *row, int d, bool there, Frag
     }
 }
 
+// The largest of three (fmaxf would make each operand canonical first).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 // Rows that are whole after range 0 are written by it; others leave a part for each range.
 __device__ __forceinline__ bool row_is_whole(const AttnArgs &p, int limit) {
     return p.splits == 1 || limit <= p.chunk;
@@ -619,28 +626,30 @@ template <int W, int NW>
 struct ManyLds {
     alignas(16) uint16_t k[2][64 * (W + 8)];
     alignas(16) uint16_t v[2][W * (64 + 8)];
-    float scales[2][8];  // ks c of the tile's four groups of 16 tokens, then vs
-    uint32_t flags[2];
+    // of the tile's four groups of 16 tokens: ks c, vs, log2 vs and 1 / vs
+    v4f scales[2][4];
+    // (1: the page is outside the pool, 2: vs is a plain number)
+    alignas(4) uint8_t flags[2][4];
     int most[NW];
 };
 
 template <typename T, int W, int NW>
 __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, NW> &lds) {
     constexpr int ROWS = 32 * NW;
-    constexpr int NT = 64 * NW;
     constexpr int QP = std::is_same<T, float>::value ? 3 : 1;
     constexpr int PP = QP;
     constexpr int ST = W / 16;       // steps of the first product
     constexpr int DT = W / 32;       // blocks of the second product
+    constexpr int VA = W <= 128 && QP == 1 ? 2 : 1;  // groups of 16 tokens read ahead
     constexpr int KR = W + 8;        // LDS rows, in bf16
     constexpr int VR = 64 + 8;
-    constexpr int CH = W / 16;       // units of 16 bytes in a row of K
-    constexpr int MU = (4 * W + NT - 1) / NT;  // units of K, and of V, that a thread moves
-    constexpr bool EVEN = 4 * W % NT == 0;     // (as many for every thread)
+    constexpr int CH = W / 16;          // units of 16 bytes in a row of K
+    constexpr int MU = (W + 63) / 64;   // units of K, and of V, that a thread moves
+    constexpr bool EVEN = W % 64 == 0;  // (as many for every thread)
     auto &k_lds = lds.k;
     auto &v_lds = lds.v;
     auto &scale_lds = lds.scales;
-    auto &lost_lds = lds.flags;
+    auto &flags_lds = lds.flags;
     auto &most_lds = lds.most;
 
     const CacheAttention &a = p.a;
@@ -695,66 +704,68 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
     // What the first tile needs is asked for at once, before it is known whether any row sees it
     // (a work-group's beginning is a chain of loads that wait for each other).
     const int lo = split * p.chunk;
-    // this thread's units of 16 bytes of a tile: of K row unit / CH (a token), of V row unit / 4
-    // (a feature) and group unit % 4 (of 16 tokens)
-    v4i kb[MU], vb[MU];
-    float sc = 0.f;
-    auto entry_at = [&](int t) { return table[min(t, p.cap - 1) >> p.shift]; };
-    auto page_of = [&](int entry) { return entry >= 0 && entry < a.c.pages ? entry : -1; };
-    auto token_of = [&](int i) { return min((tid + NT * i) / CH, 63); };
-    // A tile's table entries are read a tile before its bytes, and looked at only then (a check
-    // at once would wait for them, and as loads come back in order, for every load before).
-    int kentry[MU], ventry = -1;
-    auto find = [&](int t0) {
-#pragma unroll
-        for (int i = 0; i < MU; ++i) kentry[i] = entry_at(t0 + (token_of(i) & 48));
-        ventry = entry_at(t0 + 16 * (tid & 3));
+    // A wavefront moves 16 tokens' rows of K, so that their page is one for the wavefront and its
+    // address scalar; of V it moves the same tokens of all features or, where a page holds whole
+    // tiles, a quarter of the features of all 64 (rows of 64 neighbouring bytes). A thread's
+    // place in the page never changes.
+    const bool whole = P >= 64;
+    const int vrow = whole ? tid >> 2 : lane;      // and vrow + 64, ...
+    const int vgroup = whole ? tid & 3 : wave;
+    auto unit_of = [&](int i) { return EVEN ? lane + 64 * i : min(lane + 64 * i, W - 1); };
+    auto row_of = [&](int i) { return EVEN ? vrow + 64 * i : min(vrow + 64 * i, W - 1); };
+    uint32_t zero = 0;  // (keeps the loads below vector loads: scalar ones return out of order)
+    asm("v_mov_b32 %0, 0" : "=v"(zero));
+    auto at = [&](const auto *x, int64_t i) {
+        return *reinterpret_cast<decltype(x)>(reinterpret_cast<const char *>(x + i) + zero);
     };
-    uint32_t gone = 0;
+    // A tile's table entry is read a tile before its bytes, and looked at only then (a check at
+    // once would wait for it, and as loads come back in order, for every load before).
+    v4i kb[MU], vb[MU];
+    int entry = -1;
+    float ks_next = 0.f, vs_next = 0.f;
+    bool gone = false;
+    auto find = [&](int t0) { entry = at(table, min(t0 + 16 * wave, p.cap - 1) >> p.shift); };
     auto load = [&](int t0) {
-        int kpage[MU];
-#pragma unroll
-        for (int i = 0; i < MU; ++i) kpage[i] = page_of(kentry[i]);
-        const int vpage = page_of(ventry);
-        gone = (uint32_t)__ballot(lane < 4 && vpage < 0);
+        const int page = __builtin_amdgcn_readfirstlane(entry);
+        gone = page < 0 || page >= a.c.pages;
+        const int64_t block = (int64_t)(gone ? 0 : page) * a.c.heads + h;
+        const int in = (t0 + 16 * wave) & (P - 1);
+        const int8_t *kp = a.c.keys + block * page_bytes + in * W;
+        const int8_t *vp = a.c.values + block * page_bytes + (whole ? t0 & (P - 1) : in);
 #pragma unroll
         for (int i = 0; i < MU; ++i)
-            kb[i] = *reinterpret_cast<const v4i *>(
-                a.c.keys + ((int64_t)max(kpage[i], 0) * a.c.heads + h) * page_bytes +
-                ((t0 + token_of(i)) & (P - 1)) * W + (tid + NT * i) % CH * 16);
-        const int8_t *vp = a.c.values + ((int64_t)max(vpage, 0) * a.c.heads + h) * page_bytes +
-                           ((t0 + 16 * (tid & 3)) & (P - 1));
+            kb[i] = *reinterpret_cast<const v4i *>(kp + (uint32_t)(unit_of(i) * 16));
 #pragma unroll
-        for (int i = 0; i < MU; ++i) {
-            const int d = (tid + NT * i) >> 2;
-            vb[i] = *reinterpret_cast<const v4i *>(vp + (EVEN ? d : min(d, W - 1)) * P);
-        }
-        if (tid < 8) {  // tid & 3: the group
-            const int64_t at = (int64_t)max(vpage, 0) * a.c.heads + h;
-            sc = tid < 4 ? a.c.key_scales[at] * p.c : a.c.value_scales[at];
-        }
+        for (int i = 0; i < MU; ++i)
+            vb[i] = *reinterpret_cast<const v4i *>(
+                vp + (uint32_t)(row_of(i) * P + (whole ? vgroup * 16 : 0)));
+        ks_next = at(a.c.key_scales, block);
+        vs_next = at(a.c.value_scales, block);
     };
     auto stage = [&](int b) {
 #pragma unroll
         for (int i = 0; i < MU; ++i) {
-            const int unit = tid + NT * i;
-            if (EVEN || unit < 4 * W) {
-                pin(kb[i]);
-                pin(vb[i]);
-                uint16_t *kp = k_lds[b] + unit / CH * KR + unit % CH * 16;
+            pin(kb[i]);
+            pin(vb[i]);
+            if (EVEN || lane + 64 * i < W) {
+                const int unit = lane + 64 * i;
+                uint16_t *kp = k_lds[b] + (16 * wave + unit / CH) * KR + unit % CH * 16;
                 *reinterpret_cast<v8bf *>(kp) = bytes8_to_bf16(kb[i][0], kb[i][1]);
                 *reinterpret_cast<v8bf *>(kp + 8) = bytes8_to_bf16(kb[i][2], kb[i][3]);
+            }
+            if (EVEN || vrow + 64 * i < W) {
                 // a half-wavefront's eight tokens of each 16 are neighbours: 0-3, 8-11 and
                 // 4-7, 12-15, as the rows of the first product fall
-                uint16_t *vp = v_lds[b] + (unit >> 2) * VR + (tid & 3) * 16;
+                uint16_t *vp = v_lds[b] + (vrow + 64 * i) * VR + vgroup * 16;
                 *reinterpret_cast<v8bf *>(vp) = bytes8_to_bf16(vb[i][0], vb[i][2]);
                 *reinterpret_cast<v8bf *>(vp + 8) = bytes8_to_bf16(vb[i][1], vb[i][3]);
             }
         }
-        if (tid < 8) scale_lds[b][tid] = sc;
-        // (bit 4: the four value scales are plain numbers)
-        const bool plain = (__ballot(sc >= 0x1p-90f) >> 4 & 15) == 15;
-        if (tid == 0) lost_lds[b] = gone | (uint32_t)plain << 4;
+        if (lane == 0) {
+            scale_lds[b][wave] = v4f{ks_next * p.c, vs_next, __builtin_amdgcn_logf(vs_next),
+                                     __builtin_amdgcn_rcpf(vs_next)};
+            flags_lds[b][wave] = (uint8_t)((gone ? 1 : 0) | (vs_next >= 0x1p-90f ? 2 : 0));
+        }
     };
 
     find(lo);
@@ -803,46 +814,56 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
         if (more) load(t0 + 64);
         find(t0 + 128);  // (always: a value that only a branch loads is copied, and waited for)
         if (t0 < mine) {  // (else none of this wavefront's rows sees the tile)
-        // pages of the tile that are outside the pool (one bit for each group of 16 tokens)
-        const uint32_t flags = __builtin_amdgcn_readfirstlane(lost_lds[buf]);
-        const uint32_t lost = flags & 15;
+        const uint32_t flags = __builtin_amdgcn_readfirstlane(
+            *reinterpret_cast<const uint32_t *>(flags_lds[buf]));
+        const uint32_t lost = flags & 0x01010101u;
 
-        // The first product's and the second's operands are read from LDS a step ahead; the
-        // accumulators of neighbouring instructions are different ones.
+        // The products' operands are read from LDS several steps ahead (a read takes longer than
+        // a step's instructions); the accumulators of neighbouring instructions are different
+        // ones.
+        constexpr int KA = ST < 4 ? ST : 4;  // steps ahead
         v16f s[2];
-        const v16f zero = {};
+        const v16f none = {};
         const uint16_t *kp = k_lds[buf] + lo32 * KR + 8 * hi32;
-        v8bf kf[2][2];
+        v8bf kf[KA][2];
+        auto read_k = [&](int st) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) kf[0][b] = *reinterpret_cast<const v8bf *>(kp + 32 * b * KR);
+            for (int b = 0; b < 2; ++b)
+                kf[st % KA][b] = *reinterpret_cast<const v8bf *>(kp + 32 * b * KR + 16 * st);
+        };
+#pragma unroll
+        for (int st = 0; st < KA; ++st) read_k(st);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int st = 0; st < ST; ++st) {
-            if (st + 1 < ST) {
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-                    kf[(st + 1) & 1][b] =
-                        *reinterpret_cast<const v8bf *>(kp + 32 * b * KR + 16 * (st + 1));
-            }
 #pragma unroll
             for (int n = QP - 1; n >= 0; --n)
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
                     s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                        kf[st & 1][b], q[st][n].v, st == 0 && n == QP - 1 ? zero : s[b], 0, 0,
+                        kf[st % KA][b], q[st][n].v, st == 0 && n == QP - 1 ? none : s[b], 0, 0,
                         0);
+            if (st + KA < ST) read_k(st + KA);
         }
-        float ks[4], vs[4];
+        const uint16_t *vp = v_lds[buf] + lo32 * VR + 8 * hi32;
+        v8bf vf[VA][DT];
+        auto read_v = [&](int x) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            ks[w] = scale_lds[buf][w];
-            vs[w] = scale_lds[buf][4 + w];
-        }
+            for (int d = 0; d < DT; ++d)
+                vf[x % VA][d] = *reinterpret_cast<const v8bf *>(vp + 32 * d * VR + 16 * x);
+        };
+#pragma unroll
+        for (int x = 0; x < VA; ++x) read_v(x);
+        __builtin_amdgcn_sched_barrier(0);
+        float ks[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) ks[w] = scale_lds[buf][w][0];
         // Scores are s * ks. Where some are masked, a ks that -inf could not be multiplied with
         // (0, tiny, NaN) is multiplied first.
         if (t0 + 64 > least || lost != 0) {  // the same for the wavefront
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const int seen = lost >> w & 1 ? 0 : limit - t0 - 16 * w - 4 * hi32;
+                const int seen = lost >> 8 * w & 1 ? 0 : limit - t0 - 16 * w - 4 * hi32;
                 const bool odd = !(ks[w] >= 0x1p-100f);
                 const float by = odd ? ks[w] : 1.f;
 #pragma unroll
@@ -856,10 +877,11 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            float x = s[w >> 1][8 * (w & 1)];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) x = fmaxf(x, s[w >> 1][8 * (w & 1) + i]);
-            top = fmaxf(top, x * ks[w]);
+            const v16f &x = s[w >> 1];
+            const int i = 8 * (w & 1);
+            const float big = max3(max3(max3(x[i], x[i + 1], x[i + 2]), x[i + 3], x[i + 4]),
+                                   x[i + 5], max3(x[i + 6], x[i + 7], x[i]));
+            top = fmaxf(top, big * ks[w]);
         }
         top = fmaxf(top, __shfl_xor(top, 32));
         // m is any number near the largest score: it follows only where it would be left behind
@@ -876,13 +898,13 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
         }
         const float base = m == -INFINITY ? 0.f : m;
         Frag w[4][PP];
-        if (PP == 1 && flags >> 4 != 0) {
+        if (PP == 1 && (flags & 0x02020202u) == 0x02020202u) {
             // one part: the sum is taken over the rounded weights, so that numerator and
             // denominator round alike (a row that sees one key gives its value, whatever the
             // scale's bits; p vs alone would be off by the same 2^-9 in all of a page)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const float less = __builtin_amdgcn_logf(vs[x]) - base;  // (log2)
+                const float less = scale_lds[buf][x][2] - base;
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -896,7 +918,7 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
                         __builtin_bit_cast(v2bf, w[x][0].u[i]), v2bf{(__bf16)1.f, (__bf16)1.f},
                         sum, false);
                 }
-                l = fmaf(sum, __builtin_amdgcn_rcpf(vs[x]), l);
+                l = fmaf(sum, scale_lds[buf][x][3], l);
             }
         } else {  // (a scale of 0, a tiny one, NaN, or float32)
 #pragma unroll
@@ -909,7 +931,7 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
                         const float z = fmaf(s[x >> 1][8 * (x & 1) + 2 * i + k], ks[x], -base);
                         e[k] = __builtin_amdgcn_exp2f(z);
                         l += e[k];
-                        e[k] = z != -INFINITY ? e[k] * vs[x] : 0.f;
+                        e[k] = z != -INFINITY ? e[k] * scale_lds[buf][x][1] : 0.f;
                     }
                     uint32_t part[PP];
                     split_pair<PP>(e[0], e[1], part);
@@ -917,24 +939,15 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
                     for (int n = 0; n < PP; ++n) w[x][n].u[i] = part[n];
                 }
         }
-        const uint16_t *vp = v_lds[buf] + lo32 * VR + 8 * hi32;
-        v8bf vf[2][DT];
-#pragma unroll
-        for (int d = 0; d < DT; ++d) vf[0][d] = *reinterpret_cast<const v8bf *>(vp + 32 * d * VR);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            if (x < 3) {
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-                    vf[(x + 1) & 1][d] =
-                        *reinterpret_cast<const v8bf *>(vp + 32 * d * VR + 16 * (x + 1));
-            }
 #pragma unroll
             for (int n = PP - 1; n >= 0; --n)
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x & 1][d], w[x][n].v, o[d],
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x % VA][d], w[x][n].v, o[d],
                                                                    0, 0, 0);
+            if (x + VA < 4) read_v(x + VA);
         }
         }
         if (more) stage(buf ^ 1);
