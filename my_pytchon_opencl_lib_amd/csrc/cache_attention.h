@@ -45,9 +45,7 @@ struct AttnArgs {
 constexpr int kFewRows = 16;
 constexpr int kShareRequests = 1022;  // few_shares keeps a scan of the requests in LDS
 constexpr int kSnap = 2;              // (its cuts)
-// Wavefronts (of 32 rows) of a many-rows work-group: eight, two on each SIMD, where the
-// registers allow that.
-constexpr int many_waves(int width, int bytes) { return 4; }
+constexpr int kManyRows = 128;        // of a many-rows work-group
 constexpr float kLag = 8.f;  // (weights stay below 2^8)
 
 namespace {
@@ -117,11 +115,10 @@ __device__ __forceinline__ void query_frag(const T *row, int d, bool there, Frag
     }
 }
 
-// The largest of three (fmaxf would make each operand canonical first).
+// The largest of three, NaN if one is (fmaxf would make each operand canonical first, an
+// instruction of its own).
 __device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
 // Rows that are whole after range 0 are written by it; others leave a part for each range.
@@ -143,10 +140,10 @@ __device__ __forceinline__ bool row_is_whole(const AttnArgs &p, int limit) {
 // v_mfma_i32_16x16x64_i8: row m of subtile u is token 16 (m / 4) + 4 u + m % 4 of the tile, so
 // that lane group g ends up with the scores of tokens 16 g .. 16 g + 15, whose bytes of V^T are
 // 16 neighbours: one load a row of V.
-template <int W, int NW = 4>
+template <int W>
 struct FewLds {
-    alignas(16) float o[NW * 16 * (W + 4)];
-    float m[NW][16], l[NW][16];
+    alignas(16) float o[4 * 16 * (W + 4)];
+    float m[4][16], l[4][16];
 };
 
 // 16 rows from row0 on of request r (tokens from s0 on) and kv head h, over its keys lo .. end - 1
@@ -154,11 +151,11 @@ struct FewLds {
 // row_is_whole.
 constexpr int kWhole = -1;
 
-template <typename T, int W, int NW>
+template <typename T, int W>
 __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, int rows, int h,
                                             int row0, int lo, int end, int part,
-                                            FewLds<W, NW> &lds) {
-    constexpr int STEP = 64 * NW;  // tokens that the work-group takes at a time
+                                            FewLds<W> &lds) {
+    constexpr int STEP = 256;  // tokens that the work-group takes at a time
     constexpr int PP = std::is_same<T, float>::value ? 3 : 1;
     constexpr int SK = (W + 63) / 64;  // steps of 64 features of the first product
     constexpr bool HALF = W % 64 != 0; // of the last one only 32 are there: lane groups 2 and 3
@@ -422,7 +419,7 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
     __syncthreads();
     float top = m_lds[0][col];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) top = fmaxf(top, m_lds[w][col]);
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][col]);
     const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -435,7 +432,7 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
     if (lane < 16 && wave == 0) {  // (m_lds, l_lds: now the joined ones)
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
+        for (int w = 0; w < 4; ++w) {
             const float mw = m_lds[w][col], lw = l_lds[w][col];
             sum += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f(mw - top);
         }
@@ -449,7 +446,7 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
         if (jj >= rows) continue;
         v4f x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
+        for (int w = 0; w < 4; ++w) {
             const v4f y = *reinterpret_cast<const v4f *>(o_lds + (w * 16 + c) * OS + d);
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] += y[i];
@@ -487,8 +484,8 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
 }
 
 // One request, kv head and range of its keys, all its rows.
-template <typename T, int W, int NW>
-__device__ __forceinline__ void few_rows(const AttnArgs &p, int id, FewLds<W, NW> &lds) {
+template <typename T, int W>
+__device__ __forceinline__ void few_rows(const AttnArgs &p, int id, FewLds<W> &lds) {
     const CacheAttention &a = p.a;
     const int split = id % p.splits;
     id /= p.splits;
@@ -500,7 +497,7 @@ __device__ __forceinline__ void few_rows(const AttnArgs &p, int id, FewLds<W, NW
     if (p.both && rows > kFewRows) return;
     const int lo = split * p.chunk;
     for (int row0 = 0; row0 < rows; row0 += 16)
-        few_segment<T, W, NW>(p, r, s0, rows, h, row0, lo,
+        few_segment<T, W>(p, r, s0, rows, h, row0, lo,
                               split == p.splits - 1 ? p.cap : lo + p.chunk, -2 - split, lds);
 }
 
@@ -527,8 +524,8 @@ struct ShareLds {
     int rows[kShareRequests + 2];
 };
 
-template <typename T, int W, int NW>
-__device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W, NW> &lds,
+template <typename T, int W>
+__device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W> &lds,
                                            ShareLds &scan) {
     const CacheAttention &a = p.a;
     auto &first = scan.first;
@@ -536,7 +533,7 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W, NW> &lds
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     auto &sums = lds.m[0];
     int before = 0;
-    for (int base = 0; base <= a.requests; base += 64 * NW) {
+    for (int base = 0; base <= a.requests; base += 256) {
         const int r = base + tid;
         int n = 0, unit = 1;
         if (r <= a.requests) {
@@ -560,7 +557,7 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W, NW> &lds
         __syncthreads();
         int all = 0;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
+        for (int w = 0; w < 4; ++w) {
             const int x = __float_as_int(sums[w]);
             upto += w < wave ? x : 0;
             all += x;
@@ -572,7 +569,7 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W, NW> &lds
     if (tid == 0) first[0] = 0;
     __syncthreads();
     if (blockIdx.x == 0)
-        for (int i = tid; i <= a.requests + 1; i += 64 * NW) {
+        for (int i = tid; i <= a.requests + 1; i += 256) {
             p.firsts[i] = first[i];
             p.firsts[a.requests + 2 + i] = i <= a.requests ? units[i] : 1;
         }
@@ -608,7 +605,7 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W, NW> &lds
         const bool ends = last == unit;
         const int s0 = __builtin_amdgcn_readfirstlane(scan.token[r]);
         const int rows = __builtin_amdgcn_readfirstlane(scan.rows[r]);
-        few_segment<T, W, NW>(p, r, s0, rows, h, block * 16, tile * 64,
+        few_segment<T, W>(p, r, s0, rows, h, block * 16, tile * 64,
                               last * 64,
                               tile == 0 && ends ? kWhole : 2 * w + (tile == 0 ? 1 : 0), lds);
         at += last - tile;
@@ -622,44 +619,28 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W, NW> &lds
 // work, one barrier a tile). Bound by the matrix cores and by the exponentials and
 // conversions beside them. LDS rows are padded by 16 bytes: the 16 lanes of a read phase fall
 // on different banks.
-template <int W, int NW>
+template <int W>
 struct ManyLds {
-    alignas(16) uint16_t k[2][64 * (W + 8)];
-    alignas(16) uint16_t v[2][W * (64 + 8)];
+    static constexpr int KR = W + 8, VR = 64 + 8;  // LDS rows, in bf16
+    alignas(16) uint16_t k[2][64 * KR];
+    alignas(16) uint16_t v[2][W * VR];
     // of the tile's four groups of 16 tokens: ks c, vs, log2 vs and 1 / vs
     v4f scales[2][4];
     // (1: the page is outside the pool, 2: vs is a plain number)
     alignas(4) uint8_t flags[2][4];
-    int most[NW];
+    int most[4];
 };
 
-template <typename T, int W, int NW>
-__device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, NW> &lds) {
-    constexpr int ROWS = 32 * NW;
-    constexpr int QP = std::is_same<T, float>::value ? 3 : 1;
-    constexpr int PP = QP;
-    constexpr int ST = W / 16;       // steps of the first product
-    constexpr int DT = W / 32;       // blocks of the second product
-    constexpr int VA = W <= 128 && QP == 1 ? 2 : 1;  // groups of 16 tokens read ahead
-    constexpr int KR = W + 8;        // LDS rows, in bf16
-    constexpr int VR = 64 + 8;
-    constexpr int CH = W / 16;          // units of 16 bytes in a row of K
-    constexpr int MU = (W + 63) / 64;   // units of K, and of V, that a thread moves
-    constexpr bool EVEN = W % 64 == 0;  // (as many for every thread)
-    auto &k_lds = lds.k;
-    auto &v_lds = lds.v;
-    auto &scale_lds = lds.scales;
-    auto &flags_lds = lds.flags;
-    auto &most_lds = lds.most;
-
+// A work-group's share: request r's rows from tile * kManyRows on, of kv head h, and a range of keys.
+struct ManyTile {
+    int r, tile, s0, rows, h, split;
+};
+__device__ __forceinline__ bool many_tile(const AttnArgs &p, int id, ManyTile &x) {
     const CacheAttention &a = p.a;
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int lo32 = lane & 31, hi32 = lane >> 5;
-
-    const int h = id % a.c.heads;
+    const int lane = threadIdx.x & 63;
+    x.h = id % a.c.heads;
     id /= a.c.heads;
-    const int split = id % p.splits;
+    x.split = id % p.splits;
     id /= p.splits;
     // which request's tile: requests in order (tiles that run together share keys in L2), 64 at
     // a time
@@ -669,7 +650,7 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
         if (base + lane <= a.requests) {
             request_tokens(a, base + lane, x0, x1);
             const int rows = (x1 - x0) * p.group;
-            n = rows > kFewRows ? (rows + ROWS - 1) / ROWS : 0;
+            n = rows > kFewRows ? (rows + kManyRows - 1) / kManyRows : 0;
         }
         int upto = n;
 #pragma unroll
@@ -688,87 +669,164 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
         }
         before += __shfl(upto, 63);
     }
-    if (r < 0) return;
-    r = __builtin_amdgcn_readfirstlane(r);
-    s0 = __builtin_amdgcn_readfirstlane(s0);
-    s1 = __builtin_amdgcn_readfirstlane(s1);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-    const int rows = (s1 - s0) * p.group;
-    const int P = a.c.page_size;
-    const int *table = a.table + (int64_t)(r < a.requests ? r : 0) * a.max_pages;
-    const int64_t page_bytes = (int64_t)P * W;
+    x.r = __builtin_amdgcn_readfirstlane(r);
+    x.s0 = __builtin_amdgcn_readfirstlane(s0);
+    x.rows = (__builtin_amdgcn_readfirstlane(s1) - x.s0) * p.group;
+    x.tile = __builtin_amdgcn_readfirstlane(tile);
+    return r >= 0;
+}
 
-    const int j = tile * ROWS + wave * 32 + lo32;
+// How a work-group of four wavefronts brings tiles of 64 tokens into LDS. A wavefront moves 16
+// tokens' rows of K, so that their page is one for the wavefront and its address scalar; of V it
+// moves the same tokens of all features or, where a page holds whole tiles, a quarter of the
+// features of all 64 (rows of 64 neighbouring bytes). A thread's place in the page never changes.
+template <int W>
+struct ManyStage {
+    static constexpr int CH = W / 16;          // units of 16 bytes in a row of K
+    static constexpr int MU = (W + 63) / 64;   // units of K, and of V, that a thread moves
+    static constexpr bool EVEN = W % 64 == 0;  // (as many for every thread)
+    static constexpr int KR = ManyLds<W>::KR, VR = ManyLds<W>::VR;
+    const AttnArgs &p;
+    ManyLds<W> &lds;
+    const int *table;
+    int lane, wave, h, P, vrow, vgroup;
+    bool whole, gone = false;
+    uint32_t zero;
+    v4i kb[MU], vb[MU];
+    int entry = -1;
+    int64_t block = 0;  // of the tile whose K was loaded last
+    float ks = 0.f, vs = 0.f;
+
+    __device__ __forceinline__ ManyStage(const AttnArgs &args, ManyLds<W> &l, int r, int head)
+        : p(args), lds(l) {
+        const CacheAttention &a = p.a;
+        lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        h = head;
+        P = a.c.page_size;
+        table = a.table + (int64_t)(r < a.requests ? r : 0) * a.max_pages;
+        whole = P >= 64;
+        vrow = whole ? threadIdx.x >> 2 : lane;  // and vrow + 64, ...
+        vgroup = whole ? threadIdx.x & 3 : wave;
+        // (keeps the loads below vector loads: scalar ones return out of order)
+        asm("v_mov_b32 %0, 0" : "=v"(zero));
+    }
+    template <typename X>
+    __device__ __forceinline__ X at(const X *x, int64_t i) const {
+        return *reinterpret_cast<const X *>(reinterpret_cast<const char *>(x + i) + zero);
+    }
+    __device__ __forceinline__ int clip(int u) const { return EVEN ? u : min(u, W - 1); }
+    // A tile's table entry is read a tile before its bytes, and looked at only then (a check at
+    // once would wait for it, and as loads come back in order, for every load before).
+    __device__ __forceinline__ void find(int t) {
+        entry = at(table, min(t + 16 * wave, p.cap - 1) >> p.shift);
+    }
+    __device__ __forceinline__ void load_k(int t) {
+        const CacheAttention &a = p.a;
+        const int page = __builtin_amdgcn_readfirstlane(entry);
+        gone = page < 0 || page >= a.c.pages;
+        block = (int64_t)(gone ? 0 : page) * a.c.heads + h;
+        const int8_t *kp =
+            a.c.keys + block * P * W + ((t + 16 * wave) & (P - 1)) * W;
+#pragma unroll
+        for (int i = 0; i < MU; ++i)
+            kb[i] = *reinterpret_cast<const v4i *>(kp + (uint32_t)(clip(lane + 64 * i) * 16));
+        ks = at(a.c.key_scales, block);
+        vs = at(a.c.value_scales, block);
+    }
+    // (of the tile whose K was loaded last)
+    __device__ __forceinline__ void load_v(int t) {
+        const int8_t *vp = p.a.c.values + block * P * W + ((whole ? t : t + 16 * wave) & (P - 1));
+#pragma unroll
+        for (int i = 0; i < MU; ++i)
+            vb[i] = *reinterpret_cast<const v4i *>(
+                vp + (uint32_t)(clip(vrow + 64 * i) * P + (whole ? vgroup * 16 : 0)));
+    }
+    // Half n of 2 MU of K, then of V.
+    __device__ __forceinline__ void put_k(int b, int n) {
+        const int i = n >> 1, half = n & 1, unit = lane + 64 * i;
+        if (EVEN || unit < W) {
+            uint16_t *kp =
+                lds.k[b] + (16 * wave + unit / CH) * KR + unit % CH * 16 + 8 * half;
+            *reinterpret_cast<v8bf *>(kp) = bytes8_to_bf16(kb[i][2 * half], kb[i][2 * half + 1]);
+        }
+    }
+    // a half-wavefront's eight tokens of each 16 are neighbours: 0-3, 8-11 and 4-7, 12-15, as
+    // the rows of the first product fall
+    __device__ __forceinline__ void put_v(int b, int n) {
+        const int i = n >> 1, half = n & 1, row = vrow + 64 * i;
+        if (EVEN || row < W) {
+            uint16_t *vp = lds.v[b] + row * VR + vgroup * 16 + 8 * half;
+            *reinterpret_cast<v8bf *>(vp) = bytes8_to_bf16(vb[i][half], vb[i][half + 2]);
+        }
+    }
+    __device__ __forceinline__ void put_scales(int b) {
+        if (lane == 0) {
+            lds.scales[b][wave] = v4f{ks * p.c, vs, __builtin_amdgcn_logf(vs),
+                                      __builtin_amdgcn_rcpf(vs)};
+            lds.flags[b][wave] = (uint8_t)((gone ? 1 : 0) | (vs >= 0x1p-90f ? 2 : 0));
+        }
+    }
+    __device__ __forceinline__ void pin_k() {
+#pragma unroll
+        for (int i = 0; i < MU; ++i) pin(kb[i]);
+    }
+    __device__ __forceinline__ void pin_v() {
+#pragma unroll
+        for (int i = 0; i < MU; ++i) pin(vb[i]);
+    }
+    __device__ __forceinline__ void stage_k(int b) {
+        pin_k();
+#pragma unroll
+        for (int n = 0; n < 2 * MU; ++n) put_k(b, n);
+        put_scales(b);
+    }
+    __device__ __forceinline__ void stage_v(int b) {
+        pin_v();
+#pragma unroll
+        for (int n = 0; n < 2 * MU; ++n) put_v(b, n);
+    }
+};
+
+template <typename T, int W>
+__device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W> &lds) {
+    constexpr int QP = std::is_same<T, float>::value ? 3 : 1;
+    constexpr int PP = QP;
+    constexpr int ST = W / 16;       // steps of the first product
+    constexpr int DT = W / 32;       // blocks of the second product
+    constexpr int VA = W <= 128 && QP == 1 ? 2 : 1;  // groups of 16 tokens read ahead
+    constexpr int KR = ManyLds<W>::KR, VR = ManyLds<W>::VR;
+    auto &k_lds = lds.k;
+    auto &v_lds = lds.v;
+    auto &scale_lds = lds.scales;
+    auto &flags_lds = lds.flags;
+    auto &most_lds = lds.most;
+
+    const CacheAttention &a = p.a;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lo32 = lane & 31, hi32 = lane >> 5;
+    ManyTile x;
+    if (!many_tile(p, id, x)) return;
+    const int r = x.r, tile = x.tile, s0 = x.s0, rows = x.rows, h = x.h, split = x.split;
+    ManyStage<W> st(p, lds, r, h);
+
+    const int j = tile * kManyRows + wave * 32 + lo32;
     const int tok = j < rows ? s0 + j / p.group : s0;
     const int head = j < rows ? h * p.group + j % p.group : 0;
     // What the first tile needs is asked for at once, before it is known whether any row sees it
     // (a work-group's beginning is a chain of loads that wait for each other).
     const int lo = split * p.chunk;
-    // A wavefront moves 16 tokens' rows of K, so that their page is one for the wavefront and its
-    // address scalar; of V it moves the same tokens of all features or, where a page holds whole
-    // tiles, a quarter of the features of all 64 (rows of 64 neighbouring bytes). A thread's
-    // place in the page never changes.
-    const bool whole = P >= 64;
-    const int vrow = whole ? tid >> 2 : lane;      // and vrow + 64, ...
-    const int vgroup = whole ? tid & 3 : wave;
-    auto unit_of = [&](int i) { return EVEN ? lane + 64 * i : min(lane + 64 * i, W - 1); };
-    auto row_of = [&](int i) { return EVEN ? vrow + 64 * i : min(vrow + 64 * i, W - 1); };
-    uint32_t zero = 0;  // (keeps the loads below vector loads: scalar ones return out of order)
-    asm("v_mov_b32 %0, 0" : "=v"(zero));
-    auto at = [&](const auto *x, int64_t i) {
-        return *reinterpret_cast<decltype(x)>(reinterpret_cast<const char *>(x + i) + zero);
-    };
-    // A tile's table entry is read a tile before its bytes, and looked at only then (a check at
-    // once would wait for it, and as loads come back in order, for every load before).
-    v4i kb[MU], vb[MU];
-    int entry = -1;
-    float ks_next = 0.f, vs_next = 0.f;
-    bool gone = false;
-    auto find = [&](int t0) { entry = at(table, min(t0 + 16 * wave, p.cap - 1) >> p.shift); };
-    auto load = [&](int t0) {
-        const int page = __builtin_amdgcn_readfirstlane(entry);
-        gone = page < 0 || page >= a.c.pages;
-        const int64_t block = (int64_t)(gone ? 0 : page) * a.c.heads + h;
-        const int in = (t0 + 16 * wave) & (P - 1);
-        const int8_t *kp = a.c.keys + block * page_bytes + in * W;
-        const int8_t *vp = a.c.values + block * page_bytes + (whole ? t0 & (P - 1) : in);
-#pragma unroll
-        for (int i = 0; i < MU; ++i)
-            kb[i] = *reinterpret_cast<const v4i *>(kp + (uint32_t)(unit_of(i) * 16));
-#pragma unroll
-        for (int i = 0; i < MU; ++i)
-            vb[i] = *reinterpret_cast<const v4i *>(
-                vp + (uint32_t)(row_of(i) * P + (whole ? vgroup * 16 : 0)));
-        ks_next = at(a.c.key_scales, block);
-        vs_next = at(a.c.value_scales, block);
+    auto load = [&](int t) {
+        st.load_k(t);
+        st.load_v(t);
     };
     auto stage = [&](int b) {
-#pragma unroll
-        for (int i = 0; i < MU; ++i) {
-            pin(kb[i]);
-            pin(vb[i]);
-            if (EVEN || lane + 64 * i < W) {
-                const int unit = lane + 64 * i;
-                uint16_t *kp = k_lds[b] + (16 * wave + unit / CH) * KR + unit % CH * 16;
-                *reinterpret_cast<v8bf *>(kp) = bytes8_to_bf16(kb[i][0], kb[i][1]);
-                *reinterpret_cast<v8bf *>(kp + 8) = bytes8_to_bf16(kb[i][2], kb[i][3]);
-            }
-            if (EVEN || vrow + 64 * i < W) {
-                // a half-wavefront's eight tokens of each 16 are neighbours: 0-3, 8-11 and
-                // 4-7, 12-15, as the rows of the first product fall
-                uint16_t *vp = v_lds[b] + (vrow + 64 * i) * VR + vgroup * 16;
-                *reinterpret_cast<v8bf *>(vp) = bytes8_to_bf16(vb[i][0], vb[i][2]);
-                *reinterpret_cast<v8bf *>(vp + 8) = bytes8_to_bf16(vb[i][1], vb[i][3]);
-            }
-        }
-        if (lane == 0) {
-            scale_lds[b][wave] = v4f{ks_next * p.c, vs_next, __builtin_amdgcn_logf(vs_next),
-                                     __builtin_amdgcn_rcpf(vs_next)};
-            flags_lds[b][wave] = (uint8_t)((gone ? 1 : 0) | (vs_next >= 0x1p-90f ? 2 : 0));
-        }
+        st.stage_k(b);
+        st.stage_v(b);
     };
 
-    find(lo);
+    st.find(lo);
     const int position = j < rows && r < a.requests ? a.positions[tok] : -1;
     Frag q[ST][QP];
     {
@@ -781,7 +839,7 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
         }
     }
     load(lo);
-    find(lo + 64);
+    st.find(lo + 64);
     const int limit = keys_of(position, p.cap);
     // the work-group's longest row, this wavefront's and its shortest
     int most = limit, least = j < rows ? limit : INT32_MAX;
@@ -796,7 +854,7 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
     stage(0);
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) most = max(most, most_lds[w]);
+    for (int w = 0; w < 4; ++w) most = max(most, most_lds[w]);
     most = __builtin_amdgcn_readfirstlane(most);
     const int hi = split == p.splits - 1 ? most : min(most, lo + p.chunk);
     if (split > 0 && lo >= most) return;
@@ -812,7 +870,7 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
     for (int t0 = lo; t0 < hi; t0 += 64, buf ^= 1) {
         const bool more = t0 + 64 < hi;
         if (more) load(t0 + 64);
-        find(t0 + 128);  // (always: a value that only a branch loads is copied, and waited for)
+        st.find(t0 + 128);  // (always: a value that only a branch loads is copied, and waited for)
         if (t0 < mine) {  // (else none of this wavefront's rows sees the tile)
         const uint32_t flags = __builtin_amdgcn_readfirstlane(
             *reinterpret_cast<const uint32_t *>(flags_lds[buf]));
@@ -826,24 +884,24 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W, 
         const v16f none = {};
         const uint16_t *kp = k_lds[buf] + lo32 * KR + 8 * hi32;
         v8bf kf[KA][2];
-        auto read_k = [&](int st) {
+        auto read_k = [&](int i) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
-                kf[st % KA][b] = *reinterpret_cast<const v8bf *>(kp + 32 * b * KR + 16 * st);
+                kf[i % KA][b] = *reinterpret_cast<const v8bf *>(kp + 32 * b * KR + 16 * i);
         };
 #pragma unroll
-        for (int st = 0; st < KA; ++st) read_k(st);
+        for (int i = 0; i < KA; ++i) read_k(i);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int st = 0; st < ST; ++st) {
+        for (int i = 0; i < ST; ++i) {
 #pragma unroll
             for (int n = QP - 1; n >= 0; --n)
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
                     s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                        kf[st % KA][b], q[st][n].v, st == 0 && n == QP - 1 ? none : s[b], 0, 0,
+                        kf[i % KA][b], q[i][n].v, i == 0 && n == QP - 1 ? none : s[b], 0, 0,
                         0);
-            if (st + KA < ST) read_k(st + KA);
+            if (i + KA < ST) read_k(i + KA);
         }
         const uint16_t *vp = v_lds[buf] + lo32 * VR + 8 * hi32;
         v8bf vf[VA][DT];
@@ -1125,29 +1183,29 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W <= 1
 attention_share_kernel(AttnArgs p) {
     __shared__ FewLds<W> lds;
     __shared__ ShareLds scan;
-    few_shares<T, W, 4>(p, lds, scan);
+    few_shares<T, W>(p, lds, scan);
 }
 
 template <typename T, int W>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W <= 128 ? 2 : 1)))
 attention_few_kernel(AttnArgs p) {
     __shared__ FewLds<W> lds;
-    few_rows<T, W, 4>(p, blockIdx.x, lds);
+    few_rows<T, W>(p, blockIdx.x, lds);
 }
 
 // Both in one launch, each request's rows where they belong: the few-rows work-groups first.
-template <typename T, int W, int NW>
-__global__ void __launch_bounds__(64 * NW)
+template <typename T, int W>
+__global__ void __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 || W > 128 ? 1 : 2)))
 attention_both_kernel(AttnArgs p, int few) {
     __shared__ union {
-        FewLds<W, NW> few;
-        ManyLds<W, NW> many;
+        FewLds<W> few;
+        ManyLds<W> many;
     } lds;
     if ((int)blockIdx.x < few) {
-        few_rows<T, W, NW>(p, blockIdx.x, lds.few);
+        few_rows<T, W>(p, blockIdx.x, lds.few);
     } else {
-        many_rows<T, W, NW>(p, blockIdx.x - few, lds.many);
+        many_rows<T, W>(p, blockIdx.x - few, lds.many);
     }
 }
 
@@ -1163,10 +1221,9 @@ int launch_width(hipStream_t stream, const AttnArgs &p) {
         return launch_status("attention_share_join_kernel launch");
     }
     const int few = p.splits * p.a.c.heads * (p.a.requests + 1);
-    constexpr int NW = many_waves(W, sizeof(T));
     if (p.both)
-        MIGEMM_LAUNCH((attention_both_kernel<T, W, NW>),
-                      dim3((unsigned)(few + p.units * p.splits * p.a.c.heads)), dim3(64 * NW),
+        MIGEMM_LAUNCH((attention_both_kernel<T, W>),
+                      dim3((unsigned)(few + p.units * p.splits * p.a.c.heads)), dim3(256),
                       0, stream, p, few);
     else
         MIGEMM_LAUNCH((attention_few_kernel<T, W>), dim3((unsigned)few), dim3(256), 0, stream,

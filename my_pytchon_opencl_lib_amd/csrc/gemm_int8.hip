@@ -31,10 +31,12 @@ __device__ __forceinline__ void put(T *c, int sum, float sa, float sb, float bia
     *c = from_f32<T>((float)sum * sa * sb + bias);
 }
 
+constexpr int BK = 32;  // words of four values of K in a stage
+
 // This lane's 16 bytes of each load of the tail tile kt, zero at k >= K. K is a multiple of 16
 // bytes, so each is wholly inside or outside; all loads are made (outside: at the row's start)
 // and fly together.
-template <int BK, typename Op>
+template <typename Op>
 __device__ __forceinline__ void fetch_tail(const Op &op, typename Op::Tail &t, int kt, int K,
                                            int64_t ld) {
     const char *tb = op.tile_base(kt, ld);
@@ -53,7 +55,7 @@ __device__ __forceinline__ void fetch_tail(const Op &op, typename Op::Tail &t, i
 // 16 bytes a lane is one operand of v_mfma_i32_32x32x32_i8. The order of waits, barrier and
 // loads is gemm_direct_kernel's: a tile's loads run D tiles ahead, and every fragment read of
 // a stage is issued before the barrier that frees it.
-template <typename T, int BM, int BN, int WM, int WN, int S, int D, int OCC, int BK>
+template <typename T, int BM, int BN, int WM, int WN, int S, int D, int OCC>
 __global__ void __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(OCC)))
 gemm_int8_kernel(Int8Args p) {
     constexpr int NT = WM * WN * 64;
@@ -136,8 +138,8 @@ gemm_int8_kernel(Int8Args p) {
     typename OpA::Tail ta;
     typename OpB::Tail tb;
     if (EARLY && kf < kt1) {
-        fetch_tail<BK>(opa, ta, kf, K, p.t.lda);
-        fetch_tail<BK>(opb, tb, kf, K, p.t.ldb);
+        fetch_tail(opa, ta, kf, K, p.t.lda);
+        fetch_tail(opb, tb, kf, K, p.t.ldb);
     }
 
     int kt = kt0;
@@ -165,8 +167,8 @@ gemm_int8_kernel(Int8Args p) {
     wait_vmcnt<0>();
     if (kt < kt1) {  // the tail tile: k >= K zero in both operands
         if (!EARLY) {
-            fetch_tail<BK>(opa, ta, kt, K, p.t.lda);
-            fetch_tail<BK>(opb, tb, kt, K, p.t.ldb);
+            fetch_tail(opa, ta, kt, K, p.t.lda);
+            fetch_tail(opb, tb, kt, K, p.t.ldb);
         }
         __syncthreads();
         opa.tail_put(ta, lds_a, lane);
@@ -246,7 +248,7 @@ join_int8_kernel(const int32_t *partial, int splits, int M, int N, int64_t plane
             bias != nullptr ? bias[col + e] : 0.f);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int S, int D, int OCC, int BK = 32>
+template <typename T, int BM, int BN, int WM, int WN, int S, int D, int OCC>
 int launch_tiles(hipStream_t stream, const Int8Product &p, int splits) {
     Int8Args a{};
     TiledArgs &t = a.t;
@@ -283,7 +285,7 @@ int launch_tiles(hipStream_t stream, const Int8Product &p, int splits) {
             workspace(stream, (size_t)t.splits * plane * sizeof(int32_t), &rc, 0));
         if (a.partial == nullptr) return rc;
     }
-    MIGEMM_LAUNCH((gemm_int8_kernel<T, BM, BN, WM, WN, S, D, OCC, BK>), dim3(t.total),
+    MIGEMM_LAUNCH((gemm_int8_kernel<T, BM, BN, WM, WN, S, D, OCC>), dim3(t.total),
                   dim3(WM * WN * 64), 0, stream, a);
     if (const int rc = launch_status("gemm_int8_kernel launch")) return rc;
     if (t.splits > 1) {

@@ -477,15 +477,14 @@ int launch_cache_attention(hipStream_t stream, const CacheAttention &a) {
         return a.type == MIGEMM_FLOAT32 ? launch_attention_f32(stream, p)
                                         : launch_attention_bf16(stream, p);
     }
-    const int tile = 32 * many_waves(a.c.width, type_size(a.type));
-    const int64_t units = (int64_t)a.tokens * p.group / tile + a.requests + 1;
+    const int64_t units = (int64_t)a.tokens * p.group / kManyRows + a.requests + 1;
     p.units = (int)units;
     // Contexts are cut in ranges (of whole rounds of a few-rows work-group, 256 tokens) where the
     // requests, tiles and kv heads alone make too few work-groups: single tokens until there are
     // about 1024 (they wait for memory), prompts only until there is one for each CU (their
     // partial results, four bytes a feature and row and range, cost more than an uneven end).
     const int64_t base =
-        (a.requests + (many ? (int64_t)a.tokens * p.group / tile : 0)) * a.c.heads;
+        (a.requests + (many ? (int64_t)a.tokens * p.group / kManyRows : 0)) * a.c.heads;
     const int64_t want = many ? (base < 256 ? 256 / base : 1) : (1024 + base - 1) / base;
     int64_t chunk = (length + want - 1) / want;
     chunk = (chunk + 255) / 256 * 256;
