@@ -438,7 +438,7 @@ int migemm_matmul_int8(void *stream, const int8_t *A, int64_t lda, const float *
 
 /* Y = the product above of the quantised rows of X [M, cols] (X and Y of `type`) and
  * W [N, K], K = cols rounded up to 16 (as migemm_quantize_rows leaves a weight [N, cols]).
- * One launch for a few rows; otherwise the quantised rows go to the stream's workspace. */
+ * One launch for one or two rows; otherwise the quantised rows go to the stream's workspace. */
 int migemm_linear_int8(void *stream, const void *X, int type, int64_t ldx, const int8_t *W,
                        int64_t ldw, const float *w_scales, const float *bias, void *Y,
                        int64_t ldy, int M, int N, int cols);
@@ -460,9 +460,9 @@ int migemm_linear_int8(void *stream, const void *X, int type, int64_t ldx, const
  * slots[t] and positions[t] are token t's, -1 where its request is not admitted or t is past
  * the step's tokens. new_lengths = lengths + counts where admitted, else lengths; *new_free =
  * the pages left. Negative lengths and counts are read as 0, a page number that is negative
- * or has no int32 slot gives slot and position -1. Only table, slots, positions, starts, new_lengths and new_free are
- * written: the same call again gives the same results, until the caller takes new_lengths and
- * new_free as its lengths and free_count. */
+ * or has no int32 slot gives slot and position -1. Only table, slots, positions, starts,
+ * new_lengths and new_free are written: the same call again gives the same results, until the
+ * caller takes new_lengths and new_free as its lengths and free_count. */
 int migemm_cache_tables(void *stream, const int *lengths, const int *counts, int requests,
                         int *table, int max_pages, int page_size, const int *free_pages,
                         const int *free_count, int free_capacity, int *slots,
@@ -510,8 +510,8 @@ int migemm_cache_read(void *stream, const int8_t *keys, const int8_t *values,
  * cached tokens whose table entry is outside the pool are left out.
  * max_count (most tokens of one request, 0: unknown) and max_length (longest request after
  * the step, 0: unknown) shape the launch; results are right whatever they say.
- * Contexts are cut in ranges where the requests alone do not fill the GPU; their partial
- * results go to the stream's workspace and are joined in order: the same bits every time. */
+ * Contexts are cut, in ranges or in even shares of all of them, where the requests alone do
+ * not fill the GPU or fill it unevenly; their partial results go to the stream's workspace and are joined in order: the same bits every time. */
 int migemm_cache_attention(void *stream, const void *Q, int type, int64_t ldq,
                            const int8_t *keys, const int8_t *values, const float *key_scales,
                            const float *value_scales, int pages, int kv_heads, int head_dim,

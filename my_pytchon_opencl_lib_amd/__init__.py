@@ -2,8 +2,9 @@
 
 The compute lives in libmigemm.so (hand-written HIP kernels behind the C ABI of
 include/migemm.h); this package is the Python host side: ctypes bindings (_native), the
-operator dispatcher mirroring the reference's NnClGlob (nncl_glob) and the gradient nodes
-(autograd).
+operator dispatcher mirroring the reference's NnClGlob (nncl_glob), the gradient nodes
+(autograd), and for serving in 8 bits the layers (layers.LinearInt8) and the paged cache of keys
+and values (cache.Int8Cache).
 """
 from . import _native
 from .nncl_glob import NnClGlob, ShapeError

@@ -30,7 +30,8 @@ __device__ __forceinline__ int scan_block(int v, int *part, F op) {
 // counts for the tokens' places, a scan of the pages asked for their pages; 8 bytes a request
 // from L2) and keeps, in LDS, what the requests that own tokens of its window of 1024 tokens
 // need; then one thread a token. Bound by latency: a step of a few hundred requests is one
-// round of loads, two scans and one more dependent load. The token at a new page's first
+// round of loads, two scans and one more dependent load (32 requests, a token each: 4.9 us; 512
+// requests with 180000 tokens: 7.5 us). The token at a new page's first
 // place writes that page to the table, so each entry has one writer; tokens in new pages take
 // them from the free list and never read an entry that another work-group may be writing.
 // GROW false: slots of the pages that the table already names, nothing is allocated.
@@ -176,7 +177,8 @@ struct AppendArgs {
 // values; what is beyond is read again). Values are transposed through LDS so that a page's rows
 // are written in whole words. Bound by memory for prompts; for single tokens by latency: two
 // loads that wait for each other (slots; tokens and scale). A page is rounded anew only where
-// its scale grew.
+// its scale grew. 64 tokens, 8 heads of 128, pages of 64: 6.9 us; 12500 float32 tokens (128 MB):
+// 23 us, 5.6 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4)))
 cache_append_kernel(AppendArgs a) {
@@ -360,7 +362,7 @@ cache_append_kernel(AppendArgs a) {
 // 64 tokens of one head, of K or of V: a thread takes four tokens' eight features at a time.
 // Values are read along a page's tokens, four neighbouring slots a load (wherever they begin),
 // and turned in registers. Two loads that wait for each other (slots; bytes and scales), then
-// 16 bytes or more a store: bound by memory.
+// 16 bytes or more a store: bound by memory (12500 float32 tokens, 128 MB: 22 us, 5.8 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256)
 cache_read_kernel(Cache8 c, const int *slots, int tokens, T *K, T *V, int shift) {

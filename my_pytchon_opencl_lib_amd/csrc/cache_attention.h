@@ -128,9 +128,8 @@ __device__ __forceinline__ bool row_is_whole(const AttnArgs &p, int limit) {
 
 // ------------------------------------------------------------------------- few rows
 // Up to 16 rows (queries x heads that share a kv head): decoding. Bound by reading the cache
-// once, if little enough is done for each byte: the vector units have about 40 instructions'
-// time for each 64 bytes of the cache. A work-group takes one request, kv head and range of
-// keys; its four wavefronts take tiles of 64 tokens in turn, straight from memory to registers
+// once, if little enough is done for each byte. A work-group takes one request, kv head and
+// range of keys; its four wavefronts take tiles of 64 tokens in turn, straight from memory to registers
 // (K of the next tile flies from the first product on, V from the second).
 //
 // The first product runs on the int8 matrix cores, so K needs no conversion at all: a row of q
@@ -147,8 +146,8 @@ struct FewLds {
 };
 
 // 16 rows from row0 on of request r (tokens from s0 on) and kv head h, over its keys lo .. end - 1
-// (as far as a row sees them). part: kWhole (all its keys: the result), a place for a part, or -2 - range where rows go by
-// row_is_whole.
+// (as far as a row sees them). part: kWhole (all its keys: the result), a place for a part, or
+// -2 - range where rows go by row_is_whole.
 constexpr int kWhole = -1;
 
 template <typename T, int W>
@@ -498,12 +497,14 @@ __device__ __forceinline__ void few_rows(const AttnArgs &p, int id, FewLds<W> &l
     const int lo = split * p.chunk;
     for (int row0 = 0; row0 < rows; row0 += 16)
         few_segment<T, W>(p, r, s0, rows, h, row0, lo,
-                              split == p.splits - 1 ? p.cap : lo + p.chunk, -2 - split, lds);
+                          split == p.splits - 1 ? p.cap : lo + p.chunk, -2 - split, lds);
 }
 
 // Single tokens in even shares: the tiles (of 64 tokens) of all requests and kv heads in one
 // line, cut into p.shares equal pieces, one a work-group, all of which run at once; a decoding
 // batch's contexts differ, and work-groups of whole ranges would leave CUs idle at the end.
+// 32 requests of 4096 tokens, 8 kv heads of 128: 38 us (172 MB, 4.6 TB/s; 51 in ranges), 2 of
+// 131072: 70 us (5.9 TB/s; 87 in ranges).
 // A unit is one request, kv head and 16 rows (its rows beyond 16 are further units, and a unit
 // without keys has one tile, which writes its zeros). Cuts within two tiles of a unit's end
 // are moved there. A unit that is cut is joined afterwards (attention_share_join_kernel, which
@@ -605,20 +606,26 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W> &lds,
         const bool ends = last == unit;
         const int s0 = __builtin_amdgcn_readfirstlane(scan.token[r]);
         const int rows = __builtin_amdgcn_readfirstlane(scan.rows[r]);
-        few_segment<T, W>(p, r, s0, rows, h, block * 16, tile * 64,
-                              last * 64,
-                              tile == 0 && ends ? kWhole : 2 * w + (tile == 0 ? 1 : 0), lds);
+        few_segment<T, W>(p, r, s0, rows, h, block * 16, tile * 64, last * 64,
+                          tile == 0 && ends ? kWhole : 2 * w + (tile == 0 ? 1 : 0), lds);
         at += last - tile;
     }
 }
 
 // ------------------------------------------------------------------------ many rows
-// Prompts: 32 rows (queries x heads that share a kv head) a wavefront, 4 or 8 wavefronts, on
+// Prompts: 32 rows (queries x heads that share a kv head) a wavefront, four wavefronts, on
 // v_mfma_f32_32x32x16_bf16. Tiles of 64 tokens are read as bytes, turned into bf16 once for
 // the work-group and shared in LDS (two buffers: the next tile's bytes fly during a tile's
-// work, one barrier a tile). Bound by the matrix cores and by the exponentials and
-// conversions beside them. LDS rows are padded by 16 bytes: the 16 lanes of a read phase fall
+// work, one barrier a tile). LDS rows are padded by 16 bytes: the 16 lanes of a read phase fall
 // on different banks.
+//
+// 4 x 4096 tokens, 32 heads on 8 of 128: 646 to 660 us, 0.85 PFLOP/s; 16 x 1024: 251 us. Of a
+// wavefront's 2900 cycles a tile the matrix cores have 1024, the vector instructions (softmax
+// 110, maxima 35, conversions 96, exponentials at a quarter of the rate) about 1350, and the
+// LDS reads, a kilobyte an instruction, as long as the matrix cores have: each has a half of
+// the time, and the two work-groups of a CU overlap them in part. Tried and slower: eight
+// wavefronts, two on a SIMD a phase apart (690); 64 rows a wavefront, which halves the LDS
+// reads, with a SIMD to itself (1420: the registers do not hold it).
 template <int W>
 struct ManyLds {
     static constexpr int KR = W + 8, VR = 64 + 8;  // LDS rows, in bf16
@@ -631,7 +638,8 @@ struct ManyLds {
     int most[4];
 };
 
-// A work-group's share: request r's rows from tile * kManyRows on, of kv head h, and a range of keys.
+// A work-group's share: request r's rows from tile * kManyRows on, of kv head h, and a range of
+// keys.
 struct ManyTile {
     int r, tile, s0, rows, h, split;
 };
