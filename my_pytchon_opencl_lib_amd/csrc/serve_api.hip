@@ -1,5 +1,6 @@
 // C ABI of the 8-bit serving operators (include/migemm.h, 6): argument validation before any
 // HIP call, and the shape of the attention's launches.
+#include <algorithm>
 #include <initializer_list>
 
 #include "cache_attention.h"
@@ -454,16 +455,20 @@ int launch_cache_attention(hipStream_t stream, const CacheAttention &a) {
     const int64_t count = a.max_count > 0 && a.max_count < a.tokens ? a.max_count : a.tokens;
     const int64_t length =
         a.max_length > 0 && a.max_length < p.cap ? a.max_length : p.cap;
-    // Requests of at most 16 rows are computed one way, others another; where one request may
-    // bring more, one launch holds both ways.
-    const bool many = count * p.group > kFewRows;
-    p.both = many;
+    const int64_t count_rows = count * p.group;
     // Single tokens in even shares, two work-groups a CU (one where a head's registers allow no
     // more): int32 holds the number of tiles, and their scan is kept on the chip. Short contexts
     // in ranges, without the scan (8 requests of 200 tokens: 11.4 us, 15.7 in shares).
     const int64_t tiles = ((int64_t)a.tokens * p.group / 16 + a.requests + 1) *
                           ((p.cap + 63) / 64) * a.c.heads;
-    if (!many && length > 512 && a.requests <= kShareRequests && tiles < (int64_t)1 << 30) {
+    const bool even = length > 512 && a.requests <= kShareRequests && tiles < (int64_t)1 << 30;
+    // Requests of at most 16 rows are computed one way, others another; where one request may
+    // bring more, one launch holds both ways. Up to 32 float32 rows go the first way twice, in
+    // shares (32 requests of 4096 tokens, 20 rows each, 8 kv heads of 128: 93 us, 183 the other
+    // way, which has six products for one; 48 rows: 154 and 194, 64: 197 and 193).
+    const bool many = count_rows > (even && a.type == MIGEMM_FLOAT32 ? 2 * kFewRows : kFewRows);
+    p.both = many;
+    if (!many && even) {
         p.shares = a.c.width <= 128 ? 512 : 256;
         MIGEMM_TRY(check_grid("cache_attention", (int64_t)a.requests * a.heads, 256));
         const size_t parts = (size_t)p.shares * 2 * 16;
@@ -481,11 +486,18 @@ int launch_cache_attention(hipStream_t stream, const CacheAttention &a) {
     p.units = (int)units;
     // Contexts are cut in ranges (of whole rounds of a few-rows work-group, 256 tokens) where the
     // requests, tiles and kv heads alone make too few work-groups: single tokens until there are
-    // about 1024 (they wait for memory), prompts only until there is one for each CU (their
-    // partial results, four bytes a feature and row and range, cost more than an uneven end).
+    // about 1024 (they wait for memory), more rows until there is one for each CU, or two where
+    // the registers hold two (bfloat16, heads up to 128) and the rows are fewer than the keys
+    // (their partial results, four bytes a feature and row and range, cost more otherwise). 32
+    // requests of 4096 tokens, 20 rows each, 8 kv heads of 128: 115 us with one, 70 with two; 8
+    // of 8192, 512 rows: 221 and 198; float32 with two: 375 and 411.
     const int64_t base =
-        (a.requests + (many ? (int64_t)a.tokens * p.group / kManyRows : 0)) * a.c.heads;
-    const int64_t want = many ? (base < 256 ? 256 / base : 1) : (1024 + base - 1) / base;
+        std::max<int64_t>(a.requests, many ? (int64_t)a.tokens * p.group / kManyRows : 0) *
+        a.c.heads;
+    const bool two = a.type == MIGEMM_BFLOAT16 && a.c.width <= 128 &&
+                     (int64_t)a.tokens * p.group <= a.requests * length;
+    const int64_t fill = two ? 512 : 256;
+    const int64_t want = many ? (base < fill ? fill / base : 1) : (1024 + base - 1) / base;
     int64_t chunk = (length + want - 1) / want;
     chunk = (chunk + 255) / 256 * 256;
     p.chunk = (int)chunk;

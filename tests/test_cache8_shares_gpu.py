@@ -56,7 +56,18 @@ def test_shares_of_contexts_of_any_length(nncl, heads, kv, dim, page, requests, 
 def test_shares_of_several_tokens_and_wrong_hints(nncl, heads, kv, dim, page, lengths, counts,
                                                   kind):
     run(nncl, heads, kv, dim, page, lengths, counts, kind,
-        [(1, max(lengths)), (1, 100000), (2, 513)])
+        [(1, max(lengths)), (1, 100000), (2, 513), (max(counts), max(lengths))])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("heads,kv,dim,page,lengths,counts", [
+    (4, 1, 128, 64, [2100, 64, 1500], [5, 8, 6]),         # 20 to 32 rows: float32 in shares
+    (8, 2, 64, 16, [1300, 900], [8, 1]),
+    (2, 1, 256, 32, [1100, 30, 600], [12, 16, 9]),
+    (4, 1, 96, 64, [3000, 1200], [30, 100]),              # more rows: two ranges a CU
+    (8, 1, 128, 32, [1024], [64])])
+def test_few_queries_over_long_contexts(nncl, heads, kv, dim, page, lengths, counts, kind):
+    run(nncl, heads, kv, dim, page, lengths, counts, kind, [(max(counts), max(lengths)), (0, 0)])
 
 
 @pytest.mark.parametrize("page", [16, 64])
