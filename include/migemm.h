@@ -438,7 +438,7 @@ int migemm_matmul_int8(void *stream, const int8_t *A, int64_t lda, const float *
 
 /* Y = the product above of the quantised rows of X [M, cols] (X and Y of `type`) and
  * W [N, K], K = cols rounded up to 16 (as migemm_quantize_rows leaves a weight [N, cols]).
- * One launch for one or two rows; otherwise the quantised rows go to the stream's workspace. */
+ * One launch for up to three rows; otherwise the quantised rows go to the stream's workspace. */
 int migemm_linear_int8(void *stream, const void *X, int type, int64_t ldx, const int8_t *W,
                        int64_t ldw, const float *w_scales, const float *bias, void *Y,
                        int64_t ldy, int M, int N, int cols);

@@ -10,7 +10,7 @@
 //                        cores (and the loads that feed them) for large M
 //   rows_int8_kernel     few rows: bound by streaming B once; a work-group takes 16 rows of B,
 //                        its wavefronts split K, operands go straight to registers
-//   rows_int8_kernel with x in float: the same for one or two rows, x quantised by every
+//   rows_int8_kernel with x in float: the same for up to three rows, x quantised by every
 //                        work-group (x is small and in L2): one launch instead of two
 #include "gemm_direct.h"
 #include "int8_common.h"
@@ -311,7 +311,7 @@ int launch_tiles(hipStream_t stream, const Int8Product &p, int splits) {
 // (45 MB) 9.5 us, 4.7 TB/s; 24 x 2048 to 4096 4.1 to 4.9 us.
 // X != void: A is not given but x [M, K] in X, and each work-group quantises it into LDS
 // itself (its first loads of B are on their way meanwhile).
-constexpr int kKeep = 2;  // steps of x (NW * 512 values each) that stay in registers
+constexpr int kKeep = 3;  // steps of x (NW * 512 values each) that stay in registers
 struct RowsArgs {
     const int8_t *A, *B;
     const void *X;
@@ -506,10 +506,14 @@ constexpr TileChoice kTiles[] = {
 
 template <typename T>
 int launch_product(hipStream_t stream, const Int8Product &p) {
-    // Few rows over few columns: 16 columns a work-group (24 x 4096 x 2048: 4.2 us, tiles 6.8);
-    // over many the tiles stream B as well and read A once for 64 columns (16 x 11008 x 4096:
-    // 11.1 us, 14.3 by rows).
-    if (p.M <= 32 && (int64_t)p.N * p.K <= (int64_t)12 << 20) {
+    // Few rows: 16 columns a work-group (24 x 4096 x 2048: 4.2 us, tiles 6.8; with the quantising
+    // before it 16 x 4096 x 4096 10.2, 12.5; 16 x 8192 x 8192 23.2, 29.7), where that makes
+    // enough work-groups (8 x 1024 x 16384: 18.4, 15.6 in k ranges of tiles) and not so many that
+    // A, read by each, costs more than it saves: over many columns the tiles stream B as well
+    // and read A once for 64 columns (16 x 11008 x 4096: 18.4, 17.6; 16 x 32000 x 4096 35.5,
+    // 25.9; 24 x 4096 x 11008 22.4, 20.5).
+    if ((p.M <= 32 && (int64_t)p.N * p.K <= (int64_t)12 << 20) ||
+        (p.M <= 16 && p.N >= 2048 && p.N <= 8192)) {
         const RowsArgs a = rows_args(p);
         return p.M <= 16 ? launch_rows<T, void, 1, 8>(stream, a)
                          : launch_rows<T, void, 2, 8>(stream, a);
@@ -541,9 +545,10 @@ int launch_product(hipStream_t stream, const Int8Product &p) {
     return launch_tiles<T, 64, 64, 2, 2, 3, 3, 3>(stream, p, splits < most ? splits : most);
 }
 
-// One or two rows that a work-group of 8 wavefronts holds in its registers: quantised by each
+// Up to three rows that a work-group of 8 wavefronts holds in its registers: quantised by each
 // (1 x 4096 to 11008, weights from HBM: 10.4 us, against 3 and 10.5 by two launches; 2 x 4096
-// to 4096: 5.9, and 3 and 5.0).
+// to 4096: 5.9, and 3 and 5.0; 3 x 4096 to 11008 13.1 and 17.0 together, 1 x 11008 to 4096 12.9
+// and 17.1). Room for a fourth step costs a wavefront a SIMD (1 x 4096 to 11008: 12.5).
 bool fused_rows(int M, int K) { return M <= kKeep && M * ((K + 4095) / 4096) <= kKeep; }
 }  // namespace
 

@@ -573,7 +573,7 @@ class NnClGlob:
     def LinearInt8(self, x, weight, scales, bias=None):
         """y[..., N] = x[..., K] @ W^T (+ bias[N], float32) with W [N, K] as QuantizeRows left
         it (weight int8 [N, K rounded up to 16], scales [N]); the rows of x are quantised on
-        the way. y has the type of x. One launch for one or two rows."""
+        the way. y has the type of x. One launch for up to three rows."""
         code = _check_rows("x", x)
         _check_typed("weight", weight, torch.int8, dim=2)
         n, kp = weight.shape

@@ -125,7 +125,8 @@ def int8(seed, *shape):
 SIZES = [(1, 1, 16), (1, 17, 48), (2, 16, 128), (5, 100, 144), (16, 257, 4112), (17, 33, 1024),
          (32, 1000, 528), (33, 15, 272), (64, 300, 2064), (65, 64, 16), (65, 70, 4112),
          (100, 1, 8208), (130, 257, 144), (300, 300, 1040), (1000, 3000, 784), (257, 2048, 128),
-         (1500, 1100, 2048), (4000, 3100, 144), (4097, 3333, 640)]
+         (1500, 1100, 2048), (4000, 3100, 144), (4097, 3333, 640), (16, 2048, 8208),
+         (9, 8192, 2064), (3, 8193, 1600), (17, 4096, 4112)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -142,7 +143,8 @@ def test_product(nncl, m, n, k, kind):
         check(full, *product64(a, sa, b, sb, bias))
         assert torch.equal(got, full.to(TYPES[kind]))
     plan = _native.last_plan()
-    assert plan.startswith("int8-rows" if m <= 32 and n * k <= 12 << 20 else "int8-tiles"), plan
+    rows = (m <= 32 and n * k <= 12 << 20) or (m <= 16 and 2048 <= n <= 8192)
+    assert plan.startswith("int8-rows" if rows else "int8-tiles"), plan
 
 
 def test_product_takes_strided_rows_and_keeps_to_its_output(nncl):
@@ -181,7 +183,8 @@ def test_product_sums_are_exact_at_the_longest_k(nncl, m):
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 11008, 4096), (1, 5, 30001), (2, 100, 33), (3, 1000, 777),
                                    (4, 64, 8192), (4, 50, 8209), (5, 64, 777), (24, 500, 100),
-                                   (70, 130, 777), (600, 520, 1000)])
+                                   (70, 130, 777), (600, 520, 1000), (3, 600, 4096), (1, 300, 12000),
+                                   (2, 200, 4100), (9, 2050, 6000)])
 def test_layer_is_the_product_of_its_rows(nncl, m, n, k, kind):
     """One launch or two, quantised by every work-group or once: the same bits as the two
     operators called one after the other, and within the rule's distance of x W^T: half a step
@@ -193,7 +196,7 @@ def test_layer_is_the_product_of_its_rows(nncl, m, n, k, kind):
     w8, ws = nncl.QuantizeRows(w)
     y = nncl.LinearInt8(x, w8, ws, bias)
     plan = _native.last_plan()
-    assert plan.startswith("int8-rows-fused") == (m * -(-k // 4096) <= 2)
+    assert plan.startswith("int8-rows-fused") == (m * -(-k // 4096) <= 3)
     x8, xs = nncl.QuantizeRows(x)
     assert torch.equal(y, nncl.MatmulInt8(x8, xs, w8, ws, bias, dtype=x.dtype))
     assert y.dtype == x.dtype
