@@ -126,7 +126,8 @@ SIZES = [(1, 1, 16), (1, 17, 48), (2, 16, 128), (5, 100, 144), (16, 257, 4112), 
          (32, 1000, 528), (33, 15, 272), (64, 300, 2064), (65, 64, 16), (65, 70, 4112),
          (100, 1, 8208), (130, 257, 144), (300, 300, 1040), (1000, 3000, 784), (257, 2048, 128),
          (1500, 1100, 2048), (4000, 3100, 144), (4097, 3333, 640), (16, 2048, 8208),
-         (9, 8192, 2064), (3, 8193, 1600), (17, 4096, 4112)]
+         (9, 8192, 2064), (3, 8193, 1600), (17, 4096, 4112),
+         (128, 4090, 4112)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
