@@ -10,7 +10,9 @@ table that NnClGlob.CacheTables fills on the GPU from a list of free pages.
 import torch
 
 from . import _native
-from .nncl_glob import ShapeError, _require
+from .nncl_glob import ShapeError, _check_typed, _require
+
+_INT8, _FLOAT = torch.int8, torch.float32
 
 
 def width(headDim):
@@ -41,10 +43,37 @@ class Int8Cache:
         self.keyScales = torch.zeros((self.pages, self.kvHeads), dtype=torch.float32,
                                      device=device)
         self.valueScales = torch.zeros_like(self.keyScales)
-        # what the C entries take
-        self.pointers = tuple(t.data_ptr() for t in (self.keys, self.values, self.keyScales,
-                                                     self.valueScales))
-        self.sizes = (self.pages, self.kvHeads, self.headDim, self.pageSize)
+
+    @property
+    def pointers(self):
+        """Where the four tensors are now. Nothing is remembered: a copy of a cache (deepcopy,
+        pickle, torch.save) has memory of its own, and a tensor may be replaced by another."""
+        return (self.keys.data_ptr(), self.values.data_ptr(), self.keyScales.data_ptr(),
+                self.valueScales.data_ptr())
+
+    @property
+    def sizes(self):
+        return self.pages, self.kvHeads, self.headDim, self.pageSize
+
+    def operands(self):
+        """(the four tensors, their addresses and the sizes as the C entries take them), after a
+        look at the tensors: types, shapes and layout may have been changed since (the devices
+        are looked at with those of a call's other operands)."""
+        k, v, ks, vs = held = self.keys, self.values, self.keyScales, self.valueScales
+        pages, heads, dim, page = sizes = self.sizes
+        w = width(dim)
+        flat = (pages, heads)
+        if not (k.dtype is _INT8 and v.dtype is _INT8 and ks.dtype is _FLOAT and
+                vs.dtype is _FLOAT and k.shape == (pages, heads, page, w) and
+                v.shape == (pages, heads, w, page) and ks.shape == flat and vs.shape == flat and
+                k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and
+                vs.is_contiguous()):
+            for name, t, dtype, shape in (("keys", k, _INT8, (pages, heads, page, w)),
+                                          ("values", v, _INT8, (pages, heads, w, page)),
+                                          ("keyScales", ks, _FLOAT, flat),
+                                          ("valueScales", vs, _FLOAT, flat)):
+                _check_typed(name + " of the cache", t, dtype, shape)
+        return held, (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()) + sizes
 
     def freePages(self):
         """(free [pages], freeCount [1]) int32: every page free, for CacheTables."""

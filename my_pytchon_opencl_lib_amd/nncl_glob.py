@@ -661,10 +661,10 @@ class NnClGlob:
             raise ShapeError(f"k and v must be {list(want)} (got {list(k.shape)} and "
                              f"{list(v.shape)})")
         _check_typed("slots", slots, torch.int32, (tokens,))
+        held, place = cache.operands()
         if tokens:
-            _launch("migemm_cache_append", (k, v, slots, cache.keys), _ptr(k), _ptr(v), code,
-                    _row_stride("k", k), _row_stride("v", v), _ptr(slots), tokens,
-                    *cache.pointers, *cache.sizes)
+            _launch("migemm_cache_append", (k, v, slots) + held, _ptr(k), _ptr(v), code,
+                    _row_stride("k", k), _row_stride("v", v), _ptr(slots), tokens, *place)
 
     def CacheRead(self, cache, slots, dtype=torch.float32):
         """(k, v) [tokens, kv heads, head size] of dtype: what the cache holds at slots (e.g.
@@ -672,13 +672,14 @@ class NnClGlob:
         if dtype not in _TYPES:
             raise ShapeError(f"dtype must be float32 or bfloat16 (got {dtype})")
         _check_typed("slots", slots, torch.int32, dim=1)
+        held, place = cache.operands()
         tokens = slots.numel()
         k = torch.empty((tokens, cache.kvHeads, cache.headDim), dtype=dtype,
                         device=slots.device)
         v = torch.empty_like(k)
         if tokens:
-            _launch("migemm_cache_read", (slots, cache.keys, k, v), *cache.pointers,
-                    *cache.sizes, _ptr(slots), tokens, _ptr(k), _ptr(v), _TYPES[dtype])
+            _launch("migemm_cache_read", (slots, k, v) + held, *place, _ptr(slots), tokens,
+                    _ptr(k), _ptr(v), _TYPES[dtype])
         return k, v
 
     def CacheAttention(self, q, cache, table, starts, positions, scale=None, maxCount=0,
@@ -700,12 +701,12 @@ class NnClGlob:
         requests, columns = table.shape
         _check_typed("starts", starts, torch.int32, (requests + 1,))
         _check_typed("positions", positions, torch.int32, (tokens,))
+        held, place = cache.operands()
         o = q.new_empty((tokens, heads, dim))
         if tokens:
-            _launch("migemm_cache_attention",
-                    (q, cache.keys, table, starts, positions, o), _ptr(q), code,
-                    _row_stride("q", q), *cache.pointers, *cache.sizes, _ptr(table),
-                    columns, _ptr(starts), _ptr(positions), requests, tokens, heads,
+            _launch("migemm_cache_attention", (q, table, starts, positions, o) + held, _ptr(q),
+                    code, _row_stride("q", q), *place, _ptr(table), columns, _ptr(starts),
+                    _ptr(positions), requests, tokens, heads,
                     dim ** -0.5 if scale is None else float(scale), int(maxCount),
                     int(maxLength), _ptr(o))
         return o
