@@ -484,8 +484,9 @@ int migemm_cache_release(void *stream, const int *finished, int *lengths, int re
                          int *free_count);
 
 /* Writes K and V [tokens, kv_heads, head_dim] (tokens ldk / ldv elements apart) into their
- * slots. The tokens of one page are neighbours in the call (as migemm_cache_tables gives
- * them); slots outside the pool are skipped. For each page and head that gets tokens the new
+ * slots. Slots outside the pool are skipped; but for skipped ones, which may stand anywhere,
+ * the tokens of one page are neighbours in the call (as migemm_cache_tables gives them), and no
+ * more than a page holds. For each page and head that gets tokens the new
  * scale is the larger of the old one and of the new tokens', the old one dropped where the
  * page's first slot is among the new; where it grew, what the page holds is rounded anew:
  * rint(fl(v * fl(old / new))). A value that is not finite makes its page's scale NaN for that

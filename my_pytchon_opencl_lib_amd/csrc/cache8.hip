@@ -170,22 +170,67 @@ struct AppendArgs {
     FastDiv d8;  // head_dim / 8
 };
 
+// The slot of token t, -1 past the call's tokens or where it is outside the pool: skipped.
+__device__ __forceinline__ int slot_at(const AppendArgs &a, int t) {
+    const int slot = a.slots[min(max(t, 0), a.tokens - 1)];
+    return t >= 0 && t < a.tokens && page_of(slot, a.shift, a.c.pages) >= 0 ? slot : -1;
+}
+
+// The slot of the last token before `end` that is not skipped, -1 if there is none; 256 tokens at
+// a time (a wavefront's work, the same in each).
+__device__ __forceinline__ int last_slot(const AppendArgs &a, int end) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll 1
+    for (int hi = end; hi > 0; hi -= 256) {
+        int slot[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) slot[j] = slot_at(a, hi - 1 - lane - 64 * j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint64_t is = __ballot(slot[j] >= 0);
+            if (is != 0) return __shfl(slot[j], __builtin_ctzll(is));
+        }
+    }
+    return -1;
+}
+
+// The first token from `begin` on that is not skipped, a.tokens if there is none.
+__device__ __forceinline__ int next_token(const AppendArgs &a, int begin) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll 1
+    for (int lo = begin; lo < a.tokens; lo += 256) {
+        int slot[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) slot[j] = slot_at(a, lo + lane + 64 * j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint64_t is = __ballot(slot[j] >= 0);
+            if (is != 0) return lo + 64 * j + __builtin_ctzll(is);
+        }
+    }
+    return a.tokens;
+}
+
 // A work-group takes the pages that begin (in the order of tokens) in its chunk of tokens, for
 // one head and one of K and V, one after the other, so that each page and head has one owner:
 // no atomics, and the scale, the rounding anew and the new tokens follow each other behind
-// barriers. New tokens stay in registers between the maximum and the rounding (up to 8192
+// barriers. Skipped tokens neither begin nor end a page, however many lie between two of its
+// tokens: both searches look past them, beyond the window only where it holds nothing else (256
+// of them cost a load). New tokens stay in registers between the maximum and the rounding (up to 8192
 // values; what is beyond is read again). Values are transposed through LDS so that a page's rows
 // are written in whole words. Bound by memory for prompts; for single tokens by latency: two
 // loads that wait for each other (slots; tokens and scale). A page is rounded anew only where
 // its scale grew. 64 tokens, 8 heads of 128, pages of 64: 6.9 us; 12500 float32 tokens (128 MB):
 // 23 us, 5.6 TB/s.
 template <typename T>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4)))
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(5)))
 cache_append_kernel(AppendArgs a) {
     constexpr int KEEP = 4;  // items of 8 values that a thread keeps
     __shared__ uint32_t most_part[4];
     __shared__ int token_at[128];
-    __shared__ int window[256];  // slots of tokens c0 - 1 ..: -1 outside the pool and the call
+    __shared__ int window[256];  // slots of tokens c0 - 1 ..: -1 where skipped
+    __shared__ int run_token[128];  // the run's tokens (after its first), and their places in the
+    __shared__ int run_off[128];    // page
     extern __shared__ __attribute__((aligned(16))) int8_t tile[];  // values: [page_size][W + 4]
     const int tid = threadIdx.x, lane = tid & 63;
     const int h = blockIdx.y;
@@ -199,17 +244,18 @@ cache_append_kernel(AppendArgs a) {
         e = i - t * d8;
     };
     const int c0 = blockIdx.x * a.chunk;
-    {  // chunk <= 64 and a page's 128 tokens: a window of 193 at most
-        const int t = c0 - 1 + tid;
-        const int slot = t >= 0 && t < a.tokens ? a.slots[t] : -1;
-        window[tid] = page_of(slot, a.shift, a.c.pages) >= 0 ? slot : -1;
-    }
-    __syncthreads();
-    // which tokens of the chunk begin a page (every wavefront finds the same); slots of -1 have
-    // the page -1
-    const bool begins = lane < a.chunk && window[lane + 1] >= 0 &&
-                        window[lane] >> a.shift != window[lane + 1] >> a.shift;
-    uint64_t todo = __ballot(begins);
+    window[tid] = slot_at(a, c0 - 1 + tid);  // (chunk <= 64 and a page's 128 tokens: 193 without
+    __syncthreads();                         // skipped ones)
+    // which tokens of the chunk begin a page: those whose last token before that is not skipped
+    // is in another one, or is not there (every wavefront finds the same; -1 has the page -1)
+    const int its = lane < a.chunk ? window[lane + 1] : -1;
+    const uint64_t held = __ballot(its >= 0);
+    if (held == 0) return;
+    const uint64_t before = held & ((1ull << lane) - 1);
+    int prior = window[0];
+    if (prior < 0) prior = last_slot(a, c0 - 1);
+    if (before != 0) prior = window[64 - __builtin_clzll(before)];
+    uint64_t todo = __ballot(its >= 0 && prior >> a.shift != its >> a.shift);
 #pragma unroll 1
     while (todo != 0) {
         const int at = __builtin_ctzll(todo) + 1;  // the page's first token in the window
@@ -219,32 +265,54 @@ cache_append_kernel(AppendArgs a) {
         const int64_t ph = (int64_t)page * a.c.heads + h;
         float *scale = (is_v ? a.c.value_scales : a.c.key_scales) + ph;
         const float was = *scale;
-        // the run: the tokens from t0 on that stay in the page, at most as many as it holds
-        // (every wavefront finds the same)
+        // the run: the tokens from t0 on, past skipped ones, until one is in another page; at
+        // most as many as the page holds (every wavefront finds the same)
         int n = 0;
-        bool fresh = false;
+        bool fresh = false, dense = true;  // dense: neighbours
 #pragma unroll 1
-        for (int base = 0; base < P; base += 64) {
-            const int i = at + base + lane;
-            const int slot = base + lane < P ? window[i] : -1;
+        for (int base = at;;) {
+            const int i = base + lane;
+            const int slot = base + 63 < 256 ? window[i] : slot_at(a, c0 - 1 + i);
             const uint64_t in = __ballot(slot >= 0 && slot >> a.shift == page);
-            const int run = in == ~0ull ? 64 : __builtin_ctzll(~in);
-            const uint64_t zero = __ballot(lane < run && (slot & (P - 1)) == 0);
-            fresh = fresh || zero != 0;
-            n += run;
-            if (run < 64) break;
+            const uint64_t other = __ballot(slot >= 0 && slot >> a.shift != page);
+            const uint64_t run = other == 0 ? in : in & ((other & -other) - 1);
+            const int place = n + __builtin_popcountll(run & ((1ull << lane) - 1));
+            const bool here = (run >> lane & 1) != 0 && place < P;
+            const int off = slot & (P - 1);
+            if (here && tid < 64) {
+                run_token[place] = i - at;
+                run_off[place] = off;
+            }
+            fresh = fresh || __ballot(here && off == 0) != 0;
+            dense = dense && __ballot(here && place != i - at) == 0;
+            n = min(n + __builtin_popcountll(run), P);
+            base += 64;
+            if (other != 0 || n == P || c0 - 1 + base >= a.tokens) break;
+            if (base + 63 >= 256) {
+                const int t = next_token(a, c0 - 1 + base);
+                if (t >= a.tokens) break;
+                base = t - (c0 - 1);
+            }
         }
         const int items = n * d8;
-        float v[KEEP][8];
+        // the first items' tokens (past the run: its first item again, so that no register of
+        // the loads depends on a branch)
+        int from[KEEP], feature[KEEP];
 #pragma unroll
         for (int k = 0; k < KEEP; ++k) {
             const int i = tid + 256 * k;
-            int t, e;
-            split(i, t, e);
-            // (past the run: its first item again, so that no register depends on a branch)
-            load_f32<T, 8>(x + (i < items ? (int64_t)(t0 + t) * ld + e * 8 : (int64_t)t0 * ld), 8,
-                           v[k]);
+            split(i < items ? i : 0, from[k], feature[k]);
         }
+        if (!dense) {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < KEEP; ++k) from[k] = run_token[from[k]];
+        }
+        float v[KEEP][8];
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k)
+            load_f32<T, 8>(x + (int64_t)(t0 + from[k]) * ld + feature[k] * 8, 8, v[k]);
+        auto token = [&](int t) { return t0 + (dense ? t : run_token[t]); };
         if (tid < P) token_at[tid] = -1;
         uint32_t most = 0;
         auto largest = [&most](const float(&y)[8]) {
@@ -261,7 +329,7 @@ cache_append_kernel(AppendArgs a) {
             int t, e;
             split(i, t, e);
             float y[8];
-            load_f32<T, 8>(x + (int64_t)(t0 + t) * ld + e * 8, 8, y);
+            load_f32<T, 8>(x + (int64_t)token(t) * ld + e * 8, 8, y);
             largest(y);
         }
 #pragma unroll
@@ -273,7 +341,7 @@ cache_append_kernel(AppendArgs a) {
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < 4; ++w) most = most_part[w] > most ? most_part[w] : most;
-        if (tid < n) atomicMax(&token_at[window[at + tid] & (P - 1)], tid);
+        if (tid < n) atomicMax(&token_at[run_off[tid]], tid);
         const float old = fresh ? 0.0f : was;
         const float mine = scale_of(most);
         // the larger; NaN where either is
@@ -302,7 +370,7 @@ cache_append_kernel(AppendArgs a) {
         auto put = [&](const float(&y)[8], int i) {
             int t, e;
             split(i, t, e);
-            const int off = window[at + t] & (P - 1);
+            const int off = run_off[t];
             if (token_at[off] != t) return;
             uint2 q;
             q.x = pack4(held_byte(y[0], inv), held_byte(y[1], inv), held_byte(y[2], inv),
@@ -324,12 +392,12 @@ cache_append_kernel(AppendArgs a) {
             int t, e;
             split(i, t, e);
             float y[8];
-            load_f32<T, 8>(x + (int64_t)(t0 + t) * ld + e * 8, 8, y);
+            load_f32<T, 8>(x + (int64_t)token(t) * ld + e * 8, 8, y);
             put(y, i);
         }
         if (is_v) __syncthreads();
         if (is_v && n == 1) {  // (a single token's bytes lie apart)
-            const int off = window[at] & (P - 1);
+            const int off = run_off[0];
 #pragma unroll 1
             for (int d = tid; d < D; d += 256) base[(int64_t)d * P + off] = tile[off * (W + 4) + d];
         } else if (is_v) {

@@ -649,8 +649,8 @@ class NnClGlob:
 
     def CacheAppend(self, k, v, slots, cache):
         """Writes the keys k and values v [tokens, kv heads, head size] of a step into their
-        slots of an Int8Cache (slots of CacheTables; -1 skips a token; the tokens of one page
-        are neighbours). A page and head whose scale is too small for the new tokens gets
+        slots of an Int8Cache (slots of CacheTables; -1 skips a token, wherever it stands;
+        the other tokens of one page are neighbours). A page and head whose scale is too small for the new tokens gets
         theirs, and what it holds is rounded anew."""
         code = _check_rows("k", k, 3)
         if _check_rows("v", v, 3) != code:
