@@ -10,7 +10,7 @@
 // parts whose products add up in the fp32 accumulator: three parts (24 bits) for float32
 // calls, so that they are as exact as float32 arithmetic. For bf16 calls p vs is one part, and
 // the denominator is summed over the rounded weights too: their roundings average over the
-// keys and stay below the result's. (The few-rows kernel's first product is integer, below.)
+// keys and stay below the result's.
 //
 // The transposed products S^T = K Q^T and O^T = V^T P^T keep everything in registers: a lane
 // holds keys of one row, the exponentials come out where the second product wants them, and
@@ -115,6 +115,21 @@ __device__ __forceinline__ void query_frag(const T *row, int d, bool there, Frag
     }
 }
 
+// Whether one of eight bf16 values is not finite; and the values made NaN. A float32 query that is
+// not finite has parts that are NaN, so its row is; a bf16 one is held as it is, and against keys
+// of one sign an infinity gives scores that are all -inf, as of a row without keys.
+__device__ __forceinline__ bool not_finite(const Frag &f) {
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        odd = odd || (f.u[i] & 0x7f80u) == 0x7f80u || (f.u[i] & 0x7f800000u) == 0x7f800000u;
+    return odd;
+}
+__device__ __forceinline__ void spoil(Frag &f, bool odd) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.u[i] = odd ? 0x7fc07fc0u : f.u[i];
+}
+
 // The largest of three, NaN if one is (fmaxf would make each operand canonical first, an
 // instruction of its own).
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -132,13 +147,9 @@ __device__ __forceinline__ bool row_is_whole(const AttnArgs &p, int limit) {
 // range of keys; its four wavefronts take tiles of 64 tokens in turn, straight from memory to registers
 // (K of the next tile flies from the first product on, V from the second).
 //
-// The first product runs on the int8 matrix cores, so K needs no conversion at all: a row of q
-// is held as three signed bytes a value, q = max|q| / (127 * 2^16) * (h 2^16 + m 2^8 + l) to
-// 2^-24 of the row's largest, and the three sums are exact.
-//
-// v_mfma_i32_16x16x64_i8: row m of subtile u is token 16 (m / 4) + 4 u + m % 4 of the tile, so
+// v_mfma_f32_16x16x32_bf16: row m of subtile u is token 16 (m / 4) + 4 u + m % 4 of the tile, so
 // that lane group g ends up with the scores of tokens 16 g .. 16 g + 15, whose bytes of V^T are
-// 16 neighbours: one load a row of V.
+// 16 neighbours: one load a row of V. Of K a lane's 16 bytes are two steps' operands.
 template <int W>
 struct FewLds {
     alignas(16) float o[4 * 16 * (W + 4)];
@@ -155,8 +166,8 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
                                             int row0, int lo, int end, int part,
                                             FewLds<W> &lds) {
     constexpr int STEP = 256;  // tokens that the work-group takes at a time
-    constexpr int PP = std::is_same<T, float>::value ? 3 : 1;
-    constexpr int SK = (W + 63) / 64;  // steps of 64 features of the first product
+    constexpr int PP = std::is_same<T, float>::value ? 3 : 1;  // parts of q and of the weights
+    constexpr int SK = (W + 63) / 64;  // pairs of steps of 32 features of the first product
     constexpr bool HALF = W % 64 != 0; // of the last one only 32 are there: lane groups 2 and 3
                                        // take 0 and 1's bytes of K, and zeros of q
     constexpr int DT = W / 16;         // blocks of the second product
@@ -178,7 +189,7 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
     const int tok = j < rows ? s0 + j / p.group : min(s0, a.tokens - 1);
     const int head = h * p.group + j % p.group;
 
-    uint32_t kb[4][4 * SK];
+    v4i kb[4][SK];
     v4i vb[DT];
     float ks = 0.f, vs = 0.f;
     int page = -1;
@@ -202,10 +213,8 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
 #pragma unroll
             for (int i = 0; i < SK; ++i) {
                 const int group = HALF && i == SK - 1 ? g & 1 : g;
-                const v4i x = __builtin_nontemporal_load(
+                kb[u][i] = __builtin_nontemporal_load(
                     reinterpret_cast<const v4i *>(kp + u * 4 * W + 64 * i + 16 * group));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) kb[u][4 * i + e] = x[e];
             }
         }
     };
@@ -226,53 +235,27 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
     load_k(t0, entry, t0 < end);
     load_v(t0, t0 < end);
 
-    // q's bytes: lane (col, g) holds features 64 i + 16 g .. + 15
-    uint32_t q[3][4 * SK];
-    float qs;
+    // q: lane (col, g) holds features 64 i + 16 g .. + 15, eight a step
+    Frag q[2 * SK][PP];
     {
         const T *qp = static_cast<const T *>(a.Q) +
                       (j < rows ? (int64_t)tok * a.ldq + (int64_t)head * a.c.dim : 0);
-        float x[2 * SK][8];
-        uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 2 * SK; ++i) {
             const int d = 64 * (i / 2) + 16 * g + 8 * (i % 2);
-            query_values(qp, d, j < rows && d < a.c.dim, x[i]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t bits = __float_as_uint(x[i][e]) & 0x7fffffffu;
-                top = bits > top ? bits : top;
-            }
+            query_frag<T, PP>(qp, d, j < rows && d < a.c.dim, q[i]);
         }
+        if constexpr (PP == 1) {
+            bool odd = false;
 #pragma unroll
-        for (int o = 16; o < 64; o <<= 1) {
-            const uint32_t other = __shfl_xor(top, o);
-            top = other > top ? other : top;
+            for (int i = 0; i < 2 * SK; ++i) odd = odd || not_finite(q[i][0]);
+            // (lanes col, col + 16, ... have the row)
+            uint64_t rows_odd = __ballot(odd);
+            rows_odd |= rows_odd >> 32;
+            rows_odd |= rows_odd >> 16;
+#pragma unroll
+            for (int i = 0; i < 2 * SK; ++i) spoil(q[i][0], (rows_odd >> col & 1) != 0);
         }
-        // (subnormal rows count as 0; where a value is not finite the scale is NaN)
-        const float big = __uint_as_float(top);
-        const bool fine = big >= 0x1p-126f && top < 0x7f800000u;
-        const float inv = fine ? 1.f / big : 0.f;
-        qs = (top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fine ? big : 0.f) *
-             (1.f / 8323072.f) * p.c;
-#pragma unroll
-        for (int i = 0; i < 2 * SK; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                uint32_t byte[3][4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int t = __float2int_rn(x[i][4 * e + k] * inv * 8323072.f);
-                    const int t1 = (t - (int8_t)t) >> 8;
-                    byte[2][k] = (uint32_t)t;
-                    byte[1][k] = (uint32_t)t1;
-                    byte[0][k] = (uint32_t)((t1 - (int8_t)t1) >> 8);
-                }
-#pragma unroll
-                for (int n = 0; n < 3; ++n)
-                    q[n][2 * i + e] =
-                        pack4(byte[n][0], byte[n][1], byte[n][2], byte[n][3]);
-            }
     }
 
     const int limit = j < rows && r < a.requests ? keys_of(position, p.cap) : 0;
@@ -287,34 +270,24 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
     v4f o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
-    const v4i zero = {0, 0, 0, 0};
 
     for (; t0 < hi; t0 += STEP) {
         v4f s[4];
         float top = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            v4i sum[3];
+        for (int u = 0; u < 4; ++u) s[u] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int n = 0; n < 3; ++n) {
-                sum[n] = zero;
+        for (int i = 0; i < 2 * SK; ++i)
 #pragma unroll
-                for (int i = 0; i < SK; ++i) {
-                    v4i k, x;
+            for (int u = 0; u < 4; ++u) {
+                if (i % 2 == 0) pin(kb[u][i / 2]);
+                const v8bf k =
+                    bytes8_to_bf16(kb[u][i / 2][i % 2 * 2], kb[u][i / 2][i % 2 * 2 + 1]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        k[e] = (int)kb[u][4 * i + e];
-                        x[e] = (int)q[n][4 * i + e];
-                    }
-                    sum[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, x, sum[n], 0, 0, 0);
-                }
+                for (int n = PP - 1; n >= 0; --n)
+                    s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[i][n].v, s[u], 0, 0, 0);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                s[u][i] = fmaf((float)((sum[0][i] << 8) + sum[1][i]), 256.f,
-                               (float)sum[2][i]);
-        }
-        float sc = ks * qs;
+        float sc = ks * p.c;
         const float vscale = vs;
         const int seen = page < 0 ? 0 : limit - t0 - 16 * g;  // of this lane's 16 tokens
         // The next tile's loads, behind the last one too: loads in a branch would make every
