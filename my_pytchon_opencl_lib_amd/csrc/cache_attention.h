@@ -115,19 +115,22 @@ __device__ __forceinline__ void query_frag(const T *row, int d, bool there, Frag
     }
 }
 
-// Whether one of eight bf16 values is not finite; and the values made NaN. A float32 query that is
-// not finite has parts that are NaN, so its row is; a bf16 one is held as it is, and against keys
-// of one sign an infinity gives scores that are all -inf, as of a row without keys.
-__device__ __forceinline__ bool not_finite(const Frag &f) {
-    bool odd = false;
+// A float32 query that is not finite has parts that are NaN, and with them all scores of its row.
+// A bf16 one is held as it is, and against keys of one sign an infinity would give scores that
+// are all -inf, as of a row without keys: where one of a lane's values is not finite (times 0 it is
+// NaN), its first ones become NaN.
+template <int N>
+__device__ __forceinline__ void spoil(Frag (&q)[N][1]) {
+    float odd[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        odd = odd || (f.u[i] & 0x7f80u) == 0x7f80u || (f.u[i] & 0x7f800000u) == 0x7f800000u;
-    return odd;
-}
-__device__ __forceinline__ void spoil(Frag &f, bool odd) {
+    for (int s = 0; s < N; ++s)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f.u[i] = odd ? 0x7fc07fc0u : f.u[i];
+        for (int i = 0; i < 4; ++i)
+            odd[i & 1] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, q[s][0].u[i]),
+                                                         v2bf{(__bf16)0.f, (__bf16)0.f},
+                                                         odd[i & 1], false);
+    const float sum = odd[0] + odd[1];
+    q[0][0].u[0] = sum != sum ? 0x7fc07fc0u : q[0][0].u[0];
 }
 
 // The largest of three, NaN if one is (fmaxf would make each operand canonical first, an
@@ -245,17 +248,7 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
             const int d = 64 * (i / 2) + 16 * g + 8 * (i % 2);
             query_frag<T, PP>(qp, d, j < rows && d < a.c.dim, q[i]);
         }
-        if constexpr (PP == 1) {
-            bool odd = false;
-#pragma unroll
-            for (int i = 0; i < 2 * SK; ++i) odd = odd || not_finite(q[i][0]);
-            // (lanes col, col + 16, ... have the row)
-            uint64_t rows_odd = __ballot(odd);
-            rows_odd |= rows_odd >> 32;
-            rows_odd |= rows_odd >> 16;
-#pragma unroll
-            for (int i = 0; i < 2 * SK; ++i) spoil(q[i][0], (rows_odd >> col & 1) != 0);
-        }
+        if constexpr (PP == 1) spoil(q);
     }
 
     const int limit = j < rows && r < a.requests ? keys_of(position, p.cap) : 0;
@@ -821,6 +814,7 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W> 
     }
     load(lo);
     st.find(lo + 64);
+    if constexpr (QP == 1) spoil(q);  // (behind the loads: it waits for q)
     const int limit = keys_of(position, p.cap);
     // the work-group's longest row, this wavefront's and its shortest
     int most = limit, least = j < rows ? limit : INT32_MAX;

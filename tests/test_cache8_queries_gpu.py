@@ -56,3 +56,27 @@ def test_rows_of_any_size(nncl, lengths, counts, hints, kind):
     got = nncl.CacheAttention(q, cache, ints(table), starts, positions, maxCount=hints[0],
                               maxLength=hints[1])
     check_attention(got, attention64(q, cache, table, starts, positions, 1.0 / 8), max(lengths))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lengths,counts,hints", FORMS)
+@pytest.mark.parametrize("value", ["inf", "-inf", "nan"])
+def test_queries_that_are_not_finite_are_seen(nncl, lengths, counts, hints, value, kind):
+    """Against keys of one sign an infinite query's scores are all inf or all -inf, neither of
+    which has a softmax: NaN, never zeros, in its row and no other; 0 where the row has no key."""
+    dim = 64
+    cache = filled(2, dim, 16, sum(-(-n // 16) for n in lengths) + 2, dim)
+    cache.keys[..., 11] = cache.keys[..., 11].abs().clamp(min=1)
+    table, starts, positions, tokens = step_of(nncl, cache, lengths, counts, 0, 5)
+    q = torch.randn(tokens, 4, dim, generator=gen(9), device="cuda").to(TYPES[kind])
+    args = dict(maxCount=hints[0], maxLength=hints[1])
+    clean = nncl.CacheAttention(q, cache, ints(table), starts, positions, **args)
+    bad = torch.zeros(tokens, 4, dtype=torch.bool, device="cuda")
+    bad[0, 1] = bad[-1, 3] = bad[tokens // 2, 0] = True
+    q[:, :, 11] = torch.where(bad, float(value), q[:, :, 11])
+    got = nncl.CacheAttention(q, cache, ints(table), starts, positions, **args)
+    assert torch.equal(got.isnan(), bad[:, :, None].expand_as(got))
+    assert torch.equal(got[~bad], clean[~bad])
+    positions[0] = -1
+    got = nncl.CacheAttention(q, cache, ints(table), starts, positions, **args)
+    assert not got[0].any()
