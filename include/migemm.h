@@ -506,9 +506,11 @@ int migemm_cache_read(void *stream, const int8_t *keys, const int8_t *values,
 /* O[t, h] = softmax(scale * Q[t, h] . keys) values over positions 0 .. positions[t] of token
  * t's request, head h / (heads / kv_heads) of the cache: Q (tokens ldq elements apart) and O
  * (contiguous) [tokens, heads, head_dim] of `type`, heads a multiple of kv_heads. Request i
- * has tokens starts[i] .. starts[i + 1]; tokens past starts[requests] and those with position
- * -1 give 0. Positions are read as below max_pages * page_size, starts as within [0, tokens];
- * cached tokens whose table entry is outside the pool are left out.
+ * has tokens starts[i] .. starts[i + 1]; tokens before starts[0], past starts[requests] and
+ * those with position -1 give 0. Positions are read as below max_pages * page_size, starts as
+ * within [0, tokens] and not below the one before; starts must not descend otherwise (where
+ * they do, rows that several requests claim, or none, have no defined result). Cached tokens
+ * whose table entry is outside the pool are left out.
  * max_count (most tokens of one request, 0: unknown) and max_length (longest request after
  * the step, 0: unknown) shape the launch; results are right whatever they say.
  * Contexts are cut, in ranges or in even shares of all of them, where the requests alone do

@@ -37,7 +37,8 @@ struct AttnArgs {
     int both;           // few and many rows in one launch, each part takes its requests
     int units;          // many rows: tiles of rows that the grid covers
     int shares;         // work-groups of few_shares (0: ranges)
-    int *firsts;        // [2][requests + 2]: its scan, for the join
+    int tiles;          // its bound of one kv head's tiles
+    int *firsts;        // [2][requests + kNoRequest + 1]: its scan, for the join
     float *part_o;      // [tokens * heads][splits][width], or [2 shares][16][width]
     float *part_ml;     // likewise, 2 (the largest score, the sum)
 };
@@ -52,12 +53,16 @@ namespace {
 
 __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
-// Tokens [s0, s1) of request r; r == requests: the tokens past the last request's, without
-// keys.
+// Tokens [s0, s1) of request r. Two more "requests", without keys, have the tokens that belong to
+// none: r == requests those past the last one's, r == requests + 1 those before the first one's.
+constexpr int kNoRequest = 2;
 __device__ __forceinline__ void request_tokens(const CacheAttention &a, int r, int &s0,
                                                int &s1) {
-    s0 = clamp_int(a.starts[r], 0, a.tokens);
-    s1 = r < a.requests ? clamp_int(a.starts[r + 1], s0, a.tokens) : a.tokens;
+    const bool leading = r > a.requests;
+    const int at = clamp_int(a.starts[leading ? 0 : r], 0, a.tokens);
+    const int next = a.starts[min(r + 1, a.requests)];
+    s0 = leading ? 0 : at;
+    s1 = leading ? at : r < a.requests ? clamp_int(next, s0, a.tokens) : a.tokens;
 }
 
 // Keys that a row sees: its position's and those before it.
@@ -485,10 +490,10 @@ __device__ __forceinline__ Shares shares_of(const AttnArgs &p, int tiles) {
 }
 
 struct ShareLds {
-    int first[kShareRequests + 2];  // tiles of one head of the requests before r
-    int units[kShareRequests + 2];  // tiles of a unit of r
-    int token[kShareRequests + 2];  // r's first token
-    int rows[kShareRequests + 2];
+    int first[kShareRequests + kNoRequest + 1];  // tiles of one head of the requests before r
+    int units[kShareRequests + kNoRequest];      // tiles of a unit of r
+    int token[kShareRequests + kNoRequest];      // r's first token
+    int rows[kShareRequests + kNoRequest];
 };
 
 template <typename T, int W>
@@ -499,11 +504,14 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W> &lds,
     auto &units = scan.units;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     auto &sums = lds.m[0];
+    const int all_requests = a.requests + kNoRequest;
+    // (Sums end at p.tiles, which starts that do not descend never reach: no index below leaves its
+    // array, and no int32 overflows, whatever the device's memory holds.)
     int before = 0;
-    for (int base = 0; base <= a.requests; base += 256) {
+    for (int base = 0; base < all_requests; base += 256) {
         const int r = base + tid;
         int n = 0, unit = 1;
-        if (r <= a.requests) {
+        if (r < all_requests) {
             int s0, s1, most = 0;
             request_tokens(a, r, s0, s1);
             if (r < a.requests)
@@ -514,39 +522,38 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W> &lds,
             scan.token[r] = s0;
             scan.rows[r] = (s1 - s0) * p.group;
         }
-        int upto = n;
+        int upto = min(n, p.tiles);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int u = __shfl_up(upto, o);
-            if (lane >= o) upto += u;
+            if (lane >= o) upto = min(upto + u, p.tiles);
         }
         if (lane == 63) sums[wave] = __int_as_float(upto);
         __syncthreads();
-        int all = 0;
+        int all = before;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const int x = __float_as_int(sums[w]);
-            upto += w < wave ? x : 0;
-            all += x;
+            if (w == wave) upto = min(upto + all, p.tiles);
+            all = min(all + __float_as_int(sums[w]), p.tiles);
         }
-        if (r <= a.requests) first[r + 1] = before + upto;
-        before += all;
+        if (r < all_requests) first[r + 1] = upto;
+        before = all;
         __syncthreads();
     }
     if (tid == 0) first[0] = 0;
     __syncthreads();
     if (blockIdx.x == 0)
-        for (int i = tid; i <= a.requests + 1; i += 256) {
+        for (int i = tid; i <= all_requests; i += 256) {
             p.firsts[i] = first[i];
-            p.firsts[a.requests + 2 + i] = i <= a.requests ? units[i] : 1;
+            p.firsts[all_requests + 1 + i] = i < all_requests ? units[i] : 1;
         }
     const Shares s = shares_of(p, before);
     auto request_at = [&](int tile) {  // the last request that begins at or before the tile
         int r = -1;
-        for (int base = 0; base <= a.requests; base += 64)
+        for (int base = 0; base < all_requests; base += 64)
             r += __builtin_popcountll(__ballot(
-                base + lane <= a.requests && first[min(base + lane, a.requests)] *
-                                                     a.c.heads <= tile));
+                base + lane < all_requests && first[min(base + lane, all_requests)] *
+                                                      a.c.heads <= tile));
         return r;
     };
     auto cut = [&](int w) {
@@ -555,7 +562,7 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W> &lds,
         const int r = request_at((int)at);
         const int in = ((int)at - first[r] * a.c.heads) % units[r];
         if (in <= kSnap) return (int)at - in;
-        return units[r] - in <= kSnap ? (int)at + units[r] - in : (int)at;
+        return units[r] - in <= kSnap ? min((int)at + units[r] - in, s.total) : (int)at;
     };
     const int w = blockIdx.x;
     int at = __builtin_amdgcn_readfirstlane(cut(w));
@@ -619,9 +626,9 @@ __device__ __forceinline__ bool many_tile(const AttnArgs &p, int id, ManyTile &x
     // which request's tile: requests in order (tiles that run together share keys in L2), 64 at
     // a time
     int r = -1, tile = 0, s0 = 0, s1 = 0;
-    for (int base = 0, before = 0; base <= a.requests; base += 64) {
+    for (int base = 0, before = 0; base < a.requests + kNoRequest; base += 64) {
         int x0 = 0, x1 = 0, n = 0;
-        if (base + lane <= a.requests) {
+        if (base + lane < a.requests + kNoRequest) {
             request_tokens(a, base + lane, x0, x1);
             const int rows = (x1 - x0) * p.group;
             n = rows > kFewRows ? (rows + kManyRows - 1) / kManyRows : 0;
@@ -1033,7 +1040,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnArgs p) {
     const CacheAttention &a = p.a;
     const int64_t row = blockIdx.x;
     const int tok = (int)(row / a.heads);
-    if (tok >= clamp_int(a.starts[a.requests], 0, a.tokens)) return;
+    if (tok < a.starts[0] || tok >= clamp_int(a.starts[a.requests], 0, a.tokens)) return;
     const int limit = keys_of(a.positions[tok], p.cap);
     if (row_is_whole(p, limit)) return;
     const int n = min(p.splits, (limit + p.chunk - 1) / p.chunk);
@@ -1092,7 +1099,8 @@ __global__ void __launch_bounds__(256) attention_share_join_kernel(AttnArgs p) {
     const int r = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
     const int h = head / p.group;
     const int before = p.firsts[r], n = p.firsts[r + 1] - before;
-    const int tiles = p.firsts[a.requests + 1], unit = p.firsts[a.requests + 2 + r];
+    const int all_requests = a.requests + kNoRequest;
+    const int tiles = p.firsts[all_requests], unit = p.firsts[all_requests + 1 + r];
     if (n == 0 || unit <= 2 * kSnap) return;
     const Shares s = shares_of(p, tiles);
     int s0, s1;
@@ -1102,8 +1110,8 @@ __global__ void __launch_bounds__(256) attention_share_join_kernel(AttnArgs p) {
         const int j = (tok - s0) * p.group + head % p.group;
         const int begin = before * a.c.heads + h * n + j / 16 * unit;
         const int cut0 = (begin + kSnap) / s.each + 1;         // the first cut inside
-        const int cut1 = (begin + unit - kSnap - 1) / s.each;  // and the last
-        const int parts = cut1 - cut0 + 2;
+        const int cut1 = min(begin + unit - kSnap, s.total) - 1;
+        const int parts = cut1 / s.each - cut0 + 2;            // (to the last one)
         if (parts < 2) continue;
         auto place = [&](int k) {
             return (int64_t)(k == 0 ? 2 * (cut0 - 1) + 1 : 2 * (cut0 + k - 1)) * 16 + j % 16;
@@ -1195,7 +1203,7 @@ int launch_width(hipStream_t stream, const AttnArgs &p) {
                       dim3((unsigned)(p.a.requests * p.a.heads)), dim3(256), 0, stream, p);
         return launch_status("attention_share_join_kernel launch");
     }
-    const int few = p.splits * p.a.c.heads * (p.a.requests + 1);
+    const int few = p.splits * p.a.c.heads * (p.a.requests + kNoRequest);
     if (p.both)
         MIGEMM_LAUNCH((attention_both_kernel<T, W>),
                       dim3((unsigned)(few + p.units * p.splits * p.a.c.heads)), dim3(256),

@@ -459,9 +459,10 @@ int launch_cache_attention(hipStream_t stream, const CacheAttention &a) {
     // Single tokens in even shares, two work-groups a CU (one where a head's registers allow no
     // more): int32 holds the number of tiles, and their scan is kept on the chip. Short contexts
     // in ranges, without the scan (8 requests of 200 tokens: 11.4 us, 15.7 in shares).
-    const int64_t tiles = ((int64_t)a.tokens * p.group / 16 + a.requests + 1) *
-                          ((p.cap + 63) / 64) * a.c.heads;
-    const bool even = length > 512 && a.requests <= kShareRequests && tiles < (int64_t)1 << 30;
+    const int64_t tiles = ((int64_t)a.tokens * p.group / 16 + a.requests + kNoRequest) *
+                          ((p.cap + 63) / 64);
+    const bool even = length > 512 && a.requests <= kShareRequests &&
+                      tiles * a.c.heads < (int64_t)1 << 30;
     // Requests of at most 16 rows are computed one way, others another; where one request may
     // bring more, one launch holds both ways. Up to 32 float32 rows go the first way twice, in
     // shares (32 requests of 4096 tokens, 20 rows each, 8 kv heads of 128: 93 us, 183 the other
@@ -470,9 +471,10 @@ int launch_cache_attention(hipStream_t stream, const CacheAttention &a) {
     p.both = many;
     if (!many && even) {
         p.shares = a.c.width <= 128 ? 512 : 256;
+        p.tiles = (int)tiles;
         MIGEMM_TRY(check_grid("cache_attention", (int64_t)a.requests * a.heads, 256));
         const size_t parts = (size_t)p.shares * 2 * 16;
-        const size_t scan = ((size_t)a.requests + 2) * 2 * sizeof(int);
+        const size_t scan = ((size_t)a.requests + kNoRequest + 1) * 2 * sizeof(int);
         int rc = MIGEMM_OK;
         p.part_o = static_cast<float *>(workspace(
             stream, parts * (a.c.width + 2) * sizeof(float) + scan, &rc, 0));
@@ -482,7 +484,7 @@ int launch_cache_attention(hipStream_t stream, const CacheAttention &a) {
         return a.type == MIGEMM_FLOAT32 ? launch_attention_f32(stream, p)
                                         : launch_attention_bf16(stream, p);
     }
-    const int64_t units = (int64_t)a.tokens * p.group / kManyRows + a.requests + 1;
+    const int64_t units = (int64_t)a.tokens * p.group / kManyRows + a.requests + kNoRequest;
     p.units = (int)units;
     // Contexts are cut in ranges (of whole rounds of a few-rows work-group, 256 tokens) where the
     // requests, tiles and kv heads alone make too few work-groups: single tokens until there are
@@ -504,7 +506,7 @@ int launch_cache_attention(hipStream_t stream, const CacheAttention &a) {
     p.splits = (int)((length + chunk - 1) / chunk);
     const int64_t rows = (int64_t)a.tokens * a.heads;
     MIGEMM_TRY(check_grid("cache_attention", (int64_t)p.splits * a.c.heads *
-                                                  (a.requests + 1 + (many ? units : 0)), 512));
+                                                  (a.requests + kNoRequest + (many ? units : 0)), 512));
     if (p.splits > 1) {
         MIGEMM_TRY(check_grid("cache_attention", rows, 256));
         const size_t parts = (size_t)rows * p.splits;

@@ -688,7 +688,8 @@ class NnClGlob:
         query t of request i (starts[i] <= t < starts[i + 1]) sees the request's tokens 0 ..
         positions[t] (its own, already appended, among them), head h the kv head
         h // (heads / kv heads). scale: 1 / sqrt(head size) if None. Tokens without a position
-        (-1) or request give 0. starts and positions are CacheTables'; maxCount (most tokens of
+        (-1) or request (before starts[0], past the last start) give 0. starts and positions are
+        CacheTables' (starts never descend); maxCount (most tokens of
         one request) and maxLength (longest request) shape the launches if the caller knows
         them, the result does not depend on them. Returns [tokens, heads, head size] of q's
         type."""
