@@ -438,7 +438,10 @@ int migemm_matmul_int8(void *stream, const int8_t *A, int64_t lda, const float *
 
 /* Y = the product above of the quantised rows of X [M, cols] (X and Y of `type`) and
  * W [N, K], K = cols rounded up to 16 (as migemm_quantize_rows leaves a weight [N, cols]).
- * One launch for up to three rows; otherwise the quantised rows go to the stream's workspace. */
+ * One launch where M * ceil(cols / 4096) <= 3 (three rows of up to 4096 columns, one of up to
+ * 12288); otherwise the quantised rows, M * (K + 4) bytes, go to the stream's workspace first.
+ * Products of few tiles and many columns (both entries) also keep their k ranges' sums there:
+ * reserve it before a capture. */
 int migemm_linear_int8(void *stream, const void *X, int type, int64_t ldx, const int8_t *W,
                        int64_t ldw, const float *w_scales, const float *bias, void *Y,
                        int64_t ldy, int M, int N, int cols);

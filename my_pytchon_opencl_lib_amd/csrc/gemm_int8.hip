@@ -10,8 +10,8 @@
 //                        cores (and the loads that feed them) for large M
 //   rows_int8_kernel     few rows: bound by streaming B once; a work-group takes 16 rows of B,
 //                        its wavefronts split K, operands go straight to registers
-//   rows_int8_kernel with x in float: the same for up to three rows, x quantised by every
-//                        work-group (x is small and in L2): one launch instead of two
+//   rows_int8_kernel with x in float: the same for up to three rows (fused_rows), x quantised by
+//                        every work-group (x is small and in L2): one launch instead of two
 #include "gemm_direct.h"
 #include "int8_common.h"
 

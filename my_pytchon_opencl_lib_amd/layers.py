@@ -53,7 +53,8 @@ class Linear:
 class LinearInt8:
     """A Linear layer for serving, its weight held in 8 bits with a scale for each output:
     y[..., out] = x[..., in] @ weight^T (+ bias). weight [out, in] is a float tensor or array
-    (e.g. Linear.weight), quantised here once; x and y are float32 or bfloat16."""
+    (e.g. Linear.weight), quantised here once; x and y are float32 or bfloat16. For inference: y
+    carries no gradient."""
 
     def __init__(self, weight, bias=None, nnclglob=None):
         self.nnclglob = nnclglob if nnclglob is not None else NnClGlob()

@@ -520,7 +520,7 @@ class NnClGlob:
     # ---------------------------------------------------------------- serving in 8 bits
     # The reference has no counterpart. Activations are float32 or bfloat16; rows of a larger
     # tensor (a slice of a fused projection) are taken as they lie. All of these only enqueue
-    # work on the current stream; nothing is read back.
+    # work on the current stream; nothing is read back, and no gradient is recorded.
     def QuantizeRows(self, x):
         """(values, scales) of x[..., K] in 8 bits, a scale for each row: scales [rows] =
         max |x| / 127 over the row, values int8 [rows, K rounded up to 16] = x / scale rounded
@@ -573,7 +573,9 @@ class NnClGlob:
     def LinearInt8(self, x, weight, scales, bias=None):
         """y[..., N] = x[..., K] @ W^T (+ bias[N], float32) with W [N, K] as QuantizeRows left
         it (weight int8 [N, K rounded up to 16], scales [N]); the rows of x are quantised on
-        the way. y has the type of x. One launch for up to three rows."""
+        the way. y has the type of x. One launch where rows * ceil(K / 4096) <= 3; otherwise
+        the quantised rows go through the stream's workspace (reserve_workspace before a
+        capture). For inference: the result carries no gradient."""
         code = _check_rows("x", x)
         _check_typed("weight", weight, torch.int8, dim=2)
         n, kp = weight.shape
