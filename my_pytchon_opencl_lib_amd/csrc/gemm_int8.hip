@@ -507,12 +507,15 @@ constexpr TileChoice kTiles[] = {
 template <typename T>
 int launch_product(hipStream_t stream, const Int8Product &p) {
     // Few rows: 16 columns a work-group (24 x 4096 x 2048: 4.2 us, tiles 6.8; with the quantising
-    // before it 16 x 4096 x 4096 10.2, 12.5; 16 x 8192 x 8192 23.2, 29.7), where that makes
-    // enough work-groups (8 x 1024 x 16384: 18.4, 15.6 in k ranges of tiles) and not so many that
-    // A, read by each, costs more than it saves: over many columns the tiles stream B as well
-    // and read A once for 64 columns (16 x 11008 x 4096: 18.4, 17.6; 16 x 32000 x 4096 35.5,
-    // 25.9; 24 x 4096 x 11008 22.4, 20.5).
-    if ((p.M <= 32 && (int64_t)p.N * p.K <= (int64_t)12 << 20) ||
+    // before it 16 x 4096 x 4096 10.2, 12.5; 16 x 8192 x 8192 23.2, 29.7). Not where many columns
+    // read A, each work-group all of it: there the tiles stream B as well and read A once for 64
+    // columns (16 x 11008 x 4096: 18.4, 17.6; 16 x 32000 x 4096 35.5, 25.9; 24 x 4096 x 11008
+    // 22.4, 20.5). And not over long K of few columns, as a work-group's time grows with K (alone, up
+    // to a work-group a CU) and tiles cut it in ranges: M <= 16 8.1 us at 512 x 8192 (tiles 9.9), 9.7
+    // (10.4) at 10240, 11.0 (11.1) at 12288, 13.7 (11.4) at 16384, 64.7 (22.7) at 64 x 131056; M <=
+    // 32 9.1 (10.7) at 512 x 5120, 10.3 (10.3) at 6144, 11.6 (10.2) at 8192.
+    if ((p.M <= 32 && (int64_t)p.N * p.K <= (int64_t)12 << 20 &&
+         p.K <= (p.M <= 16 ? 10240 : 6144)) ||
         (p.M <= 16 && p.N >= 2048 && p.N <= 8192)) {
         const RowsArgs a = rows_args(p);
         return p.M <= 16 ? launch_rows<T, void, 1, 8>(stream, a)
