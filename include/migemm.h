@@ -481,7 +481,9 @@ int migemm_cache_slots(void *stream, const int *lengths, const int *counts, int 
 
 /* Gives the pages of each request i with finished[i] != 0 back: they are added at the end of
  * free_pages (which holds `pages`), *free_count grows, its table entries become -1 and its
- * length 0. Pages outside the pool, or beyond what free_pages holds, are dropped. */
+ * length 0. Pages outside the pool, or beyond what free_pages holds, are dropped. Pages are not
+ * counted: one that rows of several requests name is given back with the first of them, so it is
+ * taken out of the others' reach before (an entry of -1 is passed over). */
 int migemm_cache_release(void *stream, const int *finished, int *lengths, int requests,
                          int *table, int max_pages, int page_size, int *free_pages, int pages,
                          int *free_count);

@@ -121,7 +121,9 @@ __global__ void __launch_bounds__(TW) cache_tables_kernel(TablesArgs a, int shif
     a.positions[t] = pos;
 }
 
-// One work-group: a scheduler frees a few requests at a time, in order.
+// One work-group: a scheduler frees a few requests at a time, in order. It looks at one request
+// after the other, a load that is waited for each: 512 requests with one finished take 45 us, with 8
+// of 64 pages 53, with all 631.
 __global__ void __launch_bounds__(TW)
 cache_release_kernel(const int *finished, int *lengths, int requests, int *table, int max_pages,
                      int shift, int *free_pages, int pages, int *free_count) {
@@ -220,8 +222,9 @@ __device__ __forceinline__ int next_token(const AppendArgs &a, int begin) {
 // values; what is beyond is read again). Values are transposed through LDS so that a page's rows
 // are written in whole words. Bound by memory for prompts; for single tokens by latency: two
 // loads that wait for each other (slots; tokens and scale). A page is rounded anew only where
-// its scale grew. 64 tokens, 8 heads of 128, pages of 64: 6.9 us; 12500 float32 tokens (128 MB):
-// 23 us, 5.6 TB/s.
+// its scale grew, a third load that waits for the first two and the bytes of the page, read and
+// written. 63 tokens, 8 heads of 128, pages of 64: 6.7 us where no scale grows, 8.7 where all do;
+// 8767 float32 tokens in pages of 32 (90 MB): 28 and 30.6 us, 3.2 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(5)))
 cache_append_kernel(AppendArgs a) {
@@ -430,7 +433,8 @@ cache_append_kernel(AppendArgs a) {
 // 64 tokens of one head, of K or of V: a thread takes four tokens' eight features at a time.
 // Values are read along a page's tokens, four neighbouring slots a load (wherever they begin),
 // and turned in registers. Two loads that wait for each other (slots; bytes and scales), then
-// 16 bytes or more a store: bound by memory (12500 float32 tokens, 128 MB: 22 us, 5.8 TB/s).
+// 16 bytes or more a store: bound by memory (8972 float32 tokens, 92 MB: 22.8 us, 4.0 TB/s).
+// A step's 64 pages of 64 tokens, bfloat16 (25 MB): 8.2 us.
 template <typename T>
 __global__ void __launch_bounds__(256)
 cache_read_kernel(Cache8 c, const int *slots, int tokens, T *K, T *V, int shift) {

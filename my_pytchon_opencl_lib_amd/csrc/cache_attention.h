@@ -474,8 +474,10 @@ __device__ __forceinline__ void few_rows(const AttnArgs &p, int id, FewLds<W> &l
 // Single tokens in even shares: the tiles (of 64 tokens) of all requests and kv heads in one
 // line, cut into p.shares equal pieces, one a work-group, all of which run at once; a decoding
 // batch's contexts differ, and work-groups of whole ranges would leave CUs idle at the end.
-// 32 requests of 4096 tokens, 8 kv heads of 128: 38 us (172 MB, 4.6 TB/s; 51 in ranges), 2 of
-// 131072: 70 us (5.9 TB/s; 87 in ranges).
+// 32 requests of up to 4096 tokens, 8 kv heads of 128: 38.7 us (172 MB, 4.4 TB/s; 42.3 in ranges), 2
+// of up to 131072: 74 us (415 MB, 5.6 TB/s). float32 queries 41.8 and 77.9. Where all contexts
+// have one length ranges are as good (32 x 4096: bfloat16 51.9 us in shares and 49.7 in ranges with
+// the join, float32 55.4 and 49.3).
 // A unit is one request, kv head and 16 rows (its rows beyond 16 are further units, and a unit
 // without keys has one tile, which writes its zeros). Cuts within two tiles of a unit's end
 // are moved there. A unit that is cut is joined afterwards (attention_share_join_kernel, which
@@ -592,7 +594,7 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W> &lds,
 // work, one barrier a tile). LDS rows are padded by 16 bytes: the 16 lanes of a read phase fall
 // on different banks.
 //
-// 4 x 4096 tokens, 32 heads on 8 of 128: 646 to 660 us, 0.85 PFLOP/s; 16 x 1024: 251 us. Of a
+// 4 x 4096 tokens, 32 heads on 8 of 128: 637 to 660 us, 0.85 PFLOP/s; 16 x 1024: 228 us. Of a
 // wavefront's 2900 cycles a tile the matrix cores have 1024, the vector instructions (softmax
 // 110, maxima 35, conversions 96, exponentials at a quarter of the rate) about 1350, and the
 // LDS reads, a kilobyte an instruction, as long as the matrix cores have: each has a half of

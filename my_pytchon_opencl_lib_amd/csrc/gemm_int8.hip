@@ -56,8 +56,10 @@ __device__ __forceinline__ void fetch_tail(const Op &op, typename Op::Tail &t, i
 // loads is gemm_direct_kernel's: a tile's loads run D tiles ahead, and every fragment read of
 // a stage is issued before the barrier that frees it. 256 x 256 tiles have 16 wavefronts of
 // 32 x 128, four on a SIMD, so that one's fragment reads and waits pass under the others'
-// products (8 wavefronts of 64 x 128: 401 us, 16: 348 at 8192 x 11008 x 4096, 2.1 POP/s); K in
-// stages of 64 bytes and four of them: 376. Bound by the matrix cores and their clock.
+// products (8 wavefronts of 64 x 128: 401 us, 16: 348 at 8192 x 11008 x 4096); K in stages of 64
+// bytes and four of them: 376. Bound by the matrix cores and their clock, which follows the data:
+// random bytes 471 us at 8192^3 (2.33 POP/s; a library's product 447) and 362 at 8192 x 11008 x
+// 4096 (2.04; 340), zeros 305 (3.60; 307) and 263 (263), on one card.
 template <typename T, int BM, int BN, int WM, int WN, int S, int D, int OCC>
 __global__ void __launch_bounds__(WM *WN * 64) __attribute__((amdgpu_waves_per_eu(OCC)))
 gemm_int8_kernel(Int8Args p) {
@@ -308,7 +310,7 @@ int launch_tiles(hipStream_t stream, const Int8Product &p, int splits) {
 // v_mfma_i32_16x16x64_i8 hold 16 bytes of one row a lane, in any order of k that is the same
 // for both: lane group g = lane / 16 takes bytes 32 g .. 32 g + 31 of a piece, so a piece of a
 // row is one whole 128-byte line and two instructions. Bound by streaming B: 1 x 4096 to 11008
-// (45 MB) 9.5 us, 4.7 TB/s; 24 x 2048 to 4096 4.1 to 4.9 us.
+// (45 MB, quantising its row) 10.2 us a call, 4.4 TB/s; 24 x 2048 to 4096 5.5 us.
 // X != void: A is not given but x [M, K] in X, and each work-group quantises it into LDS
 // itself (its first loads of B are on their way meanwhile).
 constexpr int kKeep = 3;  // steps of x (NW * 512 values each) that stay in registers
@@ -496,7 +498,9 @@ RowsArgs rows_args(const Int8Product &p) {
 
 // What a choice costs, in work of one CU at the best tiles' rate: rounds of work-groups over
 // the 256 CUs, a tile's products over the rate that its shape reaches. Rates measured against
-// 256 x 256 (2500 TOP/s at 8192^3): 128 x 256 0.88, 128 x 128 0.84, 64 x 128 0.70, 64 x 64 0.55.
+// 256 x 256 (at 8192^3): 128 x 256 0.88, 128 x 128 0.84, 64 x 128 0.70, 64 x 64 0.55. (Where a
+// round is not full the choice hardly matters: 1000 x 3000 x 784 takes 12.5 us in 128 x 128, 12.8 in
+// 64 x 128, 12.6 in 64 x 64, 17.3 in 128 x 256.)
 struct TileChoice {
     int bm, bn;
     float rate;

@@ -4,7 +4,7 @@
 //
 // (scale_of, held_byte). One pass over the data: a row stays in registers between the
 // maximum and the rounding, so x is read once and a byte a value written: bound by memory
-// (8192 x 4096 bfloat16: 20 us, 5.0 TB/s; 1000 x 777 float32: 2.8 to 3.7 us, a launch's latency).
+// (8192 x 4096 bfloat16: 22 us, 4.5 TB/s; 1000 x 777 float32: 3.0 to 4.0 us, a launch's latency).
 // A wavefront takes a row of up to 2048 values (four rows a work-group, no barrier); longer
 // ones take a work-group of 256 threads, which keeps 16384 values and reads what is beyond
 // them twice (from L2).

@@ -458,15 +458,17 @@ int launch_cache_attention(hipStream_t stream, const CacheAttention &a) {
     const int64_t count_rows = count * p.group;
     // Single tokens in even shares, two work-groups a CU (one where a head's registers allow no
     // more): int32 holds the number of tiles, and their scan is kept on the chip. Short contexts
-    // in ranges, without the scan (8 requests of 200 tokens: 11.4 us, 15.7 in shares).
+    // in ranges, without the scan (8 requests of 200 tokens: 6.5 us, 9.4 in shares; 32 of 500: 15.5,
+    // 17.5; 32 of 1000: 23.0, 22.3).
     const int64_t tiles = ((int64_t)a.tokens * p.group / 16 + a.requests + kNoRequest) *
                           ((p.cap + 63) / 64);
     const bool even = length > 512 && a.requests <= kShareRequests &&
                       tiles * a.c.heads < (int64_t)1 << 30;
     // Requests of at most 16 rows are computed one way, others another; where one request may
     // bring more, one launch holds both ways. Up to 32 float32 rows go the first way twice, in
-    // shares (32 requests of 4096 tokens, 20 rows each, 8 kv heads of 128: 93 us, 183 the other
-    // way, which has six products for one; 48 rows: 154 and 194, 64: 197 and 193).
+    // shares (32 requests of 4096 tokens, 20 rows each, 8 kv heads of 128: 97 us, 183 the other
+    // way, whose work-groups hold 128; 48 rows: 159 and 213, 64: 199 and 215; bfloat16 20 rows 93
+    // and 73).
     const bool many = count_rows > (even && a.type == MIGEMM_FLOAT32 ? 2 * kFewRows : kFewRows);
     p.both = many;
     if (!many && even) {

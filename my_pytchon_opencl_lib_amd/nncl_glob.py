@@ -640,7 +640,8 @@ class NnClGlob:
     def CacheRelease(self, finished, lengths, table, free, freeCount, pageSize):
         """Gives the pages of every request with finished[i] != 0 back: added at the end of
         free[0 .. freeCount) (free has room for the whole pool), its table row becomes -1 and
-        its length 0. In place."""
+        its length 0. In place. Pages are not counted: set the entries of a page that another
+        request goes on using to -1 before."""
         requests, columns = _check_table(lengths, table)
         _check_typed("finished", finished, torch.int32, (requests,))
         _check_typed("free", free, torch.int32, dim=1)
