@@ -8,9 +8,15 @@
 // The bytes are exact in bf16 (7 bits), so products run on the bf16 matrix cores with the
 // cache's side exact. A bf16 query is exact too. A float32 query, and p vs, are cut into bf16
 // parts whose products add up in the fp32 accumulator: three parts (24 bits) for float32
-// calls, so that they are as exact as float32 arithmetic. For bf16 calls p vs is one part, and
-// the denominator is summed over the rounded weights too: their roundings average over the
-// keys and stay below the result's.
+// calls, so that they are as exact as float32 arithmetic. For bf16 calls p vs is one f16 number
+// (11 bits, an eighth of the result's own rounding; the bytes of V are exact in f16 too). f16's
+// range is small, so weights have a running maximum of their own, over score + log2 vs, in whose
+// unit they and the sums of weights times V are held (Weights, below): a row's weights come to
+// at most 2^14, whatever its pages' scales, and what f16 rounds as subnormal is below 2^-20 of the
+// row's largest. The denominator is summed over the rounded weights where a tile's scales are not far
+// below the row's, else over the exponentials. (With one bf16 number, 8 bits, results were 2.3e-3 off
+// the formula in norm; the result's own rounding is 1.7e-3, and so are they now. Single tokens take
+// the same time, prompts 2 % more: 4 x 4096 tokens 636 and 652 us.)
 //
 // The transposed products S^T = K Q^T and O^T = V^T P^T keep everything in registers: a lane
 // holds keys of one row, the exponentials come out where the second product wants them, and
@@ -86,6 +92,33 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[N])
 union Frag {
     uint32_t u[4];
     v8bf v;
+    v8h h;
+};
+
+// bf16 calls: a row's weights, in units of 2^(top - kUnit). top follows score + log2 vs as m
+// follows the scores, and whenever m does, so that over = top - m is log2 of a scale that the row
+// saw. Rows that saw no key: over = -inf; nothing but zeros: inf.
+constexpr float kUnit = 6.f;
+constexpr float kFar = -5.f;  // scales below 2^kFar of the row's: the denominator from exponentials
+struct Weights {
+    float top = -INFINITY, over = -INFINITY;
+    __device__ __forceinline__ float unit() const {
+        return (top == -INFINITY ? 0.f : top) - kUnit;
+    }
+    // Returns what the sums are multiplied with.
+    __device__ __forceinline__ float follow(float now, float m) {
+        now = fmaxf(top, now);
+        const float alpha = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.f : now));
+        top = now;
+        over = top == -INFINITY ? (m == -INFINITY ? -INFINITY : INFINITY) : top - m;
+        return alpha;
+    }
+    // What brings a sum of weights over vs to units of 2^m.
+    __device__ __forceinline__ float to_m() const { return __builtin_amdgcn_exp2f(over - kUnit); }
+    // What brings the sums to units of 2^m, times 2^kUnit (2^over alone stays a normal number).
+    __device__ __forceinline__ float natural() const {
+        return over == INFINITY ? 0.f : __builtin_amdgcn_exp2f(over);
+    }
 };
 
 // Eight neighbouring values of a query row as float32 (head sizes are multiples of 8: all of
@@ -265,6 +298,7 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
     if (split > 0 && lo >= most) return;  // (the same for the whole work-group)
 
     float m = -INFINITY, l = 0.f;
+    Weights weights;
     v4f o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -310,42 +344,46 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
                 }
             sc = 1.f;
         }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
         // m is any number near the largest score: it follows only where it would be left
         // behind by more than kLag, so the sums are rarely scaled anew
-        if (__ballot(top > m + kLag) != 0) {
+        const float lg = __builtin_amdgcn_logf(vscale);  // (log2)
+        float big = PP == 1 ? top + lg : 0.f;
+        if (__ballot(top > m + kLag || (PP == 1 && big > weights.top + kLag)) != 0) {
+#pragma unroll
+            for (int x = 16; x < 64; x <<= 1) {
+                top = fmaxf(top, __shfl_xor(top, x));
+                if constexpr (PP == 1) big = fmaxf(big, __shfl_xor(big, x));
+            }
             const float now = fmaxf(m, top);
             const float alpha = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.f : now));
             l *= alpha;
+            m = now;
+            const float by = PP == 1 ? weights.follow(big, m) : alpha;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
-            m = now;
+                for (int i = 0; i < 4; ++i) o[d][i] *= by;
         }
-        const float base = m == -INFINITY ? 0.f : m;
         Frag w[2][PP];
-        if (PP == 1 && __ballot(!(vscale >= 0x1p-90f)) == 0) {
-            // one part: the sum is taken over the rounded weights, so that numerator and
-            // denominator round alike (a row that sees one key gives its value, whatever
-            // the scale's bits; p vs alone would be off by the same 2^-9 in all of a page)
-            const float less = __builtin_amdgcn_logf(vscale) - base;  // (log2)
+        const float less = lg - weights.unit();
+        if (PP == 1 && __ballot(!(vscale >= 0x1p-90f) || lg - weights.over < kFar) == 0) {
+            // the sum is taken over the rounded weights, so that numerator and denominator round
+            // alike (a row that sees one key gives its value, whatever the scale's bits)
             float sum = 0.f;
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const uint32_t e =
-                        pack_bf16(__builtin_amdgcn_exp2f(fmaf(s[u][2 * i], sc, less)),
-                                  __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], sc, less)));
+                        pack_f16(__builtin_amdgcn_exp2f(fmaf(s[u][2 * i], sc, less)),
+                                 __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], sc, less)));
                     w[u / 2][0].u[2 * (u & 1) + i] = e;
-                    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, e),
-                                                          v2bf{(__bf16)1.f, (__bf16)1.f},
-                                                          sum, false);
+                    sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, e),
+                                                 v2h{(_Float16)1.f, (_Float16)1.f}, sum, false);
                 }
-            l = fmaf(sum, __builtin_amdgcn_rcpf(vscale), l);
-        } else {  // (a scale of 0, a tiny one, NaN, or float32)
+            l = fmaf(sum, __builtin_amdgcn_rcpf(vscale) * weights.to_m(), l);
+        } else {  // (a scale of 0, a tiny one, NaN, one far below the row's, or float32)
+            const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -356,24 +394,39 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
                         const float z = fmaf(s[u][2 * i + k], sc, -base);
                         e[k] = __builtin_amdgcn_exp2f(z);
                         l += e[k];
-                        e[k] = z != -INFINITY ? e[k] * vscale : 0.f;
+                        if constexpr (PP == 1)
+                            e[k] = __builtin_amdgcn_exp2f(z + (less + base));
+                        else
+                            e[k] *= vscale;
+                        e[k] = z != -INFINITY ? e[k] : 0.f;
                     }
-                    uint32_t part[PP];
-                    split_pair<PP>(e[0], e[1], part);
+                    if constexpr (PP == 1) {
+                        w[u / 2][0].u[2 * (u & 1) + i] = pack_f16(e[0], e[1]);
+                    } else {
+                        uint32_t part[PP];
+                        split_pair<PP>(e[0], e[1], part);
 #pragma unroll
-                    for (int n = 0; n < PP; ++n)
-                        w[u / 2][n].u[2 * (u & 1) + i] = part[n];
+                        for (int n = 0; n < PP; ++n)
+                            w[u / 2][n].u[2 * (u & 1) + i] = part[n];
+                    }
                 }
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             pin(vb[d]);
-            const v8bf x = bytes8_to_bf16(vb[d][0], vb[d][1]);
-            const v8bf y = bytes8_to_bf16(vb[d][2], vb[d][3]);
+            if constexpr (PP == 1) {
+                const v8h x = bytes8_to_f16(vb[d][0], vb[d][1]);
+                const v8h y = bytes8_to_f16(vb[d][2], vb[d][3]);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w[0][0].h, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, w[1][0].h, o[d], 0, 0, 0);
+            } else {
+                const v8bf x = bytes8_to_bf16(vb[d][0], vb[d][1]);
+                const v8bf y = bytes8_to_bf16(vb[d][2], vb[d][3]);
 #pragma unroll
-            for (int n = PP - 1; n >= 0; --n) {
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, w[0][n].v, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, w[1][n].v, o[d], 0, 0, 0);
+                for (int n = PP - 1; n >= 0; --n) {
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, w[0][n].v, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, w[1][n].v, o[d], 0, 0, 0);
+                }
             }
         }
         load_v(t0 + STEP, more);
@@ -391,11 +444,13 @@ __device__ __forceinline__ void few_segment(const AttnArgs &p, int r, int s0, in
 #pragma unroll
     for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][col]);
     const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - top);
+    const float natural = PP == 1 ? weights.natural() : 1.f;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
         v4f x = o[d];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] *= f;
+        for (int i = 0; i < 4; ++i)
+            x[i] = (PP == 1 ? x[i] * 0x1p-6f * natural : x[i]) * f;  // (2^-kUnit)
         *reinterpret_cast<v4f *>(o_lds + (wave * 16 + col) * OS + d * 16 + 4 * g) = x;
     }
     __syncthreads();
@@ -589,10 +644,10 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W> &lds,
 
 // ------------------------------------------------------------------------ many rows
 // Prompts: 32 rows (queries x heads that share a kv head) a wavefront, four wavefronts, on
-// v_mfma_f32_32x32x16_bf16. Tiles of 64 tokens are read as bytes, turned into bf16 once for
-// the work-group and shared in LDS (two buffers: the next tile's bytes fly during a tile's
-// work, one barrier a tile). LDS rows are padded by 16 bytes: the 16 lanes of a read phase fall
-// on different banks.
+// v_mfma_f32_32x32x16_bf16 (bf16 calls' second product: _f16). Tiles of 64 tokens are read as
+// bytes, turned into 16 bits once for the work-group and shared in LDS (two buffers: the next
+// tile's bytes fly during a tile's work, one barrier a tile). LDS rows are padded by 16 bytes: the
+// 16 lanes of a read phase fall on different banks.
 //
 // 4 x 4096 tokens, 32 heads on 8 of 128: 637 to 660 us, 0.85 PFLOP/s; 16 x 1024: 228 us. Of a
 // wavefront's 2900 cycles a tile the matrix cores have 1024, the vector instructions (softmax
@@ -603,7 +658,7 @@ __device__ __forceinline__ void few_shares(const AttnArgs &p, FewLds<W> &lds,
 // reads, with a SIMD to itself (1420: the registers do not hold it).
 template <int W>
 struct ManyLds {
-    static constexpr int KR = W + 8, VR = 64 + 8;  // LDS rows, in bf16
+    static constexpr int KR = W + 8, VR = 64 + 8;  // LDS rows, in 16-bit values
     alignas(16) uint16_t k[2][64 * KR];
     alignas(16) uint16_t v[2][W * VR];
     // of the tile's four groups of 16 tokens: ks c, vs, log2 vs and 1 / vs
@@ -663,7 +718,7 @@ __device__ __forceinline__ bool many_tile(const AttnArgs &p, int id, ManyTile &x
 // tokens' rows of K, so that their page is one for the wavefront and its address scalar; of V it
 // moves the same tokens of all features or, where a page holds whole tiles, a quarter of the
 // features of all 64 (rows of 64 neighbouring bytes). A thread's place in the page never changes.
-template <int W>
+template <int W, bool F16>  // (V in f16, or bf16)
 struct ManyStage {
     static constexpr int CH = W / 16;          // units of 16 bytes in a row of K
     static constexpr int MU = (W + 63) / 64;   // units of K, and of V, that a thread moves
@@ -740,7 +795,10 @@ struct ManyStage {
         const int i = n >> 1, half = n & 1, row = vrow + 64 * i;
         if (EVEN || row < W) {
             uint16_t *vp = lds.v[b] + row * VR + vgroup * 16 + 8 * half;
-            *reinterpret_cast<v8bf *>(vp) = bytes8_to_bf16(vb[i][half], vb[i][half + 2]);
+            if constexpr (F16)
+                *reinterpret_cast<v8h *>(vp) = bytes8_to_f16(vb[i][half], vb[i][half + 2]);
+            else
+                *reinterpret_cast<v8bf *>(vp) = bytes8_to_bf16(vb[i][half], vb[i][half + 2]);
         }
     }
     __device__ __forceinline__ void put_scales(int b) {
@@ -792,7 +850,7 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W> 
     ManyTile x;
     if (!many_tile(p, id, x)) return;
     const int r = x.r, tile = x.tile, s0 = x.s0, rows = x.rows, h = x.h, split = x.split;
-    ManyStage<W> st(p, lds, r, h);
+    ManyStage<W, QP == 1> st(p, lds, r, h);
 
     const int j = tile * kManyRows + wave * 32 + lo32;
     const int tok = j < rows ? s0 + j / p.group : s0;
@@ -844,6 +902,7 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W> 
     if (split > 0 && lo >= most) return;
 
     float m = -INFINITY, l = 0.f;
+    Weights weights;
     v16f o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -916,37 +975,47 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W> 
                 ks[w] = odd ? 1.f : ks[w];
             }
         }
-        float top = -INFINITY;
+        float top = -INFINITY, big = -INFINITY;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const v16f &x = s[w >> 1];
             const int i = 8 * (w & 1);
-            const float big = max3(max3(max3(x[i], x[i + 1], x[i + 2]), x[i + 3], x[i + 4]),
-                                   x[i + 5], max3(x[i + 6], x[i + 7], x[i]));
-            top = fmaxf(top, big * ks[w]);
+            const float most = max3(max3(max3(x[i], x[i + 1], x[i + 2]), x[i + 3], x[i + 4]),
+                                    x[i + 5], max3(x[i + 6], x[i + 7], x[i])) * ks[w];
+            top = fmaxf(top, most);
+            if constexpr (PP == 1) big = fmaxf(big, most + scale_lds[buf][w][2]);
         }
-        top = fmaxf(top, __shfl_xor(top, 32));
         // m is any number near the largest score: it follows only where it would be left behind
         // by more than kLag, so the sums are rarely scaled anew
-        if (__ballot(top > m + kLag) != 0) {
+        if (__ballot(top > m + kLag || (PP == 1 && big > weights.top + kLag)) != 0) {
+            top = fmaxf(top, __shfl_xor(top, 32));
             const float now = fmaxf(m, top);
             const float alpha = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.f : now));
             l *= alpha;
+            m = now;
+            float by = alpha;
+            if constexpr (PP == 1) by = weights.follow(fmaxf(big, __shfl_xor(big, 32)), m);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
-            m = now;
+                for (int i = 0; i < 16; ++i) o[d][i] *= by;
         }
-        const float base = m == -INFINITY ? 0.f : m;
         Frag w[4][PP];
-        if (PP == 1 && (flags & 0x02020202u) == 0x02020202u) {
-            // one part: the sum is taken over the rounded weights, so that numerator and
-            // denominator round alike (a row that sees one key gives its value, whatever the
-            // scale's bits; p vs alone would be off by the same 2^-9 in all of a page)
+        const float unit = weights.unit();
+        bool near = false;
+        if constexpr (PP == 1) {
+            const float low = fminf(fminf(scale_lds[buf][0][2], scale_lds[buf][1][2]),
+                                    fminf(scale_lds[buf][2][2], scale_lds[buf][3][2]));
+            near = (flags & 0x02020202u) == 0x02020202u &&
+                   __ballot(low - weights.over < kFar) == 0;
+        }
+        if (near) {
+            // the sum is taken over the rounded weights, so that numerator and denominator round
+            // alike (a row that sees one key gives its value, whatever the scale's bits)
+            const float to_m = weights.to_m();
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const float less = scale_lds[buf][x][2] - base;
+                const float less = scale_lds[buf][x][2] - unit;
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -955,14 +1024,14 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W> 
                     for (int k = 0; k < 2; ++k)
                         e[k] = __builtin_amdgcn_exp2f(
                             fmaf(s[x >> 1][8 * (x & 1) + 2 * i + k], ks[x], less));
-                    w[x][0].u[i] = pack_bf16(e[0], e[1]);
-                    sum = __builtin_amdgcn_fdot2_f32_bf16(
-                        __builtin_bit_cast(v2bf, w[x][0].u[i]), v2bf{(__bf16)1.f, (__bf16)1.f},
-                        sum, false);
+                    w[x][0].u[i] = pack_f16(e[0], e[1]);
+                    sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w[x][0].u[i]),
+                                                 v2h{(_Float16)1.f, (_Float16)1.f}, sum, false);
                 }
-                l = fmaf(sum, scale_lds[buf][x][3], l);
+                l = fmaf(sum, scale_lds[buf][x][3] * to_m, l);
             }
-        } else {  // (a scale of 0, a tiny one, NaN, or float32)
+        } else {  // (a scale of 0, a tiny one, NaN, one far below a row's, or float32)
+            const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -973,12 +1042,20 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W> 
                         const float z = fmaf(s[x >> 1][8 * (x & 1) + 2 * i + k], ks[x], -base);
                         e[k] = __builtin_amdgcn_exp2f(z);
                         l += e[k];
-                        e[k] = z != -INFINITY ? e[k] * scale_lds[buf][x][1] : 0.f;
+                        if constexpr (PP == 1)
+                            e[k] = __builtin_amdgcn_exp2f(z + (scale_lds[buf][x][2] + base - unit));
+                        else
+                            e[k] *= scale_lds[buf][x][1];
+                        e[k] = z != -INFINITY ? e[k] : 0.f;
                     }
-                    uint32_t part[PP];
-                    split_pair<PP>(e[0], e[1], part);
+                    if constexpr (PP == 1) {
+                        w[x][0].u[i] = pack_f16(e[0], e[1]);
+                    } else {
+                        uint32_t part[PP];
+                        split_pair<PP>(e[0], e[1], part);
 #pragma unroll
-                    for (int n = 0; n < PP; ++n) w[x][n].u[i] = part[n];
+                        for (int n = 0; n < PP; ++n) w[x][n].u[i] = part[n];
+                    }
                 }
         }
 #pragma unroll
@@ -986,9 +1063,14 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W> 
 #pragma unroll
             for (int n = PP - 1; n >= 0; --n)
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x % VA][d], w[x][n].v, o[d],
-                                                                   0, 0, 0);
+                for (int d = 0; d < DT; ++d) {
+                    if constexpr (PP == 1)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                            __builtin_bit_cast(v8h, vf[x % VA][d]), w[x][n].h, o[d], 0, 0, 0);
+                    else
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x % VA][d], w[x][n].v,
+                                                                       o[d], 0, 0, 0);
+                }
             if (x + VA < 4) read_v(x + VA);
         }
         }
@@ -996,6 +1078,13 @@ __device__ __forceinline__ void many_rows(const AttnArgs &p, int id, ManyLds<W> 
         __syncthreads();
     }
     l += __shfl_xor(l, 32);
+    if constexpr (PP == 1) {
+        const float natural = weights.natural();
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * 0x1p-6f * natural;  // (2^-kUnit)
+    }
 
     if (j < rows) {
         const int64_t row = (int64_t)tok * a.heads + head;

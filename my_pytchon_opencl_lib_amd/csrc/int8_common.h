@@ -165,11 +165,35 @@ __device__ __forceinline__ v8bf bytes8_to_bf16(uint32_t a, uint32_t b) {
     bytes_to_bf16(b, r.u[2], r.u[3]);
     return r.v;
 }
+// Four signed bytes as f16, exact: byte + 128 as the low bits of 1024 + x, less 1152.
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ void bytes_to_f16(uint32_t v, uint32_t &lo, uint32_t &hi) {
+    const uint32_t x = v ^ 0x80808080u;
+    const v2h less = {(_Float16)-1152.f, (_Float16)-1152.f};
+    const v2h a = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(x, 0x64646464u, 0x00050004u));
+    const v2h b = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(x, 0x64646464u, 0x00070006u));
+    lo = __builtin_bit_cast(uint32_t, a + less);
+    hi = __builtin_bit_cast(uint32_t, b + less);
+}
+__device__ __forceinline__ v8h bytes8_to_f16(uint32_t a, uint32_t b) {
+    union {
+        uint32_t u[4];
+        v8h v;
+    } r;
+    bytes_to_f16(a, r.u[0], r.u[1]);
+    bytes_to_f16(b, r.u[2], r.u[3]);
+    return r.v;
+}
 // Two floats as two bf16, rounded to nearest even.
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2bf));
+}
+// The same as two f16.
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2h));
 }
 __device__ __forceinline__ float bf16_low(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t u) {
