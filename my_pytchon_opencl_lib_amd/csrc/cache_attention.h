@@ -529,10 +529,10 @@ __device__ __forceinline__ void few_rows(const AttnArgs &p, int id, FewLds<W> &l
 // Single tokens in even shares: the tiles (of 64 tokens) of all requests and kv heads in one
 // line, cut into p.shares equal pieces, one a work-group, all of which run at once; a decoding
 // batch's contexts differ, and work-groups of whole ranges would leave CUs idle at the end.
-// 32 requests of up to 4096 tokens, 8 kv heads of 128: 38.7 us (172 MB, 4.4 TB/s; 42.3 in ranges), 2
-// of up to 131072: 74 us (415 MB, 5.6 TB/s). float32 queries 41.8 and 77.9. Where all contexts
-// have one length ranges are as good (32 x 4096: bfloat16 51.9 us in shares and 49.7 in ranges with
-// the join, float32 55.4 and 49.3).
+// 32 requests of up to 4096 tokens, 8 kv heads of 128: 38.4 us (172 MB, 4.5 TB/s; 41.8 in ranges), 2
+// of up to 131072: 74 us (415 MB, 5.6 TB/s). float32 queries 41.6 and 77.6. Where all contexts
+// have one length ranges are as good (32 x 4096: bfloat16 50.9 us in shares and 49.1 in ranges with
+// the join, float32 54.3 and 49.1).
 // A unit is one request, kv head and 16 rows (its rows beyond 16 are further units, and a unit
 // without keys has one tile, which writes its zeros). Cuts within two tiles of a unit's end
 // are moved there. A unit that is cut is joined afterwards (attention_share_join_kernel, which

@@ -466,9 +466,9 @@ int launch_cache_attention(hipStream_t stream, const CacheAttention &a) {
                       tiles * a.c.heads < (int64_t)1 << 30;
     // Requests of at most 16 rows are computed one way, others another; where one request may
     // bring more, one launch holds both ways. Up to 32 float32 rows go the first way twice, in
-    // shares (32 requests of 4096 tokens, 20 rows each, 8 kv heads of 128: 97 us, 183 the other
-    // way, whose work-groups hold 128; 48 rows: 159 and 213, 64: 199 and 215; bfloat16 20 rows 93
-    // and 73).
+    // shares (32 requests of 4096 tokens, 20 rows each, 8 kv heads of 128: 95 us, 183 the other
+    // way, whose work-groups hold 128; 48 rows: 154 and 198, 64: 198 and 213; bfloat16 20 rows 92
+    // and 71).
     const bool many = count_rows > (even && a.type == MIGEMM_FLOAT32 ? 2 * kFewRows : kFewRows);
     p.both = many;
     if (!many && even) {
