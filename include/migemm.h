@@ -424,10 +424,28 @@ int migemm_gemm_plan(int transA, int transB, int M, int N, int K,
 #define MIGEMM_FLOAT32 0
 #define MIGEMM_BFLOAT16 1
 
+/* Activations: none; x < 0 ? 0 : x; x / (1 + exp(-x)); x (1 + erf(x / sqrt 2)) / 2;
+ * x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2. */
+#define MIGEMM_ACT_NONE 0
+#define MIGEMM_ACT_RELU 1
+#define MIGEMM_ACT_SILU 2
+#define MIGEMM_ACT_GELU 3
+#define MIGEMM_ACT_GELU_TANH 4
+
 /* values[r, k] and scales[r] of the rows of X [rows, cols]. ldv >= cols rounded up to 16
  * (the added columns are written as 0), ldv % 16 == 0, values 16-byte aligned. */
 int migemm_quantize_rows(void *stream, const void *X, int type, int64_t ldx, int8_t *values,
                          int64_t ldv, float *scales, int rows, int cols);
+
+/* The quantised rows of a root-mean-square norm, after a residual's addition: with t = X + R
+ * (rounded to `type`; t = X where R is NULL), q = 1 / sqrt(mean_k t[r, k]^2 + eps) (in 64 bits,
+ * rounded to 32 once) and y[r, k] = fl(fl(t[r, k] * q[r]) * weight[k]), values and scales are the
+ * rows of y as migemm_quantize_rows lays them out. S [rows, cols] of `type`, lds apart, gets t
+ * (NULL: not kept; it needs an R). weight is float32 [cols], NULL for ones; eps finite and > 0. A
+ * row with a value that is not finite gets the scale NaN. */
+int migemm_norm_int8(void *stream, const void *X, int64_t ldx, const void *R, int64_t ldr,
+                     int type, const float *weight, float eps, void *S, int64_t lds,
+                     int8_t *values, int64_t ldv, float *scales, int rows, int cols);
 
 /* C[m, n] = (sum_k A[m, k] * B[n, k]) * a_scales[m] * b_scales[n] (+ bias[n] if not NULL):
  * A [M, K] and B [N, K] int8, C [M, N] of `type`. The sum is exact (int32; K <= 131071).
@@ -445,6 +463,22 @@ int migemm_matmul_int8(void *stream, const int8_t *A, int64_t lda, const float *
 int migemm_linear_int8(void *stream, const void *X, int type, int64_t ldx, const int8_t *W,
                        int64_t ldw, const float *w_scales, const float *bias, void *Y,
                        int64_t ldy, int M, int N, int cols);
+
+/* The two products with what closes a layer, in the same launches: with c as above (scales and
+ * bias applied),
+ *   gated == 0:  out[m, n] = act(c[m, n]) (+ residual[m, n] if not NULL), weight [N, K]
+ *   gated == 1:  out[m, n] = act(c[m, n]) * c[m, N + n] (+ residual[m, n]), weight [2 N, K]: the N
+ *                rows of the gate, then the N rows that it multiplies; scales and bias [2 N]
+ * in float32, rounded to `type` once. residual [M, N] of `type`, rows ldr apart; out may not
+ * overlap it. N is the number of out's columns. */
+int migemm_matmul_int8_ex(void *stream, const int8_t *A, int64_t lda, const float *a_scales,
+                          const int8_t *B, int64_t ldb, const float *b_scales, const float *bias,
+                          int activation, int gated, const void *residual, int64_t ldr, void *C,
+                          int type, int64_t ldc, int M, int N, int K);
+int migemm_linear_int8_ex(void *stream, const void *X, int type, int64_t ldx, const int8_t *W,
+                          int64_t ldw, const float *w_scales, const float *bias, int activation,
+                          int gated, const void *residual, int64_t ldr, void *Y, int64_t ldy,
+                          int M, int N, int cols);
 
 /* The paged cache: keys int8 [pages, kv_heads, page_size, width], values int8 [pages,
  * kv_heads, width, page_size] (a head's values transposed within a page), float32 scales

@@ -25,6 +25,12 @@ MIGEMM_GEMM_ACCUMULATE = 1  # migemm_gemm_strided_batched_ex flag: C += result
 # Activation types of the 8-bit operators
 MIGEMM_FLOAT32 = 0
 MIGEMM_BFLOAT16 = 1
+# Activations of the 8-bit products
+MIGEMM_ACT_NONE = 0
+MIGEMM_ACT_RELU = 1
+MIGEMM_ACT_SILU = 2
+MIGEMM_ACT_GELU = 3
+MIGEMM_ACT_GELU_TANH = 4
 
 # Kernel-family policies (migemm_set_gemm_policy)
 MIGEMM_POLICY_AUTO = 0
@@ -142,10 +148,16 @@ SIGNATURES = {
     "migemm_gemm_plan": ([_i32, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
                           _vp, _i64, _i64, _i32, _i32, ctypes.c_char_p, _sz], _i32),
     "migemm_quantize_rows": ([_vp, _vp, _i32, _i64, _vp, _i64, _vp, _i32, _i32], _i32),
+    "migemm_norm_int8": ([_vp, _vp, _i64, _vp, _i64, _i32, _vp, _f32, _vp, _i64, _vp, _i64, _vp,
+                          _i32, _i32], _i32),
     "migemm_matmul_int8": ([_vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _i64, _i32,
                             _i32, _i32], _i32),
     "migemm_linear_int8": ([_vp, _vp, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32,
                             _i32], _i32),
+    "migemm_matmul_int8_ex": ([_vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _i32, _vp, _i64,
+                               _vp, _i32, _i64, _i32, _i32, _i32], _i32),
+    "migemm_linear_int8_ex": ([_vp, _vp, _i32, _i64, _vp, _i64, _vp, _vp, _i32, _i32, _vp, _i64,
+                               _vp, _i64, _i32, _i32, _i32], _i32),
     "migemm_cache_tables": ([_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32] +
                             [_vp] * 5 + [_i32], _i32),
     "migemm_cache_slots": ([_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _i32], _i32),

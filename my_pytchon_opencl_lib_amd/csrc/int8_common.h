@@ -12,10 +12,25 @@ struct Int8Product {
     const float *sa, *sb, *bias;
     void *C;
     int64_t lda, ldb, ldc;
-    int M, N, K, type;
+    int M, N, K, type;  // N: columns of C
+    int act;            // MIGEMM_ACT_*
+    bool gated;         // B holds 2 N rows (and sb, bias 2 N values): the gate's first
+    const void *residual;  // [M, N] of `type`, rows ldr values apart, or null
+    int64_t ldr;
 };
 int launch_quantize_rows(hipStream_t stream, const void *X, int type, int64_t ldx,
                          int8_t *values, int64_t ldv, float *scales, int rows, int cols);
+struct NormInt8 {
+    const void *X, *R;  // [rows, cols] of `type`, rows ldx / ldr values apart; R may be null
+    void *S;            // their sum, or null
+    const float *weight;  // [cols], or null: ones
+    int8_t *values;
+    float *scales;
+    int64_t ldx, ldr, lds, ldv;
+    int rows, cols, type;
+    float eps;
+};
+int launch_norm_int8(hipStream_t stream, const NormInt8 &p);
 int launch_product_int8(hipStream_t stream, const Int8Product &p);
 // The layer: x quantised by rows, then the product (one launch for a few rows).
 int launch_linear_int8(hipStream_t stream, const void *X, int64_t ldx, int cols,

@@ -100,6 +100,20 @@ int check_int8_rows(const char *what, const char *name, const int8_t *p, int64_t
     return MIGEMM_OK;
 }
 
+int64_t padded16(int cols) { return ((int64_t)cols + 15) / 16 * 16; }
+
+// Rows that are written in 8 bits, a work-group of 256 threads each.
+int check_quantized(const char *what, const int8_t *values, int64_t ldv, int rows, int cols) {
+    if (rows < 1 || cols < 1 || cols > INT32_MAX - 65536)
+        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: sizes must be >= 1 (rows=%d cols=%d)", what,
+                         rows, cols);
+    MIGEMM_TRY(check_ld(what, "ldv", ldv, padded16(cols)));
+    if (ldv % 16 != 0 || !aligned(values, 16))
+        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: values must be 16-byte aligned and ldv=%lld "
+                         "a multiple of 16", what, (long long)ldv);
+    return check_grid(what, rows, 256);
+}
+
 int check_cache(const char *what, const Cache8 &c) {
     MIGEMM_TRY(check_pointers(what, {c.keys, c.values, c.key_scales, c.value_scales}));
     if (c.pages < 1 || c.heads < 1 || c.heads > 65535)
@@ -158,54 +172,47 @@ int check_table(const char *what, int requests, int max_pages, int page_size, in
     return MIGEMM_OK;
 }
 
-}  // namespace
-}  // namespace migemm
+// What closes a product: an activation, a gate, a residual.
+struct Closing {
+    int activation = MIGEMM_ACT_NONE, gated = 0;
+    const void *residual = nullptr;
+    int64_t ldr = 0;
+};
 
-using namespace migemm;
-
-extern "C" {
-
-int migemm_quantize_rows(void *stream, const void *X, int type, int64_t ldx, int8_t *values,
-                         int64_t ldv, float *scales, int rows, int cols) {
-    const char *w = "quantize_rows";
-    clear_error();
-    MIGEMM_TRY(check_pointers(w, {X, values, scales}));
-    MIGEMM_TRY(check_type(w, type));
-    if (rows < 1 || cols < 1 || cols > INT32_MAX - 65536)
-        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: sizes must be >= 1 (rows=%d cols=%d)", w,
-                         rows, cols);
-    const int64_t padded = ((int64_t)cols + 15) / 16 * 16;
-    MIGEMM_TRY(check_ld(w, "ldx", ldx, cols));
-    MIGEMM_TRY(check_ld(w, "ldv", ldv, padded));
-    if (ldv % 16 != 0 || !aligned(values, 16))
-        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: values must be 16-byte aligned and ldv=%lld "
-                         "a multiple of 16", w, (long long)ldv);
-    MIGEMM_TRY(check_grid(w, rows, 256));
-    MIGEMM_TRY(check_alias(w, {{values, rows_bytes(rows, ldv, padded, 1)},
-                               {scales, (int64_t)rows * 4}},
-                           {{X, rows_bytes(rows, ldx, cols, type_size(type))}}));
-    return launch_quantize_rows((hipStream_t)stream, X, type, ldx, values, ldv, scales, rows,
-                                cols);
+int check_closing(const char *what, const Closing &e, int N) {
+    if (e.activation < MIGEMM_ACT_NONE || e.activation > MIGEMM_ACT_GELU_TANH)
+        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: activation %d is none of MIGEMM_ACT_*", what,
+                         e.activation);
+    if (e.gated != 0 && e.gated != 1)
+        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: gated=%d must be 0 or 1", what, e.gated);
+    if (e.gated && N > INT32_MAX / 2 - 32)
+        return set_error(MIGEMM_ERR_UNSUPPORTED, "%s: a gated N=%d exceeds the int32 rows of the "
+                         "weight", what, N);
+    if (e.residual != nullptr) MIGEMM_TRY(check_ld(what, "ldr", e.ldr, N));
+    return MIGEMM_OK;
 }
 
-int migemm_matmul_int8(void *stream, const int8_t *A, int64_t lda, const float *a_scales,
-                       const int8_t *B, int64_t ldb, const float *b_scales, const float *bias,
-                       void *C, int type, int64_t ldc, int M, int N, int K) {
-    const char *w = "matmul_int8";
+int matmul_int8(const char *w, void *stream, const int8_t *A, int64_t lda, const float *a_scales,
+                const int8_t *B, int64_t ldb, const float *b_scales, const float *bias, void *C,
+                int type, int64_t ldc, int M, int N, int K, const Closing &e) {
     clear_error();
     MIGEMM_TRY(check_pointers(w, {A, a_scales, B, b_scales, C}));
     MIGEMM_TRY(check_type(w, type));
-    MIGEMM_TRY(check_product(w, M, N, K));
+    MIGEMM_TRY(check_closing(w, e, N));
+    MIGEMM_TRY(check_product(w, M, e.gated ? 2 * N : N, K));
     if (K % 16 != 0)
         return set_error(MIGEMM_ERR_INVALID_ARG, "%s: K=%d must be a multiple of 16 (rows padded "
                          "with zeros, as quantize_rows leaves them)", w, K);
     MIGEMM_TRY(check_int8_rows(w, "a", A, lda, K));
     MIGEMM_TRY(check_int8_rows(w, "b", B, ldb, K));
     MIGEMM_TRY(check_ld(w, "ldc", ldc, N));
-    MIGEMM_TRY(check_alias(w, {{C, rows_bytes(M, ldc, N, type_size(type))}},
-                           {{A, rows_bytes(M, lda, K, 1)}, {B, rows_bytes(N, ldb, K, 1)},
-                            {a_scales, (int64_t)M * 4}, {b_scales, (int64_t)N * 4},
-                            {bias, bias != nullptr ? (int64_t)N * 4 : 0}}));
+    const int64_t wide = e.gated ? 2 * (int64_t)N : N;
+    MIGEMM_TRY(check_alias(
+        w, {{C, rows_bytes(M, ldc, N, type_size(type))}},
+        {{A, rows_bytes(M, lda, K, 1)}, {B, rows_bytes(wide, ldb, K, 1)},
+         {a_scales, (int64_t)M * 4}, {b_scales, wide * 4},
+         {bias, bias != nullptr ? wide * 4 : 0},
+         {e.residual, e.residual != nullptr ? rows_bytes(M, e.ldr, N, type_size(type)) : 0}}));
     Int8Product p{};
     p.A = A;
     p.B = B;
@@ -220,17 +227,21 @@ int migemm_matmul_int8(void *stream, const int8_t *A, int64_t lda, const float *
     p.N = N;
     p.K = K;
     p.type = type;
+    p.act = e.activation;
+    p.gated = e.gated != 0;
+    p.residual = e.residual;
+    p.ldr = e.ldr;
     return launch_product_int8((hipStream_t)stream, p);
 }
 
-int migemm_linear_int8(void *stream, const void *X, int type, int64_t ldx, const int8_t *W,
-                       int64_t ldw, const float *w_scales, const float *bias, void *Y,
-                       int64_t ldy, int M, int N, int cols) {
-    const char *w = "linear_int8";
+int linear_int8(const char *w, void *stream, const void *X, int type, int64_t ldx, const int8_t *W,
+                int64_t ldw, const float *w_scales, const float *bias, void *Y, int64_t ldy, int M,
+                int N, int cols, const Closing &e) {
     clear_error();
     MIGEMM_TRY(check_pointers(w, {X, W, w_scales, Y}));
     MIGEMM_TRY(check_type(w, type));
-    MIGEMM_TRY(check_product(w, M, N, cols));
+    MIGEMM_TRY(check_closing(w, e, N));
+    MIGEMM_TRY(check_product(w, M, e.gated ? 2 * N : N, cols));
     const int K = (cols + 15) / 16 * 16;
     if (K > 131071)
         return set_error(MIGEMM_ERR_UNSUPPORTED, "%s: K=%d, int32 sums hold K <= 131071", w, K);
@@ -238,10 +249,12 @@ int migemm_linear_int8(void *stream, const void *X, int type, int64_t ldx, const
     MIGEMM_TRY(check_int8_rows(w, "w", W, ldw, K));
     MIGEMM_TRY(check_ld(w, "ldy", ldy, N));
     MIGEMM_TRY(check_grid(w, M, 256));
-    MIGEMM_TRY(check_alias(w, {{Y, rows_bytes(M, ldy, N, type_size(type))}},
-                           {{X, rows_bytes(M, ldx, cols, type_size(type))},
-                            {W, rows_bytes(N, ldw, K, 1)}, {w_scales, (int64_t)N * 4},
-                            {bias, bias != nullptr ? (int64_t)N * 4 : 0}}));
+    const int64_t wide = e.gated ? 2 * (int64_t)N : N;
+    MIGEMM_TRY(check_alias(
+        w, {{Y, rows_bytes(M, ldy, N, type_size(type))}},
+        {{X, rows_bytes(M, ldx, cols, type_size(type))}, {W, rows_bytes(wide, ldw, K, 1)},
+         {w_scales, wide * 4}, {bias, bias != nullptr ? wide * 4 : 0},
+         {e.residual, e.residual != nullptr ? rows_bytes(M, e.ldr, N, type_size(type)) : 0}}));
     Int8Product p{};
     p.B = W;
     p.sb = w_scales;
@@ -253,7 +266,106 @@ int migemm_linear_int8(void *stream, const void *X, int type, int64_t ldx, const
     p.N = N;
     p.K = K;
     p.type = type;
+    p.act = e.activation;
+    p.gated = e.gated != 0;
+    p.residual = e.residual;
+    p.ldr = e.ldr;
     return launch_linear_int8((hipStream_t)stream, X, ldx, cols, p);
+}
+
+}  // namespace
+}  // namespace migemm
+
+using namespace migemm;
+
+extern "C" {
+
+int migemm_quantize_rows(void *stream, const void *X, int type, int64_t ldx, int8_t *values,
+                         int64_t ldv, float *scales, int rows, int cols) {
+    const char *w = "quantize_rows";
+    clear_error();
+    MIGEMM_TRY(check_pointers(w, {X, values, scales}));
+    MIGEMM_TRY(check_type(w, type));
+    MIGEMM_TRY(check_quantized(w, values, ldv, rows, cols));
+    MIGEMM_TRY(check_ld(w, "ldx", ldx, cols));
+    MIGEMM_TRY(check_alias(w, {{values, rows_bytes(rows, ldv, padded16(cols), 1)},
+                               {scales, (int64_t)rows * 4}},
+                           {{X, rows_bytes(rows, ldx, cols, type_size(type))}}));
+    return launch_quantize_rows((hipStream_t)stream, X, type, ldx, values, ldv, scales, rows,
+                                cols);
+}
+
+int migemm_norm_int8(void *stream, const void *X, int64_t ldx, const void *R, int64_t ldr,
+                     int type, const float *weight, float eps, void *S, int64_t lds,
+                     int8_t *values, int64_t ldv, float *scales, int rows, int cols) {
+    const char *w = "norm_int8";
+    clear_error();
+    MIGEMM_TRY(check_pointers(w, {X, values, scales}));
+    MIGEMM_TRY(check_type(w, type));
+    MIGEMM_TRY(check_quantized(w, values, ldv, rows, cols));
+    MIGEMM_TRY(check_ld(w, "ldx", ldx, cols));
+    if (R != nullptr) MIGEMM_TRY(check_ld(w, "ldr", ldr, cols));
+    if (S != nullptr) {
+        if (R == nullptr)
+            return set_error(MIGEMM_ERR_INVALID_ARG, "%s: a sum needs a residual", w);
+        MIGEMM_TRY(check_ld(w, "lds", lds, cols));
+    }
+    if (!(eps > 0.f && eps <= 3.4e38f))
+        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: eps=%g must be finite and > 0", w,
+                         (double)eps);
+    const int size = type_size(type);
+    MIGEMM_TRY(check_alias(
+        w, {{values, rows_bytes(rows, ldv, padded16(cols), 1)}, {scales, (int64_t)rows * 4},
+            {S, S != nullptr ? rows_bytes(rows, lds, cols, size) : 0}},
+        {{X, rows_bytes(rows, ldx, cols, size)},
+         {R, R != nullptr ? rows_bytes(rows, ldr, cols, size) : 0},
+         {weight, weight != nullptr ? (int64_t)cols * 4 : 0}}));
+    NormInt8 p{};
+    p.X = X;
+    p.R = R;
+    p.S = S;
+    p.weight = weight;
+    p.values = values;
+    p.scales = scales;
+    p.ldx = ldx;
+    p.ldr = ldr;
+    p.lds = lds;
+    p.ldv = ldv;
+    p.rows = rows;
+    p.cols = cols;
+    p.type = type;
+    p.eps = eps;
+    return launch_norm_int8((hipStream_t)stream, p);
+}
+
+int migemm_matmul_int8(void *stream, const int8_t *A, int64_t lda, const float *a_scales,
+                       const int8_t *B, int64_t ldb, const float *b_scales, const float *bias,
+                       void *C, int type, int64_t ldc, int M, int N, int K) {
+    return matmul_int8("matmul_int8", stream, A, lda, a_scales, B, ldb, b_scales, bias, C, type,
+                       ldc, M, N, K, Closing{});
+}
+
+int migemm_matmul_int8_ex(void *stream, const int8_t *A, int64_t lda, const float *a_scales,
+                          const int8_t *B, int64_t ldb, const float *b_scales, const float *bias,
+                          int activation, int gated, const void *residual, int64_t ldr, void *C,
+                          int type, int64_t ldc, int M, int N, int K) {
+    return matmul_int8("matmul_int8_ex", stream, A, lda, a_scales, B, ldb, b_scales, bias, C,
+                       type, ldc, M, N, K, Closing{activation, gated, residual, ldr});
+}
+
+int migemm_linear_int8(void *stream, const void *X, int type, int64_t ldx, const int8_t *W,
+                       int64_t ldw, const float *w_scales, const float *bias, void *Y,
+                       int64_t ldy, int M, int N, int cols) {
+    return linear_int8("linear_int8", stream, X, type, ldx, W, ldw, w_scales, bias, Y, ldy, M, N,
+                       cols, Closing{});
+}
+
+int migemm_linear_int8_ex(void *stream, const void *X, int type, int64_t ldx, const int8_t *W,
+                          int64_t ldw, const float *w_scales, const float *bias, int activation,
+                          int gated, const void *residual, int64_t ldr, void *Y, int64_t ldy,
+                          int M, int N, int cols) {
+    return linear_int8("linear_int8_ex", stream, X, type, ldx, W, ldw, w_scales, bias, Y, ldy, M,
+                       N, cols, Closing{activation, gated, residual, ldr});
 }
 
 int migemm_cache_tables(void *stream, const int *lengths, const int *counts, int requests,

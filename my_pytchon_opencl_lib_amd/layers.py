@@ -13,7 +13,7 @@ NnClGlob.LinearForward) is the bias-epilogue form.
 import numpy as np
 import torch
 
-from .nncl_glob import NnClGlob, ShapeError, _check_typed, _require
+from .nncl_glob import NnClGlob, ShapeError, _check_typed, _closing, _require
 
 
 class Linear:
@@ -54,15 +54,19 @@ class LinearInt8:
     """A Linear layer for serving, its weight held in 8 bits with a scale for each output:
     y[..., out] = x[..., in] @ weight^T (+ bias). weight [out, in] is a float tensor or array
     (e.g. Linear.weight), quantised here once; x and y are float32 or bfloat16. For inference: y
-    carries no gradient."""
+    carries no gradient. activation ("relu", "silu", "gelu", "gelu_tanh") and a residual given
+    with x are applied in the product's launch; gated: weight [2 * out, in] holds the rows of a
+    gate, then those that it multiplies: y = activation(gate) * up."""
 
-    def __init__(self, weight, bias=None, nnclglob=None):
+    def __init__(self, weight, bias=None, nnclglob=None, activation=None, gated=False):
         self.nnclglob = nnclglob if nnclglob is not None else NnClGlob()
         dev = self.nnclglob.device
         w = weight if isinstance(weight, torch.Tensor) else torch.as_tensor(
             np.asarray(weight, dtype=np.float32))
         _require(w.dim() == 2, "weight must be [out, in]")
-        self.out_channels, self.in_features = w.shape
+        rows, self.in_features = w.shape
+        self.out_channels, _ = _closing(rows, activation, gated)
+        self.activation, self.gated = activation, bool(gated)
         if w.dtype != torch.bfloat16:
             w = w.to(torch.float32)
         self.weight, self.scales = self.nnclglob.QuantizeRows(w.to(dev).contiguous())
@@ -70,15 +74,21 @@ class LinearInt8:
         if bias is not None:
             b = bias if isinstance(bias, torch.Tensor) else torch.as_tensor(np.asarray(bias))
             self.bias = b.to(dev, torch.float32).contiguous()
-            _check_typed("bias", self.bias, torch.float32, (self.out_channels,))
+            _check_typed("bias", self.bias, torch.float32, (rows,))
 
-    def forward(self, x):
+    def forward(self, x, residual=None):
         if not isinstance(x, torch.Tensor) or not x.dim() or x.shape[-1] != self.in_features:
             raise ShapeError(f"x must end in {self.in_features} features (got "
                              f"{list(getattr(x, 'shape', []))})")
-        return self.nnclglob.LinearInt8(x, self.weight, self.scales, self.bias)
+        return self.nnclglob.LinearInt8(x, self.weight, self.scales, self.bias, self.activation,
+                                        self.gated, residual)
 
     __call__ = forward
+
+    def forwardRows(self, values, scales, dtype=torch.float32, residual=None):
+        """The same layer over rows that are in 8 bits already (of QuantizeRows or NormInt8)."""
+        return self.nnclglob.MatmulInt8(values, scales, self.weight, self.scales, self.bias, dtype,
+                                        self.activation, self.gated, residual)
 
     def parameters(self):
         return [self.weight, self.scales] + ([self.bias] if self.bias is not None else [])

@@ -35,6 +35,7 @@ Deliberate differences from the reference, each an aliasing or safety fix:
     leaves unchecked (an out-of-bounds read there).
 """
 import ctypes
+import math
 import operator
 import struct
 
@@ -190,6 +191,35 @@ def _check_typed(name, t, dtype, shape=None, dim=None):
     raise ShapeError(f"{name} must have the shape {list(shape)} (got {list(t.shape)})"
                      if shape is not None else
                      f"{name} must have {dim} axes (got {list(t.shape)})")
+
+
+_ACTIVATIONS = {None: _native.MIGEMM_ACT_NONE, "relu": _native.MIGEMM_ACT_RELU,
+                "silu": _native.MIGEMM_ACT_SILU, "gelu": _native.MIGEMM_ACT_GELU,
+                "gelu_tanh": _native.MIGEMM_ACT_GELU_TANH}
+
+
+def _closing(wide, activation, gated):
+    """(columns of the output, (activation, gated) as the C entries take them; None for the product
+    alone) of a weight of `wide` rows."""
+    if activation is None and not gated:
+        return wide, None
+    if activation not in _ACTIVATIONS:
+        names = [a for a in _ACTIVATIONS if a]
+        raise ShapeError(f"activation must be None or one of {names} (got {activation!r})")
+    if gated and wide % 2:
+        raise ShapeError(f"a gated weight must have an even number of rows (got {wide})")
+    return wide // 2 if gated else wide, (_ACTIVATIONS[activation], int(bool(gated)))
+
+
+def _check_residual(t, out):
+    """A residual [rows, columns] of the output's type and shape; its rows may lie apart."""
+    if _check_rows("residual", t, 2) != _TYPES[out.dtype] or t.shape != out.shape:
+        raise ShapeError(f"residual must be {out.dtype} {list(out.shape)} (got {t.dtype} "
+                         f"{list(t.shape)})")
+
+
+def _residual_at(t):
+    return (None, 0) if t is None else (_ptr(t), _row_stride("residual", t))
 
 
 def _check_table(lengths, table):
@@ -539,10 +569,52 @@ class NnClGlob:
                     _row_stride("x", x2), _ptr(values), values.shape[1], _ptr(scales), rows, k)
         return values, scales
 
-    def MatmulInt8(self, a, aScales, b, bScales, bias=None, dtype=torch.float32):
-        """C[M, N] = (a[M, K] @ b[N, K]^T) * aScales[M] * bScales[N] (+ bias[N]) of dtype: int8
-        rows as QuantizeRows gives them (K a multiple of 16, at most 131071; rows may lie
-        further apart than K). The integer sum is exact."""
+    def NormInt8(self, x, weight=None, residual=None, eps=1e-6):
+        """(values, scales, sum) of the rows x[..., K] after a residual's addition: sum =
+        x + residual of x's type (x itself where residual is None), and in 8 bits, as
+        QuantizeRows lays them out, the rows of sum / sqrt(mean(sum^2) + eps) * weight (float32
+        [K]; None: ones). They are the a and aScales of MatmulInt8, and the sum is the residual of
+        what follows. residual has the shape of x; eps > 0."""
+        code = _check_rows("x", x)
+        k = x.shape[-1] if x.dim() else 0
+        if k < 1:
+            raise ShapeError(f"x must have rows of at least one value (got {list(x.shape)})")
+        eps = float(eps)
+        _require(0.0 < eps < math.inf, "eps must be finite and greater than 0")
+        x2 = x if x.dim() == 2 else x.reshape(-1, k)
+        rows = x2.shape[0]
+        operands = (x2,)
+        if weight is not None:
+            _check_typed("weight", weight, torch.float32, (k,))
+            operands += (weight,)
+        r2 = total = None
+        if residual is not None:
+            if _check_rows("residual", residual) != code or residual.shape != x.shape:
+                raise ShapeError(f"residual must be {x.dtype} {list(x.shape)} (got "
+                                 f"{residual.dtype} {list(residual.shape)})")
+            r2 = residual if x.dim() == 2 else residual.reshape(-1, k)
+            total = x.new_empty(x.shape)
+            operands += (r2, total)
+        values = x.new_empty((rows, (k + 15) // 16 * 16), dtype=torch.int8)
+        scales = x.new_empty(rows, dtype=torch.float32)
+        if rows:
+            _launch("migemm_norm_int8", operands + (values, scales), _ptr(x2),
+                    _row_stride("x", x2), _ptr(r2) if r2 is not None else None,
+                    _row_stride("residual", r2) if r2 is not None else 0, code,
+                    _ptr(weight) if weight is not None else None, eps,
+                    _ptr(total) if total is not None else None, k, _ptr(values),
+                    values.shape[1], _ptr(scales), rows, k)
+        return values, scales, x if total is None else total
+
+    def MatmulInt8(self, a, aScales, b, bScales, bias=None, dtype=torch.float32, activation=None,
+                   gated=False, residual=None):
+        """C[M, N] of dtype from c = (a[M, K] @ b[N, K]^T) * aScales[M] * bScales[N] (+ bias[N]):
+        int8 rows as QuantizeRows or NormInt8 gives them (K a multiple of 16, at most 131071; rows
+        may lie further apart than K). The integer sum is exact. In the same launch:
+        activation ("relu", "silu", "gelu", "gelu_tanh"; None: C = c) gives C = activation(c);
+        gated C = activation(gate) * up, with b [2N, K] (bScales and bias [2N]): N rows of the
+        gate, then N of up; residual [M, N] of dtype is added to either. All of it is float32,
+        rounded to dtype once."""
         if dtype not in _TYPES:
             raise ShapeError(f"dtype must be float32 or bfloat16 (got {dtype})")
         for name, t in (("a", a), ("b", b)):
@@ -552,48 +624,75 @@ class NnClGlob:
                                  f"{list(t.shape)})")
             _require(t.is_cuda, f"{name} must live on the GPU: there is no CPU fallback")
         m, k = a.shape
-        n = b.shape[0]
+        wide = b.shape[0]
         if b.shape[1] != k:
             raise ShapeError(f"inner dimensions differ: {k} != {b.shape[1]}")
         _check_typed("aScales", aScales, torch.float32, (m,))
-        _check_typed("bScales", bScales, torch.float32, (n,))
+        _check_typed("bScales", bScales, torch.float32, (wide,))
         if bias is not None:
-            _check_typed("bias", bias, torch.float32, (n,))
+            _check_typed("bias", bias, torch.float32, (wide,))
+        n, closing = _closing(wide, activation, gated)
         c = torch.empty((m, n), dtype=dtype, device=a.device)
+        if residual is not None:
+            _check_residual(residual, c)
         if m and n:
             if not k:
                 raise ShapeError("K must be at least 1")
             extra = (bias,) if bias is not None else ()
-            _launch("migemm_matmul_int8", (a, b, aScales, bScales, c) + extra, _ptr(a),
-                    _row_stride("a", a), _ptr(aScales), _ptr(b), _row_stride("b", b),
-                    _ptr(bScales), _ptr(bias) if bias is not None else None, _ptr(c),
-                    _TYPES[dtype], n, m, n, k)
+            product = (_ptr(a), _row_stride("a", a), _ptr(aScales), _ptr(b), _row_stride("b", b),
+                       _ptr(bScales), _ptr(bias) if bias is not None else None)
+            out = (_ptr(c), _TYPES[dtype], n, m, n, k)
+            if closing is None and residual is None:
+                _launch("migemm_matmul_int8", (a, b, aScales, bScales, c) + extra, *product, *out)
+            else:
+                if residual is not None:
+                    extra += (residual,)
+                _launch("migemm_matmul_int8_ex", (a, b, aScales, bScales, c) + extra, *product,
+                        *(closing or (0, 0)), *_residual_at(residual), *out)
         return c
 
-    def LinearInt8(self, x, weight, scales, bias=None):
-        """y[..., N] = x[..., K] @ W^T (+ bias[N], float32) with W [N, K] as QuantizeRows left
+    def LinearInt8(self, x, weight, scales, bias=None, activation=None, gated=False,
+                   residual=None):
+        """y[..., N] from x[..., K] @ W^T (+ bias[N], float32) with W [N, K] as QuantizeRows left
         it (weight int8 [N, K rounded up to 16], scales [N]); the rows of x are quantised on
-        the way. y has the type of x. One launch where rows * ceil(K / 4096) <= 3; otherwise
+        the way. y has the type of x. activation, gated (W [2N, K]) and residual (y's shape and
+        type) as MatmulInt8's. One launch where rows * ceil(K / 4096) <= 3; otherwise
         the quantised rows go through the stream's workspace (reserve_workspace before a
         capture). For inference: the result carries no gradient."""
         code = _check_rows("x", x)
         _check_typed("weight", weight, torch.int8, dim=2)
-        n, kp = weight.shape
+        wide, kp = weight.shape
         k = x.shape[-1] if x.dim() else 0
         if k < 1 or (k + 15) & -16 != kp:
             raise ShapeError(f"x must end in the weight's features (got {list(x.shape)} and "
                              f"rows of {kp} bytes)")
-        _check_typed("scales", scales, torch.float32, (n,))
+        _check_typed("scales", scales, torch.float32, (wide,))
         if bias is not None:
-            _check_typed("bias", bias, torch.float32, (n,))
+            _check_typed("bias", bias, torch.float32, (wide,))
+        n, closing = _closing(wide, activation, gated)
         x2 = x if x.dim() == 2 else x.reshape(-1, k)
         m = x2.shape[0]
         y = x.new_empty((m, n))
+        if residual is not None:
+            if x.dim() != 2:
+                _check_rows("residual", residual)
+                if residual.shape != x.shape[:-1] + (n,):
+                    raise ShapeError(f"residual must be {list(x.shape[:-1]) + [n]} (got "
+                                     f"{list(residual.shape)})")
+                residual = residual.reshape(m, n)
+            _check_residual(residual, y)
         if m and n:
             extra = (bias,) if bias is not None else ()
-            _launch("migemm_linear_int8", (x2, weight, scales, y) + extra, _ptr(x2), code,
-                    _row_stride("x", x2), _ptr(weight), kp, _ptr(scales),
-                    _ptr(bias) if bias is not None else None, _ptr(y), n, m, n, k)
+            layer = (_ptr(x2), code, _row_stride("x", x2), _ptr(weight), kp, _ptr(scales),
+                     _ptr(bias) if bias is not None else None)
+            out = (_ptr(y), n, m, n, k)
+            if closing is None and residual is None:
+                _launch("migemm_linear_int8", (x2, weight, scales, y) + extra, *layer, *out)
+            else:
+                if residual is not None:
+                    extra += (residual,)
+                _launch("migemm_linear_int8_ex", (x2, weight, scales, y) + extra, *layer,
+                        *(closing or (0, 0)), *_residual_at(residual), *out)
         return y if x.dim() == 2 else y.reshape(list(x.shape[:-1]) + [n])
 
     def CacheTables(self, lengths, counts, table, free, freeCount, tokens, pageSize):
