@@ -158,6 +158,8 @@ SIGNATURES = {
                                _vp, _i32, _i64, _i32, _i32, _i32], _i32),
     "migemm_linear_int8_ex": ([_vp, _vp, _i32, _i64, _vp, _i64, _vp, _vp, _i32, _i32, _vp, _i64,
                                _vp, _i64, _i32, _i32, _i32], _i32),
+    "migemm_sample": ([_vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _f32, _vp, _i32, _vp, _f32,
+                       _vp, _f32, _vp, _vp], _i32),
     "migemm_cache_tables": ([_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32] +
                             [_vp] * 5 + [_i32], _i32),
     "migemm_cache_slots": ([_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _i32], _i32),

@@ -76,6 +76,23 @@ struct CacheAttention {
 };
 int launch_cache_attention(hipStream_t stream, const CacheAttention &a);
 
+struct SampleArgs {
+    const void *logits;
+    int64_t ld;
+    int rows, vocab, type;
+    const float *uniforms;
+    // a value for each row, or (null) one for all
+    const float *temperatures, *top_ps, *min_ps;
+    const int *top_ks;
+    float temperature, top_p, min_p;
+    int top_k;
+    int *tokens;
+    float *probabilities;
+    int bits;  // weights are integers of this many fractional bits
+    double unit;
+};
+int launch_sample(hipStream_t stream, const SampleArgs &a);
+
 #ifdef __HIPCC__
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));

@@ -553,6 +553,60 @@ int migemm_cache_attention(void *stream, const void *Q, int type, int64_t ldq,
     return launch_cache_attention((hipStream_t)stream, a);
 }
 
+int migemm_sample(void *stream, const void *logits, int type, int64_t ld, int rows, int vocab,
+                  const float *uniforms, const float *temperatures, float temperature,
+                  const int *top_ks, int top_k, const float *top_ps, float top_p,
+                  const float *min_ps, float min_p, int *tokens, float *probabilities) {
+    const char *w = "sample";
+    clear_error();
+    MIGEMM_TRY(check_pointers(w, {logits, uniforms, tokens, probabilities}));
+    MIGEMM_TRY(check_type(w, type));
+    if (rows < 1 || vocab < 1)
+        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: sizes must be >= 1 (rows=%d vocab=%d)", w,
+                         rows, vocab);
+    if (vocab > 1 << 20)
+        return set_error(MIGEMM_ERR_UNSUPPORTED, "%s: vocab=%d, must be at most 2^20", w, vocab);
+    MIGEMM_TRY(check_ld(w, "ld", ld, vocab));
+    MIGEMM_TRY(check_grid(w, rows, 1024));
+    if (temperatures == nullptr && !(temperature >= 0.f && temperature <= 3.4e38f))
+        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: temperature=%g must be finite and >= 0", w,
+                         (double)temperature);
+    if (top_ks == nullptr && top_k < 0)
+        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: top_k=%d must be >= 0", w, top_k);
+    if (top_ps == nullptr && !(top_p > 0.f && top_p <= 1.f))
+        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: top_p=%g must be in (0, 1]", w,
+                         (double)top_p);
+    if (min_ps == nullptr && !(min_p >= 0.f && min_p <= 1.f))
+        return set_error(MIGEMM_ERR_INVALID_ARG, "%s: min_p=%g must be in [0, 1]", w,
+                         (double)min_p);
+    const int64_t r4 = (int64_t)rows * 4;
+    MIGEMM_TRY(check_alias(w, {{tokens, r4}, {probabilities, r4}},
+                           {{logits, rows_bytes(rows, ld, vocab, type_size(type))},
+                            {uniforms, r4},
+                            {temperatures, temperatures != nullptr ? r4 : 0},
+                            {top_ks, top_ks != nullptr ? r4 : 0},
+                            {top_ps, top_ps != nullptr ? r4 : 0},
+                            {min_ps, min_ps != nullptr ? r4 : 0}}));
+    SampleArgs p{};
+    p.logits = logits;
+    p.ld = ld;
+    p.rows = rows;
+    p.vocab = vocab;
+    p.type = type;
+    p.uniforms = uniforms;
+    p.temperatures = temperatures;
+    p.top_ks = top_ks;
+    p.top_ps = top_ps;
+    p.min_ps = min_ps;
+    p.temperature = temperature;
+    p.top_k = top_k;
+    p.top_p = top_p;
+    p.min_p = min_p;
+    p.tokens = tokens;
+    p.probabilities = probabilities;
+    return launch_sample((hipStream_t)stream, p);
+}
+
 }  // extern "C"
 
 namespace migemm {

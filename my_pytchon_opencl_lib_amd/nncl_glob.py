@@ -193,6 +193,8 @@ def _check_typed(name, t, dtype, shape=None, dim=None):
                      f"{name} must have {dim} axes (got {list(t.shape)})")
 
 
+_MOST = torch.finfo(torch.float32).max
+
 _ACTIVATIONS = {None: _native.MIGEMM_ACT_NONE, "relu": _native.MIGEMM_ACT_RELU,
                 "silu": _native.MIGEMM_ACT_SILU, "gelu": _native.MIGEMM_ACT_GELU,
                 "gelu_tanh": _native.MIGEMM_ACT_GELU_TANH}
@@ -813,3 +815,43 @@ class NnClGlob:
                     dim ** -0.5 if scale is None else float(scale), int(maxCount),
                     int(maxLength), _ptr(o))
         return o
+
+    def Sample(self, logits, uniforms, temperature=1.0, topK=0, topP=1.0, minP=0.0):
+        """(tokens int32 [rows], probabilities float32 [rows]): a token for each row of logits
+        [rows, vocabulary] (float32 or bfloat16, at most 2^20 tokens) from its random number
+        uniforms [rows] in [0, 1) (float32). Tokens stand by logit, largest first, equal ones by
+        index, and weigh w = exp((logit - largest) / temperature). minP: those with w < minP weigh
+        nothing; topK: so do those beyond the first topK (0: no limit); topP: of the others the
+        fewest are kept that hold topP of their sum. The token is the first whose weights up to
+        its own are more than uniform times the kept ones' sum; its probability is its share of
+        that. temperature 0: the largest logit's first token. Every parameter is a number, or a
+        tensor [rows] (float32; topK int32) with one for each row. Rows that allow no token (all
+        -inf), that hold a NaN, or whose tensors' parameters are NaN or a temperature negative or
+        infinite give token -1 and probability 0."""
+        code = _check_rows("logits", logits, 2)
+        rows, vocab = logits.shape
+        _check_typed("uniforms", uniforms, torch.float32, (rows,))
+        operands = (logits, uniforms)
+        params = []
+        for name, v, dtype, low, high in (("temperature", temperature, torch.float32, 0, _MOST),
+                                          ("topK", topK, torch.int32, 0, 2 ** 31 - 1),
+                                          ("topP", topP, torch.float32, 0, 1),
+                                          ("minP", minP, torch.float32, 0, 1)):
+            if isinstance(v, torch.Tensor):
+                _check_typed(name, v, dtype, (rows,))
+                operands += (v,)
+                params += (_ptr(v), 0)
+            else:
+                v = operator.index(v) if dtype is torch.int32 else float(v)
+                if not low <= v <= high:
+                    raise ShapeError(f"{name} must be in {low}..{high} (got {v})")
+                params += (None, v)
+        if not vocab:
+            raise ShapeError("logits must have at least one token")
+        tokens = logits.new_empty(rows, dtype=torch.int32)
+        probabilities = logits.new_empty(rows, dtype=torch.float32)
+        if rows:
+            _launch("migemm_sample", operands + (tokens, probabilities), _ptr(logits), code,
+                    _row_stride("logits", logits), rows, vocab, _ptr(uniforms), *params,
+                    _ptr(tokens), _ptr(probabilities))
+        return tokens, probabilities

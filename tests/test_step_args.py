@@ -1,5 +1,5 @@
 """CPU tests of the argument checks of the operators that close a decoder's step in 8 bits: the
-norm and the products with activation, gate and residual. Every C entry refuses bad
+norm, the products with activation, gate and residual, and sampling. Every C entry refuses bad
 arguments with a message before it touches HIP (the pointers here are never followed), and the
 Python operators refuse CPU tensors."""
 import pytest
@@ -23,13 +23,17 @@ def entries():
                N=9, K=48)
     lin = dict(stream=None, X=P(0), type=1, ldx=50, W=P(1), ldw=64, w_scales=P(2), bias=P(5),
                activation=4, gated=1, residual=P(6), ldr=9, Y=P(3), ldy=9, M=7, N=9, cols=50)
-    return {"norm_int8": norm, "matmul_int8_ex": mat, "linear_int8_ex": lin}
+    sam = dict(stream=None, logits=P(0), type=1, ld=100, rows=3, vocab=100, uniforms=P(1),
+               temperatures=P(2), temperature=0.0, top_ks=P(3), top_k=0, top_ps=P(4), top_p=0.0,
+               min_ps=P(5), min_p=0.0, tokens=P(6), probabilities=P(7))
+    return {"norm_int8": norm, "matmul_int8_ex": mat, "linear_int8_ex": lin, "sample": sam}
 
 
 OPTIONAL = {"norm_int8": ("R", "weight", "S"), "matmul_int8_ex": ("bias", "residual"),
-            "linear_int8_ex": ("bias", "residual")}
+            "linear_int8_ex": ("bias", "residual"),
+            "sample": ("temperatures", "top_ks", "top_ps", "min_ps")}
 OUTPUTS = {"norm_int8": ["S", "values", "scales"], "matmul_int8_ex": ["C"],
-           "linear_int8_ex": ["Y"]}
+           "linear_int8_ex": ["Y"], "sample": ["tokens", "probabilities"]}
 
 
 def refused(lib, name, code, fragment, **change):
@@ -107,6 +111,23 @@ def test_closings(lib):
     refused(lib, "linear_int8_ex", UNSUPPORTED, "131071", cols=131071, ldx=131071, ldw=131072)
 
 
+def test_sample(lib):
+    for bad in (dict(rows=0), dict(vocab=0), dict(rows=-1)):
+        refused(lib, "sample", INVALID, "sizes must be >= 1", **bad)
+    refused(lib, "sample", UNSUPPORTED, "2^20", vocab=(1 << 20) + 1, ld=1 << 21)
+    refused(lib, "sample", UNSUPPORTED, "exceed one launch", rows=1 << 22)
+    for ld in (99, -100, (1 << 28) + 1):
+        refused(lib, "sample", INVALID, "ld", ld=ld)
+    nan, inf = float("nan"), float("inf")
+    for v in (-1.0, inf, nan):
+        refused(lib, "sample", INVALID, "temperature", temperatures=None, temperature=v)
+    refused(lib, "sample", INVALID, "top_k", top_ks=None, top_k=-1)
+    for v in (0.0, -1.0, 1.01, nan):
+        refused(lib, "sample", INVALID, "top_p", top_ps=None, top_p=v)
+    for v in (-0.01, 1.01, nan):
+        refused(lib, "sample", INVALID, "min_p", min_ps=None, min_p=v)
+
+
 def test_python_operators_refuse_cpu_tensors():
     import torch
     from my_pytchon_opencl_lib_amd import NnClGlob, ShapeError
@@ -115,6 +136,7 @@ def test_python_operators_refuse_cpu_tensors():
     for call in (lambda: g.NormInt8(x), lambda: g.NormInt8(x, residual=x),
                  lambda: g.MatmulInt8(x.to(torch.int8), x[:, 0], x.to(torch.int8), x[:, 0],
                                       activation="silu"),
-                 lambda: g.LinearInt8(x, x.to(torch.int8), x[:, 0], gated=True)):
+                 lambda: g.LinearInt8(x, x.to(torch.int8), x[:, 0], gated=True),
+                 lambda: g.Sample(x, x[:, 0])):
         with pytest.raises(ShapeError, match="no CPU fallback"):
             call()
