@@ -572,8 +572,8 @@ int migemm_cache_attention(void *stream, const void *Q, int type, int64_t ldq,
  * sum. probabilities[r] is its weight over that sum. temperature 0 gives the largest logit's
  * first token, with probability 1. Each parameter is one for all rows, or (temperatures, top_ks,
  * top_ps, min_ps [rows] on the GPU, where not NULL) one a row. Weights are 64-bit numbers rounded to 2^-42
- * of the largest or finer; their sums are exact. A logit of -inf is never chosen (inf
- * weighs 1, everything else then nothing); a row without a logit above -inf, with a NaN, or with
+ * of the largest or finer; their sums are exact. A logit of -inf is never chosen, inf counts as the
+ * largest float32; a row without a logit above -inf, with a NaN, or with
  * a parameter that is NaN or a temperature that is negative or not finite gives token -1 and
  * probability 0. */
 int migemm_sample(void *stream, const void *logits, int type, int64_t ld, int rows, int vocab,
