@@ -107,6 +107,7 @@ struct Weights {
     double rate;     // log2(e) / T
     double width;    // of a bin, in log2 of the weight
     double cut;      // l - top below which a token weighs nothing
+    float least;     // the smallest logit that is not below it
     double unit;     // 2^bits
 
     __device__ __forceinline__ void init(const SampleArgs &p, float high, float low,
@@ -138,6 +139,21 @@ struct Weights {
         top = high * scale;
         bins = (float)(per / (double)scale);
         width = bins > 0.f ? rate / ((double)bins * (double)scale) : 0.0;
+        least = smallest(kBins - 1);
+    }
+    // The smallest logit of bins 0 .. b, by all lanes of a wavefront: bin and cut go by the order
+    // of logits, so 64 of them at a time narrow it down.
+    __device__ __forceinline__ float smallest(uint32_t b) const {
+        uint32_t lo = order_of((float)top64), hi = order_of(-kMost);
+        while (hi > lo) {
+            const uint32_t step = (hi - lo) / 64 + 1;
+            const u64 at = lo + (u64)step * (threadIdx.x & 63);
+            const float l = logit_of((at < hi ? at : hi) << kIndexBits);
+            const int in = __popcll(__ballot(at <= hi && bin(l) <= b && below(l) >= cut));
+            lo += step * (in - 1);
+            hi = (u64)lo + step - 1 < hi ? lo + step - 1 : hi;
+        }
+        return logit_of((u64)lo << kIndexBits);
     }
     __device__ __forceinline__ double below(float l) const { return (double)l - top64; }
     // (two roundings, each of which keeps the order)
@@ -180,7 +196,10 @@ struct Asked {
         valid = temperature >= 0.f && temperature < INFINITY && top_p == top_p &&
                 min_p == min_p && uniform == uniform;
     }
+    __device__ __forceinline__ bool wide() const { return temperature > 2.f; }
     __device__ __forceinline__ bool greedy() const { return temperature == 0.f || top_k == 1; }
+    // Whether the row's histogram holds numbers: top-k comes first.
+    __device__ __forceinline__ bool counted(int n) const { return top_k > 0 && top_k < n; }
     // The running weight that ends the tokens that top-p keeps of a sum, and the one to draw.
     __device__ __forceinline__ u64 kept(u64 total) const {
         const u64 t = (u64)ceil((double)fmaxf(top_p, 0.f) * (double)total);
@@ -213,24 +232,33 @@ __device__ __forceinline__ void each(const T *row, int first, int end, const F &
     }
 }
 
-// The largest logit and the smallest above -inf of a range, and whether one is NaN, in every lane.
+// The largest logit of a range and whether one is NaN, in every lane, and with `wide` the smallest
+// above -inf (otherwise it is -inf). At low temperatures the logits that weigh something span
+// less than all of them, so the smallest does not matter, and costs half of the pass.
 template <int THREADS, typename T>
-__device__ __forceinline__ void extremes(const T *row, int first, int end, float &high, float &low,
-                                         bool &nan) {
+__device__ __forceinline__ void extremes(const T *row, int first, int end, bool wide, float &high,
+                                         float &low, bool &nan) {
     high = -INFINITY;
-    low = INFINITY;
+    low = wide ? INFINITY : -INFINITY;
     nan = false;
-    each<THREADS>(row, first, end, [&](float x, int) {
-        nan |= x != x;
-        const float l = bounded(x);
-        high = fmaxf(high, l);
-        low = l > -INFINITY ? fminf(low, l) : low;
-    });
+    if (wide)
+        each<THREADS>(row, first, end, [&](float x, int) {
+            nan |= x != x;
+            high = fmaxf(high, x);
+            low = x > -INFINITY ? fminf(low, x) : low;
+        });
+    else
+        each<THREADS>(row, first, end, [&](float x, int) {
+            nan |= x != x;
+            high = fmaxf(high, x);
+        });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         high = fmaxf(high, __shfl_xor(high, o));
         low = fminf(low, __shfl_xor(low, o));
     }
+    high = bounded(high);
+    low = fminf(low, kMost);
     nan = __ballot(nan) != 0;
 }
 
@@ -240,13 +268,32 @@ template <bool COUNT, typename T>
 __device__ __forceinline__ void fill(u64 *mass, const T *row, int first, int end, const Weights &w,
                                      u64 limit) {
     each<kThreads>(row, first, end, [&](float x, int i) {
+        if (!(x >= w.least)) return;
         const float l = bounded(x);
-        const double d = w.below(l);
-        if (!(d >= w.cut)) return;
         if (limit != ~(u64)0 && key_of(l, i) > limit) return;
         const uint32_t b = w.bin(l);
-        atomicAdd(&mass[b], COUNT ? (u64)1 : w.over_middle(d, b));
+        atomicAdd(&mass[b], COUNT ? (u64)1 : w.over_middle(w.below(l), b));
     });
+}
+
+// Running sums over a wavefront's lanes (within rows of 16, then over the rows).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 moved(u64 x) {
+    return (u64)moved<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | moved<CTRL, ROWS>((uint32_t)x);
+}
+template <typename N>
+__device__ __forceinline__ N run_up_lanes(N x) {
+    x += moved<0x111, 0xf>(x);
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
+    x += moved<0x142, 0xa>(x);
+    x += moved<0x143, 0xc>(x);
+    return x;
 }
 
 // Running sums of 2 * kThreads masses (and counts), in place. Ends with a barrier.
@@ -254,29 +301,23 @@ template <bool COUNTS>
 __device__ __forceinline__ void run_up(Shared &s, u64 *mass, uint32_t *count) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const u64 m1 = mass[2 * tid + 1];
-    u64 m = mass[2 * tid] + m1;
+    u64 m = run_up_lanes(mass[2 * tid] + m1);
     uint32_t c = 0, c1 = 0;
     if (COUNTS) {
         c1 = count[2 * tid + 1];
-        c = count[2 * tid] + c1;
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 pm = __shfl_up(m, o);
-        if (lane >= o) m += pm;
-        if (COUNTS) {
-            const uint32_t pc = __shfl_up(c, o);
-            if (lane >= o) c += pc;
-        }
+        c = run_up_lanes(count[2 * tid] + c1);
     }
     if (lane == 63) {
         s.wave_mass[wave] = m;
         s.wave_count[wave] = c;
     }
     __syncthreads();
-    for (int w = 0; w < wave; ++w) {
-        m += s.wave_mass[w];
-        c += s.wave_count[w];
+    // the sums of the wavefronts before: each lane of a row of 16 takes one
+    const u64 wm = run_up_lanes(lane < wave ? s.wave_mass[lane & (kWaves - 1)] : 0);
+    m += __shfl(wm, kWaves - 1);
+    if (COUNTS) {
+        const uint32_t wc = run_up_lanes(lane < wave ? s.wave_count[lane & (kWaves - 1)] : 0);
+        c += __shfl(wc, kWaves - 1);
     }
     mass[2 * tid] = m - m1;
     mass[2 * tid + 1] = m;
@@ -405,22 +446,21 @@ struct Row {
         hi = hi < limit ? hi : limit;
         if (tid == 0) s.listed = 0;
         __syncthreads();
-        const auto take = [&](float l, u64 key) {
+        const auto take = [&](u64 key) {
             if (key < lo || key > hi) return;
             const uint32_t place = atomicAdd(&s.listed, 1u);
             if (place < kList) s.list[place] = key;
         };
         if (given != nullptr) {
             for (int i = tid; i < gathered; i += kThreads) {
-                const float l = logit_of(given[i]);
-                const int at = (int)w.bin(l);
-                if (at >= a && at <= b) take(l, given[i]);
+                const int at = (int)w.bin(logit_of(given[i]));
+                if (at >= a && at <= b) take(given[i]);
             }
         } else {
+            const float from = w.smallest(b);
+            const float below = a ? w.smallest(a - 1) : INFINITY;
             each<kThreads>(logits, 0, n, [&](float x, int i) {
-                const float l = bounded(x);
-                const int at = (int)w.bin(l);
-                if (at >= a && at <= b && w.below(l) >= w.cut) take(l, key_of(l, i));
+                if (x >= from && (x < below || a == 0)) take(key_of(bounded(x), i));
             });
         }
         __syncthreads();
@@ -463,7 +503,7 @@ struct Row {
             __syncthreads();
             each<kThreads>(logits, 0, n, [&](float x, int i) {
                 const float l = bounded(x);
-                if ((int)w.bin(l) != b || !(w.below(l) >= w.cut)) return;
+                if ((int)w.bin(l) != b || !(l >= w.least)) return;
                 const u64 key = key_of(l, i);
                 if (key < lo || key > hi || key > limit) return;
                 const int at = (int)((key - lo) >> shift);
@@ -553,7 +593,8 @@ __device__ __forceinline__ void nothing(const SampleArgs &p, int r) {
 
 // ------------------------------------------------------------- a row in one work-group
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleArgs p) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4)))
+sample_row_kernel(SampleArgs p) {
     __shared__ Shared s;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = blockIdx.x, n = p.vocab;
@@ -565,7 +606,7 @@ __global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleArgs p) {
         s.bad = 0;
         s.found = n;
     }
-    extremes<kThreads>(logits, 0, n, high, low, nan);
+    extremes<kThreads>(logits, 0, n, q.wide(), high, low, nan);
     if (lane == 0) {
         s.high[wave] = high;
         s.low[wave] = low;
@@ -594,7 +635,7 @@ __global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleArgs p) {
     }
     Weights w;
     w.init(p, high, low, q.temperature, q.min_p);
-    const bool counted = q.top_k > 0 && q.top_k < n;
+    const bool counted = q.counted(n);
     if (counted)
         fill<true>(s.mass, logits, 0, n, w, ~(u64)0);
     else
@@ -607,6 +648,214 @@ __global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleArgs p) {
     Row<T> row{s, logits, n, nullptr, 0, w, ~(u64)0, false, 1, 0, 0};
     row.answer(p, r, q, counted, plan_of(s, q, counted));
 }
+// ------------------------------------------------------------- rows cut over work-groups
+// Four launches: the largest logit of each part of a row; the parts' histograms, added up; the tokens
+// of the bins that the answer may need; and the answer, from the histogram and those tokens. Each
+// work-group of the last two reads the whole histogram and plans the same. A row that the list does
+// not hold is walked by the last kernel's work-group alone.
+struct SplitArgs {
+    SampleArgs p;
+    int splits, chunk;  // parts of a row, tokens of a part
+    u64 *mass;          // [rows][kBins]
+    u64 *list;          // [rows][kList]
+    float4 *parts;      // [rows][splits]: largest, smallest, whether one is NaN
+    uint32_t *listed;   // [rows]
+    uint32_t *best;     // [rows]: where the largest logit stands first
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sample_top_kernel(SplitArgs a) {
+    __shared__ float highs[kWaves], lows[kWaves];
+    __shared__ int bad;
+    const SampleArgs &p = a.p;
+    const int tid = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
+    const T *logits = static_cast<const T *>(p.logits) + (int64_t)r * p.ld;
+    for (int i = part * kThreads + tid; i < kBins; i += a.splits * kThreads)
+        a.mass[(int64_t)r * kBins + i] = 0;
+    if (part == 0 && tid == 0) {
+        a.listed[r] = 0;
+        a.best[r] = ~0u;
+    }
+    if (tid == 0) bad = 0;
+    const int first = part * a.chunk, end = min(first + a.chunk, p.vocab);
+    float high, low;
+    bool nan;
+    extremes<kThreads>(logits, first, end, Asked(p, r).wide(), high, low, nan);
+    if ((tid & 63) == 0) {
+        highs[tid >> 6] = high;
+        lows[tid >> 6] = low;
+    }
+    __syncthreads();
+    if (nan) bad = 1;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < kWaves; ++w) {
+            high = fmaxf(high, highs[w]);
+            low = fminf(low, lows[w]);
+        }
+        a.parts[(int64_t)r * a.splits + part] = make_float4(high, low, bad ? 1.f : 0.f, 0.f);
+    }
+}
+
+// A row's extremes from its parts', in every lane; false where there is nothing to choose from.
+__device__ __forceinline__ bool joined(const SplitArgs &a, int r, const Asked &q, float &high,
+                                       float &low) {
+    const int lane = threadIdx.x & 63;
+    float4 x = make_float4(-INFINITY, INFINITY, 0.f, 0.f);
+    if (lane < a.splits) x = a.parts[(int64_t)r * a.splits + lane];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        x.x = fmaxf(x.x, __shfl_xor(x.x, o));
+        x.y = fminf(x.y, __shfl_xor(x.y, o));
+    }
+    high = x.x;
+    low = x.y;
+    return q.valid && __ballot(x.z != 0.f) == 0 && high > -INFINITY;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sample_bins_kernel(SplitArgs a) {
+    __shared__ u64 mass[kBins];
+    const SampleArgs &p = a.p;
+    const int tid = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
+    const T *logits = static_cast<const T *>(p.logits) + (int64_t)r * p.ld;
+    const Asked q(p, r);
+    float high, low;
+    if (!joined(a, r, q, high, low) || q.greedy()) return;
+    Weights w;
+    w.init(p, high, low, q.temperature, q.min_p);
+    for (int i = tid; i < kBins; i += kThreads) mass[i] = 0;
+    __syncthreads();
+    const int first = part * a.chunk, end = min(first + a.chunk, p.vocab);
+    if (q.counted(p.vocab))
+        fill<true>(mass, logits, first, end, w, ~(u64)0);
+    else
+        fill<false>(mass, logits, first, end, w, ~(u64)0);
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kThreads)
+        if (mass[i] != 0) atomicAdd(&a.mass[(int64_t)r * kBins + i], mass[i]);
+}
+
+// The running sums of a row's histogram.
+__device__ __forceinline__ void load_bins(Shared &s, const SplitArgs &a, int r, const Weights &w,
+                                          bool counted) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = a.mass[(int64_t)r * kBins + i];
+    if (counted)
+        finish<true>(s, w);
+    else
+        finish<false>(s, w);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sample_gather_kernel(SplitArgs a) {
+    __shared__ Shared s;
+    const SampleArgs &p = a.p;
+    const int tid = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
+    const T *logits = static_cast<const T *>(p.logits) + (int64_t)r * p.ld;
+    const Asked q(p, r);
+    float high, low;
+    if (!joined(a, r, q, high, low)) return;
+    const int first = part * a.chunk, end = min(first + a.chunk, p.vocab);
+    const float mine = a.parts[(int64_t)r * a.splits + part].x;
+    if (q.greedy()) {
+        if (mine != high) return;
+        uint32_t best = ~0u;
+        each<kThreads>(logits, first, end, [&](float x, int i) {
+            best = bounded(x) == high && (uint32_t)i < best ? i : best;
+        });
+        if (best != ~0u) atomicMin(&a.best[r], best);
+        return;
+    }
+    Weights w;
+    w.init(p, high, low, q.temperature, q.min_p);
+    const bool counted = q.counted(p.vocab);
+    load_bins(s, a, r, w, counted);
+    const Plan plan = plan_of(s, q, counted);
+    if (!plan.listed) return;
+    // the bins to draw from, and the one where top-p ends, which is not before them
+    const int lowest = plan.whole || plan.kept >= plan.last ? plan.kept : plan.last;
+    const float from = w.smallest(lowest);
+    if (!(mine >= from)) return;
+    if (tid == 0) s.listed = 0;
+    __syncthreads();
+    each<kThreads>(logits, first, end, [&](float x, int i) {
+        if (!(x >= from)) return;
+        const float l = bounded(x);
+        if (!plan.has((int)w.bin(l))) return;
+        const uint32_t place = atomicAdd(&s.listed, 1u);
+        if (place < kList) s.list[place] = key_of(l, i);
+    });
+    __syncthreads();
+    const uint32_t found = min(s.listed, (uint32_t)kList);
+    if (found == 0) return;
+    if (tid == 0) s.found = atomicAdd(&a.listed[r], found);
+    __syncthreads();
+    const uint32_t to = s.found;
+    for (uint32_t i = tid; i < found && to + i < kList; i += kThreads)
+        a.list[(int64_t)r * kList + to + i] = s.list[i];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sample_pick_kernel(SplitArgs a) {
+    __shared__ Shared s;
+    const SampleArgs &p = a.p;
+    const int r = blockIdx.x;
+    const T *logits = static_cast<const T *>(p.logits) + (int64_t)r * p.ld;
+    const Asked q(p, r);
+    float high, low;
+    if (!joined(a, r, q, high, low)) return nothing(p, r);
+    if (q.greedy()) {
+        if (threadIdx.x == 0) {
+            p.tokens[r] = (int)a.best[r];
+            p.probabilities[r] = 1.f;
+        }
+        return;
+    }
+    Weights w;
+    w.init(p, high, low, q.temperature, q.min_p);
+    const bool counted = q.counted(p.vocab);
+    load_bins(s, a, r, w, counted);
+    const Plan plan = plan_of(s, q, counted);
+    const u64 *given = plan.listed ? a.list + (int64_t)r * kList : nullptr;
+    const int gathered = plan.listed ? (int)min(a.listed[r], (uint32_t)kList) : 0;
+    Row<T> row{s, logits, p.vocab, given, gathered, w, ~(u64)0, false, 1, 0, 0};
+    row.answer(p, r, q, counted, plan);
+}
+
+template <typename T>
+int launch_split(hipStream_t stream, SplitArgs a) {
+    const SampleArgs &p = a.p;
+    const size_t row = (kBins + kList) * sizeof(u64) + a.splits * sizeof(float4) + 8;
+    int rc = MIGEMM_OK;
+    a.mass = static_cast<u64 *>(workspace(stream, p.rows * row, &rc, 0));
+    if (a.mass == nullptr) return rc;
+    a.list = a.mass + (int64_t)p.rows * kBins;
+    a.parts = reinterpret_cast<float4 *>(a.list + (int64_t)p.rows * kList);
+    a.listed = reinterpret_cast<uint32_t *>(a.parts + (int64_t)p.rows * a.splits);
+    a.best = a.listed + p.rows;
+    const dim3 grid(a.splits, p.rows), block(kThreads);
+    MIGEMM_LAUNCH((sample_top_kernel<T>), grid, block, 0, stream, a);
+    MIGEMM_LAUNCH((sample_bins_kernel<T>), grid, block, 0, stream, a);
+    MIGEMM_LAUNCH((sample_gather_kernel<T>), grid, block, 0, stream, a);
+    MIGEMM_LAUNCH((sample_pick_kernel<T>), dim3(p.rows), block, 0, stream, a);
+    return launch_status("sample_pick_kernel launch");
+}
+
+template <typename T>
+int launch(hipStream_t stream, const SampleArgs &p) {
+    SplitArgs a{};
+    a.p = p;
+    const int most = p.vocab / 4096 < 64 ? p.vocab / 4096 : 64;
+    a.splits = 512 / p.rows < most ? 512 / p.rows : most;
+    if (a.splits >= 2) {
+        // (whole vectors: a part begins at a multiple of 8 tokens)
+        a.chunk = ((p.vocab + a.splits - 1) / a.splits + 7) / 8 * 8;
+        a.splits = (p.vocab + a.chunk - 1) / a.chunk;
+        return launch_split<T>(stream, a);
+    }
+    MIGEMM_LAUNCH((sample_row_kernel<T>), dim3(p.rows), dim3(kThreads), 0, stream, p);
+    return launch_status("sample_row_kernel launch");
+}
 }  // namespace
 
 int launch_sample(hipStream_t stream, const SampleArgs &a) {
@@ -615,11 +864,7 @@ int launch_sample(hipStream_t stream, const SampleArgs &a) {
     while (((int64_t)1 << log2) < p.vocab) ++log2;
     p.bits = 62 - log2 < 46 ? 62 - log2 : 46;
     p.unit = (double)((uint64_t)1 << p.bits);
-    if (p.type == MIGEMM_FLOAT32)
-        MIGEMM_LAUNCH((sample_row_kernel<float>), dim3(p.rows), dim3(kThreads), 0, stream, p);
-    else
-        MIGEMM_LAUNCH((sample_row_kernel<Bf16>), dim3(p.rows), dim3(kThreads), 0, stream, p);
-    return launch_status("sample_kernel launch");
+    return p.type == MIGEMM_FLOAT32 ? launch<float>(stream, p) : launch<Bf16>(stream, p);
 }
 
 }  // namespace migemm
