@@ -6,8 +6,7 @@
 // more than u times the kept ones' sum. So every step asks one question: where in the order does a
 // running count or sum cross a value? It is answered without sorting the row:
 //
-//   * A histogram of the row, in bins of equal width in (top - l), a monotone function of the logit
-//     in float32. Its running sums name the bin that a value falls in. With top_k it holds counts
+//   * A histogram of the row, in bins of equal width in (top - l). Its running sums name the bin that a value falls in. With top_k it holds counts
 //     (the few tokens that are left get their weights later), otherwise weights.
 //   * The tokens of that bin, or of all bins up to it where they are few, are collected into LDS
 //     and sorted there by logit and index; the running sums over them name the token. A bin of more
@@ -16,8 +15,8 @@
 //
 // Weights come from 64-bit arithmetic, because a sum of 10^5 float32 weights is off by more than a
 // token's share, and are summed as integers: exactly, in any order (atomics among them), so that a
-// result does not depend on how a row was walked. Within a bin's width of at most 0.023 in log2 w
-// a token's weight over its bin's middle one is a polynomial of degree 5 (off by 2^-50); these are
+// result does not depend on how a row was walked. Within a bin's width of at most 0.047 in log2 w
+// a token's weight over its bin's middle one is a polynomial of degree 4 (off by 2^-39 at most); these are
 // summed with 43 fractional bits, and a bin's sum is multiplied by its middle weight once, to 42 bits
 // below the point or more (62 - log2(vocabulary), at most 46). Tokens that weigh less than half of
 // the last bit are left out.
@@ -29,10 +28,10 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kBins = 2 * kThreads;
-constexpr int kList = 2 * kThreads;
-constexpr int kWhole = 512;     // all bins up to the one in question are sorted together up to here
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kBins = 2048;
+constexpr int kList = kBins;
+constexpr int kWhole = 256;     // all bins up to the one in question are sorted together up to here
 constexpr int kIndexBits = 20;  // of a token, below the bits of its logit in an order's key
 constexpr int kFraction = 43;   // bits of a weight over its bin's middle one (2^20 of them fit)
 constexpr double kOne = (double)((u64)1 << kFraction);
@@ -50,6 +49,7 @@ struct Shared {
             uint32_t part_count[kBins];
         };
     };
+    u64 gathered[kList];  // keys of the bins that the answer may need, in any order
     u64 wave_mass[kWaves];
     uint32_t wave_count[kWaves];
     float high[kWaves], low[kWaves];
@@ -71,7 +71,9 @@ __device__ __forceinline__ u64 key_of(float l, uint32_t index) {
 }
 // inf counts as the largest number.
 __device__ __forceinline__ float bounded(float l) {
-    return __builtin_amdgcn_fmed3f(l, -INFINITY, kMost);
+    float r;
+    asm("v_min_f32 %0, %1, %2" : "=v"(r) : "s"(kMost), "v"(l));  // (one step: no NaN comes here)
+    return r;
 }
 
 // 2^x for x > -1000. 2^f for |f| <= 1/2 is 1 + f q(f), q of degree 9 through the Chebyshev nodes of
@@ -93,90 +95,95 @@ __device__ __forceinline__ double power(double x) {
     return __longlong_as_double(
         (long long)((u64)__double_as_longlong(q) + ((u64)__double_as_longlong(t) << 52)));
 }
+// a b + c with c in scalar registers (the compiler's form copies c for each use).
+__device__ __forceinline__ double step(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
+}
 // A number in [0, 2^52) rounded to an integer, in the adder.
 __device__ __forceinline__ u64 rounded(double x, double unit) {
     const double y = __builtin_fma(x, unit, 4503599627370496.0);
     return (u64)__double_as_longlong(y) & (((u64)1 << 52) - 1);
 }
 
-// What a row's logits weigh, and its bins.
+// What a row's logits weigh, and its bins: 2^j of them a unit of log2 of the weight, each around its
+// middle, a multiple of 2^-j.
 struct Weights {
-    float scale, top;  // the largest logit times the scale
-    float bins;        // bins a unit of (top - l) scale
-    double top64;
-    double rate;     // log2(e) / T
-    double width;    // of a bin, in log2 of the weight
-    double cut;      // l - top below which a token weighs nothing
-    float least;     // the smallest logit that is not below it
-    double unit;     // 2^bits
+    float least;   // the smallest logit that weighs something
+    double top;    // the largest
+    double rate;   // log2(e) / T
+    double cut;    // how far below the top the smallest weight is
+    double magic;  // 1.5 2^(52 - j): adding it rounds to multiples of 2^-j
+    double width;  // 2^-j
+    double unit;   // 2^bits
 
     __device__ __forceinline__ void init(const SampleArgs &p, float high, float low,
                                          float temperature, float min_p) {
-        top64 = high;
+        top = high;
         rate = 1.4426950408889634074 / (double)temperature;
         unit = p.unit;
         // bins over the logits that weigh something, or over all of them where that is less
-        const double spread = top64 - (double)low;
-        double span = (double)(p.bits + 1) / rate;
-        span = spread < span ? spread : span;
-        cut = -span;
+        const double spread = top - (double)low;
+        cut = (double)(p.bits + 1) * 0.69314718055994530942 * (double)temperature;
+        cut = spread < cut ? spread : cut;
+        // cut rate = m 2^e with 1 <= m < 2: 1024 to 2047 bins of 2^(e - 10)
+        const int e = (int)((u64)__double_as_longlong(cut * rate * 1.001) >> 52) - 1023;
+        const int j = 10 - e < 900 ? 10 - e : 900;  // (no spread at all)
+        width = ldexp(1.0, -j);
+        magic = 6755399441055744.0 * width;
         if (min_p > 0.f) {
-            const double least = min_p < 1.f ? log2((double)min_p) / rate : 0.0;
-            cut = least > cut ? least : cut;
+            const double most = min_p < 1.f ? -log2((double)min_p) / rate : 0.0;
+            cut = most < cut ? most : cut;
         }
-        // (the float32 coordinate of a token at the cut stays below kBins - 1)
-        double per = span > 0.0 ? (kBins - 2) / span : 0.0;
-        // Halves, so that the difference of the largest numbers is one too. Spans that are too
-        // small for float32's range of bins a unit: logits that are small as well are scaled up,
-        // larger ones have no neighbour within such a span.
-        scale = 0.5f;
-        if (per > 1e30) {
-            if (fabsf(high) < 1.f)
-                scale = 0x1p100f;
-            else
-                per = 0.0;
-        }
-        top = high * scale;
-        bins = (float)(per / (double)scale);
-        width = bins > 0.f ? rate / ((double)bins * (double)scale) : 0.0;
         least = smallest(kBins - 1);
     }
     // The smallest logit of bins 0 .. b, by all lanes of a wavefront: bin and cut go by the order
     // of logits, so 64 of them at a time narrow it down.
     __device__ __forceinline__ float smallest(uint32_t b) const {
-        uint32_t lo = order_of((float)top64), hi = order_of(-kMost);
+        uint32_t lo = order_of((float)top), hi = order_of(-kMost);
         while (hi > lo) {
             const uint32_t step = (hi - lo) / 64 + 1;
             const u64 at = lo + (u64)step * (threadIdx.x & 63);
             const float l = logit_of((at < hi ? at : hi) << kIndexBits);
-            const int in = __popcll(__ballot(at <= hi && bin(l) <= b && below(l) >= cut));
+            const int in = __popcll(__ballot(at <= hi && bin(l) <= b && below(l) <= cut));
             lo += step * (in - 1);
             hi = (u64)lo + step - 1 < hi ? lo + step - 1 : hi;
         }
         return logit_of((u64)lo << kIndexBits);
     }
-    __device__ __forceinline__ double below(float l) const { return (double)l - top64; }
-    // (two roundings, each of which keeps the order)
+    // How far a logit is below the top.
+    __device__ __forceinline__ double below(float l) const { return top - (double)l; }
+    // The bin whose middle is nearest is in the low bits of d rate + magic. (For logits beyond the
+    // cut they are any.)
+    __device__ __forceinline__ double placed(double d) const {
+        return __builtin_fma(d, rate, magic);
+    }
+    static __device__ __forceinline__ uint32_t index(double t) {
+        return (uint32_t)__double_as_longlong(t) & (kBins - 1);
+    }
     __device__ __forceinline__ uint32_t bin(float l) const {
-        return (uint32_t)fminf(__builtin_fmaf(-scale, l, top) * bins, (float)(kBins - 1));
+        const double d = below(l);
+        return index(placed(d < cut ? d : cut));
     }
-    // 2^(log2 w + width (b + 1/2)) with kFraction bits: the weight over the middle one of its bin
-    __device__ __forceinline__ u64 over_middle(double d, uint32_t b) const {
-        const double f = __builtin_fma(d, rate, __builtin_fma((double)b, width, 0.5 * width));
-        double q = 0.0013333558146428443;  // ln2^k / k!
-        q = __builtin_fma(q, f, 0.009618129107628477);
-        q = __builtin_fma(q, f, 0.05550410866482158);
-        q = __builtin_fma(q, f, 0.24022650695910072);
-        q = __builtin_fma(q, f, 0.6931471805599453);
-        q = __builtin_fma(q, f, 1.0);
-        return rounded(q, kOne);
+    // The weight over the middle one of its bin, 2^f for |f| <= width / 2, with kFraction bits: 1 + f
+    // q(f), q of degree 3 through the Chebyshev nodes of (2^f - 1) / f (off by 2^-39 at the bin's
+    // ends). Eight 64-bit steps: the middle comes from adding and taking off `magic`, and the
+    // last step of the polynomial rounds to an integer, too.
+    __device__ __forceinline__ u64 over_middle(double d, uint32_t &b) const {
+        const double t = placed(d);
+        b = index(t);
+        const double f = __builtin_fma(-d, rate, t - magic);
+        double q = step(0.00961821489950097 * kOne, f, 0.05550485129481622 * kOne);
+        q = step(q, f, 0.24022650695312786 * kOne);
+        q = step(q, f, 0.6931471805082434 * kOne);
+        const double y = step(q, f, kOne + 4503599627370496.0);  // (2^52: rounds to integers)
+        return (u64)__double_as_longlong(y) & (((u64)1 << 52) - 1);
     }
-    __device__ __forceinline__ double middle(int b) const {
-        return power(-width * ((double)b + 0.5));
-    }
+    __device__ __forceinline__ double middle(int b) const { return power(-width * (double)b); }
     __device__ __forceinline__ double share(float l) const {
         const double y = below(l) * rate;
-        return y > -64.0 ? power(y) : 0.0;
+        return y < 64.0 ? power(-y) : 0.0;
     }
     __device__ __forceinline__ u64 mass(float l) const { return rounded(share(l), unit); }
 };
@@ -188,11 +195,17 @@ struct Asked {
     bool valid;
 
     __device__ __forceinline__ Asked(const SampleArgs &p, int r) {
-        temperature = p.temperatures != nullptr ? p.temperatures[r] : p.temperature;
-        top_k = p.top_ks != nullptr ? p.top_ks[r] : p.top_k;
-        top_p = p.top_ps != nullptr ? p.top_ps[r] : p.top_p;
-        min_p = p.min_ps != nullptr ? p.min_ps[r] : p.min_p;
+        // (loaded whether there or not, from somewhere that is: five loads that fly together)
         uniform = p.uniforms[r];
+        const float t = (p.temperatures != nullptr ? p.temperatures : p.uniforms)[r];
+        const float tp = (p.top_ps != nullptr ? p.top_ps : p.uniforms)[r];
+        const float mp = (p.min_ps != nullptr ? p.min_ps : p.uniforms)[r];
+        const int k = (p.top_ks != nullptr ? p.top_ks
+                                           : reinterpret_cast<const int *>(p.uniforms))[r];
+        temperature = p.temperatures != nullptr ? t : p.temperature;
+        top_p = p.top_ps != nullptr ? tp : p.top_p;
+        min_p = p.min_ps != nullptr ? mp : p.min_p;
+        top_k = p.top_ks != nullptr ? k : p.top_k;
         valid = temperature >= 0.f && temperature < INFINITY && top_p == top_p &&
                 min_p == min_p && uniform == uniform;
     }
@@ -212,45 +225,131 @@ struct Asked {
     }
 };
 
-// Calls f(logit, index) for the logits first .. end of a row, those of a thread in ascending order.
-template <int THREADS, typename T, typename F>
-__device__ __forceinline__ void each(const T *row, int first, int end, const F &f) {
-    constexpr int V = 16 / sizeof(T), U = sizeof(T) == 4 ? 4 : 2;
-    for (int part = first; part < end; part += THREADS * V * U) {
-        const int at = part + threadIdx.x * V;
-        float x[U][V];
+// The 16 bytes of logits of a row from place `at`; those at and after `end` are -inf.
+template <typename T>
+__device__ __forceinline__ uint4 load_logits(const T *row, int at, int end) {
+    constexpr int V = 16 / sizeof(T);
+    uint4 raw;
+    if (at + V <= end) {
+        __builtin_memcpy(&raw, row + at, sizeof(raw));
+        return raw;
+    }
+    T x[V];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            load_f32<T, V>(row + at + u * THREADS * V, end - at - u * THREADS * V, x[u]);
+    for (int e = 0; e < V; ++e) x[e] = at + e < end ? row[at + e] : from_f32<T>(-INFINITY);
+    __builtin_memcpy(&raw, x, sizeof(raw));
+    return raw;
+}
+// Calls f(logits, place of the first) with their float32 values.
+template <typename T, typename F>
+__device__ __forceinline__ void of_logits(const uint4 &raw, int at, const F &f) {
+    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+    constexpr int V = 16 / sizeof(T);
+    float x[V];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (V == 4) {
+            x[e] = __uint_as_float(u[e]);
+        } else {
+            x[2 * e] = bf16_low(u[e]);
+            x[2 * e + 1] = bf16_high(u[e]);
+        }
+    }
+    f(x, at);
+}
+
+// Calls f(logits, place of the first) for the logits first .. end of a row, 16 bytes at a time, those of
+// a thread in ascending order (and with -inf for places behind the end). The first HELD vectors of a thread stay in registers
+// from start() on, for as many walks as there are; what is beyond comes in parts of four vectors,
+// each on its way while the one before is looked at.
+template <typename T, int HELD>
+struct Walk {
+    static constexpr int V = 16 / sizeof(T), STEP = kThreads * V, U = 4;
+    const T *row;
+    int first, end;
+    uint4 held[HELD];
+
+    __device__ __forceinline__ int place(int vector) const {
+        return first + vector * STEP + threadIdx.x * V;
+    }
+    __device__ __forceinline__ void start(const T *r, int a, int b) {
+        row = r;
+        first = a;
+        end = b;
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int i = at + u * THREADS * V + e;
-                if (i < end) f(x[u][e], i);
+        for (int u = 0; u < HELD; u += 2)
+            if (first + u * STEP < end) {
+                held[u] = load_logits<T>(row, place(u), end);
+                held[u + 1] = load_logits<T>(row, place(u + 1), end);
             }
     }
+    template <typename F>
+    __device__ __forceinline__ void go(const F &f) const {
+#pragma unroll
+        for (int u = 0; u < HELD; u += 2) {
+            const uint4 a = held[u], b = held[u + 1];
+            if (first + u * STEP < end) {  // (two at a time: more to do while one waits)
+                of_logits<T>(a, place(u), f);
+                of_logits<T>(b, place(u + 1), f);
+            }
+        }
+        if (first + HELD * STEP < end) rest(HELD, f);
+    }
+    template <typename F>
+    __device__ __forceinline__ void rest(int vector, const F &f) const {
+        uint4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = load_logits<T>(row, place(vector + u), end);
+        for (; first + vector * STEP < end; vector += U) {
+            uint4 y[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) y[u] = x[u];
+            if (first + (vector + U) * STEP < end) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    x[u] = load_logits<T>(row, place(vector + U + u), end);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) of_logits<T>(y[u], place(vector + u), f);
+        }
+    }
+};
+// The same without vectors that stay.
+template <typename T, typename F>
+__device__ __forceinline__ void each(const T *row, int first, int end, const F &f) {
+    Walk<T, 2> walk;
+    walk.row = row;
+    walk.first = first;
+    walk.end = end;
+    walk.rest(0, f);
 }
 
 // The largest logit of a range and whether one is NaN, in every lane, and with `wide` the smallest
 // above -inf (otherwise it is -inf). At low temperatures the logits that weigh something span
 // less than all of them, so the smallest does not matter, and costs half of the pass.
-template <int THREADS, typename T>
-__device__ __forceinline__ void extremes(const T *row, int first, int end, bool wide, float &high,
+template <typename W>
+__device__ __forceinline__ void extremes(const W &walk, bool wide, float &high,
                                          float &low, bool &nan) {
     high = -INFINITY;
     low = wide ? INFINITY : -INFINITY;
     nan = false;
+    constexpr int V = W::V;
     if (wide)
-        each<THREADS>(row, first, end, [&](float x, int) {
-            nan |= x != x;
-            high = fmaxf(high, x);
-            low = x > -INFINITY ? fminf(low, x) : low;
+        walk.go([&](const auto &x, int) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                nan |= x[e] != x[e];
+                high = fmaxf(high, x[e]);
+                low = x[e] > -INFINITY ? fminf(low, x[e]) : low;
+            }
         });
     else
-        each<THREADS>(row, first, end, [&](float x, int) {
-            nan |= x != x;
-            high = fmaxf(high, x);
+        walk.go([&](const auto &x, int) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                nan |= x[e] != x[e];
+                high = fmaxf(high, x[e]);
+            }
         });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -264,15 +363,26 @@ __device__ __forceinline__ void extremes(const T *row, int first, int end, bool 
 
 // The tokens first .. end into the histogram: their weights, or with COUNT their number. Keys past
 // `limit` are left out.
-template <bool COUNT, typename T>
-__device__ __forceinline__ void fill(u64 *mass, const T *row, int first, int end, const Weights &w,
-                                     u64 limit) {
-    each<kThreads>(row, first, end, [&](float x, int i) {
-        if (!(x >= w.least)) return;
-        const float l = bounded(x);
-        if (limit != ~(u64)0 && key_of(l, i) > limit) return;
-        const uint32_t b = w.bin(l);
-        atomicAdd(&mass[b], COUNT ? (u64)1 : w.over_middle(w.below(l), b));
+template <bool COUNT, typename W>
+__device__ __forceinline__ void fill(u64 *mass, const W &walk, const Weights &w, u64 limit) {
+    walk.go([&](const auto &x, int at) {
+        constexpr int V = W::V;
+        u64 m[V];
+        uint32_t b[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const double d = w.below(bounded(x[e]));
+            m[e] = COUNT ? 1 : w.over_middle(d, b[e]);
+            if (COUNT) b[e] = w.index(w.placed(d));
+        }
+        // (here all are known: left alone, the compiler moves each token's chain of dependent steps
+        // behind its comparison, and none runs beside another)
+#pragma unroll
+        for (int e = 0; e < V; ++e) asm volatile("" : "+v"(m[e]), "+v"(b[e]));
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (x[e] >= w.least && (limit == ~(u64)0 || key_of(bounded(x[e]), at + e) <= limit))
+                atomicAdd(&mass[b[e]], m[e]);
     });
 }
 
@@ -296,40 +406,43 @@ __device__ __forceinline__ N run_up_lanes(N x) {
     return x;
 }
 
-// Running sums of 2 * kThreads masses (and counts), in place. Ends with a barrier.
+// Running sums of kBins masses (and counts), in place. Ends with a barrier.
 template <bool COUNTS>
 __device__ __forceinline__ void run_up(Shared &s, u64 *mass, uint32_t *count) {
+    constexpr int PER = kBins / kThreads;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const u64 m1 = mass[2 * tid + 1];
-    u64 m = run_up_lanes(mass[2 * tid] + m1);
-    uint32_t c = 0, c1 = 0;
-    if (COUNTS) {
-        c1 = count[2 * tid + 1];
-        c = run_up_lanes(count[2 * tid] + c1);
+    u64 m[PER];
+    uint32_t c[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        m[i] = mass[PER * tid + i] + (i ? m[i - 1] : 0);
+        if (COUNTS) c[i] = count[PER * tid + i] + (i ? c[i - 1] : 0);
     }
+    const u64 lanes_m = run_up_lanes(m[PER - 1]);
+    const uint32_t lanes_c = COUNTS ? run_up_lanes(c[PER - 1]) : 0;
     if (lane == 63) {
-        s.wave_mass[wave] = m;
-        s.wave_count[wave] = c;
+        s.wave_mass[wave] = lanes_m;
+        s.wave_count[wave] = lanes_c;
     }
     __syncthreads();
-    // the sums of the wavefronts before: each lane of a row of 16 takes one
-    const u64 wm = run_up_lanes(lane < wave ? s.wave_mass[lane & (kWaves - 1)] : 0);
-    m += __shfl(wm, kWaves - 1);
+    // the sums of the wavefronts before: the lanes of a row of 16 take one each
+    u64 before_m = run_up_lanes(lane < wave ? s.wave_mass[lane & (kWaves - 1)] : 0);
+    before_m = __shfl(before_m, kWaves - 1) + lanes_m - m[PER - 1];
+    uint32_t before_c = 0;
     if (COUNTS) {
-        const uint32_t wc = run_up_lanes(lane < wave ? s.wave_count[lane & (kWaves - 1)] : 0);
-        c += __shfl(wc, kWaves - 1);
+        before_c = run_up_lanes(lane < wave ? s.wave_count[lane & (kWaves - 1)] : 0);
+        before_c = __shfl(before_c, kWaves - 1) + lanes_c - c[PER - 1];
     }
-    mass[2 * tid] = m - m1;
-    mass[2 * tid + 1] = m;
-    if (COUNTS) {
-        count[2 * tid] = c - c1;
-        count[2 * tid + 1] = c;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        mass[PER * tid + i] = before_m + m[i];
+        if (COUNTS) count[PER * tid + i] = before_c + c[i];
     }
     __syncthreads();
 }
 
 // A filled histogram becomes its running sums. A bin's weight is its sum times its middle one; its
-// number of tokens is at most the sum over the least that a token adds to it (2^-0.012).
+// number of tokens is at most the sum over the least that a token adds to it (2^-0.023).
 template <bool COUNT>
 __device__ __forceinline__ void finish(Shared &s, const Weights &w) {
     for (int b = threadIdx.x; b < kBins; b += kThreads) {
@@ -337,7 +450,7 @@ __device__ __forceinline__ void finish(Shared &s, const Weights &w) {
         if (COUNT) {
             s.count[b] = (uint32_t)m;
         } else {
-            s.count[b] = m ? (uint32_t)((double)m * (1.01 / kOne)) + 1 : 0;
+            s.count[b] = m ? (uint32_t)((double)m * (1.02 / kOne)) + 1 : 0;
             s.mass[b] = m ? (u64)((double)m * (w.middle(b) * (w.unit / kOne)) + 0.5) : 0;
         }
     }
@@ -358,15 +471,40 @@ __device__ __forceinline__ int reach(Shared &s, const N *sums, int n, N target) 
     return i;
 }
 
-// Sorts the first `size` (a power of two, at least 2) keys of the list. A wavefront's threads
-// exchange within its own 128 keys while their distance is at most 64: those steps need no barrier.
-__device__ __forceinline__ void sort(Shared &s, int size) {
+// Sorts the first n keys of the list, with `upto` as room. Up to 256 keys find their places by
+// counting the smaller ones, several threads a key (64 keys: 0.3 us, 3.0 by exchanges, whose steps
+// wait for each other). More are exchanged over powers of two: a wavefront's threads within its own 128
+// keys while their distance is at most 64, which needs no barrier.
+__device__ __forceinline__ void sort(Shared &s, int n) {
     const int tid = threadIdx.x;
+    if (n <= kWhole) {
+        int per = kThreads / kWhole;  // threads a key
+        while (per < 32 && n * per * 2 <= kThreads) per *= 2;
+        const int i = tid / per, part = tid & (per - 1);
+        u64 key = 0;
+        uint32_t less = 0;
+        if (i < n) {
+            key = s.list[i];
+            for (int j = part; j < n; j += per) less += s.list[j] < key;
+        }
+        for (int o = 1; o < per; o *= 2) less += __shfl_xor(less, o);
+        if (i < n && part == 0) s.upto[less] = key;
+        __syncthreads();
+        if (tid < n) s.list[tid] = s.upto[tid];
+        __syncthreads();
+        return;
+    }
+    int size = 2 * kWhole;
+    while (size < n) size *= 2;
+    for (int i = tid; i < size; i += kThreads)
+        if (i >= n) s.list[i] = ~(u64)0;
+    __syncthreads();
+    // (pair i of a step: a thread takes neighbours' pairs within its wavefront's keys)
     for (int k = 2; k <= size; k *= 2)
         for (int j = k / 2; j > 0; j /= 2) {
             if (j > 64) __syncthreads();
-            if (tid < size / 2) {
-                const int x = 2 * tid - (tid & (j - 1)), y = x + j;
+            for (int i = tid; i < size / 2; i += kThreads) {
+                const int x = 2 * i - (i & (j - 1)), y = x + j;
                 const u64 p = s.list[x], q = s.list[y];
                 if ((p > q) == ((x & k) == 0)) {
                     s.list[x] = q;
@@ -425,11 +563,38 @@ __device__ __forceinline__ Plan plan_of(Shared &s, const Asked &q, bool counted)
     return g;
 }
 
-// A row and what is known of it. Its tokens come from its logits, or (given) from keys that an
-// earlier kernel gathered. The list holds those of bins first .. last.
-template <typename T>
+// The keys of the plan's tokens into s.gathered; returns their number.
+template <typename W>
+__device__ __forceinline__ int gather(Shared &s, const W &walk, const Weights &w,
+                                      const Plan &plan) {
+    constexpr int V = W::V;
+    // the bins to draw from, and the one where top-p ends, which is not before them
+    const float from = w.smallest(plan.kept > plan.last ? plan.kept : plan.last);
+    if (threadIdx.x == 0) s.listed = 0;
+    __syncthreads();
+    walk.go([&](const auto &x, int i) {
+        float most = x[0];  // (few are taken: one question for all of them)
+#pragma unroll
+        for (int e = 1; e < V; ++e) most = fmaxf(most, x[e]);
+        if (!(most >= from)) return;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float l = bounded(x[e]);
+            if (!(l >= from) || !(plan.whole || plan.has((int)w.bin(l)))) continue;
+            const uint32_t place = atomicAdd(&s.listed, 1u);
+            if (place < kList) s.gathered[place] = key_of(l, i + e);
+        }
+    });
+    __syncthreads();
+    return min((int)s.listed, kList);
+}
+
+// A row and what is known of it. Its tokens come from its logits, or (given) from keys that were
+// gathered. The list holds those of bins first .. last.
+template <typename T, typename W>
 struct Row {
     Shared &s;
+    const W &walk;
     const T *logits;
     int n;
     const u64 *given;
@@ -459,18 +624,20 @@ struct Row {
         } else {
             const float from = w.smallest(b);
             const float below = a ? w.smallest(a - 1) : INFINITY;
-            each<kThreads>(logits, 0, n, [&](float x, int i) {
-                if (x >= from && (x < below || a == 0)) take(key_of(bounded(x), i));
+            walk.go([&](const auto &x, int i) {
+                float most = x[0];  // (few are taken: one question for all of them)
+#pragma unroll
+                for (int e = 1; e < W::V; ++e) most = fmaxf(most, x[e]);
+                if (!(most >= from)) return;
+#pragma unroll
+                for (int e = 0; e < W::V; ++e)
+                    if (x[e] >= from && (x[e] < below || a == 0))
+                        take(key_of(bounded(x[e]), i + e));
             });
         }
         __syncthreads();
         const int found = min((int)s.listed, kList);
-        int size = 2;
-        while (size < found) size *= 2;
-        for (int i = tid; i < kList; i += kThreads)
-            if (i >= found) s.list[i] = ~(u64)0;
-        __syncthreads();
-        sort(s, size);
+        sort(s, found);
         for (int i = tid; i < kList; i += kThreads)
             s.upto[i] = i < found ? w.mass(logit_of(s.list[i])) : 0;
         __syncthreads();
@@ -501,14 +668,18 @@ struct Row {
                 s.part_mass[i] = 0;
             }
             __syncthreads();
-            each<kThreads>(logits, 0, n, [&](float x, int i) {
-                const float l = bounded(x);
-                if ((int)w.bin(l) != b || !(l >= w.least)) return;
-                const u64 key = key_of(l, i);
-                if (key < lo || key > hi || key > limit) return;
-                const int at = (int)((key - lo) >> shift);
-                atomicAdd(&s.part_count[at], 1u);
-                if (!COUNT) atomicAdd(&s.part_mass[at], w.mass(l));
+            each(logits, 0, n, [&](const auto &x, int i) {
+#pragma unroll
+                for (int e = 0; e < W::V; ++e) {
+                    const float l = bounded(x[e]);
+                    const u64 key = key_of(l, i + e);
+                    if ((int)w.bin(l) != b || !(l >= w.least) || key < lo || key > hi ||
+                        key > limit)
+                        continue;
+                    const int at = (int)((key - lo) >> shift);
+                    atomicAdd(&s.part_count[at], 1u);
+                    if (!COUNT) atomicAdd(&s.part_mass[at], w.mass(l));
+                }
             });
             __syncthreads();
             if (COUNT) {
@@ -539,8 +710,7 @@ struct Row {
 
     // The row's token, from its histogram's running sums.
     __device__ __forceinline__ void answer(const SampleArgs &p, int r, const Asked &q, bool counted,
-                                           const Plan &plan) {
-        u64 total = s.mass[kBins - 1];
+                                           const Plan &plan, u64 total) {
         if (counted) {
             const u64 k = (u64)q.top_k < total ? (u64)q.top_k : total;
             if (plan.listed) {
@@ -552,7 +722,7 @@ struct Row {
                 __syncthreads();
                 for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0;
                 __syncthreads();
-                fill<false>(s.mass, logits, 0, n, w, limit);
+                fill<false>(s.mass, walk, w, limit);
                 __syncthreads();
                 finish<false>(s, w);
                 total = s.mass[kBins - 1];
@@ -578,7 +748,7 @@ struct Row {
         const int i = whole ? reach(s, s.upto, kList, target) : by_mass(target);
         if (threadIdx.x == 0) {
             const u64 key = s.list[i];
-            p.tokens[r] = (int)(key & (((u64)1 << kIndexBits) - 1));
+            p.tokens[r] = min((int)(key & (((u64)1 << kIndexBits) - 1)), n - 1);
             p.probabilities[r] = (float)(w.share(logit_of(key)) * p.unit / (double)total);
         }
     }
@@ -606,7 +776,9 @@ sample_row_kernel(SampleArgs p) {
         s.bad = 0;
         s.found = n;
     }
-    extremes<kThreads>(logits, 0, n, q.wide(), high, low, nan);
+    Walk<T, 4> walk;
+    walk.start(logits, 0, n);
+    extremes(walk, q.wide(), high, low, nan);
     if (lane == 0) {
         s.high[wave] = high;
         s.low[wave] = low;
@@ -622,8 +794,10 @@ sample_row_kernel(SampleArgs p) {
     if (!q.valid || s.bad || !(high > -INFINITY)) return nothing(p, r);
     if (q.greedy()) {
         uint32_t best = n;
-        each<kThreads>(logits, 0, n, [&](float x, int i) {
-            best = bounded(x) == high && (uint32_t)i < best ? i : best;
+        walk.go([&](const auto &x, int i) {
+#pragma unroll
+            for (int e = 0; e < 16 / (int)sizeof(T); ++e)
+                best = bounded(x[e]) == high && (uint32_t)(i + e) < best ? i + e : best;
         });
         if (best < (uint32_t)n) atomicMin(&s.found, best);
         __syncthreads();
@@ -637,30 +811,43 @@ sample_row_kernel(SampleArgs p) {
     w.init(p, high, low, q.temperature, q.min_p);
     const bool counted = q.counted(n);
     if (counted)
-        fill<true>(s.mass, logits, 0, n, w, ~(u64)0);
+        fill<true>(s.mass, walk, w, ~(u64)0);
     else
-        fill<false>(s.mass, logits, 0, n, w, ~(u64)0);
+        fill<false>(s.mass, walk, w, ~(u64)0);
     __syncthreads();
     if (counted)
         finish<true>(s, w);
     else
         finish<false>(s, w);
-    Row<T> row{s, logits, n, nullptr, 0, w, ~(u64)0, false, 1, 0, 0};
-    row.answer(p, r, q, counted, plan_of(s, q, counted));
+    const Plan plan = plan_of(s, q, counted);
+    const u64 total = s.mass[kBins - 1];
+    const int gathered = plan.listed ? gather(s, walk, w, plan) : 0;
+    Row<T, decltype(walk)> row{s, walk, logits, n, plan.listed ? s.gathered : nullptr, gathered, w,
+                               ~(u64)0, false, 1, 0, 0};
+    row.answer(p, r, q, counted, plan, total);
 }
 // ------------------------------------------------------------- rows cut over work-groups
 // Four launches: the largest logit of each part of a row; the parts' histograms, added up; the tokens
-// of the bins that the answer may need; and the answer, from the histogram and those tokens. Each
-// work-group of the last two reads the whole histogram and plans the same. A row that the list does
-// not hold is walked by the last kernel's work-group alone.
+// of the bins that the answer may need; and the answer, from those tokens. Each part of the third
+// reads the whole histogram and plans the same. A row whose tokens the list does not hold is walked
+// by the last kernel's work-group alone. What waits for memory is loaded as a kernel begins.
+enum RowKind { kNothing, kGreedy, kDraw };
+struct RowState {
+    Weights w;        // of the second kernel's first part
+    u64 total;        // of the third's: the histogram's sum, and what the answer needs
+    Plan plan;
+    int kind;         // of the second's
+    uint32_t listed;  // tokens gathered
+    uint32_t best;    // where the largest logit stands first (kGreedy)
+};
 struct SplitArgs {
     SampleArgs p;
     int splits, chunk;  // parts of a row, tokens of a part
     u64 *mass;          // [rows][kBins]
+    u64 *running;       // [rows][kBins], its running sums
     u64 *list;          // [rows][kList]
     float4 *parts;      // [rows][splits]: largest, smallest, whether one is NaN
-    uint32_t *listed;   // [rows]
-    uint32_t *best;     // [rows]: where the largest logit stands first
+    RowState *state;    // [rows]
 };
 
 template <typename T>
@@ -670,17 +857,20 @@ __global__ void __launch_bounds__(kThreads) sample_top_kernel(SplitArgs a) {
     const SampleArgs &p = a.p;
     const int tid = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
     const T *logits = static_cast<const T *>(p.logits) + (int64_t)r * p.ld;
+    const int first = part * a.chunk, end = min(first + a.chunk, p.vocab);
+    Walk<T, 4> walk;
+    walk.start(logits, first, end);
+    const Asked q(p, r);
     for (int i = part * kThreads + tid; i < kBins; i += a.splits * kThreads)
         a.mass[(int64_t)r * kBins + i] = 0;
     if (part == 0 && tid == 0) {
-        a.listed[r] = 0;
-        a.best[r] = ~0u;
+        a.state[r].listed = 0;
+        a.state[r].best = ~0u;
     }
     if (tid == 0) bad = 0;
-    const int first = part * a.chunk, end = min(first + a.chunk, p.vocab);
     float high, low;
     bool nan;
-    extremes<kThreads>(logits, first, end, Asked(p, r).wide(), high, low, nan);
+    extremes(walk, q.wide(), high, low, nan);
     if ((tid & 63) == 0) {
         highs[tid >> 6] = high;
         lows[tid >> 6] = low;
@@ -697,53 +887,41 @@ __global__ void __launch_bounds__(kThreads) sample_top_kernel(SplitArgs a) {
     }
 }
 
-// A row's extremes from its parts', in every lane; false where there is nothing to choose from.
-__device__ __forceinline__ bool joined(const SplitArgs &a, int r, const Asked &q, float &high,
-                                       float &low) {
-    const int lane = threadIdx.x & 63;
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sample_bins_kernel(SplitArgs a) {
+    __shared__ u64 mass[kBins];
+    const SampleArgs &p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, part = blockIdx.x, r = blockIdx.y;
+    const T *logits = static_cast<const T *>(p.logits) + (int64_t)r * p.ld;
+    const int first = part * a.chunk, end = min(first + a.chunk, p.vocab);
     float4 x = make_float4(-INFINITY, INFINITY, 0.f, 0.f);
     if (lane < a.splits) x = a.parts[(int64_t)r * a.splits + lane];
+    const Asked q(p, r);
+    Walk<T, 4> walk;
+    walk.start(logits, first, end);
+    for (int i = tid; i < kBins; i += kThreads) mass[i] = 0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         x.x = fmaxf(x.x, __shfl_xor(x.x, o));
         x.y = fminf(x.y, __shfl_xor(x.y, o));
     }
-    high = x.x;
-    low = x.y;
-    return q.valid && __ballot(x.z != 0.f) == 0 && high > -INFINITY;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_bins_kernel(SplitArgs a) {
-    __shared__ u64 mass[kBins];
-    const SampleArgs &p = a.p;
-    const int tid = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
-    const T *logits = static_cast<const T *>(p.logits) + (int64_t)r * p.ld;
-    const Asked q(p, r);
-    float high, low;
-    if (!joined(a, r, q, high, low) || q.greedy()) return;
+    const bool some = q.valid && __ballot(x.z != 0.f) == 0 && x.x > -INFINITY;
+    const int kind = !some ? kNothing : q.greedy() ? kGreedy : kDraw;
     Weights w;
-    w.init(p, high, low, q.temperature, q.min_p);
-    for (int i = tid; i < kBins; i += kThreads) mass[i] = 0;
+    w.init(p, x.x, x.y, q.temperature, q.min_p);
+    if (part == 0 && tid == 0) {
+        a.state[r].w = w;
+        a.state[r].kind = kind;
+    }
+    if (kind != kDraw) return;
     __syncthreads();
-    const int first = part * a.chunk, end = min(first + a.chunk, p.vocab);
     if (q.counted(p.vocab))
-        fill<true>(mass, logits, first, end, w, ~(u64)0);
+        fill<true>(mass, walk, w, ~(u64)0);
     else
-        fill<false>(mass, logits, first, end, w, ~(u64)0);
+        fill<false>(mass, walk, w, ~(u64)0);
     __syncthreads();
     for (int i = tid; i < kBins; i += kThreads)
         if (mass[i] != 0) atomicAdd(&a.mass[(int64_t)r * kBins + i], mass[i]);
-}
-
-// The running sums of a row's histogram.
-__device__ __forceinline__ void load_bins(Shared &s, const SplitArgs &a, int r, const Weights &w,
-                                          bool counted) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = a.mass[(int64_t)r * kBins + i];
-    if (counted)
-        finish<true>(s, w);
-    else
-        finish<false>(s, w);
 }
 
 template <typename T>
@@ -752,87 +930,107 @@ __global__ void __launch_bounds__(kThreads) sample_gather_kernel(SplitArgs a) {
     const SampleArgs &p = a.p;
     const int tid = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
     const T *logits = static_cast<const T *>(p.logits) + (int64_t)r * p.ld;
-    const Asked q(p, r);
-    float high, low;
-    if (!joined(a, r, q, high, low)) return;
     const int first = part * a.chunk, end = min(first + a.chunk, p.vocab);
+    RowState &state = a.state[r];
+    for (int i = tid; i < kBins; i += kThreads) s.mass[i] = a.mass[(int64_t)r * kBins + i];
     const float mine = a.parts[(int64_t)r * a.splits + part].x;
-    if (q.greedy()) {
+    const Asked q(p, r);
+    const int kind = state.kind;
+    const Weights w = state.w;
+    Walk<T, 4> walk;
+    walk.start(logits, first, end);
+    if (kind == kNothing) return;
+    if (kind == kGreedy) {
+        const float high = (float)w.top;
         if (mine != high) return;
         uint32_t best = ~0u;
-        each<kThreads>(logits, first, end, [&](float x, int i) {
-            best = bounded(x) == high && (uint32_t)i < best ? i : best;
+        walk.go([&](const auto &x, int i) {
+#pragma unroll
+            for (int e = 0; e < 16 / (int)sizeof(T); ++e)
+                best = bounded(x[e]) == high && (uint32_t)(i + e) < best ? i + e : best;
         });
-        if (best != ~0u) atomicMin(&a.best[r], best);
+        if (best != ~0u) atomicMin(&state.best, best);
         return;
     }
-    Weights w;
-    w.init(p, high, low, q.temperature, q.min_p);
     const bool counted = q.counted(p.vocab);
-    load_bins(s, a, r, w, counted);
+    if (counted)
+        finish<true>(s, w);
+    else
+        finish<false>(s, w);
     const Plan plan = plan_of(s, q, counted);
+    if (part == 0) {
+        for (int i = tid; i < kBins; i += kThreads)
+            a.running[(int64_t)r * kBins + i] = s.mass[i];
+        if (tid == 0) {
+            state.plan = plan;
+            state.total = s.mass[kBins - 1];
+        }
+    }
     if (!plan.listed) return;
-    // the bins to draw from, and the one where top-p ends, which is not before them
-    const int lowest = plan.whole || plan.kept >= plan.last ? plan.kept : plan.last;
-    const float from = w.smallest(lowest);
-    if (!(mine >= from)) return;
-    if (tid == 0) s.listed = 0;
-    __syncthreads();
-    each<kThreads>(logits, first, end, [&](float x, int i) {
-        if (!(x >= from)) return;
-        const float l = bounded(x);
-        if (!plan.has((int)w.bin(l))) return;
-        const uint32_t place = atomicAdd(&s.listed, 1u);
-        if (place < kList) s.list[place] = key_of(l, i);
-    });
-    __syncthreads();
-    const uint32_t found = min(s.listed, (uint32_t)kList);
+    const int found = mine >= w.smallest(plan.kept > plan.last ? plan.kept : plan.last)
+                          ? gather(s, walk, w, plan) : 0;
     if (found == 0) return;
-    if (tid == 0) s.found = atomicAdd(&a.listed[r], found);
+    if (tid == 0) s.found = atomicAdd(&state.listed, (uint32_t)found);
     __syncthreads();
-    const uint32_t to = s.found;
-    for (uint32_t i = tid; i < found && to + i < kList; i += kThreads)
-        a.list[(int64_t)r * kList + to + i] = s.list[i];
+    const int to = s.found;
+    for (int i = tid; i < found && to + i < kList; i += kThreads)
+        a.list[(int64_t)r * kList + to + i] = s.gathered[i];
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_pick_kernel(SplitArgs a) {
     __shared__ Shared s;
     const SampleArgs &p = a.p;
-    const int r = blockIdx.x;
+    const int tid = threadIdx.x, r = blockIdx.x;
     const T *logits = static_cast<const T *>(p.logits) + (int64_t)r * p.ld;
+    const u64 *list = a.list + (int64_t)r * kList;
+    const RowState &state = a.state[r];
     const Asked q(p, r);
-    float high, low;
-    if (!joined(a, r, q, high, low)) return nothing(p, r);
-    if (q.greedy()) {
-        if (threadIdx.x == 0) {
-            p.tokens[r] = (int)a.best[r];
+    const int kind = state.kind;
+    if (kind == kNothing) return nothing(p, r);
+    if (kind == kGreedy) {
+        if (tid == 0) {
+            p.tokens[r] = (int)state.best;
             p.probabilities[r] = 1.f;
         }
         return;
     }
-    Weights w;
-    w.init(p, high, low, q.temperature, q.min_p);
+    const Weights w = state.w;
+    const Plan plan = state.plan;
     const bool counted = q.counted(p.vocab);
-    load_bins(s, a, r, w, counted);
-    const Plan plan = plan_of(s, q, counted);
-    const u64 *given = plan.listed ? a.list + (int64_t)r * kList : nullptr;
-    const int gathered = plan.listed ? (int)min(a.listed[r], (uint32_t)kList) : 0;
-    Row<T> row{s, logits, p.vocab, given, gathered, w, ~(u64)0, false, 1, 0, 0};
-    row.answer(p, r, q, counted, plan);
+    if (!plan.listed) {
+        for (int i = tid; i < kBins; i += kThreads) s.mass[i] = a.mass[(int64_t)r * kBins + i];
+        if (counted)
+            finish<true>(s, w);
+        else
+            finish<false>(s, w);
+    } else if (!plan.whole) {
+        for (int i = tid; i < kBins; i += kThreads) s.mass[i] = a.running[(int64_t)r * kBins + i];
+        __syncthreads();
+    }
+    Walk<T, 4> walk;  // (of a row that the list does not hold)
+    walk.row = logits;
+    walk.first = 0;
+    walk.end = p.vocab;
+    if (!plan.listed) walk.start(logits, 0, p.vocab);
+    Row<T, decltype(walk)> row{s, walk, logits, p.vocab, plan.listed ? list : nullptr,
+               plan.listed ? (int)min(state.listed, (uint32_t)kList) : 0, w, ~(u64)0, false, 1, 0,
+               0};
+    row.answer(p, r, q, counted, plan, state.total);
 }
 
 template <typename T>
 int launch_split(hipStream_t stream, SplitArgs a) {
     const SampleArgs &p = a.p;
-    const size_t row = (kBins + kList) * sizeof(u64) + a.splits * sizeof(float4) + 8;
+    const size_t row = (2 * kBins + kList) * sizeof(u64) + a.splits * sizeof(float4) +
+                       sizeof(RowState);
     int rc = MIGEMM_OK;
     a.mass = static_cast<u64 *>(workspace(stream, p.rows * row, &rc, 0));
     if (a.mass == nullptr) return rc;
-    a.list = a.mass + (int64_t)p.rows * kBins;
+    a.running = a.mass + (int64_t)p.rows * kBins;
+    a.list = a.running + (int64_t)p.rows * kBins;
     a.parts = reinterpret_cast<float4 *>(a.list + (int64_t)p.rows * kList);
-    a.listed = reinterpret_cast<uint32_t *>(a.parts + (int64_t)p.rows * a.splits);
-    a.best = a.listed + p.rows;
+    a.state = reinterpret_cast<RowState *>(a.parts + (int64_t)p.rows * a.splits);
     const dim3 grid(a.splits, p.rows), block(kThreads);
     MIGEMM_LAUNCH((sample_top_kernel<T>), grid, block, 0, stream, a);
     MIGEMM_LAUNCH((sample_bins_kernel<T>), grid, block, 0, stream, a);
