@@ -30,8 +30,8 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
-constexpr int kList = kBins;
-constexpr int kWhole = 256;     // all bins up to the one in question are sorted together up to here
+constexpr int kGather = kBins;  // tokens that are taken out of a row
+constexpr int kSort = 256;      // tokens that are sorted at once
 constexpr int kIndexBits = 20;  // of a token, below the bits of its logit in an order's key
 constexpr int kFraction = 43;   // bits of a weight over its bin's middle one (2^20 of them fit)
 constexpr double kOne = (double)((u64)1 << kFraction);
@@ -42,14 +42,14 @@ struct Shared {
     uint32_t count[kBins];  // running number of tokens, or a bound of it
     union {
         struct {
-            u64 list[kList], upto[kList];  // keys in order, and the running weight over them
+            u64 list[kSort], upto[kSort];  // keys in order, and the running weight over them
         };
         struct {
             u64 part_mass[kBins];  // the same over the parts of a bin
             uint32_t part_count[kBins];
         };
     };
-    u64 gathered[kList];  // keys of the bins that the answer may need, in any order
+    u64 gathered[kGather];  // keys of the bins that the answer may need, in any order
     u64 wave_mass[kWaves];
     uint32_t wave_count[kWaves];
     float high[kWaves], low[kWaves];
@@ -314,16 +314,6 @@ struct Walk {
         }
     }
 };
-// The same without vectors that stay.
-template <typename T, typename F>
-__device__ __forceinline__ void each(const T *row, int first, int end, const F &f) {
-    Walk<T, 2> walk;
-    walk.row = row;
-    walk.first = first;
-    walk.end = end;
-    walk.rest(0, f);
-}
-
 // The largest logit of a range and whether one is NaN, in every lane, and with `wide` the smallest
 // above -inf (otherwise it is -inf). At low temperatures the logits that weigh something span
 // less than all of them, so the smallest does not matter, and costs half of the pass.
@@ -361,11 +351,10 @@ __device__ __forceinline__ void extremes(const W &walk, bool wide, float &high,
     nan = __ballot(nan) != 0;
 }
 
-// The tokens first .. end into the histogram: their weights, or with COUNT their number. Keys past
-// `limit` are left out.
+// The tokens first .. end into the histogram: their weights, or with COUNT their number.
 template <bool COUNT, typename W>
-__device__ __forceinline__ void fill(u64 *mass, const W &walk, const Weights &w, u64 limit) {
-    walk.go([&](const auto &x, int at) {
+__device__ __forceinline__ void fill(u64 *mass, const W &walk, const Weights &w) {
+    walk.go([&](const auto &x, int) {
         constexpr int V = W::V;
         u64 m[V];
         uint32_t b[V];
@@ -381,8 +370,7 @@ __device__ __forceinline__ void fill(u64 *mass, const W &walk, const Weights &w,
         for (int e = 0; e < V; ++e) asm volatile("" : "+v"(m[e]), "+v"(b[e]));
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            if (x[e] >= w.least && (limit == ~(u64)0 || key_of(bounded(x[e]), at + e) <= limit))
-                atomicAdd(&mass[b[e]], m[e]);
+            if (x[e] >= w.least) atomicAdd(&mass[b[e]], m[e]);
     });
 }
 
@@ -458,69 +446,44 @@ __device__ __forceinline__ void finish(Shared &s, const Weights &w) {
     run_up<true>(s, s.mass, s.count);
 }
 
-// The first place whose running sum reaches target (the last one's does, or the last is returned).
-template <typename N>
-__device__ __forceinline__ int reach(Shared &s, const N *sums, int n, N target) {
-    const N last = sums[n - 1];
+// The first place whose running sum reaches target (the last one's does, or the last sum is taken for
+// it). Every wavefront looks for itself: at every N / 64-th sum, then at those between.
+template <int N>
+__device__ __forceinline__ int reach(const u64 *sums, u64 target) {
+    constexpr int STEP = N / 64;
+    static_assert(STEP >= 1 && STEP <= 64 && STEP * 64 == N, "two looks");
+    const int lane = threadIdx.x & 63;
+    const u64 last = sums[N - 1];
     target = target < last ? target : last;
-    for (int i = threadIdx.x; i < n; i += kThreads)
-        if (sums[i] >= target && (i == 0 || sums[i - 1] < target)) s.found = i;
-    __syncthreads();
-    const int i = s.found;
-    __syncthreads();
-    return i;
+    const u64 far = __ballot(sums[STEP * lane + STEP - 1] >= target);
+    const int from = STEP * (__ffsll(far) - 1);
+    const u64 near = __ballot(sums[from + (lane < STEP ? lane : STEP - 1)] >= target);
+    return from + __ffsll(near) - 1;
 }
 
-// Sorts the first n keys of the list, with `upto` as room. Up to 256 keys find their places by
-// counting the smaller ones, several threads a key (64 keys: 0.3 us, 3.0 by exchanges, whose steps
-// wait for each other). More are exchanged over powers of two: a wavefront's threads within its own 128
-// keys while their distance is at most 64, which needs no barrier.
+// Sorts the first n keys of the list, with `upto` as room: each finds its place by counting the smaller
+// ones, two threads or more a key. (64 keys: 0.3 us, 3.0 by exchanges, each of whose steps waits for
+// the one before.)
 __device__ __forceinline__ void sort(Shared &s, int n) {
     const int tid = threadIdx.x;
-    if (n <= kWhole) {
-        int per = kThreads / kWhole;  // threads a key
-        while (per < 32 && n * per * 2 <= kThreads) per *= 2;
-        const int i = tid / per, part = tid & (per - 1);
-        u64 key = 0;
-        uint32_t less = 0;
-        if (i < n) {
-            key = s.list[i];
-            for (int j = part; j < n; j += per) less += s.list[j] < key;
-        }
-        for (int o = 1; o < per; o *= 2) less += __shfl_xor(less, o);
-        if (i < n && part == 0) s.upto[less] = key;
-        __syncthreads();
-        if (tid < n) s.list[tid] = s.upto[tid];
-        __syncthreads();
-        return;
+    int per = kThreads / kSort;  // threads a key
+    while (per < 32 && n * per * 2 <= kThreads) per *= 2;
+    const int i = tid / per, part = tid & (per - 1);
+    u64 key = 0;
+    uint32_t less = 0;
+    if (i < n) {
+        key = s.list[i];
+        for (int j = part; j < n; j += per) less += s.list[j] < key;
     }
-    int size = 2 * kWhole;
-    while (size < n) size *= 2;
-    for (int i = tid; i < size; i += kThreads)
-        if (i >= n) s.list[i] = ~(u64)0;
+    for (int o = 1; o < per; o *= 2) less += __shfl_xor(less, o);
+    if (i < n && part == 0) s.upto[less] = key;
     __syncthreads();
-    // (pair i of a step: a thread takes neighbours' pairs within its wavefront's keys)
-    for (int k = 2; k <= size; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            if (j > 64) __syncthreads();
-            for (int i = tid; i < size / 2; i += kThreads) {
-                const int x = 2 * i - (i & (j - 1)), y = x + j;
-                const u64 p = s.list[x], q = s.list[y];
-                if ((p > q) == ((x & k) == 0)) {
-                    s.list[x] = q;
-                    s.list[y] = p;
-                }
-            }
-            if (j > 64)
-                __syncthreads();
-            else
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        }
+    if (tid < n) s.list[tid] = s.upto[tid];
     __syncthreads();
 }
 
-// Bins whose tokens a row's answer may need, as far as the histogram tells: all up to one of them,
-// or single ones. `listed`: they are few enough for a list.
+// Bins whose tokens a row's answer may need, as far as the histogram tells: all up to one of them that
+// can be sorted at once (whole), or single ones. `listed`: they are few enough to be gathered.
 struct Plan {
     bool whole, listed;
     int kept, first, last;  // the bin where top-k or top-p ends (-1: none does), those to draw from
@@ -538,28 +501,30 @@ __device__ __forceinline__ uint32_t count_in(const Shared &s, int a, int b) {
 __device__ __forceinline__ Plan plan_of(Shared &s, const Asked &q, bool counted) {
     Plan g{true, true, kBins - 1, 0, -1};
     const u64 total = s.mass[kBins - 1];
-    if (counted) {
-        g.kept = reach(s, s.mass, kBins, (u64)q.top_k);
-        g.listed = s.count[g.kept] <= kList;
-        return g;
-    }
     u64 low = total, high = total;
-    if (q.top_p < 1.f) {
-        g.kept = reach(s, s.mass, kBins, q.kept(total));
+    if (counted) {
+        g.kept = reach<kBins>(s.mass, (u64)q.top_k);
+    } else if (q.top_p < 1.f) {
+        g.kept = reach<kBins>(s.mass, q.kept(total));
         low = g.kept ? s.mass[g.kept - 1] : 1;
         high = s.mass[g.kept];
     }
-    if (s.count[g.kept] <= kWhole) return g;
+    if (s.count[g.kept] <= kSort) return g;
     g.whole = false;
-    g.first = reach(s, s.mass, kBins, q.drawn(low));
-    g.last = reach(s, s.mass, kBins, q.drawn(high));
+    if (counted) {
+        g.last = g.kept;
+        g.listed = s.count[g.kept] <= kGather;
+        return g;
+    }
+    g.first = reach<kBins>(s.mass, q.drawn(low));
+    g.last = reach<kBins>(s.mass, q.drawn(high));
     uint32_t n = count_in(s, g.first, g.last);
     if (q.top_p < 1.f) {
         if (g.kept > g.last) n += count_in(s, g.kept, g.kept);
     } else {
         g.kept = -1;
     }
-    g.listed = n <= kList;
+    g.listed = n <= kGather;
     return g;
 }
 
@@ -582,173 +547,164 @@ __device__ __forceinline__ int gather(Shared &s, const W &walk, const Weights &w
             const float l = bounded(x[e]);
             if (!(l >= from) || !(plan.whole || plan.has((int)w.bin(l)))) continue;
             const uint32_t place = atomicAdd(&s.listed, 1u);
-            if (place < kList) s.gathered[place] = key_of(l, i + e);
+            if (place < kGather) s.gathered[place] = key_of(l, i + e);
         }
     });
     __syncthreads();
-    return min((int)s.listed, kList);
+    return min((int)s.listed, kGather);
 }
 
-// A row and what is known of it. Its tokens come from its logits, or (given) from keys that were
-// gathered. The list holds those of bins first .. last.
-template <typename T, typename W>
+// A row and what is known of it. Its tokens come from keys that were gathered, or (keys null; a row of
+// too many, and walked simply, so that this rare case takes no registers from the other) its logits.
+template <typename T>
 struct Row {
     Shared &s;
-    const W &walk;
     const T *logits;
     int n;
-    const u64 *given;
+    const u64 *keys;
     int gathered;
-    Weights w;
-    u64 limit;   // keys past it are out (top-k)
-    bool whole;  // the list holds all tokens that may be kept
-    int first, last;
-    u64 base;    // what runs up to the list
+    const Weights &w;
+    u64 limit;  // keys past it are out (top-k)
+    u64 base;   // what runs up to the list
 
-    // The tokens of bins a .. b with keys lo .. hi (at most kList), sorted, and their running weights.
-    __device__ __forceinline__ void collect(int a, int b, u64 lo, u64 hi) {
-        const int tid = threadIdx.x;
+    // Calls f(key) for the tokens with keys lo .. hi.
+    template <typename F>
+    __device__ __forceinline__ void tokens(u64 lo, u64 hi, const F &f) const {
         hi = hi < limit ? hi : limit;
-        if (tid == 0) s.listed = 0;
-        __syncthreads();
-        const auto take = [&](u64 key) {
-            if (key < lo || key > hi) return;
-            const uint32_t place = atomicAdd(&s.listed, 1u);
-            if (place < kList) s.list[place] = key;
-        };
-        if (given != nullptr) {
-            for (int i = tid; i < gathered; i += kThreads) {
-                const int at = (int)w.bin(logit_of(given[i]));
-                if (at >= a && at <= b) take(given[i]);
-            }
-        } else {
-            const float from = w.smallest(b);
-            const float below = a ? w.smallest(a - 1) : INFINITY;
-            walk.go([&](const auto &x, int i) {
-                float most = x[0];  // (few are taken: one question for all of them)
-#pragma unroll
-                for (int e = 1; e < W::V; ++e) most = fmaxf(most, x[e]);
-                if (!(most >= from)) return;
-#pragma unroll
-                for (int e = 0; e < W::V; ++e)
-                    if (x[e] >= from && (x[e] < below || a == 0))
-                        take(key_of(bounded(x[e]), i + e));
-            });
+        if (keys != nullptr) {
+            for (int i = threadIdx.x; i < gathered; i += kThreads)
+                if (keys[i] >= lo && keys[i] <= hi) f(keys[i]);
+            return;
         }
-        __syncthreads();
-        const int found = min((int)s.listed, kList);
-        sort(s, found);
-        for (int i = tid; i < kList; i += kThreads)
-            s.upto[i] = i < found ? w.mass(logit_of(s.list[i])) : 0;
-        __syncthreads();
-        run_up<false>(s, s.upto, nullptr);
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const u64 key = key_of(bounded(to_f32(logits[i])), i);
+            if (key >= lo && key <= hi) f(key);
+        }
+    }
+    // The keys of bins a .. b lie within these.
+    __device__ __forceinline__ u64 first_key(int a) const {
+        return a ? ((u64)order_of(w.smallest(a - 1)) + 1) << kIndexBits : 0;
+    }
+    __device__ __forceinline__ u64 last_key(int b) const {
+        return (((u64)order_of(w.smallest(b)) + 1) << kIndexBits) - 1;
     }
 
-    __device__ __forceinline__ void collect_up_to(int b) {
-        whole = true;
-        base = 0;
-        collect(0, b, 0, ~(u64)0);
+    // The list: the tokens with keys lo .. hi (at most kSort), sorted, and their running weights.
+    __device__ __forceinline__ void collect(u64 lo, u64 hi) {
+        const int tid = threadIdx.x;
+        if (tid == 0) s.listed = 0;
+        __syncthreads();
+        tokens(lo, hi, [&](u64 key) {
+            const uint32_t place = atomicAdd(&s.listed, 1u);
+            if (place < kSort) s.list[place] = key;
+        });
+        __syncthreads();
+        const int n = min((int)s.listed, kSort);
+        sort(s, n);
+        if (tid < kSort) {
+            const u64 m = run_up_lanes(tid < n ? w.mass(logit_of(s.list[tid])) : 0);
+            s.upto[tid] = m;
+            if ((tid & 63) == 63) s.wave_mass[tid >> 6] = m;
+        }
+        __syncthreads();
+        if (tid < kSort) {
+            u64 m = s.upto[tid];
+            for (int k = 0; k < tid >> 6; ++k) m += s.wave_mass[k];
+            s.upto[tid] = m;
+        }
+        __syncthreads();
     }
 
     // The list comes to hold the token of bin b whose running weight (COUNT: number) reaches target.
     template <bool COUNT>
     __device__ __forceinline__ void hold(int b, u64 target) {
-        if (first <= b && b <= last) return;
         base = b ? s.mass[b - 1] : 0;
-        uint32_t left = count_in(s, b, b);
-        u64 lo = 0, hi = ((u64)1 << (32 + kIndexBits)) - 1;
-        first = last = b;
-        while (left > kList) {  // cut by the keys' bits; a range of one key holds one token
-            first = 1;
-            last = 0;  // (not the whole bin: for this target alone)
+        u64 lo = first_key(b), hi = last_key(b);
+        uint32_t left;
+        if (keys != nullptr) {
+            if (threadIdx.x == 0) s.listed = 0;
+            __syncthreads();
+            tokens(lo, hi, [&](u64) { atomicAdd(&s.listed, 1u); });
+            __syncthreads();
+            left = s.listed;
+            __syncthreads();
+        } else {
+            left = count_in(s, b, b);
+        }
+        while (left > kSort) {  // cut by the keys' bits; a range of one key holds one token
             const int bits = 64 - __clzll(hi - lo);
             const int shift = bits > 11 ? bits - 11 : 0;
+            __syncthreads();
             for (int i = threadIdx.x; i < kBins; i += kThreads) {
                 s.part_count[i] = 0;
                 s.part_mass[i] = 0;
             }
             __syncthreads();
-            each(logits, 0, n, [&](const auto &x, int i) {
-#pragma unroll
-                for (int e = 0; e < W::V; ++e) {
-                    const float l = bounded(x[e]);
-                    const u64 key = key_of(l, i + e);
-                    if ((int)w.bin(l) != b || !(l >= w.least) || key < lo || key > hi ||
-                        key > limit)
-                        continue;
-                    const int at = (int)((key - lo) >> shift);
-                    atomicAdd(&s.part_count[at], 1u);
-                    if (!COUNT) atomicAdd(&s.part_mass[at], w.mass(l));
-                }
+            tokens(lo, hi, [&](u64 key) {
+                const int at = (int)((key - lo) >> shift);
+                atomicAdd(&s.part_count[at], 1u);
+                atomicAdd(&s.part_mass[at], COUNT ? (u64)1 : w.mass(logit_of(key)));
             });
             __syncthreads();
-            if (COUNT) {
-                for (int i = threadIdx.x; i < kBins; i += kThreads)
-                    s.part_mass[i] = s.part_count[i];
-                __syncthreads();
-            }
             run_up<true>(s, s.part_mass, s.part_count);
-            const int at = reach(s, s.part_mass, kBins, target - base);
-            left = count_parts(at);
+            const int at = reach<kBins>(s.part_mass, target - base);
+            left = s.part_count[at] - (at ? s.part_count[at - 1] : 0);
             base += at ? s.part_mass[at - 1] : 0;
             lo += (u64)at << shift;
             const u64 end = lo + (((u64)1 << shift) - 1);
             hi = end < hi ? end : hi;
             __syncthreads();
         }
-        collect(b, b, lo, hi);
-    }
-    __device__ __forceinline__ uint32_t count_parts(int at) const {
-        return s.part_count[at] - (at ? s.part_count[at - 1] : 0);
+        collect(lo, hi);
     }
 
     // The place in the list of the token whose running weight reaches target.
     __device__ __forceinline__ int by_mass(u64 target) {
-        hold<false>(reach(s, s.mass, kBins, target), target);
-        return reach(s, s.upto, kList, target - base);
+        hold<false>(reach<kBins>(s.mass, target), target);
+        return reach<kSort>(s.upto, target - base);
     }
 
     // The row's token, from its histogram's running sums.
     __device__ __forceinline__ void answer(const SampleArgs &p, int r, const Asked &q, bool counted,
                                            const Plan &plan, u64 total) {
-        if (counted) {
-            const u64 k = (u64)q.top_k < total ? (u64)q.top_k : total;
-            if (plan.listed) {
-                collect_up_to(plan.kept);
-                total = s.upto[k - 1];
-            } else {  // so many that their weights need a histogram too
+        int i;
+        if (plan.whole) {  // the list holds all tokens that may be kept
+            collect(0, last_key(plan.kept));
+            if (counted)
+                total = s.upto[q.top_k < kSort ? q.top_k - 1 : kSort - 1];
+            else if (!(q.top_p < 1.f))
+                total = s.upto[kSort - 1];
+            if (q.top_p < 1.f) total = s.upto[reach<kSort>(s.upto, q.kept(total))];
+            i = reach<kSort>(s.upto, q.drawn(total));
+        } else {
+            if (counted) {  // the tokens that top-k leaves get their weights
+                const u64 k = (u64)q.top_k < total ? (u64)q.top_k : total;
                 hold<true>(plan.kept, k);
                 limit = s.list[k - base - 1];
                 __syncthreads();
-                for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0;
+                for (int b = threadIdx.x; b < kBins; b += kThreads) s.mass[b] = 0;
                 __syncthreads();
-                fill<false>(s.mass, walk, w, limit);
+                tokens(0, limit, [&](u64 key) {
+                    uint32_t b;
+                    const u64 m = w.over_middle(w.below(logit_of(key)), b);
+                    atomicAdd(&s.mass[b], m);
+                });
                 __syncthreads();
                 finish<false>(s, w);
                 total = s.mass[kBins - 1];
-                first = 1;
-                last = 0;  // (its list went by numbers)
             }
-        } else if (plan.whole) {
-            collect_up_to(plan.kept);
+            if (q.top_p < 1.f) {
+                const u64 target = q.kept(total);
+                const u64 most = s.mass[reach<kBins>(s.mass, target)];
+                const int at = by_mass(target);
+                // (roundings of the bin's weight and of its tokens' must not reach into the next)
+                total = base + s.upto[at] < most ? base + s.upto[at] : most;
+            }
+            i = by_mass(q.drawn(total));
         }
-        if (whole) {
-            if (q.top_p < 1.f)
-                total = s.upto[reach(s, s.upto, kList, q.kept(total))];
-            else if (!counted)
-                total = s.upto[kList - 1];
-        } else if (q.top_p < 1.f) {
-            const u64 target = q.kept(total);
-            const u64 most = s.mass[reach(s, s.mass, kBins, target)];
-            const int i = by_mass(target);
-            // (roundings of the bin's weight and of its tokens' must not reach into the next bin)
-            total = base + s.upto[i] < most ? base + s.upto[i] : most;
-        }
-        const u64 target = q.drawn(total);
-        const int i = whole ? reach(s, s.upto, kList, target) : by_mass(target);
         if (threadIdx.x == 0) {
             const u64 key = s.list[i];
-            p.tokens[r] = min((int)(key & (((u64)1 << kIndexBits) - 1)), n - 1);
+            p.tokens[r] = min((int)(key & (((u64)1 << kIndexBits) - 1)), p.vocab - 1);
             p.probabilities[r] = (float)(w.share(logit_of(key)) * p.unit / (double)total);
         }
     }
@@ -811,9 +767,9 @@ sample_row_kernel(SampleArgs p) {
     w.init(p, high, low, q.temperature, q.min_p);
     const bool counted = q.counted(n);
     if (counted)
-        fill<true>(s.mass, walk, w, ~(u64)0);
+        fill<true>(s.mass, walk, w);
     else
-        fill<false>(s.mass, walk, w, ~(u64)0);
+        fill<false>(s.mass, walk, w);
     __syncthreads();
     if (counted)
         finish<true>(s, w);
@@ -822,8 +778,7 @@ sample_row_kernel(SampleArgs p) {
     const Plan plan = plan_of(s, q, counted);
     const u64 total = s.mass[kBins - 1];
     const int gathered = plan.listed ? gather(s, walk, w, plan) : 0;
-    Row<T, decltype(walk)> row{s, walk, logits, n, plan.listed ? s.gathered : nullptr, gathered, w,
-                               ~(u64)0, false, 1, 0, 0};
+    Row<T> row{s, logits, n, plan.listed ? s.gathered : nullptr, gathered, w, ~(u64)0, 0};
     row.answer(p, r, q, counted, plan, total);
 }
 // ------------------------------------------------------------- rows cut over work-groups
@@ -845,7 +800,7 @@ struct SplitArgs {
     int splits, chunk;  // parts of a row, tokens of a part
     u64 *mass;          // [rows][kBins]
     u64 *running;       // [rows][kBins], its running sums
-    u64 *list;          // [rows][kList]
+    u64 *list;          // [rows][kGather]
     float4 *parts;      // [rows][splits]: largest, smallest, whether one is NaN
     RowState *state;    // [rows]
 };
@@ -916,9 +871,9 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SplitArgs a) {
     if (kind != kDraw) return;
     __syncthreads();
     if (q.counted(p.vocab))
-        fill<true>(mass, walk, w, ~(u64)0);
+        fill<true>(mass, walk, w);
     else
-        fill<false>(mass, walk, w, ~(u64)0);
+        fill<false>(mass, walk, w);
     __syncthreads();
     for (int i = tid; i < kBins; i += kThreads)
         if (mass[i] != 0) atomicAdd(&a.mass[(int64_t)r * kBins + i], mass[i]);
@@ -973,8 +928,8 @@ __global__ void __launch_bounds__(kThreads) sample_gather_kernel(SplitArgs a) {
     if (tid == 0) s.found = atomicAdd(&state.listed, (uint32_t)found);
     __syncthreads();
     const int to = s.found;
-    for (int i = tid; i < found && to + i < kList; i += kThreads)
-        a.list[(int64_t)r * kList + to + i] = s.gathered[i];
+    for (int i = tid; i < found && to + i < kGather; i += kThreads)
+        a.list[(int64_t)r * kGather + to + i] = s.gathered[i];
 }
 
 template <typename T>
@@ -982,8 +937,7 @@ __global__ void __launch_bounds__(kThreads) sample_pick_kernel(SplitArgs a) {
     __shared__ Shared s;
     const SampleArgs &p = a.p;
     const int tid = threadIdx.x, r = blockIdx.x;
-    const T *logits = static_cast<const T *>(p.logits) + (int64_t)r * p.ld;
-    const u64 *list = a.list + (int64_t)r * kList;
+    const u64 *list = a.list + (int64_t)r * kGather;
     const RowState &state = a.state[r];
     const Asked q(p, r);
     const int kind = state.kind;
@@ -1008,13 +962,8 @@ __global__ void __launch_bounds__(kThreads) sample_pick_kernel(SplitArgs a) {
         for (int i = tid; i < kBins; i += kThreads) s.mass[i] = a.running[(int64_t)r * kBins + i];
         __syncthreads();
     }
-    Walk<T, 4> walk;  // (of a row that the list does not hold)
-    walk.row = logits;
-    walk.first = 0;
-    walk.end = p.vocab;
-    if (!plan.listed) walk.start(logits, 0, p.vocab);
-    Row<T, decltype(walk)> row{s, walk, logits, p.vocab, plan.listed ? list : nullptr,
-               plan.listed ? (int)min(state.listed, (uint32_t)kList) : 0, w, ~(u64)0, false, 1, 0,
+    Row<T> row{s, static_cast<const T *>(p.logits) + (int64_t)r * p.ld, p.vocab,
+               plan.listed ? list : nullptr, (int)min(state.listed, (uint32_t)kGather), w, ~(u64)0,
                0};
     row.answer(p, r, q, counted, plan, state.total);
 }
@@ -1022,14 +971,14 @@ __global__ void __launch_bounds__(kThreads) sample_pick_kernel(SplitArgs a) {
 template <typename T>
 int launch_split(hipStream_t stream, SplitArgs a) {
     const SampleArgs &p = a.p;
-    const size_t row = (2 * kBins + kList) * sizeof(u64) + a.splits * sizeof(float4) +
+    const size_t row = (2 * kBins + kGather) * sizeof(u64) + a.splits * sizeof(float4) +
                        sizeof(RowState);
     int rc = MIGEMM_OK;
     a.mass = static_cast<u64 *>(workspace(stream, p.rows * row, &rc, 0));
     if (a.mass == nullptr) return rc;
     a.running = a.mass + (int64_t)p.rows * kBins;
     a.list = a.running + (int64_t)p.rows * kBins;
-    a.parts = reinterpret_cast<float4 *>(a.list + (int64_t)p.rows * kList);
+    a.parts = reinterpret_cast<float4 *>(a.list + (int64_t)p.rows * kGather);
     a.state = reinterpret_cast<RowState *>(a.parts + (int64_t)p.rows * a.splits);
     const dim3 grid(a.splits, p.rows), block(kThreads);
     MIGEMM_LAUNCH((sample_top_kernel<T>), grid, block, 0, stream, a);
@@ -1045,7 +994,7 @@ int launch(hipStream_t stream, const SampleArgs &p) {
     a.p = p;
     const int most = p.vocab / 4096 < 64 ? p.vocab / 4096 : 64;
     a.splits = 512 / p.rows < most ? 512 / p.rows : most;
-    if (a.splits >= 2) {
+    if (p.vocab >= 40960 && p.rows <= p.vocab / 1024 && a.splits > 1) {
         // (whole vectors: a part begins at a multiple of 8 tokens)
         a.chunk = ((p.vocab + a.splits - 1) / a.splits + 7) / 8 * 8;
         a.splits = (p.vocab + a.chunk - 1) / a.chunk;
