@@ -473,7 +473,15 @@ __device__ __forceinline__ void sort(Shared &s, int n) {
     uint32_t less = 0;
     if (i < n) {
         key = s.list[i];
-        for (int j = part; j < n; j += per) less += s.list[j] < key;
+        int j = part;
+        for (; j + 7 * per < n; j += 8 * per) {  // (eight reads fly together)
+            u64 x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = s.list[j + k * per];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) less += x[k] < key;
+        }
+        for (; j < n; j += per) less += s.list[j] < key;
     }
     for (int o = 1; o < per; o *= 2) less += __shfl_xor(less, o);
     if (i < n && part == 0) s.upto[less] = key;
@@ -487,10 +495,6 @@ __device__ __forceinline__ void sort(Shared &s, int n) {
 struct Plan {
     bool whole, listed;
     int kept, first, last;  // the bin where top-k or top-p ends (-1: none does), those to draw from
-
-    __device__ __forceinline__ bool has(int b) const {
-        return whole ? b <= kept : b == kept || (first <= b && b <= last);
-    }
 };
 
 // Of the tokens of bins a .. b.
@@ -528,26 +532,38 @@ __device__ __forceinline__ Plan plan_of(Shared &s, const Asked &q, bool counted)
     return g;
 }
 
-// The keys of the plan's tokens into s.gathered; returns their number.
+// The logits of bins a .. b: from the smallest one's up to, but not with, the one that ends the bin
+// before (NaN: there is none).
+struct Span {
+    float from, end;
+
+    __device__ __forceinline__ Span(const Weights &w, int a, int b)
+        : from(w.smallest(b)), end(a > 0 ? w.smallest(a - 1) : __uint_as_float(0x7fc00000u)) {}
+    __device__ __forceinline__ bool has(float x) const { return x >= from && !(x >= end); }
+};
+
+// The keys of the plan's tokens into s.gathered; returns their number. Top-p's bin and those to draw
+// from are two spans of logits, so no token's bin is computed.
 template <typename W>
 __device__ __forceinline__ int gather(Shared &s, const W &walk, const Weights &w,
                                       const Plan &plan) {
     constexpr int V = W::V;
-    // the bins to draw from, and the one where top-p ends, which is not before them
-    const float from = w.smallest(plan.kept > plan.last ? plan.kept : plan.last);
+    const Span draw = plan.whole ? Span(w, 0, plan.kept) : Span(w, plan.first, plan.last);
+    const bool apart = !plan.whole && plan.kept > plan.last;
+    Span kept = draw;
+    if (apart) kept = Span(w, plan.kept, plan.kept);
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
     walk.go([&](const auto &x, int i) {
         float most = x[0];  // (few are taken: one question for all of them)
 #pragma unroll
         for (int e = 1; e < V; ++e) most = fmaxf(most, x[e]);
-        if (!(most >= from)) return;
+        if (!(most >= kept.from)) return;  // (kept is not before draw)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float l = bounded(x[e]);
-            if (!(l >= from) || !(plan.whole || plan.has((int)w.bin(l)))) continue;
+            if (!(draw.has(x[e]) || kept.has(x[e]))) continue;
             const uint32_t place = atomicAdd(&s.listed, 1u);
-            if (place < kGather) s.gathered[place] = key_of(l, i + e);
+            if (place < kGather) s.gathered[place] = key_of(bounded(x[e]), i + e);
         }
     });
     __syncthreads();
