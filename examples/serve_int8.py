@@ -2,9 +2,11 @@
 tables kept on the GPU.
 
 Each step takes any mix of prompts and single tokens: CacheTables finds pages and slots for the
-new tokens, and every layer runs LinearInt8 (q, k and v in one product), CacheAppend,
-CacheAttention and LinearInt8 again. The weights are random; `main` serves three requests of
-different lengths side by side, frees one and admits another in its place.
+new tokens, and every block runs NormInt8, a product of its rows (q, k and v in one), CacheAppend,
+CacheAttention, LinearInt8 with the residual, and the same for its two inner layers, the first with
+its activation. Sample chooses each request's next token. The weights are random; `main` serves
+three requests of different lengths side by side, each with its own temperature and top-p, frees one
+and admits another in its place.
 
     python examples/serve_int8.py
 """
@@ -22,31 +24,35 @@ from my_pytchon_opencl_lib_amd.layers import LinearInt8  # noqa: E402
 
 
 def normed(x):
+    """What NormInt8 holds in 8 bits, in the type of x (to compare with)."""
     return x / (x.float().square().mean(-1, keepdim=True) + 1e-6).sqrt().to(x.dtype)
 
 
 class Block:
     def __init__(self, nncl, width, heads, kvHeads, inner, g):
-        def layer(out, fan):
+        def layer(out, fan, activation=None):
             bound = 1 / math.sqrt(fan)
             return LinearInt8((torch.rand(out, fan, generator=g) * 2 - 1) * bound * 1.7,
-                              nnclglob=nncl)
+                              nnclglob=nncl, activation=activation)
         self.nncl, self.heads, self.kvHeads, self.dim = nncl, heads, kvHeads, width // heads
         self.qkv = layer((heads + 2 * kvHeads) * self.dim, width)
         self.out = layer(width, width)
-        self.up = layer(inner, width)
+        self.up = layer(inner, width, "silu")
         self.down = layer(width, inner)
 
     def __call__(self, x, cache, step):
         h, kv = self.heads, self.kvHeads
+        rows, scales, _ = self.nncl.NormInt8(x)
+        y = self.qkv.forwardRows(rows, scales, x.dtype)
+        q, k, v = y.unflatten(1, (h + 2 * kv, self.dim)).split((h, kv, kv), 1)
         # three slices of one product, taken by the operators as they lie
-        q, k, v = self.qkv(normed(x)).unflatten(1, (h + 2 * kv, self.dim)).split((h, kv, kv), 1)
         self.nncl.CacheAppend(k, v, step["slots"], cache)
         o = self.nncl.CacheAttention(q, cache, step["table"], step["starts"],
                                      step["positions"], maxCount=step["maxCount"],
                                      maxLength=step["maxLength"])
-        x = x + self.out(o.flatten(1))
-        return x + self.down(torch.nn.functional.silu(self.up(normed(x))))
+        x = self.out(o.flatten(1), residual=x)
+        rows, scales, _ = self.nncl.NormInt8(x)
+        return self.down(self.up.forwardRows(rows, scales, x.dtype), residual=x)
 
 
 class Server:
@@ -86,7 +92,12 @@ class Server:
         x = self.embed[flat.to(dev)] + torch.cat([angle.sin(), angle.cos()], 1).to(self.dtype)
         for block, cache in zip(self.blocks, self.caches):
             x = block(x, cache, step)
-        return self.head(normed(x))
+        rows, scales, _ = self.nncl.NormInt8(x)
+        return self.head.forwardRows(rows, scales, self.dtype)
+
+    def choose(self, logits, uniforms, temperature=1.0, topK=0, topP=1.0, minP=0.0):
+        """A token for each row of logits, from one random number a row, as a list."""
+        return self.nncl.Sample(logits, uniforms, temperature, topK, topP, minP)[0].tolist()
 
     def release(self, finished):
         """Frees the requests i with finished[i]: their pages may be given out again."""
@@ -101,6 +112,10 @@ def main():
     prompts = [list(range(1, 38)), [5, 6, 7], list(range(100, 180)), []]
     said = [[] for _ in prompts]
     new = prompts
+    # request 0 takes the likeliest token, the others sample
+    temperature = torch.tensor([0.0, 0.8, 1.0, 1.0], device="cuda")
+    topP = torch.tensor([1.0, 0.9, 0.95, 1.0], device="cuda")
+    rng = torch.Generator(device="cuda").manual_seed(1)
     for i in range(12):
         if i == 6:  # request 1 is done; another comes in its place
             server.release([False, True, False, False])
@@ -108,13 +123,17 @@ def main():
             said[1] = []
             new[1] = list(range(200, 220))
         logits = server.step(new)
-        at = -1
-        following = []
-        for r, t in enumerate(new):
-            at += len(t)
-            following.append([int(logits[at].argmax())] if t else [])
-            said[r] += following[r]
-        new = following
+        active = [r for r, t in enumerate(new) if t]
+        last, at = [], -1
+        for r in active:
+            at += len(new[r])
+            last.append(at)
+        chosen = server.choose(logits[last], torch.rand(len(active), generator=rng, device="cuda"),
+                               temperature[active], topP=topP[active])
+        new = [[] for _ in prompts]
+        for r, token in zip(active, chosen):
+            new[r] = [token]
+            said[r].append(token)
     for r, s in enumerate(said):
         if s:
             print("request", r, "said", s)

@@ -561,21 +561,24 @@ int migemm_cache_attention(void *stream, const void *Q, int type, int64_t ldq,
                            const int *positions, int requests, int tokens, int heads,
                            float scale, int max_count, int max_length, void *O);
 
-/* A token for each row of logits [rows, vocab] of `type` (rows ld apart; vocab <= 2^20), from one
- * random number a row, uniforms [rows] in [0, 1). Tokens are ordered by logit, largest first, equal
- * ones by index. A token weighs w = exp((logit - the row's largest) / temperature); then
+/* A token for each row of logits [rows, vocab] of `type` (rows ld apart; vocab <= 2^20), from
+ * one random number a row, uniforms [rows] in [0, 1). Tokens are ordered by logit, largest
+ * first, equal ones by index. A token weighs w = exp((logit - the row's largest) /
+ * temperature); then
  *   min_p   tokens with w < min_p weigh nothing (0: none)
  *   top_k   those beyond the first top_k weigh nothing (0 or less: none)
  *   top_p   of the others the fewest, first in the order, that hold top_p of their sum are kept
  *           (1 or more: all; 0 or less: one)
- * and the token is the first whose weights, up to its own, are more than uniform times the kept ones'
- * sum. probabilities[r] is its weight over that sum. temperature 0 gives the largest logit's
- * first token, with probability 1. Each parameter is one for all rows, or (temperatures, top_ks,
- * top_ps, min_ps [rows] on the GPU, where not NULL) one a row. Weights are 64-bit numbers rounded to 2^-42
- * of the largest or finer; their sums are exact. A logit of -inf is never chosen, inf counts as the
- * largest float32; a row without a logit above -inf, with a NaN, or with
- * a parameter that is NaN or a temperature that is negative or not finite gives token -1 and
- * probability 0. */
+ * and the token is the first whose weights, up to its own, are more than uniform times the kept
+ * ones' sum. probabilities[r] is its weight over that sum. temperature 0 gives the largest
+ * logit's first token, with probability 1. Each parameter is one for all rows, or
+ * (temperatures, top_ks, top_ps, min_ps [rows] on the GPU, where not NULL) one a row. Weights
+ * are held to 2^-39 of themselves and 2^-42 of the largest, and summed exactly. A logit of -inf
+ * is never chosen, inf counts as the largest float32; a row without a logit above -inf, with a
+ * NaN, or with a parameter that is NaN or a temperature that is negative or not finite gives
+ * token -1 and probability 0. One launch; rows of 40960 tokens or more, at most vocab / 1024 of
+ * them, are cut over work-groups in four, which use the stream's workspace (53 KB a row at
+ * most): reserve it before a capture. */
 int migemm_sample(void *stream, const void *logits, int type, int64_t ld, int rows, int vocab,
                   const float *uniforms, const float *temperatures, float temperature,
                   const int *top_ks, int top_k, const float *top_ps, float top_p,

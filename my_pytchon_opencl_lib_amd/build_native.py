@@ -17,7 +17,8 @@ SOURCES = ["cache_attention_f32.hip", "cache_attention_bf16.hip", "gemm_int8.hip
            "gemm_direct_64.hip", "gemm_split_256x128.hip", "gemm_split_128.hip",
            "gemm_split.hip", "gemm_mfma.hip", "api.hip", "gemm_direct.hip", "gemm_small.hip",
            "gemm_skinny.hip", "aux_kernels.hip", "runtime.hip", "gemm_panel.hip",
-           "gemm_tiny.hip", "quantize_rows.hip", "norm8.hip", "sample.hip", "cache8.hip", "serve_api.hip"]
+           "gemm_tiny.hip", "quantize_rows.hip", "norm8.hip", "sample.hip", "cache8.hip",
+           "serve_api.hip"]
 ARCH = "gfx950"
 
 

@@ -71,8 +71,8 @@ struct Relu {
 // exp(-2 u)), with a = 2 sqrt(2 / pi), b = 0.044715 a. log2(e) is folded into the constants, and
 // exponential and reciprocal are the hardware's (each within 1 ulp; about 45 cycles a wavefront
 // against 130 by division and a library exponential, on values that no product hides): off by
-// less than (4 + 1.5 |x (a + b x^2)|) 2^-23 of the value (the exponent's three roundings, then one of
-// each step), and 0 where the reciprocal is less than 2^-126.
+// less than (4 + 1.5 |x (a + b x^2)|) 2^-23 of the value (the exponent's three roundings, then one
+// of each step), and 0 where the reciprocal is less than 2^-126.
 template <bool CUBIC>
 struct Sigmoid {
     float a, b;
@@ -487,7 +487,8 @@ __global__ void __launch_bounds__(256) join_int8_kernel(Int8Args p, int64_t plan
     const int N = KIND == kGated ? p.outputs : p.t.N;
     const int n = min(4, N - col);
     const int64_t ld = (p.t.N + 3) & ~3;  // (rows padded to 4)
-    const int32_t *from = p.partial + row * ld + (KIND == kGated ? 2 * (col & ~15) + (col & 15) : col);
+    const int32_t *from =
+        p.partial + row * ld + (KIND == kGated ? 2 * (col & ~15) + (col & 15) : col);
     int sum[4] = {0, 0, 0, 0}, up[4] = {0, 0, 0, 0};
     for (int s = 0; s < p.t.splits; ++s) {
         const v4i x = *reinterpret_cast<const v4i *>(from + s * plane);

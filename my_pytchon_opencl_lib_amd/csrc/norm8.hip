@@ -106,7 +106,8 @@ __global__ void __launch_bounds__(256) norm_int8_kernel(NormInt8 p) {
         const int k = (c * TPR + t) * 8;
         if (RES && sum != nullptr) store_sum<T>(sum + k, cols - k, v[c]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) squares = __builtin_fma((double)v[c][i], (double)v[c][i], squares);
+        for (int i = 0; i < 8; ++i)
+            squares = __builtin_fma((double)v[c][i], (double)v[c][i], squares);
     }
     for (int k = (CH * TPR + t) * 8; k < cols; k += TPR * 8) {
         float a[8];

@@ -6,21 +6,28 @@
 // more than u times the kept ones' sum. So every step asks one question: where in the order does a
 // running count or sum cross a value? It is answered without sorting the row:
 //
-//   * A histogram of the row, in bins of equal width in (top - l). Its running sums name the bin that a value falls in. With top_k it holds counts
-//     (the few tokens that are left get their weights later), otherwise weights.
-//   * The tokens of that bin, or of all bins up to it where they are few, are collected into LDS
-//     and sorted there by logit and index; the running sums over them name the token. A bin of more
-//     tokens than the list holds (equal logits, mostly) is cut again by bits of logit and index
-//     until few are left.
+//   * A histogram of the row, in bins of equal width in (top - l). Its running sums name the bin that
+//     a value falls in. With top_k it holds counts (the few tokens that are left get their weights
+//     later), otherwise weights.
+//   * The tokens of the bins in question are gathered, those that can matter are sorted by logit and
+//     index, and the running sums over them name the token. A bin of more tokens than are sorted at
+//     once (equal logits, mostly) is first cut by bits of logit and index until few are left.
 //
 // Weights come from 64-bit arithmetic, because a sum of 10^5 float32 weights is off by more than a
 // token's share, and are summed as integers: exactly, in any order (atomics among them), so that a
 // result does not depend on how a row was walked. Within a bin's width of at most 0.047 in log2 w
-// a token's weight over its bin's middle one is a polynomial of degree 4 (off by 2^-39 at most); these are
-// summed with 43 fractional bits, and a bin's sum is multiplied by its middle weight once, to 42 bits
-// below the point or more (62 - log2(vocabulary), at most 46). Tokens that weigh less than half of
-// the last bit are left out.
+// a token's weight over its bin's middle one is a polynomial of degree 4 (off by 2^-39 at most);
+// these are summed with 43 fractional bits, and a bin's sum is multiplied by its middle weight
+// once, to 42 bits below the point or more (62 - log2(vocabulary), at most 46). Tokens that weigh
+// less than half of the last bit are left out.
 //
+// Logits are read three times: for the largest, for the histogram, for the gathering. One
+// work-group a row, two of them a CU, is bound by these reads (512 x 65536 float32: 70 us, of
+// which 20, 15 and 15 to 18 for 134 MB each; a copy's rate gives 26) and, with fewer rows than
+// CUs, by the 64-bit steps of the histogram (half of the float32 rate: 11 us for 65536 tokens) and
+// by what waits for what: 17 us for 1 x 32000, 4.5 of them the histogram. Few rows of many tokens
+// are cut over work-groups, in four launches (1 x 131072: 21 us with top-k, 38 for half of the
+// tokens' weight, against 39 and 92 in one work-group).
 #include "int8_common.h"
 
 namespace migemm {
@@ -107,8 +114,8 @@ __device__ __forceinline__ u64 rounded(double x, double unit) {
     return (u64)__double_as_longlong(y) & (((u64)1 << 52) - 1);
 }
 
-// What a row's logits weigh, and its bins: 2^j of them a unit of log2 of the weight, each around its
-// middle, a multiple of 2^-j.
+// What a row's logits weigh, and its bins: 2^j of them a unit of log2 of the weight, each around
+// its middle, a multiple of 2^-j.
 struct Weights {
     float least;   // the smallest logit that weighs something
     double top;    // the largest
@@ -166,10 +173,10 @@ struct Weights {
         const double d = below(l);
         return index(placed(d < cut ? d : cut));
     }
-    // The weight over the middle one of its bin, 2^f for |f| <= width / 2, with kFraction bits: 1 + f
-    // q(f), q of degree 3 through the Chebyshev nodes of (2^f - 1) / f (off by 2^-39 at the bin's
-    // ends). Eight 64-bit steps: the middle comes from adding and taking off `magic`, and the
-    // last step of the polynomial rounds to an integer, too.
+    // The weight over the middle one of its bin, 2^f for |f| <= width / 2, with kFraction bits: 1
+    // + f q(f), q of degree 3 through the Chebyshev nodes of (2^f - 1) / f (off by 2^-39 at the
+    // bin's ends). Eight 64-bit steps: the middle comes from adding and taking off `magic`, and
+    // the last step of the polynomial rounds to an integer, too.
     __device__ __forceinline__ u64 over_middle(double d, uint32_t &b) const {
         const double t = placed(d);
         b = index(t);
@@ -258,10 +265,10 @@ __device__ __forceinline__ void of_logits(const uint4 &raw, int at, const F &f) 
     f(x, at);
 }
 
-// Calls f(logits, place of the first) for the logits first .. end of a row, 16 bytes at a time, those of
-// a thread in ascending order (and with -inf for places behind the end). The first HELD vectors of a thread stay in registers
-// from start() on, for as many walks as there are; what is beyond comes in parts of four vectors,
-// each on its way while the one before is looked at.
+// Calls f(logits, place of the first) for the logits first .. end of a row, 16 bytes at a time,
+// those of a thread in ascending order (and with -inf for places behind the end). The first HELD
+// vectors of a thread stay in registers from start() on, for as many walks as there are; what is
+// beyond comes in parts of four vectors, each on its way while the one before is looked at.
 template <typename T, int HELD>
 struct Walk {
     static constexpr int V = 16 / sizeof(T), STEP = kThreads * V, U = 4;
@@ -446,8 +453,8 @@ __device__ __forceinline__ void finish(Shared &s, const Weights &w) {
     run_up<true>(s, s.mass, s.count);
 }
 
-// The first place whose running sum reaches target (the last one's does, or the last sum is taken for
-// it). Every wavefront looks for itself: at every N / 64-th sum, then at those between.
+// The first place whose running sum reaches target (the last one's does, or the last sum is taken
+// for it). Every wavefront looks for itself: at every N / 64-th sum, then at those between.
 template <int N>
 __device__ __forceinline__ int reach(const u64 *sums, u64 target) {
     constexpr int STEP = N / 64;
@@ -461,9 +468,9 @@ __device__ __forceinline__ int reach(const u64 *sums, u64 target) {
     return from + __ffsll(near) - 1;
 }
 
-// Sorts the first n keys of the list, with `upto` as room: each finds its place by counting the smaller
-// ones, two threads or more a key. (64 keys: 0.3 us, 3.0 by exchanges, each of whose steps waits for
-// the one before.)
+// Sorts the first n keys of the list, with `upto` as room: each finds its place by counting the
+// smaller ones, two threads or more a key. (64 keys: 0.3 us, 3.0 by exchanges, each of whose steps
+// waits for the one before.)
 __device__ __forceinline__ void sort(Shared &s, int n) {
     const int tid = threadIdx.x;
     int per = kThreads / kSort;  // threads a key
@@ -490,8 +497,9 @@ __device__ __forceinline__ void sort(Shared &s, int n) {
     __syncthreads();
 }
 
-// Bins whose tokens a row's answer may need, as far as the histogram tells: all up to one of them that
-// can be sorted at once (whole), or single ones. `listed`: they are few enough to be gathered.
+// Bins whose tokens a row's answer may need, as far as the histogram tells: all up to one of them
+// that can be sorted at once (whole), or single ones. `listed`: they are few enough to be
+// gathered.
 struct Plan {
     bool whole, listed;
     int kept, first, last;  // the bin where top-k or top-p ends (-1: none does), those to draw from
@@ -542,8 +550,8 @@ struct Span {
     __device__ __forceinline__ bool has(float x) const { return x >= from && !(x >= end); }
 };
 
-// The keys of the plan's tokens into s.gathered; returns their number. Top-p's bin and those to draw
-// from are two spans of logits, so no token's bin is computed.
+// The keys of the plan's tokens into s.gathered; returns their number. Top-p's bin and those to
+// draw from are two spans of logits, so no token's bin is computed.
 template <typename W>
 __device__ __forceinline__ int gather(Shared &s, const W &walk, const Weights &w,
                                       const Plan &plan) {
@@ -570,8 +578,9 @@ __device__ __forceinline__ int gather(Shared &s, const W &walk, const Weights &w
     return min((int)s.listed, kGather);
 }
 
-// A row and what is known of it. Its tokens come from keys that were gathered, or (keys null; a row of
-// too many, and walked simply, so that this rare case takes no registers from the other) its logits.
+// A row and what is known of it. Its tokens come from keys that were gathered, or (keys null; a
+// row of too many, and walked simply, so that this rare case takes no registers from the other)
+// its logits.
 template <typename T>
 struct Row {
     Shared &s;
@@ -631,7 +640,8 @@ struct Row {
         __syncthreads();
     }
 
-    // The list comes to hold the token of bin b whose running weight (COUNT: number) reaches target.
+    // The list comes to hold the token of bin b whose running weight (COUNT: number) reaches
+    // target.
     template <bool COUNT>
     __device__ __forceinline__ void hold(int b, u64 target) {
         base = b ? s.mass[b - 1] : 0;

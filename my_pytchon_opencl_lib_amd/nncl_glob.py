@@ -17,9 +17,11 @@ Reference interfaces mirrored (paths relative to the reference repository;
   permute(x, axes)                    :148     NnClGlob.permute(x, axes)
   bmm_backward(grad_output, A, B)     :283     NnClGlob.bmm_backward(grad_output, A, B)
 
-Beyond the reference, for serving in 8 bits: QuantizeRows, MatmulInt8, LinearInt8 (layers with
-int8 weights) and CacheTables, CacheSlots, CacheRelease, CacheAppend, CacheRead,
-CacheAttention (an int8 paged cache, cache.Int8Cache, and the attention that reads it).
+Beyond the reference, for serving in 8 bits: QuantizeRows, NormInt8 (rows of activations in 8
+bits, as they are or normed), MatmulInt8, LinearInt8 (layers with int8 weights; an activation, a
+gate and a residual in their launch), CacheTables, CacheSlots, CacheRelease, CacheAppend, CacheRead,
+CacheAttention (an int8 paged cache, cache.Int8Cache, and the attention that reads it) and Sample
+(a token for each row of logits).
 
 Tensors are torch float32 tensors resident on the GPU (torch is only the device-memory and
 stream plumbing); every operator enqueues a HIP kernel of libmigemm.so on the current torch
@@ -827,7 +829,9 @@ class NnClGlob:
         that. temperature 0: the largest logit's first token. Every parameter is a number, or a
         tensor [rows] (float32; topK int32) with one for each row. Rows that allow no token (all
         -inf), that hold a NaN, or whose tensors' parameters are NaN or a temperature negative or
-        infinite give token -1 and probability 0."""
+        infinite give token -1 and probability 0; a logit of inf counts as the largest float32. Few
+        rows (at most vocabulary / 1024) of 40960 tokens or more use the stream's workspace
+        (reserve_workspace before a capture)."""
         code = _check_rows("logits", logits, 2)
         rows, vocab = logits.shape
         _check_typed("uniforms", uniforms, torch.float32, (rows,))

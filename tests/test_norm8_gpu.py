@@ -1,5 +1,5 @@
-"""GPU tests of NnClGlob.NormInt8: the residual's addition, the root-mean-square norm and its rows in
-8 bits.
+"""GPU tests of NnClGlob.NormInt8: the residual's addition, the root-mean-square norm and its rows
+in 8 bits.
 
 Its rule is compared bit for bit with numpy: the sum is one float32 addition (rounded to bfloat16
 where that is the type), the sum of squares and its root are taken in 64 bits and rounded to

@@ -1,11 +1,11 @@
 """GPU tests of NnClGlob.Sample against the definition in 64 bits.
 
-The tokens have to be the same. The kernel rounds a weight to 2^-42 of the largest or finer (and its
-power is off by 2^-50), so that its sums are off by less than 2^-30 of them for the vocabularies here;
-a token differs only where u times the sum lies that near the border of two shares: for one row
-in 2^30 / vocabulary, at least 10^3 (all weights equal and inexact), far more for others; inputs are
-fixed, and where all weights are equal they are exact. A probability is a quotient of such
-numbers rounded to float32: within 2^-24 + 2^-30 of it, relatively."""
+The tokens have to be the same. The kernel's weights are off by 2^-39 of themselves and 2^-43 of the
+largest, at most, so that their sums are off by less than 2^-30 of them for the vocabularies here
+(2^17 2^-43 of the largest, which is part of the sum, and 2^-39); a token differs only where u times
+the sum lies that near the border of two shares, on one row in 10^3 for the worst of them and far
+fewer for others; inputs are fixed, and where all weights are equal they are exact. A probability
+is a quotient of such numbers rounded to float32: within 2^-24 + 2^-30 of it, relatively."""
 import numpy as np
 import pytest
 import torch
@@ -32,7 +32,7 @@ def one(v, i):
 
 def row64(x, u, t, k, p, least):
     """(token, probability) of one row of float64 logits."""
-    if np.isnan(x).any() or not x.max() > -INF or not 0 <= t < INF or any(map(np.isnan, (u, p, least))):
+    if np.isnan(x).any() or not x.max() > -INF or not 0 <= t < INF or np.isnan(u + p + least):
         return -1, 0.0
     order = np.argsort(-x, kind="stable")
     if t == 0:
@@ -219,7 +219,8 @@ def test_shares_of_many_draws(nncl):
     p = torch.softmax(x[0].double(), 0)
     got = torch.bincount(tokens.long(), minlength=6).double()
     assert bool(((got - n * p).abs() <= 1.0).all())
-    assert bool(((chances.double() - p[tokens.long()]).abs() <= 2.0 ** -23 * p[tokens.long()]).all())
+    drawn = p[tokens.long()]
+    assert bool(((chances.double() - drawn).abs() <= 2.0 ** -23 * drawn).all())
 
 
 def test_another_stream_and_replayed_graph(nncl):
@@ -241,6 +242,71 @@ def test_another_stream_and_replayed_graph(nncl):
         x.copy_(2 * torch.randn(20, 50001, generator=gen(10 + i), device="cuda"))
         u.copy_(torch.rand(20, generator=gen(20 + i), device="cuda"))
         expect = nncl.Sample(x, u, 0.9, 0, 0.9, 0.01)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], expect[0]) and torch.equal(got[1], expect[1])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_whole_rows_and_rows_cut_over_work_groups_agree(nncl, kind):
+    """49152 tokens: up to 48 rows are cut over work-groups, more are not. Both give the same bits,
+    with filters of every kind (single numbers and one a row), and those of the definition."""
+    g = gen(31)
+    rows, vocab = 64, 49152
+    x = (2.5 * torch.randn(rows, vocab, generator=g, device="cuda")).to(TYPES[kind])
+    x[5] = 1.25
+    x[6, 100:] = -INF
+    x[7] = -INF
+    x[8, 9] = float("nan")
+    u = torch.rand(rows, generator=g, device="cuda")
+    for f in FILTERS + [(1.0, 700, 0.8, 0.0), (1.5, 20000, 0.9, 0.0)]:
+        say(f)
+        whole = nncl.Sample(x, u, *f)
+        for a, b in ((0, 1), (1, 9), (9, 40), (16, 64)):
+            cut = nncl.Sample(x[a:b], u[a:b], *f)
+            assert torch.equal(cut[0], whole[0][a:b]) and torch.equal(cut[1], whole[1][a:b])
+        check(nncl, x[4:12], u[4:12], *f)
+
+
+def test_two_streams_at_once(nncl):
+    """Calls on two streams, each with its own workspace, give the bits of calls one by one."""
+    xs = [torch.randn(3, 131072, generator=gen(i), device="cuda") for i in range(2)]
+    us = [torch.rand(3, generator=gen(10 + i), device="cuda") for i in range(2)]
+    want = [nncl.Sample(x, u, 0.8, 0, 0.9) for x, u in zip(xs, us)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(nncl.Sample(xs[i], us[i], 0.8, 0, 0.9))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(t, want[i][0]) and torch.equal(c, want[i][1]) for t, c in got[i])
+
+
+@pytest.mark.parametrize("rows,vocab,uses", [(1, 40959, False), (41, 40960, False),
+                                             (40, 40960, True), (1, 131072, True)])
+def test_capture_needs_a_workspace_where_the_header_says(nncl, rows, vocab, uses):
+    x = torch.randn(rows, vocab, generator=gen(vocab), device="cuda")
+    u = torch.rand(rows, generator=gen(rows), device="cuda")
+    stream = torch.cuda.Stream()
+    _native.call("migemm_workspace_release", stream.cuda_stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    if uses:
+        with pytest.raises(_native.MigemmRuntimeError, match="WORKSPACE"):
+            with torch.cuda.graph(graph, stream=stream):
+                nncl.Sample(x, u)
+        torch.cuda.synchronize()
+        nncl.reserve_workspace(stream, 8 << 20)
+        graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = nncl.Sample(x, u)
+    for i in range(3):
+        u.copy_(torch.rand(rows, generator=gen(50 + i), device="cuda"))
+        expect = nncl.Sample(x, u)
         torch.cuda.synchronize()
         graph.replay()
         torch.cuda.synchronize()
