@@ -192,7 +192,11 @@ struct Weights {
         const double y = below(l) * rate;
         return y < 64.0 ? power(-y) : 0.0;
     }
-    __device__ __forceinline__ u64 mass(float l) const { return rounded(share(l), unit); }
+    // (A token that is not beyond the cut weighs something.)
+    __device__ __forceinline__ u64 mass(float l) const {
+        const u64 m = rounded(share(l), unit);
+        return m < 1 ? 1 : m;
+    }
 };
 
 // What a row asks for.
@@ -888,8 +892,9 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SplitArgs a) {
     }
     const bool some = q.valid && __ballot(x.z != 0.f) == 0 && x.x > -INFINITY;
     const int kind = !some ? kNothing : q.greedy() ? kGreedy : kDraw;
-    Weights w;
-    w.init(p, x.x, x.y, q.temperature, q.min_p);
+    Weights w{};
+    w.top = x.x;
+    if (kind == kDraw) w.init(p, x.x, x.y, q.temperature, q.min_p);
     if (part == 0 && tid == 0) {
         a.state[r].w = w;
         a.state[r].kind = kind;

@@ -81,10 +81,11 @@ def test_against_the_definition(nncl, rows, vocab, kind):
         check(nncl, logits, torch.rand(rows, generator=g, device="cuda"), *f)
 
 
+@pytest.mark.parametrize("rows,vocab", [(96, 5003), (44, 50001), (30, 70003)])
 @pytest.mark.parametrize("kind", TYPES)
-def test_parameters_of_each_row(nncl, kind):
+def test_parameters_of_each_row(nncl, rows, vocab, kind):
     """Every filter on and off in one call, among rows whose parameters say nothing."""
-    rows, vocab = 96, 5003
+    say("mixed", rows, vocab, kind)
     g = gen(5)
     logits = (2 * torch.randn(rows, vocab, generator=g, device="cuda")).to(TYPES[kind])
     logits[torch.rand(rows, vocab, generator=g, device="cuda") < 0.3] = -INF
