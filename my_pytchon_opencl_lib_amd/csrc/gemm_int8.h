@@ -199,21 +199,25 @@ __device__ __forceinline__ int block_row(int r) {
     return (r & ~5) | ((r >> 2) & 1) | ((r & 1) << 2);
 }
 
-// Four neighbouring values, those at and after `left` as the first (which is there).
-__device__ __forceinline__ void load_four(const float *from, int left, float (&v)[4]) {
-    if (left >= 4) {
-        const v4f x = load_any<v4f>(from);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = x[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = from[e < left ? e : 0];
-    }
+// The scales and bias of a tile's rows and columns, one value a thread: loaded as the kernel begins,
+// kept in a register and put into LDS for its end (read there as they are used, each block waits for
+// them). By place: the rows' scales, the columns' (of a gated tile the gate's outputs, then the other
+// half's), the columns' bias.
+template <int KIND, int BM, int BN>
+__device__ __forceinline__ float closing_value(const Int8Args &p, int m0, int n0, int i) {
+    if (i < BM) return p.sa[min(m0 + i, p.t.M - 1)];
+    const int c = (i - BM) % BN;
+    const float *from = i < BM + BN ? p.sb : p.bias;
+    if (i >= BM + 2 * BN || from == nullptr) return 0.f;
+    if (KIND != kGated) return from[min(n0 + c, p.outputs - 1)];
+    return from[(c < BN / 2 ? 0 : p.outputs) + min(n0 / 2 + c % (BN / 2), p.outputs - 1)];
 }
 
-template <typename T, int KIND, int FM, int FN>
-__device__ __forceinline__ void store_closed(const Int8Args &p, int32_t *block, int r0, int c0,
-                                             int lane, const v16i (&acc)[FM][FN]) {
+// block: this wavefront's 4 KB; held: the closing values. r0, c0: this wavefront's place in the tile.
+template <typename T, int KIND, int BM, int BN, int FM, int FN>
+__device__ __forceinline__ void store_closed(const Int8Args &p, int32_t *block, const float *held,
+                                             int m0, int n0, int r0, int c0, int lane,
+                                             const v16i (&acc)[FM][FN]) {
     constexpr bool GATED = KIND == kGated;
     constexpr int COLS = GATED ? 16 : 32;     // outputs of a block's row
     constexpr int LANES = COLS / 4;           // lanes that take a row
@@ -221,26 +225,28 @@ __device__ __forceinline__ void store_closed(const Int8Args &p, int32_t *block, 
     constexpr int PASSES = 32 / ROWS;
     const int lo = lane & 31, hi = lane >> 5;
     const int from = lane % LANES * 4, at = lane / LANES;
-    const int N = p.outputs;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-        const int out = (GATED ? c0 / 2 : c0) + j * COLS + from;
-        const int left = N - out, o = left > 0 ? out : 0;
-        float sb[4], bias[4] = {0.f, 0.f, 0.f, 0.f}, sb_up[4], bias_up[4] = {0.f, 0.f, 0.f, 0.f};
-        load_four(p.sb + o, left, sb);
-        if (GATED) load_four(p.sb + N + o, left, sb_up);
-        if (p.bias != nullptr) {
-            load_four(p.bias + o, left, bias);
-            if (GATED) load_four(p.bias + N + o, left, bias_up);
+        const int local = (GATED ? c0 / 2 : c0) + j * COLS + from;
+        const int out = (GATED ? n0 / 2 : n0) + local;
+        const int left = p.outputs - out, o = left > 0 ? out : 0;
+        const float *columns = held + BM + local;
+        const v4f sb = *reinterpret_cast<const v4f *>(columns);
+        const v4f bias = *reinterpret_cast<const v4f *>(columns + BN);
+        v4f sb_up = sb, bias_up = bias;
+        if (GATED) {
+            sb_up = *reinterpret_cast<const v4f *>(columns + BN / 2);
+            bias_up = *reinterpret_cast<const v4f *>(columns + BN + BN / 2);
         }
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             float sa[PASSES], add[PASSES][4];
 #pragma unroll
             for (int s = 0; s < PASSES; ++s) {
-                const int row = min(r0 + i * 32 + block_row(s * ROWS + at), p.t.M - 1);
-                sa[s] = p.sa[row];
-                load_f32<T, 4>(static_cast<const T *>(p.residual) + (int64_t)row * p.ldr + o,
+                const int row = r0 + i * 32 + block_row(s * ROWS + at);
+                sa[s] = held[row];
+                load_f32<T, 4>(static_cast<const T *>(p.residual) +
+                                   (int64_t)min(m0 + row, p.t.M - 1) * p.ldr + o,
                                p.residual != nullptr ? left : 0, add[s]);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -251,11 +257,11 @@ __device__ __forceinline__ void store_closed(const Int8Args &p, int32_t *block, 
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int s = 0; s < PASSES; ++s) {
-                const int row = r0 + i * 32 + block_row(s * ROWS + at);
-                const int32_t *held = block + (s * ROWS + at) * 32 + from;
-                const v4i sum = *reinterpret_cast<const v4i *>(held);
+                const int row = m0 + r0 + i * 32 + block_row(s * ROWS + at);
+                const int32_t *sums = block + (s * ROWS + at) * 32 + from;
+                const v4i sum = *reinterpret_cast<const v4i *>(sums);
                 v4i up = sum;
-                if (GATED) up = *reinterpret_cast<const v4i *>(held + 16);
+                if (GATED) up = *reinterpret_cast<const v4i *>(sums + 16);
                 struct Raw {
                     T v[4];
                 } y;
@@ -311,6 +317,8 @@ gemm_int8_kernel(Int8Args p) {
     __shared__ __attribute__((aligned(16))) float lds[S * (A_FL + B_FL)];
     float *const lds_a = lds, *const lds_b = lds + S * A_FL;
 
+    static_assert(NT >= BM + 2 * BN, "a closing value a thread");
+    __shared__ __attribute__((aligned(16))) float closing[KIND == kProduct ? 4 : BM + 2 * BN];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -326,6 +334,9 @@ gemm_int8_kernel(Int8Args p) {
     else
         opb.init(p.t.B, p.t.ldb, tc.n0, p.t.N, wave, lane);
 
+    float mine = 0.f;
+    if (KIND != kProduct)
+        mine = closing_value<KIND, BM, BN>(p, tc.m0, tc.n0, threadIdx.x);
     v16i acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -451,9 +462,11 @@ gemm_int8_kernel(Int8Args p) {
     T *C = static_cast<T *>(p.C);
     if constexpr (KIND != kProduct) {
         static_assert(S * (A_FL + B_FL) >= WM * WN * 1024, "4 KB of LDS a wavefront");
-        __syncthreads();  // every wavefront has read its last operands
-        store_closed<T, KIND, FM, FN>(p, reinterpret_cast<int32_t *>(lds) + wave * 1024, r0, c0,
-                                      lane, acc);
+        if ((int)threadIdx.x < BM + 2 * BN) closing[threadIdx.x] = mine;
+        __syncthreads();  // (and every wavefront has read its last operands)
+        store_closed<T, KIND, BM, BN, FM, FN>(p, reinterpret_cast<int32_t *>(lds) + wave * 1024,
+                                              closing, tc.m0, tc.n0, wm * (BM / WM),
+                                              wn * (BN / WN), lane, acc);
         return;
     }
     float sb[FN], bias[FN];

@@ -1024,7 +1024,7 @@ int launch(hipStream_t stream, const SampleArgs &p) {
     SplitArgs a{};
     a.p = p;
     const int most = p.vocab / 4096 < 64 ? p.vocab / 4096 : 64;
-    a.splits = 512 / p.rows < most ? 512 / p.rows : most;
+    a.splits = 256 / p.rows < most ? 256 / p.rows : most;
     if (p.vocab >= 40960 && p.rows <= p.vocab / 1024 && a.splits > 1) {
         // (whole vectors: a part begins at a multiple of 8 tokens)
         a.chunk = ((p.vocab + a.splits - 1) / a.splits + 7) / 8 * 8;

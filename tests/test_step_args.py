@@ -2,9 +2,14 @@
 norm, the products with activation, gate and residual, and sampling. Every C entry refuses bad
 arguments with a message before it touches HIP (the pointers here are never followed), and the
 Python operators refuse CPU tensors."""
+import os
+import re
+import subprocess
+
 import pytest
 
 from my_pytchon_opencl_lib_amd import _native
+from test_codegen import CSRC, _hipcc
 from test_serve_args import ALIAS, INVALID, UNSUPPORTED, P
 
 
@@ -140,3 +145,21 @@ def test_python_operators_refuse_cpu_tensors():
                  lambda: g.Sample(x, x[:, 0])):
         with pytest.raises(ShapeError, match="no CPU fallback"):
             call()
+
+
+@pytest.mark.skipif(_hipcc() is None, reason="hipcc not available")
+@pytest.mark.parametrize("name", ["gemm_int8_epilogue", "gemm_int8_gated"])
+def test_m0_only_feeds_the_lds_loads(tmp_path, name):
+    """The closed products' tiles are loaded by the same inline assembly as the plain ones'."""
+    out = tmp_path / (name + ".s")
+    r = subprocess.run([_hipcc(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang",
+                        "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-inline-asm",
+                        "--cuda-device-only", "-S", os.path.join(CSRC, name + ".hip"), "-o",
+                        str(out)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+    lines = [l.split(";")[0].strip() for l in out.read_text().splitlines()]
+    code = [l for l in lines if l and not l.startswith(".") and not l.endswith(":")]
+    loads = [i for i, l in enumerate(code) if re.match(r"global_load_lds_dwordx4 ", l)]
+    uses = [i for i, l in enumerate(code) if re.search(r"\bm0\b", l)]
+    assert loads and [i + 1 for i in uses] == loads
+    assert all(re.fullmatch(r"s_mov_b32 m0, s\d+", code[i]) for i in uses)
