@@ -14,10 +14,18 @@
 //
 // One pass over the data: a row stays in registers between its sum of squares, its maximum and the
 // rounding, so x and the residual are read once and the sum and a byte a value written: bound by
-// memory.
+// memory. 8192 x 4096 in bfloat16 with a residual take 47-49 us, 4.9 TB/s read and written, where
+// a large copy reaches 5.1; 1 x 4096 takes 3.5 us and 1000 x 777 in float32 5.3 us, a launch and
+// the latency of its loads. The weight is loaded with the row, so that its latency passes under
+// the sum of squares (loaded where it is used, 4096 x 777 in bfloat16 took 11.4 us and now 9.0).
+//
 // A wavefront takes a row of up to 2048 values (four rows a work-group, no barrier); longer ones
-// take a work-group of 256 threads, which keeps 16384 values and reads what is beyond them three
-// times (from L2).
+// take a work-group. What a thread keeps of a row decides how many rows are in flight: at 4096
+// rows of 8192 in bfloat16, 512 threads with 16 values each take 46 us, 256 with 32 48 us and 256
+// with 64 93 us; 2048 rows of 16384 take 48 us in 512 threads with 32 values, 56 in 1024 with 16.
+// Up to 4096 values 256 threads with 16 are ahead of 512 with 8 by 5 % in bfloat16 with many rows
+// (24.2 us against 25.4) and behind by 4 % in float32. What is beyond 16384 values is read three
+// times, from L2 (1024 x 20000: 35 us).
 #include "int8_common.h"
 
 namespace migemm {
@@ -51,16 +59,18 @@ __device__ __forceinline__ void store_sum(T *out, int left, const float (&v)[8])
     }
 }
 
-__device__ __forceinline__ void normed(float (&v)[8], float q, const float *w, int left) {
+// (Times a weight of 1 nothing is rounded.)
+__device__ __forceinline__ void load_weight(const float *w, int k, int cols, float (&a)[8]) {
     if (w != nullptr) {
-        float a[8];
-        load_f32<float, 8>(w, left, a);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] * q * a[i];
+        load_f32<float, 8>(w + k, cols - k, a);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] * q;
+        for (int i = 0; i < 8; ++i) a[i] = 1.f;
     }
+}
+__device__ __forceinline__ void normed(float (&v)[8], float q, const float (&a)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = v[i] * q * a[i];
 }
 
 __device__ __forceinline__ uint32_t magnitude(const float (&v)[8], uint32_t most) {
@@ -83,23 +93,25 @@ __device__ __forceinline__ void store_bytes(int8_t *out, const float (&v)[8], fl
 
 // TPR threads a row, each CH chunks of 8 neighbouring values in registers.
 template <typename T, bool RES, int TPR, int CH>
-__global__ void __launch_bounds__(256) norm_int8_kernel(NormInt8 p) {
-    constexpr int RPB = 256 / TPR;
+__global__ void __launch_bounds__(TPR == 64 ? 256 : TPR) norm_int8_kernel(NormInt8 p) {
+    constexpr int RPB = TPR == 64 ? 4 : 1;
     const int t = threadIdx.x % TPR;
     const int r = blockIdx.x * RPB + threadIdx.x / TPR;
-    __shared__ double part[4];
-    __shared__ uint32_t tops[4];
-    if (TPR == 64 && r >= p.rows) return;  // (a wavefront of its own; TPR 256 has a row always)
+    __shared__ double part[TPR / 64];
+    __shared__ uint32_t tops[TPR / 64];
+    if (TPR == 64 && r >= p.rows) return;  // (a wavefront of its own; a work-group has its row)
     const T *x = static_cast<const T *>(p.X) + (int64_t)r * p.ldx;
     const T *res = RES ? static_cast<const T *>(p.R) + (int64_t)r * p.ldr : nullptr;
     T *sum = RES && p.S != nullptr ? static_cast<T *>(p.S) + (int64_t)r * p.lds : nullptr;
     const int cols = p.cols;
-    float v[CH][8];
+    float v[CH][8], weight[CH][8];  // (the weight is on its way while squares are summed)
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int k = (c * TPR + t) * 8;
         load_sum<T, RES>(x + k, res + k, cols - k, v[c]);
     }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) load_weight(p.weight, (c * TPR + t) * 8, cols, weight[c]);
     double squares = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -118,24 +130,26 @@ __global__ void __launch_bounds__(256) norm_int8_kernel(NormInt8 p) {
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) squares += __shfl_xor(squares, o);
-    if constexpr (TPR == 256) {
+    if constexpr (TPR > 64) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = squares;
         __syncthreads();
-        squares = part[0] + part[1] + part[2] + part[3];
+        squares = part[0];
+#pragma unroll
+        for (int i = 1; i < TPR / 64; ++i) squares += part[i];
     }
     const float q = (float)(1.0 / __builtin_sqrt(squares / (double)cols + (double)p.eps));
 
     uint32_t most = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int k = (c * TPR + t) * 8;
-        normed(v[c], q, p.weight != nullptr ? p.weight + k : nullptr, cols - k);
+        normed(v[c], q, weight[c]);
         most = magnitude(v[c], most);
     }
     for (int k = (CH * TPR + t) * 8; k < cols; k += TPR * 8) {
-        float a[8];
+        float a[8], b[8];
         load_sum<T, RES>(x + k, res + k, cols - k, a);
-        normed(a, q, p.weight != nullptr ? p.weight + k : nullptr, cols - k);
+        load_weight(p.weight, k, cols, b);
+        normed(a, q, b);
         most = magnitude(a, most);
     }
 #pragma unroll
@@ -143,11 +157,11 @@ __global__ void __launch_bounds__(256) norm_int8_kernel(NormInt8 p) {
         const uint32_t b = __shfl_xor(most, o);
         most = b > most ? b : most;
     }
-    if constexpr (TPR == 256) {
+    if constexpr (TPR > 64) {
         if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = most;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) most = tops[i] > most ? tops[i] : most;
+        for (int i = 0; i < TPR / 64; ++i) most = tops[i] > most ? tops[i] : most;
     }
     const float s = scale_of(most);
     const float inv = inverse_scale(s);
@@ -160,9 +174,10 @@ __global__ void __launch_bounds__(256) norm_int8_kernel(NormInt8 p) {
         if (k < padded) store_bytes(out + k, v[c], inv);
     }
     for (int k = (CH * TPR + t) * 8; k < padded; k += TPR * 8) {
-        float a[8];
+        float a[8], b[8];
         load_sum<T, RES>(x + k, res + k, cols - k, a);
-        normed(a, q, p.weight != nullptr ? p.weight + k : nullptr, cols - k);
+        load_weight(p.weight, k, cols, b);
+        normed(a, q, b);
         store_bytes(out + k, a, inv);
     }
 }
@@ -172,12 +187,16 @@ void launch(hipStream_t stream, const NormInt8 &p) {
     const dim3 waves((p.rows + 3) / 4), groups(p.rows), block(256);
     if (p.cols <= 512)
         MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 64, 1>), waves, block, 0, stream, p);
+    else if (p.cols <= 1024)
+        MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 64, 2>), waves, block, 0, stream, p);
     else if (p.cols <= 2048)
         MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 64, 4>), waves, block, 0, stream, p);
     else if (p.cols <= 4096)
         MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 256, 2>), groups, block, 0, stream, p);
+    else if (p.cols <= 8192)
+        MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 512, 2>), groups, dim3(512), 0, stream, p);
     else
-        MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 256, 8>), groups, block, 0, stream, p);
+        MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 512, 4>), groups, dim3(512), 0, stream, p);
 }
 }  // namespace
 

@@ -51,7 +51,8 @@ def check(nncl, x, residual, weight, eps=1e-6):
 
 
 SIZES = [(1, 1), (3, 7), (5, 16), (4, 500), (9, 512), (6, 513), (2, 2048), (3, 2049), (1, 4096),
-         (3, 4095), (2, 4100), (2, 16384), (2, 16400), (1, 40003), (1000, 777)]
+         (3, 4095), (2, 4100), (2, 16384), (2, 16400), (1, 40003), (1000, 777),
+         (5, 1024), (5, 1025), (2, 4096), (2, 8192), (2, 8193), (1, 12000), (2, 16385)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
