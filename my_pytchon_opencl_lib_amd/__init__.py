@@ -3,8 +3,8 @@
 The compute lives in libmigemm.so (hand-written HIP kernels behind the C ABI of
 include/migemm.h); this package is the Python host side: ctypes bindings (_native), the
 operator dispatcher mirroring the reference's NnClGlob (nncl_glob), the gradient nodes
-(autograd), and for serving in 8 bits the layers (layers.LinearInt8) and the paged cache of keys
-and values (cache.Int8Cache).
+(autograd), and for serving in 8 bits the layers (layers.LinearInt8), the paged cache of keys
+and values (cache.Int8Cache), and NnClGlob's norm to 8 bits (NormInt8) and sampling (Sample).
 """
 from . import _native
 from .nncl_glob import NnClGlob, ShapeError

@@ -6,12 +6,13 @@
 // more than u times the kept ones' sum. So every step asks one question: where in the order does a
 // running count or sum cross a value? It is answered without sorting the row:
 //
-//   * A histogram of the row, in bins of equal width in (top - l). Its running sums name the bin that
-//     a value falls in. With top_k it holds counts (the few tokens that are left get their weights
-//     later), otherwise weights.
-//   * The tokens of the bins in question are gathered, those that can matter are sorted by logit and
-//     index, and the running sums over them name the token. A bin of more tokens than are sorted at
-//     once (equal logits, mostly) is first cut by bits of logit and index until few are left.
+//   * A histogram of the row, in bins of equal width in (top - l). Its running sums name the bin
+//     that a value falls in. With top_k it holds counts (the few tokens that are left get their
+//     weights later), otherwise weights.
+//   * The tokens of the bins in question are gathered, those that can matter are sorted by logit
+//     and index, and the running sums over them name the token. A bin of more tokens than are
+//     sorted at once (equal logits, mostly) is first cut by bits of logit and index until few are
+//     left.
 //
 // Weights come from 64-bit arithmetic, because a sum of 10^5 float32 weights is off by more than a
 // token's share, and are summed as integers: exactly, in any order (atomics among them), so that a
@@ -22,12 +23,12 @@
 // less than half of the last bit are left out.
 //
 // Logits are read three times: for the largest, for the histogram, for the gathering. One
-// work-group a row, two of them a CU, is bound by these reads (512 x 65536 float32: 70 us, of
-// which 20, 15 and 15 to 18 for 134 MB each; a copy's rate gives 26) and, with fewer rows than
-// CUs, by the 64-bit steps of the histogram (half of the float32 rate: 11 us for 65536 tokens) and
-// by what waits for what: 17 us for 1 x 32000, 4.5 of them the histogram. Few rows of many tokens
-// are cut over work-groups, in four launches (1 x 131072: 21 us with top-k, 38 for half of the
-// tokens' weight, against 39 and 92 in one work-group).
+// work-group a row, two of them a CU, is bound by these reads (512 x 65536 float32: 73 us, of
+// which 20, 15 and 15 to 18 for 134 MB each; one read at a streaming read's rate gives 19) and,
+// with fewer rows than CUs, by the 64-bit steps of the histogram (half of the float32 rate: 11 us
+// for 65536 tokens) and by what waits for what: 18 us for 1 x 32000, 4.5 of them the histogram.
+// Few rows of many tokens are cut over work-groups, in four launches (1 x 131072: 21 us with
+// top-k 50, 33 to 38 with top-p 0.9 and no top-k, against 39 and 92 in one work-group).
 #include "int8_common.h"
 
 namespace migemm {
@@ -812,10 +813,10 @@ sample_row_kernel(SampleArgs p) {
     row.answer(p, r, q, counted, plan, total);
 }
 // ------------------------------------------------------------- rows cut over work-groups
-// Four launches: the largest logit of each part of a row; the parts' histograms, added up; the tokens
-// of the bins that the answer may need; and the answer, from those tokens. Each part of the third
-// reads the whole histogram and plans the same. A row whose tokens the list does not hold is walked
-// by the last kernel's work-group alone. What waits for memory is loaded as a kernel begins.
+// Four launches: the largest logit of each part of a row; the parts' histograms, added up; the
+// tokens of the bins that the answer may need; and the answer, from those tokens. Each part of the
+// third reads the whole histogram and plans the same. A row whose tokens the list does not hold is
+// walked by the last kernel's work-group alone. What waits for memory is loaded as a kernel begins.
 enum RowKind { kNothing, kGreedy, kDraw };
 struct RowState {
     Weights w;        // of the second kernel's first part
@@ -1021,6 +1022,12 @@ int launch_split(hipStream_t stream, SplitArgs a) {
 
 template <typename T>
 int launch(hipStream_t stream, const SampleArgs &p) {
+    // In parts or a work-group a row, us with top-k 50 and top-p 0.95 / with top-p 0.9 alone, rows
+    // of gaussian float32 logits: 1 x 32000 22 / 33 in parts, 18 / 34 whole; 1 x 65536 21 / 35 and
+    // 25 / 55; 64 x 65536 29 / 48 and 26 / 62; 128 x 65536 35 / 60 and 27.5 / 64; 1 x 131072
+    // 21 / 38 and 39 / 92; 64 x 131072 34.5 / 59 and 42 / 98; 128 x 131072 52 / 79 and 47.5 / 100;
+    // 256 x 131072 80 / 113 and 61 / 108. 256 parts in all (one a CU) of at least 4096 tokens: with 512
+    // or 1024 each reads and writes more of the histogram than it saves (1 to 4 us more).
     SplitArgs a{};
     a.p = p;
     const int most = p.vocab / 4096 < 64 ? p.vocab / 4096 : 64;
