@@ -30,6 +30,8 @@ struct NormInt8 {
     int rows, cols, type;
     float eps;
 };
+// Threads of its work-groups (a row's, or four rows' of up to 2048 values).
+constexpr int norm_int8_threads(int cols) { return cols <= 4096 ? 256 : 512; }
 int launch_norm_int8(hipStream_t stream, const NormInt8 &p);
 int launch_product_int8(hipStream_t stream, const Int8Product &p);
 // The layer: x quantised by rows, then the product (one launch for a few rows).

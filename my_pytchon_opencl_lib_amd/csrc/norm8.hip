@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(TPR == 64 ? 256 : TPR) norm_int8_kernel(NormIn
 
 template <typename T, bool RES>
 void launch(hipStream_t stream, const NormInt8 &p) {
-    const dim3 waves((p.rows + 3) / 4), groups(p.rows), block(256);
+    const dim3 waves((p.rows + 3) / 4), groups(p.rows), block(norm_int8_threads(p.cols));
     if (p.cols <= 512)
         MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 64, 1>), waves, block, 0, stream, p);
     else if (p.cols <= 1024)
@@ -194,9 +194,9 @@ void launch(hipStream_t stream, const NormInt8 &p) {
     else if (p.cols <= 4096)
         MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 256, 2>), groups, block, 0, stream, p);
     else if (p.cols <= 8192)
-        MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 512, 2>), groups, dim3(512), 0, stream, p);
+        MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 512, 2>), groups, block, 0, stream, p);
     else
-        MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 512, 4>), groups, dim3(512), 0, stream, p);
+        MIGEMM_LAUNCH((norm_int8_kernel<T, RES, 512, 4>), groups, block, 0, stream, p);
 }
 }  // namespace
 

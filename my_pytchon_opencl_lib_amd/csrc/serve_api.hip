@@ -102,8 +102,9 @@ int check_int8_rows(const char *what, const char *name, const int8_t *p, int64_t
 
 int64_t padded16(int cols) { return ((int64_t)cols + 15) / 16 * 16; }
 
-// Rows that are written in 8 bits, a work-group of 256 threads each.
-int check_quantized(const char *what, const int8_t *values, int64_t ldv, int rows, int cols) {
+// Rows that are written in 8 bits, a work-group of so many threads each.
+int check_quantized(const char *what, const int8_t *values, int64_t ldv, int rows, int cols,
+                    int threads) {
     if (rows < 1 || cols < 1 || cols > INT32_MAX - 65536)
         return set_error(MIGEMM_ERR_INVALID_ARG, "%s: sizes must be >= 1 (rows=%d cols=%d)", what,
                          rows, cols);
@@ -111,7 +112,7 @@ int check_quantized(const char *what, const int8_t *values, int64_t ldv, int row
     if (ldv % 16 != 0 || !aligned(values, 16))
         return set_error(MIGEMM_ERR_INVALID_ARG, "%s: values must be 16-byte aligned and ldv=%lld "
                          "a multiple of 16", what, (long long)ldv);
-    return check_grid(what, rows, 256);
+    return check_grid(what, rows, threads);
 }
 
 int check_cache(const char *what, const Cache8 &c) {
@@ -286,7 +287,7 @@ int migemm_quantize_rows(void *stream, const void *X, int type, int64_t ldx, int
     clear_error();
     MIGEMM_TRY(check_pointers(w, {X, values, scales}));
     MIGEMM_TRY(check_type(w, type));
-    MIGEMM_TRY(check_quantized(w, values, ldv, rows, cols));
+    MIGEMM_TRY(check_quantized(w, values, ldv, rows, cols, 256));
     MIGEMM_TRY(check_ld(w, "ldx", ldx, cols));
     MIGEMM_TRY(check_alias(w, {{values, rows_bytes(rows, ldv, padded16(cols), 1)},
                                {scales, (int64_t)rows * 4}},
@@ -302,7 +303,7 @@ int migemm_norm_int8(void *stream, const void *X, int64_t ldx, const void *R, in
     clear_error();
     MIGEMM_TRY(check_pointers(w, {X, values, scales}));
     MIGEMM_TRY(check_type(w, type));
-    MIGEMM_TRY(check_quantized(w, values, ldv, rows, cols));
+    MIGEMM_TRY(check_quantized(w, values, ldv, rows, cols, norm_int8_threads(cols)));
     MIGEMM_TRY(check_ld(w, "ldx", ldx, cols));
     if (R != nullptr) MIGEMM_TRY(check_ld(w, "ldr", ldr, cols));
     if (S != nullptr) {

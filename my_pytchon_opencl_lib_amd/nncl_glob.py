@@ -826,8 +826,8 @@ class NnClGlob:
         nothing; topK: so do those beyond the first topK (0: no limit); topP: of the others the
         fewest are kept that hold topP of their sum. The token is the first whose weights up to
         its own are more than uniform times the kept ones' sum; its probability is its share of
-        that. temperature 0: the largest logit's first token. Every parameter is a number, or a
-        tensor [rows] (float32; topK int32) with one for each row. Rows that allow no token (all
+        that. temperature 0: the largest logit's first token. Every parameter is a number (topP
+        above 0), or a tensor [rows] (float32; topK int32) with one for each row. Rows that allow no token (all
         -inf), that hold a NaN, or whose tensors' parameters are NaN or a temperature negative or
         infinite give token -1 and probability 0; a logit of inf counts as the largest float32. Few
         rows (at most vocabulary / 1024) of 40960 tokens or more use the stream's workspace

@@ -94,6 +94,8 @@ def test_norm(lib):
     refused(lib, "norm_int8", INVALID, "multiple of 16", ldv=72)
     refused(lib, "norm_int8", INVALID, "aligned", values=P(4, 8))
     refused(lib, "norm_int8", UNSUPPORTED, "exceed one launch", rows=1 << 24)
+    refused(lib, "norm_int8", UNSUPPORTED, "exceed one launch", rows=1 << 23, cols=4097, ldx=4097,
+            ldr=4097, lds=4097, ldv=4112)  # (512 threads a row)
 
 
 def test_closings(lib):
