@@ -597,14 +597,16 @@ class NnClGlob:
                 raise ShapeError(f"residual must be {x.dtype} {list(x.shape)} (got "
                                  f"{residual.dtype} {list(residual.shape)})")
             r2 = residual if x.dim() == 2 else residual.reshape(-1, k)
-            total = x.new_empty(x.shape)
+            total = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
             operands += (r2, total)
         values = x.new_empty((rows, (k + 15) // 16 * 16), dtype=torch.int8)
         scales = x.new_empty(rows, dtype=torch.float32)
         if rows:
+            added = (None, 0)
+            if r2 is not None:
+                added = (_ptr(r2), k if r2.is_contiguous() else _row_stride("residual", r2))
             _launch("migemm_norm_int8", operands + (values, scales), _ptr(x2),
-                    _row_stride("x", x2), _ptr(r2) if r2 is not None else None,
-                    _row_stride("residual", r2) if r2 is not None else 0, code,
+                    k if x2.is_contiguous() else _row_stride("x", x2), *added, code,
                     _ptr(weight) if weight is not None else None, eps,
                     _ptr(total) if total is not None else None, k, _ptr(values),
                     values.shape[1], _ptr(scales), rows, k)
