@@ -27,8 +27,8 @@
 // which 20, 15 and 15 to 18 for 134 MB each; one read at a streaming read's rate gives 19) and,
 // with fewer rows than CUs, by the 64-bit steps of the histogram (half of the float32 rate: 11 us
 // for 65536 tokens) and by what waits for what: 18 us for 1 x 32000, 4.5 of them the histogram.
-// Few rows of many tokens are cut over work-groups, in four launches (1 x 131072: 21 us with
-// top-k 50, 33 to 38 with top-p 0.9 and no top-k, against 39 and 92 in one work-group).
+// Few rows of many tokens are cut over work-groups, in three launches (1 x 131072: 19 us with
+// top-k 50, 35 with top-p 0.9 and no top-k, against 41 and 79 in one work-group).
 #include "int8_common.h"
 
 namespace migemm {
@@ -813,24 +813,24 @@ sample_row_kernel(SampleArgs p) {
     row.answer(p, r, q, counted, plan, total);
 }
 // ------------------------------------------------------------- rows cut over work-groups
-// Four launches: the largest logit of each part of a row; the parts' histograms, added up; the
-// tokens of the bins that the answer may need; and the answer, from those tokens. Each part of the
-// third reads the whole histogram and plans the same. A row whose tokens the list does not hold is
-// walked by the last kernel's work-group alone. What waits for memory is loaded as a kernel begins.
+// Three launches: the largest logit of each part of a row; the parts' histograms, added up; and the
+// tokens of the bins that the answer may need, and from them the answer. Each part of the third
+// reads the whole histogram and plans the same, and the one that comes to its end last (no other is
+// waited for) goes on to the answer, with the running sums still in LDS. A row whose tokens
+// the list does not hold is walked by that work-group alone. What waits for memory is loaded as a
+// kernel begins.
 enum RowKind { kNothing, kGreedy, kDraw };
 struct RowState {
-    Weights w;        // of the second kernel's first part
-    u64 total;        // of the third's: the histogram's sum, and what the answer needs
-    Plan plan;
-    int kind;         // of the second's
-    uint32_t listed;  // tokens gathered
-    uint32_t best;    // where the largest logit stands first (kGreedy)
+    Weights w;         // these two of the second kernel's first part
+    int kind;
+    uint32_t listed;   // tokens gathered
+    uint32_t arrived;  // parts that have gathered theirs
+    uint32_t best;     // where the largest logit stands first (kGreedy)
 };
 struct SplitArgs {
     SampleArgs p;
     int splits, chunk;  // parts of a row, tokens of a part
     u64 *mass;          // [rows][kBins]
-    u64 *running;       // [rows][kBins], its running sums
     u64 *list;          // [rows][kGather]
     float4 *parts;      // [rows][splits]: largest, smallest, whether one is NaN
     RowState *state;    // [rows]
@@ -851,6 +851,7 @@ __global__ void __launch_bounds__(kThreads) sample_top_kernel(SplitArgs a) {
         a.mass[(int64_t)r * kBins + i] = 0;
     if (part == 0 && tid == 0) {
         a.state[r].listed = 0;
+        a.state[r].arrived = 0;
         a.state[r].best = ~0u;
     }
     if (tid == 0) bad = 0;
@@ -911,8 +912,30 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SplitArgs a) {
         if (mass[i] != 0) atomicAdd(&a.mass[(int64_t)r * kBins + i], mass[i]);
 }
 
+// What a row's parts tell each other within a launch goes to memory and comes from there, past the
+// caches that they do not share.
+template <typename N>
+__device__ __forceinline__ void write_now(N *to, N x) {
+    __hip_atomic_store(to, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename N>
+__device__ __forceinline__ N read_now(const N *x) {
+    return __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Whether this work-group is the last of its row's parts to come here: all that the others wrote is
+// then there to be read. (Each thread waits until its writes are done. A fence instead writes back
+// and invalidates a whole L2, in every work-group: 64 x 131072 73 us.)
+__device__ __forceinline__ bool last_part(Shared &s, RowState &state, int parts) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");  // (no write moves behind the wait)
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) s.found = atomicAdd(&state.arrived, 1u);
+    __syncthreads();
+    return s.found == (uint32_t)parts - 1;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_gather_kernel(SplitArgs a) {
+__global__ void __launch_bounds__(kThreads) sample_answer_kernel(SplitArgs a) {
     __shared__ Shared s;
     const SampleArgs &p = a.p;
     const int tid = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
@@ -926,17 +949,25 @@ __global__ void __launch_bounds__(kThreads) sample_gather_kernel(SplitArgs a) {
     const Weights w = state.w;
     Walk<T, 4> walk;
     walk.start(logits, first, end);
-    if (kind == kNothing) return;
+    if (kind == kNothing) {
+        if (part == 0) nothing(p, r);
+        return;
+    }
     if (kind == kGreedy) {
         const float high = (float)w.top;
-        if (mine != high) return;
-        uint32_t best = ~0u;
-        walk.go([&](const auto &x, int i) {
+        if (mine == high) {
+            uint32_t best = ~0u;
+            walk.go([&](const auto &x, int i) {
 #pragma unroll
-            for (int e = 0; e < 16 / (int)sizeof(T); ++e)
-                best = bounded(x[e]) == high && (uint32_t)(i + e) < best ? i + e : best;
-        });
-        if (best != ~0u) atomicMin(&state.best, best);
+                for (int e = 0; e < 16 / (int)sizeof(T); ++e)
+                    best = bounded(x[e]) == high && (uint32_t)(i + e) < best ? i + e : best;
+            });
+            if (best != ~0u) atomicMin(&state.best, best);
+        }
+        if (last_part(s, state, a.splits) && tid == 0) {
+            p.tokens[r] = (int)read_now(&state.best);
+            p.probabilities[r] = 1.f;
+        }
         return;
     }
     const bool counted = q.counted(p.vocab);
@@ -945,89 +976,54 @@ __global__ void __launch_bounds__(kThreads) sample_gather_kernel(SplitArgs a) {
     else
         finish<false>(s, w);
     const Plan plan = plan_of(s, q, counted);
-    if (part == 0) {
-        for (int i = tid; i < kBins; i += kThreads)
-            a.running[(int64_t)r * kBins + i] = s.mass[i];
-        if (tid == 0) {
-            state.plan = plan;
-            state.total = s.mass[kBins - 1];
-        }
+    u64 *list = a.list + (int64_t)r * kGather;
+    if (plan.listed && mine >= w.smallest(plan.kept > plan.last ? plan.kept : plan.last)) {
+        const int found = gather(s, walk, w, plan);
+        if (tid == 0 && found) s.found = atomicAdd(&state.listed, (uint32_t)found);
+        __syncthreads();
+        const int to = s.found;
+        for (int i = tid; i < found && to + i < kGather; i += kThreads)
+            write_now(list + to + i, s.gathered[i]);
     }
-    if (!plan.listed) return;
-    const int found = mine >= w.smallest(plan.kept > plan.last ? plan.kept : plan.last)
-                          ? gather(s, walk, w, plan) : 0;
-    if (found == 0) return;
-    if (tid == 0) s.found = atomicAdd(&state.listed, (uint32_t)found);
-    __syncthreads();
-    const int to = s.found;
-    for (int i = tid; i < found && to + i < kGather; i += kThreads)
-        a.list[(int64_t)r * kGather + to + i] = s.gathered[i];
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_pick_kernel(SplitArgs a) {
-    __shared__ Shared s;
-    const SampleArgs &p = a.p;
-    const int tid = threadIdx.x, r = blockIdx.x;
-    const u64 *list = a.list + (int64_t)r * kGather;
-    const RowState &state = a.state[r];
-    const Asked q(p, r);
-    const int kind = state.kind;
-    if (kind == kNothing) return nothing(p, r);
-    if (kind == kGreedy) {
-        if (tid == 0) {
-            p.tokens[r] = (int)state.best;
-            p.probabilities[r] = 1.f;
-        }
-        return;
-    }
-    const Weights w = state.w;
-    const Plan plan = state.plan;
-    const bool counted = q.counted(p.vocab);
-    if (!plan.listed) {
-        for (int i = tid; i < kBins; i += kThreads) s.mass[i] = a.mass[(int64_t)r * kBins + i];
-        if (counted)
-            finish<true>(s, w);
-        else
-            finish<false>(s, w);
-    } else if (!plan.whole) {
-        for (int i = tid; i < kBins; i += kThreads) s.mass[i] = a.running[(int64_t)r * kBins + i];
+    if (!last_part(s, state, a.splits)) return;
+    const int gathered = min(read_now(&state.listed), (uint32_t)kGather);
+    if (plan.listed) {
+        for (int i = tid; i < gathered; i += kThreads) s.gathered[i] = read_now(list + i);
         __syncthreads();
     }
-    Row<T> row{s, static_cast<const T *>(p.logits) + (int64_t)r * p.ld, p.vocab,
-               plan.listed ? list : nullptr, (int)min(state.listed, (uint32_t)kGather), w, ~(u64)0,
-               0};
-    row.answer(p, r, q, counted, plan, state.total);
+    const u64 total = s.mass[kBins - 1];
+    Row<T> row{s, logits, p.vocab, plan.listed ? s.gathered : nullptr, gathered, w, ~(u64)0, 0};
+    row.answer(p, r, q, counted, plan, total);
 }
 
 template <typename T>
 int launch_split(hipStream_t stream, SplitArgs a) {
     const SampleArgs &p = a.p;
-    const size_t row = (2 * kBins + kGather) * sizeof(u64) + a.splits * sizeof(float4) +
+    const size_t row = (kBins + kGather) * sizeof(u64) + a.splits * sizeof(float4) +
                        sizeof(RowState);
     int rc = MIGEMM_OK;
     a.mass = static_cast<u64 *>(workspace(stream, p.rows * row, &rc, 0));
     if (a.mass == nullptr) return rc;
-    a.running = a.mass + (int64_t)p.rows * kBins;
-    a.list = a.running + (int64_t)p.rows * kBins;
+    a.list = a.mass + (int64_t)p.rows * kBins;
     a.parts = reinterpret_cast<float4 *>(a.list + (int64_t)p.rows * kGather);
     a.state = reinterpret_cast<RowState *>(a.parts + (int64_t)p.rows * a.splits);
     const dim3 grid(a.splits, p.rows), block(kThreads);
     MIGEMM_LAUNCH((sample_top_kernel<T>), grid, block, 0, stream, a);
     MIGEMM_LAUNCH((sample_bins_kernel<T>), grid, block, 0, stream, a);
-    MIGEMM_LAUNCH((sample_gather_kernel<T>), grid, block, 0, stream, a);
-    MIGEMM_LAUNCH((sample_pick_kernel<T>), dim3(p.rows), block, 0, stream, a);
-    return launch_status("sample_pick_kernel launch");
+    MIGEMM_LAUNCH((sample_answer_kernel<T>), grid, block, 0, stream, a);
+    return launch_status("sample_answer_kernel launch");
 }
 
 template <typename T>
 int launch(hipStream_t stream, const SampleArgs &p) {
-    // In parts or a work-group a row, us with top-k 50 and top-p 0.95 / with top-p 0.9 alone, rows
-    // of gaussian float32 logits: 1 x 32000 22 / 33 in parts, 18 / 34 whole; 1 x 65536 21 / 35 and
-    // 25 / 55; 64 x 65536 29 / 48 and 26 / 62; 128 x 65536 35 / 60 and 27.5 / 64; 1 x 131072
-    // 21 / 38 and 39 / 92; 64 x 131072 34.5 / 59 and 42 / 98; 128 x 131072 52 / 79 and 47.5 / 100;
-    // 256 x 131072 80 / 113 and 61 / 108. 256 parts in all (one a CU) of at least 4096 tokens: with 512
-    // or 1024 each reads and writes more of the histogram than it saves (1 to 4 us more).
+    // In parts or a work-group a row, us on a graph with top-k 50 and top-p 0.95 / with top-p 0.9
+    // alone, rows of gaussian float32 logits (deviation 2): 1 x 32000 20.4 / 31.6 in parts, 18.9 /
+    // 33.7 whole; 1 x 40960 19.1 / 31.1 and 20.5 / 37.7; 40 x 40960 24.3 / 37.1 and 21.6 / 40.2;
+    // 64 x 40960 28.5 / 41.6 and 23.3 / 41.6; 1 x 65536 19.0 / 33.0 and 26.3 / 50.3; 64 x 65536
+    // 28.8 / 45.4 and 29.7 / 55.4; 128 x 65536 34.0 / 54.2 and 30.4 / 56.9; 1 x 131072 19.1 / 35.0
+    // and 40.8 / 78.6; 128 x 131072 48.9 / 76.0 and 48.3 / 90.3. 256 parts in all (one a CU) of at
+    // least 4096 tokens: with 512 or 1024 each reads and writes more of the histogram than it
+    // saves (1 to 4 us more).
     SplitArgs a{};
     a.p = p;
     const int most = p.vocab / 4096 < 64 ? p.vocab / 4096 : 64;
