@@ -62,7 +62,10 @@ struct Shared {
     uint32_t wave_count[kWaves];
     float high[kWaves], low[kWaves];
     int bad;
-    uint32_t listed, found;
+    // Tokens of the list (set to 0 again only behind a barrier that follows its last reading), and
+    // of `gathered`, set once a row: the list begins while some still read the other.
+    uint32_t listed, taken;
+    uint32_t found;
 };
 
 // Ascending keys: largest logit first, then lowest index.
@@ -565,7 +568,7 @@ __device__ __forceinline__ int gather(Shared &s, const W &walk, const Weights &w
     const bool apart = !plan.whole && plan.kept > plan.last;
     Span kept = draw;
     if (apart) kept = Span(w, plan.kept, plan.kept);
-    if (threadIdx.x == 0) s.listed = 0;
+    if (threadIdx.x == 0) s.taken = 0;
     __syncthreads();
     walk.go([&](const auto &x, int i) {
         float most = x[0];  // (few are taken: one question for all of them)
@@ -575,12 +578,12 @@ __device__ __forceinline__ int gather(Shared &s, const W &walk, const Weights &w
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             if (!(draw.has(x[e]) || kept.has(x[e]))) continue;
-            const uint32_t place = atomicAdd(&s.listed, 1u);
+            const uint32_t place = atomicAdd(&s.taken, 1u);
             if (place < kGather) s.gathered[place] = key_of(bounded(x[e]), i + e);
         }
     });
     __syncthreads();
-    return min((int)s.listed, kGather);
+    return min((int)s.taken, kGather);
 }
 
 // A row and what is known of it. Its tokens come from keys that were gathered, or (keys null; a
