@@ -576,9 +576,9 @@ int migemm_cache_attention(void *stream, const void *Q, int type, int64_t ldq,
  * are held to 2^-39 of themselves and 2^-42 of the largest, and summed exactly. A logit of -inf
  * is never chosen, inf counts as the largest float32; a row without a logit above -inf, with a
  * NaN, or with a parameter that is NaN or a temperature that is negative or not finite gives
- * token -1 and probability 0. One launch; rows of 40960 tokens or more, at most vocab / 1024 of
- * them, are cut over work-groups in three, which use the stream's workspace (34 KB a row at
- * most): reserve it before a capture. */
+ * token -1 and probability 0. One launch; rows of 40960 tokens or more, at most vocab / 1024 and at
+ * most 128 of them, are cut over work-groups in three, which use the stream's workspace (34 KB a
+ * row at most): reserve it before a capture. */
 int migemm_sample(void *stream, const void *logits, int type, int64_t ld, int rows, int vocab,
                   const float *uniforms, const float *temperatures, float temperature,
                   const int *top_ks, int top_k, const float *top_ps, float top_p,

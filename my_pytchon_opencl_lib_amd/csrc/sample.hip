@@ -1026,7 +1026,7 @@ int launch(hipStream_t stream, const SampleArgs &p) {
     // 28.8 / 45.4 and 29.7 / 55.4; 128 x 65536 34.0 / 54.2 and 30.4 / 56.9; 1 x 131072 19.1 / 35.0
     // and 40.8 / 78.6; 128 x 131072 48.9 / 76.0 and 48.3 / 90.3. 256 parts in all (one a CU) of at
     // least 4096 tokens: with 512 or 1024 each reads and writes more of the histogram than it
-    // saves (1 to 4 us more).
+    // saves (1 to 4 us more). A row in two parts at least, so 128 rows at most.
     SplitArgs a{};
     a.p = p;
     const int most = p.vocab / 4096 < 64 ? p.vocab / 4096 : 64;

@@ -832,8 +832,8 @@ class NnClGlob:
         above 0), or a tensor [rows] (float32; topK int32) with one for each row. Rows that allow no token (all
         -inf), that hold a NaN, or whose tensors' parameters are NaN or a temperature negative or
         infinite give token -1 and probability 0; a logit of inf counts as the largest float32. Few
-        rows (at most vocabulary / 1024) of 40960 tokens or more use the stream's workspace
-        (reserve_workspace before a capture)."""
+        rows (at most vocabulary / 1024, and at most 128) of 40960 tokens or more use the stream's
+        workspace (reserve_workspace before a capture)."""
         code = _check_rows("logits", logits, 2)
         rows, vocab = logits.shape
         _check_typed("uniforms", uniforms, torch.float32, (rows,))
