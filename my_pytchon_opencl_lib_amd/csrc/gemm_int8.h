@@ -82,11 +82,32 @@ struct Sigmoid {
         return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z));
     }
 };
-// x (1 + erf(x / sqrt 2)) / 2: off by less than |x| 2^-21.
+// x (1 + erf(x / sqrt 2)) / 2 = x P(x), P the normal distribution: P(-a) = exp(-a^2 / 2) u q(u) for a
+// = |x| and u = 1 / (1 + 0.39 a), q of degree 9 through the Chebyshev nodes of u for 0 <= a <= 13.3
+// (off by 2^-26.7), and P(a) = 1 - P(-a). Off by less than (10 + 1.5 x^2 / 2) 2^-23 of the value,
+// the small ones of negative x too (in 2^-24: 6 of u, 7 of q, 5 of the other steps, 3 x^2 / 2 of the
+// exponent; 1 + erf moves in steps of 2^-24, and at -5 is off by a tenth), and 0 where the
+// exponential is less than 2^-126 (beyond 13.2).
 struct Gelu {
     __device__ __forceinline__ float operator()(float x) const {
 #pragma clang fp contract(off)
-        return 0.5f * x * (1.f + erff(x * 0.70710678118654752440f));
+        const float a = fabsf(x);
+        float p = 0.f;
+        if (a < 13.3f) {  // (a branch also keeps the values of a thread apart, so registers suffice)
+            const float u = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.39f, 1.f));
+            float q = 0.0300211515f;
+            q = __builtin_fmaf(q, u, -0.172886625f);
+            q = __builtin_fmaf(q, u, 0.398460865f);
+            q = __builtin_fmaf(q, u, -0.432662934f);
+            q = __builtin_fmaf(q, u, 0.184471577f);
+            q = __builtin_fmaf(q, u, -0.0497388989f);
+            q = __builtin_fmaf(q, u, 0.101456709f);
+            q = __builtin_fmaf(q, u, 0.129514083f);
+            q = __builtin_fmaf(q, u, 0.155783504f);
+            q = __builtin_fmaf(q, u, 0.155580565f);
+            p = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170368f) * (u * q);
+        }
+        return x * (x < 0.f ? p : 1.f - p);
     }
 };
 constexpr float kLog2e = 1.44269504088896340736f, kGeluA = 1.59576912160573071176f;
@@ -195,15 +216,16 @@ __device__ __forceinline__ void fetch_tail(const Op &op, typename Op::Tail &t, i
 // exchanged, all of it at once. (From the registers, one value a lane and access, the 256 x 256
 // tiles keep 428 values in scratch.) Row r of a block stands at r with bits 0 and 2 exchanged: the
 // two half-wavefronts that write rows r and r + 4 then meet different banks. 4096 x 4096 to
-// 11008 outputs and their gates takes 378 us (as many plain products, 8192 x 4096 to 11008, 362;
-// bound by the matrix cores as those are); 1000 x 777 to gelu of 3000 13.9 (plain 12.5).
+// 11008 outputs and their gates takes 371 us (as many plain products, 8192 x 4096 to 11008, 362;
+// bound by the matrix cores as those are); 1000 x 777 to gelu of 3000 12.9 (silu 11.7).
+// The 256 x 256 tiles keep up to 9 registers in scratch here (of a gated product none).
 __device__ __forceinline__ int block_row(int r) {
     return (r & ~5) | ((r >> 2) & 1) | ((r & 1) << 2);
 }
 
 // The scales and bias of a tile's rows and columns, one value a thread: loaded as the kernel
 // begins, kept in a register and put into LDS for its end (read from memory as they are used, each
-// block waits for them: 405 us instead of 378). By place: the rows' scales, the columns' (of a
+// block waits for them: 27 us more). By place: the rows' scales, the columns' (of a
 // gated tile the gate's outputs, then the other half's), the columns' bias.
 template <int KIND, int BM, int BN>
 __device__ __forceinline__ float closing_value(const Int8Args &p, int m0, int n0, int i) {
