@@ -273,7 +273,10 @@ int migemm_stream_synchronize(void *stream);
  * running the same calls once on that stream. A call that needs more during a capture
  * fails with MIGEMM_ERR_WORKSPACE. A buffer that a graph captured lives until the process
  * ends and is no longer used by eager calls after the capture (the next eager call on the
- * stream gets a new one), so replaying the graph on another stream cannot race with them. */
+ * stream gets a new one), so replaying the graph on another stream cannot race with them. Graphs
+ * that are captured on one stream one after the other use the same buffers, and must be replayed
+ * one after the other too, unless this call comes before each capture: it gives the stream new
+ * buffers where a graph has captured its own. */
 /* Grows each of `stream`'s two workspace buffers (the stream's device) to >= bytes. */
 int migemm_workspace_reserve(void *stream, size_t bytes);
 /* Frees the stream's workspace buffers in the stream's order (the work queued so far still
