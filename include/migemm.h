@@ -574,12 +574,13 @@ int migemm_cache_attention(void *stream, const void *Q, int type, int64_t ldq,
  *           (1 or more: all; 0 or less: one)
  * and the token is the first whose weights, up to its own, are more than uniform times the kept
  * ones' sum. probabilities[r] is its weight over that sum. temperature 0 gives the largest
- * logit's first token, with probability 1. Each parameter is one for all rows, or
- * (temperatures, top_ks, top_ps, min_ps [rows] on the GPU, where not NULL) one a row. Weights
+ * logit's first token, with probability 1. Each parameter is one for all rows (refused unless
+ * temperature >= 0 is finite, top_k >= 0, 0 < top_p <= 1 and 0 <= min_p <= 1), or (temperatures,
+ * top_ks, top_ps, min_ps [rows] on the GPU, where not NULL) one a row, not refused. Weights
  * are held to 2^-39 of themselves and 2^-42 of the largest, and summed exactly. A logit of -inf
  * is never chosen, inf counts as the largest float32; a row without a logit above -inf, with a
- * NaN, or with a parameter that is NaN or a temperature that is negative or not finite gives
- * token -1 and probability 0. One launch; rows of 40960 tokens or more, at most vocab / 1024 and at
+ * NaN, or with a parameter or random number that is NaN or a temperature that is negative or not
+ * finite gives token -1 and probability 0. One launch; rows of 40960 tokens or more, at most vocab / 1024 and at
  * most 128 of them, are cut over work-groups in three, which use the stream's workspace (34 KB a
  * row at most): reserve it before a capture. */
 int migemm_sample(void *stream, const void *logits, int type, int64_t ld, int rows, int vocab,

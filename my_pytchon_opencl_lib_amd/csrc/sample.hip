@@ -16,8 +16,8 @@
 //
 // Weights come from 64-bit arithmetic, because a sum of 10^5 float32 weights is off by more than a
 // token's share, and are summed as integers: exactly, in any order (atomics among them), so that a
-// result does not depend on how a row was walked. Within a bin's width of at most 0.047 in log2 w
-// a token's weight over its bin's middle one is a polynomial of degree 4 (off by 2^-39 at most);
+// result does not depend on how a row was walked. Within a bin's width of at most 2^-5 in log2 w
+// a token's weight over its bin's middle one is a polynomial of degree 4 (off by 2^-40 at most);
 // these are summed with 43 fractional bits, and a bin's sum is multiplied by its middle weight
 // once, to 42 bits below the point or more (62 - log2(vocabulary), at most 46). Tokens that weigh
 // less than half of the last bit are left out.
@@ -29,6 +29,13 @@
 // for 65536 tokens) and by what waits for what: 18 us for 1 x 32000, 4.5 of them the histogram.
 // Few rows of many tokens are cut over work-groups, in three launches (1 x 131072: 19 us with
 // top-k 50, 35 with top-p 0.9 and no top-k, against 41 and 79 in one work-group).
+//
+// Where more than 2048 tokens are in question (any top-k above that; rows so flat, or so alike, that
+// a bin holds as many) the row's logits are walked again for each cut and sum, one a thread and
+// step, by one work-group, so this costs most where rows are few. 1 x 131072, gaussian logits
+// of deviation 2: top-k 2500 163 us, with top-p 0.95 212 (top-k 2000: 37); of deviation 0.5, top-p
+// 0.9 245 (without 28); of 0.02 337 (150); 64 x 131072 of 0.5 428. Elementary torch operations: 340
+// to 390, 1980 for the 64 rows.
 #include "int8_common.h"
 
 namespace migemm {
@@ -178,7 +185,7 @@ struct Weights {
         return index(placed(d < cut ? d : cut));
     }
     // The weight over the middle one of its bin, 2^f for |f| <= width / 2, with kFraction bits: 1
-    // + f q(f), q of degree 3 through the Chebyshev nodes of (2^f - 1) / f (off by 2^-39 at the
+    // + f q(f), q of degree 3 through the Chebyshev nodes of (2^f - 1) / f (off by 2^-40 at the
     // bin's ends). Eight 64-bit steps: the middle comes from adding and taking off `magic`, and
     // the last step of the polynomial rounds to an integer, too.
     __device__ __forceinline__ u64 over_middle(double d, uint32_t &b) const {
@@ -445,7 +452,7 @@ __device__ __forceinline__ void run_up(Shared &s, u64 *mass, uint32_t *count) {
 }
 
 // A filled histogram becomes its running sums. A bin's weight is its sum times its middle one; its
-// number of tokens is at most the sum over the least that a token adds to it (2^-0.023).
+// number of tokens is at most the sum over the least that a token adds to it (2^-0.016, 1 / 1.011).
 template <bool COUNT>
 __device__ __forceinline__ void finish(Shared &s, const Weights &w) {
     for (int b = threadIdx.x; b < kBins; b += kThreads) {
@@ -587,8 +594,8 @@ __device__ __forceinline__ int gather(Shared &s, const W &walk, const Weights &w
 }
 
 // A row and what is known of it. Its tokens come from keys that were gathered, or (keys null; a
-// row of too many, and walked simply, so that this rare case takes no registers from the other)
-// its logits.
+// row of too many, and walked simply, so that this case takes no registers from the other) its
+// logits.
 template <typename T>
 struct Row {
     Shared &s;
@@ -926,8 +933,11 @@ __device__ __forceinline__ N read_now(const N *x) {
     return __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 // Whether this work-group is the last of its row's parts to come here: all that the others wrote is
-// then there to be read. (Each thread waits until its writes are done. A fence instead writes back
-// and invalidates a whole L2, in every work-group: 64 x 131072 73 us.)
+// then there to be read. This rests on the chip's order, not on the language's release and acquire:
+// stores and loads of agent scope go past the L2s that work-groups do not share (sc1), a
+// wavefront's wait ends when its stores have got there, and a work-group is counted behind the
+// barrier that its threads come to after that wait. (A fence, which would say it in the language,
+// writes back and invalidates a whole L2, in every work-group: 64 x 131072 73 us.)
 __device__ __forceinline__ bool last_part(Shared &s, RowState &state, int parts) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");  // (no write moves behind the wait)
     __builtin_amdgcn_s_waitcnt(0);

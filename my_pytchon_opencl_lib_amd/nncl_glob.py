@@ -829,11 +829,12 @@ class NnClGlob:
         fewest are kept that hold topP of their sum. The token is the first whose weights up to
         its own are more than uniform times the kept ones' sum; its probability is its share of
         that. temperature 0: the largest logit's first token. Every parameter is a number (topP
-        above 0), or a tensor [rows] (float32; topK int32) with one for each row. Rows that allow no token (all
-        -inf), that hold a NaN, or whose tensors' parameters are NaN or a temperature negative or
-        infinite give token -1 and probability 0; a logit of inf counts as the largest float32. Few
-        rows (at most vocabulary / 1024, and at most 128) of 40960 tokens or more use the stream's
-        workspace (reserve_workspace before a capture)."""
+        above 0), or a tensor [rows] (float32; topK int32) with one for each row, which is not
+        refused (a topP of 0 or less keeps one token, a topK of 0 or less all). Rows that allow no
+        token (all -inf), that hold a NaN, or whose uniform or parameter in a tensor is NaN or a
+        temperature negative or infinite give token -1 and probability 0; a logit of inf counts as
+        the largest float32. Few rows (at most vocabulary / 1024, and at most 128) of 40960 tokens
+        or more use the stream's workspace (reserve_workspace before a capture)."""
         code = _check_rows("logits", logits, 2)
         rows, vocab = logits.shape
         _check_typed("uniforms", uniforms, torch.float32, (rows,))
