@@ -216,7 +216,7 @@ __device__ __forceinline__ void fetch_tail(const Op &op, typename Op::Tail &t, i
 // exchanged, all of it at once. (From the registers, one value a lane and access, the 256 x 256
 // tiles keep 428 values in scratch.) Row r of a block stands at r with bits 0 and 2 exchanged: the
 // two half-wavefronts that write rows r and r + 4 then meet different banks. 4096 x 4096 to
-// 11008 outputs and their gates takes 371 us (as many plain products, 8192 x 4096 to 11008, 362;
+// 11008 outputs and their gates takes 360 to 371 us (as many plain products, 8192 x 4096 to 11008, 362;
 // bound by the matrix cores as those are); 1000 x 777 to gelu of 3000 12.9 (silu 11.7).
 // The 256 x 256 tiles keep up to 9 registers in scratch here (of a gated product none).
 __device__ __forceinline__ int block_row(int r) {
