@@ -1,6 +1,8 @@
 """GPU tests of Sample where the rows of a call decide how it runs: rows of 40960 tokens or more are
 cut over work-groups while they are at most vocabulary / 1024 and at most 128. Beyond 131072 tokens
 it is the second that counts."""
+import ctypes
+
 import pytest
 import torch
 
@@ -12,13 +14,19 @@ pytestmark = pytest.mark.gpu
 VOCAB = 262144
 
 
+def new_stream():
+    """A stream that nothing used before (torch's own come from a pool of 32, in turn)."""
+    s = ctypes.c_void_p()
+    _native.call("migemm_stream_create", ctypes.byref(s))
+    return torch.cuda.ExternalStream(s.value)
+
+
 @pytest.mark.parametrize("rows,uses", [(128, True), (129, False), (200, False)])
 def test_a_capture_needs_a_workspace_up_to_128_rows(nncl, rows, uses):
     print(rows, flush=True)
     x = torch.randn(rows, VOCAB, generator=gen(rows), device="cuda")
     u = torch.rand(rows, generator=gen(1), device="cuda")
-    stream = torch.cuda.Stream()
-    _native.call("migemm_workspace_release", stream.cuda_stream)
+    stream = new_stream()
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     if uses:

@@ -5,12 +5,13 @@ import pytest
 import torch
 
 from test_int8_gpu import gen
+from test_sample_border_gpu import new_stream
 
 pytestmark = pytest.mark.gpu
 
 
 def test_two_graphs_of_one_stream_replayed_at_once(nncl):
-    stream = torch.cuda.Stream()
+    stream = new_stream()
     xs = [torch.randn(3, 131072, generator=gen(i), device="cuda") for i in range(3)]
     us = [torch.rand(3, generator=gen(10 + i), device="cuda") for i in range(3)]
     want = [nncl.Sample(x, u, 0.8, 0, 0.9) for x, u in zip(xs, us)]
@@ -23,7 +24,7 @@ def test_two_graphs_of_one_stream_replayed_at_once(nncl):
         with torch.cuda.graph(graph, stream=stream):
             got.append(nncl.Sample(xs[i], us[i], 0.8, 0, 0.9))
         graphs.append(graph)
-    sides = [torch.cuda.Stream() for _ in graphs]
+    sides = [new_stream() for _ in graphs]
     torch.cuda.synchronize()
     for _ in range(5):
         for _ in range(8):
